@@ -174,7 +174,7 @@ def _own_pass(s):
         loss, saved = ops.linear_distill_fwd(s["x"], s["w"], s["idx"], s["val"], tau=s["tau"], offset=s["off"])
         out = {"loss": loss}
         if s["grad"]:
-            out["dx"], out["dw"] = ops.linear_distill_bwd(s["x"], s["w"], s["idx"], s["val"], saved, s["drow"], tau=s["tau"], offset=s["off"])
+            out["dx"], out["dw"] = ops.linear_distill_bwd(s["x"], s["w"], s["idx"], saved, s["drow"], tau=s["tau"], offset=s["off"])
         return out
     loss, dlogits = ops.topk_distill(s["logits"], s["idx"], s["val"], tau=s["tau"], drow=s["drow"])
     return {"loss": loss, "dlogits": dlogits}
