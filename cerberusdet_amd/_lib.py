@@ -83,6 +83,16 @@ class MatchDesc(C.Structure):
     _fields_ = [("N", i32), ("max_det", i32), ("T", i32), ("max_labels", i32)]
 
 
+class LinearLossDesc(C.Structure):
+    _fields_ = [("N", i32), ("V", i32), ("d", i32), ("dtype", i32), ("x_ld", i64), ("w_ld", i64), ("scale", f32), ("tau", f32), ("offset", vp),
+                ("label64", i32)]
+
+
+class TopkDistillDesc(C.Structure):
+    _fields_ = [("P", i32), ("G", i32), ("V", i32), ("k", i32), ("dtype", i32), ("val_dtype", i32), ("grad_dtype", i32), ("ld", i64), ("grad_ld", i64),
+                ("tau", f32), ("grad_scale", f32)]
+
+
 class WgradItem(C.Structure):
     _fields_ = [("x", vp), ("dy", vp), ("dw", vp), ("src_ld", i32), ("src_coff", i32)]
 
@@ -174,6 +184,12 @@ _SIGS = {
     "cdet_pad_targets": (i32, [vp, vp, vp, i32, i32, i32, f32, f32, vp, vp, vp]),
     "cdet_det_loss_ws_bytes": (i64, [C.POINTER(LossDesc)]),
     "cdet_det_loss": (i32, [C.POINTER(LossDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "cdet_linear_loss_ws_bytes": (i64, [C.POINTER(LinearLossDesc), i32]),
+    "cdet_linear_ce_fwd": (i32, [C.POINTER(LinearLossDesc), vp, vp, vp, vp, vp, vp, vp]),
+    "cdet_linear_ce_bwd": (i32, [C.POINTER(LinearLossDesc), vp, vp, vp, vp, vp, i32, vp, i64, vp, i64, vp, vp]),
+    "cdet_linear_distill_fwd": (i32, [C.POINTER(LinearLossDesc), vp, vp, i32, vp, vp, i32, vp, vp, vp, vp]),
+    "cdet_linear_distill_bwd": (i32, [C.POINTER(LinearLossDesc), vp, vp, i32, vp, vp, vp, i32, vp, i64, vp, i64, vp, vp]),
+    "cdet_topk_distill": (i32, [C.POINTER(TopkDistillDesc), vp, vp, vp, vp, vp, vp, vp]),
     "cdet_nms_ws_bytes": (i64, [C.POINTER(NmsDesc)]),
     "cdet_match_predictions": (i32, [C.POINTER(MatchDesc), vp, vp, vp, vp, vp, vp, vp]),
     "cdet_merge_tasks": (i32, [C.POINTER(MergeDesc), vp, vp, vp, vp]),

@@ -1,0 +1,952 @@
+// Losses of a linear class projection over a long class list, logits never in memory:
+//   z[r][v] = scale * <x_r, w_v> + offset[v]          x [N, d], w [V, d], 16-bit; everything below in fp32
+//   cross entropy   loss_r = lse_r - z[r][label_r],                       dz[r][v] = g_r (p[r][v] - [v == label_r])
+//   distillation    loss_r = tau^2 sum_j q_rj (log q_rj - log p[r][idx_rj]), dz[r][v] = g_r tau (p[r][v] - sum_{j: idx_rj == v} q_rj)
+// with p = softmax(z / tau) and q the softmax of the teacher's k logits / tau. dx = scale * dz w, dw = scale * dz^T x.
+//
+// Forward: one matrix product whose epilogue keeps, per row and per 128 (64) classes, the running maximum and the sum of exponentials; a second launch
+// joins those pairs per row in a fixed order. Backward: per piece of the class list the product is computed again, its epilogue turns the logits
+// into dz (16-bit, one [N, piece] buffer), and one launch computes the piece's dw and adds the piece to dx. dz is relative to the largest row gradient
+// (and, in fp16, times 2^12): p of a 10^5-class list times 1 / N is far below fp16's smallest number.
+//
+// One product kernel for all three (gemm_tile): an 8-wave workgroup, 256 x 256 (or 128 x 128) outputs, K in steps of 32 through a ring of four LDS
+// stages filled by LDS-DMA. The two halves of the workgroup run half a step apart: while one multiplies, the other reads its fragments.
+// Operand "A" (fragment rows) is what must come out contiguous: a lane ends up with four consecutive A rows of one B row. So A = classes in the first
+// product (a lane holds classes of ONE row of x: the softmax statistics are sums inside the lane), A = features in the other two. An operand whose
+// memory runs along the output index instead of K is staged as it lies and transposed by ds_read_b64_tr_b16 on the way to the registers.
+#include <algorithm>
+
+#include "common.h"
+
+namespace cdet {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(2))) float cf32x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 cbf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 cf16x2;
+
+constexpr int LBK = 32;                   // K elements per step
+constexpr int LRING = 4;                  // LDS stages
+constexpr unsigned LSENT = 0xE0000000u;   // offset beyond every buffer: the DMA writes zeros
+constexpr int LCAP = (int)0xD0000000u;    // extent of every buffer descriptor (offsets are at most 256 rows or 32 rows of < 4 M elements)
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <int DT>
+__device__ __forceinline__ f32x16 lmfma(const u32x4& a, const u32x4& b, const f32x16& c) {
+    if (DT == CDET_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t lpack2(float a, float b) {  // round to nearest even
+    if (DT == CDET_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(cf32x2{a, b}, cbf16x2));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(cf32x2{a, b}, cf16x2));
+}
+__device__ __forceinline__ int xcd_order(int b, int n) {  // consecutive logical ids run on one XCD (bijective)
+    const int xcd = b & 7, q = n >> 3, r = n & 7, j = b >> 3;
+    return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + j;
+}
+
+// An operand of a tile: p points at the tile's first element. TR = false: rows of K-contiguous elements, [row][k]; TR = true: [k][row].
+struct TileSrc {
+    const uint16_t* p;
+    int64_t ld;
+    int rows;  // valid rows from p on (the rest reads as zero); a multiple of 8 when TR
+};
+
+// acc[mt][nt] += A B^T over K (any K; K % 8 == 0 for the K-contiguous operands). C row of register i: grp * MT*32 + mt*32 + 8*(i>>2) + 4*(lane>>5) + (i&3);
+// C column: wave * NT*32 + nt*32 + (lane&31). Ends with every wave past its last LDS access.
+template <int DT, int MT, int NT, bool ATR, bool BTR>
+__device__ __forceinline__ void gemm_tile(unsigned char* smem, TileSrc A, TileSrc B, int K, f32x16 (&acc)[MT][NT]) {
+    constexpr int ABYTES = MT * 64 * 64, BBYTES = NT * 128 * 64, STAGE = ABYTES + BBYTES;
+    constexpr int NA = MT / 2, NB = NT, NPW = NA + NB;  // DMA instructions (1 KiB) of a wave per step
+    const int tid = (int)threadIdx.x, lane = tid & 63;
+    const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wave8 >> 2, wave = wave8 & 3;
+    const int l31 = lane & 31, h = lane >> 5;
+    const int steps = (K + LBK - 1) / LBK;
+
+    // DMA sources. K-contiguous: piece `id` = rows 16 id .. +15, four lanes (64 B) a row, 16-byte slot s of row r stored at s ^ ((r >> 2) & 3): the 16
+    // lanes that one ds_read_b128 cycle serves then cover the 16 slots of 256 bytes. Transposed: piece `id` = 64 rows x 8 k, eight lanes (128 B) a k;
+    // slot s of k stored at s ^ (4 * ((k >> 1) & 1)): the four k of a transpose read, and its two 16-row halves, fall into different banks.
+    unsigned va[NA], vb[NB];
+    int ka[NA], kb[NB];  // the lane's first k of the piece
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+        const int id = wave8 + 8 * i;
+        const int k = ATR ? 8 * (id & 3) + (lane >> 3) : 8 * ((lane & 3) ^ ((lane >> 4) & 3));
+        const int row = ATR ? (id >> 2) * 64 + 8 * ((lane & 7) ^ (((lane >> 4) & 1) << 2)) : 16 * id + (lane >> 2);
+        ka[i] = row < A.rows ? k : 0x40000000;
+        va[i] = ATR ? (unsigned)(k * A.ld + row) * 2u : (unsigned)(row * A.ld + k) * 2u;
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int id = wave8 + 8 * i;
+        const int k = BTR ? 8 * (id & 3) + (lane >> 3) : 8 * ((lane & 3) ^ ((lane >> 4) & 3));
+        const int row = BTR ? (id >> 2) * 64 + 8 * ((lane & 7) ^ (((lane >> 4) & 1) << 2)) : 16 * id + (lane >> 2);
+        kb[i] = row < B.rows ? k : 0x40000000;
+        vb[i] = BTR ? (unsigned)(k * B.ld + row) * 2u : (unsigned)(row * B.ld + k) * 2u;
+    }
+    const int64_t astep = ATR ? LBK * A.ld : LBK, bstep = BTR ? LBK * B.ld : LBK;
+    const uint16_t *ap = A.p, *bp = B.p;
+    int krem = K;  // K left from the next step to be fetched on: <= 0 beyond the end, where every lane fetches zeros and the counts stay the same
+    int fslot = 0;
+    auto fetch = [&]() {
+        const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)ap, 0, LCAP, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)bp, 0, LCAP, 0x00020000);
+        unsigned char* dst = smem + fslot * STAGE + wave8 * 1024;
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(dst + i * 8192), 16, (int)(ka[i] < krem ? va[i] : LSENT), 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void*)(dst + ABYTES + i * 8192), 16, (int)(kb[i] < krem ? vb[i] : LSENT), 0, 0, 0);
+        ap += astep;
+        bp += bstep;
+        krem -= LBK;
+        fslot = (fslot + 1) & (LRING - 1);
+    };
+
+    // fragment addresses
+    const int trl = (8 * h + ((lane & 15) >> 2)) * 128 + (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ (((lane >> 3) & 1) << 2)) << 4) + (lane & 1) * 8;
+    const int nrl = l31 * 64 + ((h ^ ((l31 >> 2) & 3)) << 4);
+    const int aoff = ATR ? trl + grp * (MT / 2) * 4096 : nrl + grp * MT * 2048;
+    const int boff = ABYTES + (BTR ? (trl ^ (((wave * NT) & 1) << 6)) + ((wave * NT) >> 1) * 4096 : nrl + wave * NT * 2048);
+    auto frag_n = [&](int base, int t, int kk) { return *reinterpret_cast<const u32x4*>(smem + ((base + t * 2048) ^ (kk << 5))); };
+    // transpose reads are asm: in front of the builtin the compiler waits for every DMA in flight. Valid behind the phase's own wait (landed())
+    const int lds0 = (int)(unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+    auto frag_t = [&](int base, int t, int kk, u32x2& lo, u32x2& hi) {
+        const int o = lds0 + (((base + (t >> 1) * 4096) ^ ((t & 1) << 6)) + kk * 2048);
+        asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(lo) : "v"(o));
+        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:512" : "=v"(hi) : "v"(o));
+    };
+
+    fetch();
+    fetch();
+    fetch();
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NPW) : "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if (grp == 1) {  // half a step behind from here to the end of the loop
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    int so = 0;
+    for (int st = 0; st < steps; ++st) {
+        u32x4 a[2][MT], b[2][NT];
+        u32x2 al[2][MT], ah[2][MT], bl[2][NT], bh[2][NT];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                if (BTR) frag_t(so + boff, i, kk, bl[kk][i], bh[kk][i]);
+                else b[kk][i] = frag_n(so + boff, i, kk);
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                if (ATR) frag_t(so + aoff, i, kk, al[kk][i], ah[kk][i]);
+                else a[kk][i] = frag_n(so + aoff, i, kk);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // stage st + 3 goes where stage st - 1 was: its last reader, the other half in ITS memory phase of step st - 1, waited for its reads before the
+        // barrier that opened this phase
+        fetch();
+        so = so + STAGE == LRING * STAGE ? 0 : so + STAGE;
+        __builtin_amdgcn_sched_barrier(0);
+        // stage st + 1 has landed for this wave (two stages stay in flight); the fragments are in registers
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * NPW) : "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        // (the registers of the transpose reads become values here, behind the wait)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            if (ATR) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    asm volatile("" : "+v"(al[kk][i]), "+v"(ah[kk][i]));
+                    a[kk][i] = u32x4{al[kk][i][0], al[kk][i][1], ah[kk][i][0], ah[kk][i][1]};
+                }
+            }
+            if (BTR) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    asm volatile("" : "+v"(bl[kk][i]), "+v"(bh[kk][i]));
+                    b[kk][i] = u32x4{bl[kk][i][0], bl[kk][i][1], bh[kk][i][0], bh[kk][i][1]};
+                }
+            }
+        }
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = lmfma<DT>(a[kk][i], b[kk][j], acc[i][j]);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (st + 1 < steps) {
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    if (grp == 0) {  // releases the other half into its last multiplication
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the (empty) trailing fetches write zeros into the ring: done before anybody reuses it
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// ---- first product: logits of a tile of classes x rows ------------------------------------------------------------------------------------------
+struct LogitArgs {
+    const uint16_t* x;
+    const uint16_t* w;
+    int64_t x_ld, w_ld;
+    const float* off;     // [V] class offsets, or null; -inf leaves the class out
+    float c, coff;        // z / tau in units of log2: acc * c + off * coff
+    int N, V, d;          // V, w, off: of the piece in the backward
+    int ntv, ntr;         // tiles
+    const void* label;    // [N] int64 / int32 (cross entropy) or null
+    int label64, v_first; // first class of the piece
+    // forward
+    float* part;          // [2][nvb][N]: maximum and sum per 32 MT classes
+    float* zlab;          // [N] logit of the label (log2 units)
+    // backward
+    const float* lse2;    // [N] (+inf: the row takes no part)
+    const float* coef;    // [N]
+    uint16_t* dz;         // [rows][dz_ld]
+    int64_t dz_ld;
+    int dz_rows;          // rows to be written (N rounded up to 32)
+};
+
+__device__ __forceinline__ int64_t load_label(const void* p, int is64, int r) {
+    return is64 ? reinterpret_cast<const int64_t*>(p)[r] : (int64_t)reinterpret_cast<const int32_t*>(p)[r];
+}
+
+// wave-private staging of 32 C columns x (MT*32) C rows of 16-bit values as whole rows of the destination
+template <int DT, int MT>
+__device__ __forceinline__ void store_rows16(unsigned char* stg, const uint2 (&pk)[MT][4], int lane, uint16_t* dst, int64_t ld, int nrows, int ncols) {
+    constexpr int RS = MT * 64 + 16, CH = MT * 4;  // +16: consecutive rows start in different banks
+    const int l31 = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<uint2*>(stg + l31 * RS + (i * 32 + q * 8 + h * 4) * 2) = pk[i][q];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int it = 0; it < 32 * CH / 64; ++it) {
+        const int id = it * 64 + lane, row = id / CH, ch = id % CH;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(stg + row * RS + ch * 16);
+        if (row < nrows && ch * 8 < ncols) *reinterpret_cast<u32x4*>(dst + row * ld + ch * 8) = v;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <int DT, int MT, int NT, bool BWD>
+__global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_logits_kernel(const LogitArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    constexpr int BM = MT * 64, BN = NT * 128, GR = 8;
+    const int tid = (int)threadIdx.x, lane = tid & 63;
+    const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wave8 >> 2, wave = wave8 & 3, l31 = lane & 31, h = lane >> 5;
+    // panels of 8 row tiles: the 32 workgroups that an XCD runs at a time share 8 row tiles and 4 class tiles
+    const int L = xcd_order((int)blockIdx.x, (int)gridDim.x);
+    const int panel = L / (GR * a.ntv), pr0 = panel * GR, pw = min(GR, a.ntr - pr0), in = L - panel * GR * a.ntv;
+    const int tv = in / pw, tr = pr0 + in % pw;
+    const int v0 = tv * BM, r0 = tr * BN;
+
+    f32x16 acc[MT][NT];
+    gemm_tile<DT, MT, NT, false, false>(smem, TileSrc{a.w + (int64_t)v0 * a.w_ld, a.w_ld, a.V - v0}, TileSrc{a.x + (int64_t)r0 * a.x_ld, a.x_ld, a.N - r0}, a.d, acc);
+
+    // class offsets of the tile in LDS (log2 units; -inf: left out, or behind the last class)
+    float* offs = reinterpret_cast<float*>(smem);
+    int* any = reinterpret_cast<int*>(smem + BM * 4);
+    if (tid == 0) *any = 0;
+    __syncthreads();
+    if (tid < BM) {
+        const int v = v0 + tid;
+        float o = -INFINITY;
+        if (v < a.V) {
+            o = a.off ? a.off[v] * a.coff : 0.f;
+            if (o == -INFINITY) *any = 1;
+        }
+        offs[tid] = o;
+    }
+    __syncthreads();
+    const float* offw = offs + grp * MT * 32 + 4 * h;
+    if (!BWD && *any) {  // a left-out class counts as nothing whatever its weights hold (0 * inf and NaN stay out)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const bool out = offw[i * 32 + 8 * (r >> 2) + (r & 3)] == -INFINITY;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j][r] = out ? 0.f : acc[i][j][r];
+            }
+    }
+    unsigned char* stg = smem + 2048 + wave8 * (32 * (MT * 64 + 16));
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int r = r0 + (wave * NT + j) * 32 + l31;
+        int64_t lab = -1;
+        if (a.label && r < a.N) lab = load_label(a.label, a.label64, r) - a.v_first;
+        const int64_t local64 = lab - v0 - grp * MT * 32;
+        const int local = local64 >= 0 && local64 < MT * 32 ? (int)local64 : -1;
+        const bool mine = local >= 0 && ((local >> 2) & 1) == h;
+        const int slot = ((local >> 3) << 2) | (local & 3);  // (i, q, r & 3) of the lane that holds it
+        if (!BWD) {
+            float m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 o = *reinterpret_cast<const f32x4*>(offw + i * 32 + q * 8);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float t = fmaf(acc[i][j][4 * q + e], a.c, o[e]);
+                        acc[i][j][4 * q + e] = t;
+                        m = fmaxf(m, t);
+                    }
+                }
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float mu = __builtin_isinf(m) ? 0.f : m;  // nothing left, or an infinite logit: exp2 of the values themselves
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(acc[i][j][e] - mu);
+            s += __shfl_xor(s, 32);
+            if (__ballot(mine)) {
+                float z = 0.f;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) z = slot == i * 16 + e ? acc[i][j][e] : z;
+                if (mine) a.zlab[r] = z;
+            }
+            if (h == 0 && r < a.N) {
+                const int64_t vb = (int64_t)tv * 2 + grp, nvb = (int64_t)a.ntv * 2;
+                a.part[vb * a.N + r] = mu;
+                a.part[(nvb + vb) * a.N + r] = s;
+            }
+        } else {
+            const bool live = r < a.N;
+            const float l2 = live ? a.lse2[r] : INFINITY;
+            const float g = live ? a.coef[r] : 0.f;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 o = *reinterpret_cast<const f32x4*>(offw + i * 32 + q * 8);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * q + e], a.c, o[e]) - l2);
+                }
+            const bool named = mine && offs[grp * MT * 32 + local] != -INFINITY;  // (a left-out class gets no gradient)
+            if (__ballot(named)) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[i][j][e] -= named && slot == i * 16 + e ? 1.f : 0.f;
+            }
+            uint2 pk[MT][4];
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    pk[i][q].x = lpack2<DT>(acc[i][j][4 * q] * g, acc[i][j][4 * q + 1] * g);
+                    pk[i][q].y = lpack2<DT>(acc[i][j][4 * q + 2] * g, acc[i][j][4 * q + 3] * g);
+                }
+            const int rr = r0 + (wave * NT + j) * 32;
+            store_rows16<DT, MT>(stg, pk, lane, a.dz + (int64_t)rr * a.dz_ld + v0 + grp * MT * 32, a.dz_ld, a.dz_rows - rr, MT * 32);
+        }
+    }
+}
+
+// ---- second product of the backward: a piece's dw tiles and dx tiles in one launch -----------------------------------------------------------------
+struct GradArgs {
+    const uint16_t* x;    // [rows32][d], rows without a part zeroed
+    const uint16_t* w;    // [Vp][w_ld], first class of the piece
+    const uint16_t* dz;   // [rows32][dz_ld]
+    int64_t w_ld, dz_ld;
+    int N, rows32, d, Vp; // Vp: classes of the piece
+    int vk;               // columns of dz that hold numbers (Vp rounded up to the tile)
+    int ntd, ndw, ndx;    // tiles along d; dw tiles, dx tiles
+    int ntr, splits, kper;// dx: row tiles, slices of the piece, classes per slice (a multiple of 32)
+    uint16_t* dw;         // [Vp][dw_ld]
+    int64_t dw_ld;
+    float* slab;          // [splits][N][d]
+    int add;              // slabs hold earlier pieces
+    const float* outscale;
+};
+
+template <int DT, int MT, int NT>
+__global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_grads_kernel(const GradArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    constexpr int BM = MT * 64, BN = NT * 128;
+    const int tid = (int)threadIdx.x, lane = tid & 63;
+    const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wave8 >> 2, wave = wave8 & 3, l31 = lane & 31, h = lane >> 5;
+    int L = xcd_order((int)blockIdx.x, (int)gridDim.x);
+    f32x16 acc[MT][NT];
+    if (L < a.ndw) {  // dw[v][f] = sum_r dz[r][v] x[r][f]
+        const int f0 = (L % a.ntd) * BM, v0 = (L / a.ntd) * BN;
+        gemm_tile<DT, MT, NT, true, true>(smem, TileSrc{a.x + f0, a.d, a.d - f0}, TileSrc{a.dz + v0, a.dz_ld, a.vk - v0}, a.rows32, acc);
+        const float os = *a.outscale;
+        unsigned char* stg = smem + wave8 * (32 * (MT * 64 + 16));
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            uint2 pk[MT][4];
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    pk[i][q].x = lpack2<DT>(acc[i][j][4 * q] * os, acc[i][j][4 * q + 1] * os);
+                    pk[i][q].y = lpack2<DT>(acc[i][j][4 * q + 2] * os, acc[i][j][4 * q + 3] * os);
+                }
+            const int v = v0 + (wave * NT + j) * 32, f = f0 + grp * MT * 32;
+            store_rows16<DT, MT>(stg, pk, lane, a.dw + (int64_t)v * a.dw_ld + f, a.dw_ld, a.Vp - v, a.d - f);
+        }
+        return;
+    }
+    L -= a.ndw;  // dx[r][f] += sum over the slice's classes of dz[r][v] w[v][f]
+    const int f0 = (L % a.ntd) * BM, r0 = (L / a.ntd % a.ntr) * BN, s = L / a.ntd / a.ntr;
+    const int k0 = s * a.kper, k = min(a.kper, a.Vp - k0);
+    gemm_tile<DT, MT, NT, true, false>(smem, TileSrc{a.w + (int64_t)k0 * a.w_ld + f0, a.w_ld, a.d - f0},
+                                       TileSrc{a.dz + (int64_t)r0 * a.dz_ld + k0, a.dz_ld, a.rows32 - r0}, k, acc);
+    float* slab = a.slab + (int64_t)s * a.N * a.d;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int r = r0 + (wave * NT + j) * 32 + l31;
+        if (r >= a.N) continue;
+        f32x4 *p = reinterpret_cast<f32x4*>(slab + (int64_t)r * a.d), old[MT][4];
+        const int c0 = f0 + grp * MT * 32 + h * 4;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                old[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (a.add && c0 + i * 32 + q * 8 < a.d) old[i][q] = p[(c0 + i * 32 + q * 8) >> 2];
+            }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c0 + i * 32 + q * 8 < a.d)
+                    p[(c0 + i * 32 + q * 8) >> 2] = old[i][q] + f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    }
+}
+
+// ---- small launches ----------------------------------------------------------------------------------------------------------------------------------
+// rows' (maximum, sum) pairs -> lse; 64 rows a workgroup, 16 threads a row that take every 16th pair, joined in a fixed order
+__global__ __launch_bounds__(1024) void class_lse_kernel(const float* part, int nvb, int N, int V, const void* label, int label64, const float* zlab, float* loss,
+                                                         float* lse) {
+    __shared__ float sm[16][64], ss[16][64];
+    const int c = (int)threadIdx.x & 63, g = (int)threadIdx.x >> 6;
+    const int r = (int)blockIdx.x * 64 + c;
+    float m = -INFINITY, s = 0.f;
+    auto join = [](float& m, float& s, float m2, float s2) {  // a sum of 0 has no maximum; one of inf or NaN keeps it
+        if (s2 == 0.f) return;
+        if (s == 0.f) {
+            m = m2;
+            s = s2;
+            return;
+        }
+        const float mn = fmaxf(m, m2);
+        s = s * __builtin_amdgcn_exp2f(m - mn) + s2 * __builtin_amdgcn_exp2f(m2 - mn);
+        m = mn;
+    };
+    if (r < N)
+        for (int b = g; b < nvb; b += 16) join(m, s, part[(int64_t)b * N + r], part[((int64_t)nvb + b) * N + r]);
+    sm[g][c] = m;
+    ss[g][c] = s;
+    __syncthreads();
+    if (g || r >= N) return;
+    for (int k = 1; k < 16; ++k) join(m, s, sm[k][c], ss[k][c]);
+    const float l2 = s == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(s);  // (v_log_f32: base 2)
+    lse[r] = l2 * kLn2;
+    if (loss) {
+        const int64_t lab = load_label(label, label64, r);
+        loss[r] = lab >= 0 && lab < V && s != 0.f ? (l2 - zlab[r]) * kLn2 : 0.f;
+    }
+}
+
+// row coefficients of dz: g_r relative to the largest |g| (a power of two above it), so that dz uses the 16-bit type's range; outscale undoes it
+__global__ __launch_bounds__(1024) void class_coef_kernel(const float* drow, int drow_stride, const void* label, int label64, const float* lse, int64_t lse_stride,
+                                                          int N, int V, float gain, float spread, float* lse2, float* coef, float* outscale) {
+    __shared__ float red[16];
+    const int t = (int)threadIdx.x;
+    auto live = [&](int r) {
+        const float l = lse[(int64_t)r * lse_stride];
+        if (l == INFINITY && !label) return false;
+        if (l == -INFINITY) return false;
+        if (!label) return true;
+        const int64_t lab = load_label(label, label64, r);
+        return lab >= 0 && lab < V;
+    };
+    float m = 0.f;
+    for (int r = t; r < N; r += 1024)
+        if (live(r)) {
+            const float g = drow ? fabsf(drow[(int64_t)r * drow_stride]) : 1.f;
+            m = __builtin_isfinite(g) ? fmaxf(m, g) : m;
+        }
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if ((t & 63) == 0) red[t >> 6] = m;
+    __syncthreads();
+    m = red[0];
+    for (int i = 1; i < 16; ++i) m = fmaxf(m, red[i]);
+    int e = 0;
+    if (m > 0.f) frexpf(m, &e);  // m < 2^e
+    e = max(-100, min(100, e));
+    const float down = ldexpf(1.f, -e);
+    for (int r = t; r < N; r += 1024) {
+        const bool on = live(r);
+        const float g = drow ? drow[(int64_t)r * drow_stride] : 1.f;
+        const float l = lse[(int64_t)r * lse_stride] * kLog2e;
+        lse2[r] = !on ? INFINITY : l == INFINITY ? NAN : l;  // +inf marks a row without a part; an infinite logit gives NaN gradients
+        coef[r] = on ? g * down * spread : 0.f;
+    }
+    if (t == 0) *outscale = ldexpf(gain, e) / spread;
+}
+
+// x -> [rows32][d] contiguous, rows without a part (and behind the last) zeroed: 0 * inf and NaN stay out of dw
+__global__ __launch_bounds__(256) void class_rows_kernel(const uint16_t* x, int64_t ld, const float* lse2, int N, int rows32, int d8, u32x4* out) {
+    const int64_t n = (int64_t)rows32 * d8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int r = (int)(i / d8), c = (int)(i - (int64_t)r * d8);
+        u32x4 v = {0, 0, 0, 0};
+        if (r < N && lse2[r] != INFINITY) v = *reinterpret_cast<const u32x4*>(x + r * ld + c * 8);
+        out[i] = v;
+    }
+}
+// a piece's weights with the left-out classes zeroed: 0 * inf and NaN stay out of dx
+__global__ __launch_bounds__(256) void class_weights_kernel(const uint16_t* w, int64_t ld, const float* off, int V, int d8, u32x4* out) {
+    const int64_t n = (int64_t)V * d8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int r = (int)(i / d8), c = (int)(i - (int64_t)r * d8);
+        u32x4 v = {0, 0, 0, 0};
+        if (off[r] != -INFINITY) v = *reinterpret_cast<const u32x4*>(w + r * ld + c * 8);
+        out[i] = v;
+    }
+}
+template <int DT>
+__global__ __launch_bounds__(256) void class_dx_kernel(const float* slab, int splits, int N, int d, const float* outscale, uint16_t* dx, int64_t ld) {
+    const int d4 = d >> 2;
+    const int64_t n = (int64_t)N * d4;
+    const float os = *outscale;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        f32x4 v = reinterpret_cast<const f32x4*>(slab)[i];
+        for (int s = 1; s < splits; ++s) v += reinterpret_cast<const f32x4*>(slab)[(int64_t)s * n + i];
+        const int64_t r = i / d4;
+        uint2 o;
+        o.x = lpack2<DT>(v[0] * os, v[1] * os);
+        o.y = lpack2<DT>(v[2] * os, v[3] * os);
+        *reinterpret_cast<uint2*>(dx + r * ld + (i - r * d4) * 4) = o;
+    }
+}
+__global__ __launch_bounds__(256) void class_zero_kernel(uint16_t* p, int64_t rows, int64_t ld, int d) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * d; i += (int64_t)gridDim.x * 256) p[i / d * ld + i % d] = 0;
+}
+
+// ---- distillation: the teacher's slots ---------------------------------------------------------------------------------------------------------------
+// One wave a row, 16 lanes a slot: the student's logits at the teacher's classes (dot products in fp32), the teacher's softmax over its filled slots, the
+// loss. saved: [N][1 + 2k] = lse of the row (+inf where the teacher says nothing), logits (log2 units), q.
+template <int DT>
+__global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, int64_t x_ld, const uint16_t* w, int64_t w_ld, const float* off, float c, float coff,
+                                                            const int32_t* idx, const void* val, int val_dtype, int k, float itau, float tau2, int N, int V, int d,
+                                                            const float* lse, float* loss, float* saved) {
+    const int lane = (int)threadIdx.x & 63;
+    const int r = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
+    if (r >= N) return;
+    const int sub = lane >> 4, l = lane & 15;
+    float* sv = saved + (int64_t)r * (1 + 2 * k);
+    const int32_t* ir = idx + (int64_t)r * k;
+    auto slot_on = [&](int j) { return j < k && (unsigned)ir[j] < (unsigned)V; };
+    auto teach = [&](int j) { return load_elem(val, (int64_t)r * k + j, val_dtype) * itau; };
+    // the teacher's maximum and sum
+    float m = -INFINITY;
+    bool some = false;
+    for (int j = lane; j < k; j += 64)
+        if (slot_on(j)) {
+            const float t = teach(j);
+            m = t != t ? t : fmaxf(m, t);
+            some = true;
+        }
+    for (int o = 32; o; o >>= 1) {
+        const float m2 = __shfl_xor(m, o);
+        m = (m != m || m2 != m2) ? NAN : fmaxf(m, m2);
+    }
+    some = __ballot(some) != 0 && m != -INFINITY;
+    float s = 0.f;
+    for (int j = lane; j < k; j += 64)
+        if (slot_on(j)) s += expf(teach(j) - m);
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+    const float ls = logf(s);
+    const float l2 = lse[r] * kLog2e;
+    some = some && l2 != -INFINITY;
+    float sum = 0.f;
+    for (int j0 = 0; j0 < k; j0 += 4) {
+        const int j = j0 + sub;
+        const bool on = some && slot_on(j);
+        float z = 0.f;
+        if (on) {
+            const int v = ir[j];
+            const uint16_t *xr = x + r * x_ld, *wr = w + v * w_ld;
+            for (int f = l * 8; f < d; f += 128) {
+                const u32x4 xv = *reinterpret_cast<const u32x4*>(xr + f), wv = *reinterpret_cast<const u32x4*>(wr + f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    z = fmaf(Elem<DT>::to_f32((uint16_t)(xv[e] & 0xffff)), Elem<DT>::to_f32((uint16_t)(wv[e] & 0xffff)), z);
+                    z = fmaf(Elem<DT>::to_f32((uint16_t)(xv[e] >> 16)), Elem<DT>::to_f32((uint16_t)(wv[e] >> 16)), z);
+                }
+            }
+        }
+        for (int o = 8; o; o >>= 1) z += __shfl_xor(z, o);
+        if (j < k && l == 0) {
+            float z2 = -INFINITY, q = 0.f;
+            if (on) {
+                const float ov = off ? off[ir[j]] : 0.f;
+                z2 = ov == -INFINITY ? -INFINITY : fmaf(z, c, ov * coff);
+                const float lq = teach(j) - m - ls;
+                q = expf(lq);
+                if (q != 0.f) sum += q * (lq - (z2 - l2) * kLn2);
+            }
+            sv[1 + j] = z2;
+            sv[1 + k + j] = q;
+        }
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (lane == 0) {
+        loss[r] = some ? sum * tau2 : 0.f;
+        sv[0] = !some ? INFINITY : lse[r] == INFINITY ? NAN : lse[r];
+    }
+}
+// dz at the teacher's classes of a piece: coef * (p - q), q summed over the slots that name the class; the slot that names it first writes
+template <int DT>
+__global__ __launch_bounds__(256) void class_teacher_dz_kernel(const int32_t* idx, const float* saved, const float* lse2, const float* coef, int k, int N, int v_first,
+                                                               int Vp, uint16_t* dz, int64_t dz_ld) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)N * k) return;
+    const int r = (int)(i / k), j = (int)(i - (int64_t)r * k);
+    const int32_t* ir = idx + (int64_t)r * k;
+    const int v = ir[j];
+    if (v < v_first || v - v_first >= Vp || lse2[r] == INFINITY) return;
+    const float* sv = saved + (int64_t)r * (1 + 2 * k);
+    if (sv[1 + j] == -INFINITY) return;  // a left-out class gets no gradient
+    float q = sv[1 + k + j];
+    for (int o = 0; o < j; ++o)
+        if (ir[o] == v) return;
+    for (int o = j + 1; o < k; ++o)
+        if (ir[o] == v) q += sv[1 + k + o];
+    const float g = (__builtin_amdgcn_exp2f(sv[1 + j] - lse2[r]) - q) * coef[r];
+    dz[r * dz_ld + (v - v_first)] = Elem<DT>::from_f32(g);
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------------------------------------
+static inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+// 256 x 256 tiles read 131 FLOP per byte staged, 128 x 128 tiles half of that, so the large ones are taken wherever they fill most of the 256 CUs
+static inline bool big_tiles(int64_t rows, int64_t cols) { return (up(rows, 256) / 256) * (up(cols, 256) / 256) >= 160; }
+
+struct LinPlan {
+    bool big_f, big_g;
+    int nvb, rows32, piece, splits, kper;
+    int64_t o_part, o_zlab, o_lse, fwd_bytes;
+    int64_t o_lse2, o_coef, o_scale, o_x, o_w, o_dz, o_slab, bwd_bytes;
+};
+static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool want_dx) {
+    LinPlan p;
+    const int64_t N = q->N, V = q->V, d = q->d;
+    p.big_f = big_tiles(N, V);
+    p.nvb = (int)(up(V, p.big_f ? 256 : 128) / (p.big_f ? 128 : 64));
+    int64_t o = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t at = o;
+        o += up(bytes, 256);
+        return at;
+    };
+    p.o_part = take(2 * (int64_t)p.nvb * N * 4);
+    p.o_zlab = take(N * 4);
+    p.o_lse = take(N * 4);
+    p.fwd_bytes = o;
+    o = 0;
+    p.rows32 = (int)up(N, 32);
+    // dz of a piece stays within 128 MiB (written once, read by two products: it should live in the 256 MiB cache), but never below 2048 classes
+    int64_t piece = std::max<int64_t>(2048, ((int64_t)64 << 20) / p.rows32 / 256 * 256);
+    const int64_t pieces = up(V, piece) / piece;
+    piece = up(up(V, pieces) / pieces, 256);  // equal pieces
+    p.piece = (int)piece;
+    // dx tiles are few (rows x features): the piece's classes are cut into slices of about the dw tiles' length (rows), as long as tiles are missing
+    auto cut = [&](int64_t bt) {
+        const int64_t dxt = (up(N, bt) / bt) * (up(d, bt) / bt);
+        int64_t n = std::min((piece + p.rows32 / 2) / p.rows32, (512 + dxt - 1) / dxt);
+        n = std::max<int64_t>(1, std::min(n, piece / 128));
+        p.kper = (int)up(up(piece, n) / n, 32);
+        p.splits = (int)(up(piece, p.kper) / p.kper);
+        return dxt * p.splits + (piece / bt) * (up(d, bt) / bt);
+    };
+    p.big_g = cut(256) >= 160;
+    if (!p.big_g) cut(128);
+    p.o_lse2 = take(N * 4);
+    p.o_coef = take(N * 4);
+    p.o_scale = take(4);
+    p.o_x = take((int64_t)p.rows32 * d * 2);
+    p.o_w = q->offset ? take(piece * d * 2) : 0;
+    p.o_dz = take((int64_t)p.rows32 * piece * 2);
+    p.o_slab = want_dx ? take((int64_t)p.splits * N * d * 4) : 0;
+    p.bwd_bytes = o;
+    return p;
+}
+
+static int lin_check(const cdet_linear_loss_desc* q, const char* who) {
+    CDET_CHECK_ARG(q, "%s: no descriptor", who);
+    CDET_CHECK_ARG(q->dtype == CDET_BF16 || q->dtype == CDET_F16, "%s: x and w must be bf16 or fp16 (dtype %d)", who, q->dtype);
+    CDET_CHECK_ARG(q->N >= 0 && q->N <= (1 << 24) && q->V >= 1 && q->V <= (1 << 24), "%s: N %d (0 .. 2^24) or V %d (1 .. 2^24)", who, q->N, q->V);
+    CDET_CHECK_ARG(q->d >= 8 && q->d % 8 == 0 && q->d <= 65536, "%s: d = %d must be a multiple of 8 in 8 .. 65536", who, q->d);
+    CDET_CHECK_ARG(q->x_ld >= 0 && q->x_ld % 8 == 0 && q->x_ld < (1 << 22) && q->w_ld >= 0 && q->w_ld % 8 == 0 && q->w_ld < (1 << 22),
+                   "%s: row pitches %lld, %lld must be multiples of 8 elements below 2^22", who, (long long)q->x_ld, (long long)q->w_ld);
+    CDET_CHECK_ARG(q->tau > 0.f && q->tau < INFINITY && q->scale == q->scale && q->scale - q->scale == 0.f, "%s: tau %g must be positive, scale %g finite", who, q->tau, q->scale);
+    return 0;
+}
+static inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <typename K>
+static void allow_lds(K kernel, size_t bytes) {
+    (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+constexpr size_t LDS_BIG = 4 * 32768, LDS_SMALL = 4 * 16384;
+
+template <bool BWD>
+static int launch_logits(LogitArgs a, int dtype, bool big, hipStream_t s) {
+    const int bt = big ? 256 : 128;
+    a.ntv = div_up(a.V, bt);
+    a.ntr = div_up(a.N, bt);
+    const int64_t n = (int64_t)a.ntv * a.ntr;
+    CDET_CHECK_ARG(n < ((int64_t)1 << 31), "linear loss: too many tiles");
+#define CDET_GO(DT_, MT_, NT_, LDS_)                                                                       \
+    do {                                                                                                   \
+        static bool once = (allow_lds(class_logits_kernel<DT_, MT_, NT_, BWD>, LDS_), true);               \
+        (void)once;                                                                                        \
+        class_logits_kernel<DT_, MT_, NT_, BWD><<<dim3((unsigned)n), dim3(512), LDS_, s>>>(a);             \
+    } while (0)
+    if (dtype == CDET_BF16) {
+        if (big) CDET_GO(CDET_BF16, 4, 2, LDS_BIG);
+        else CDET_GO(CDET_BF16, 2, 1, LDS_SMALL);
+    } else {
+        if (big) CDET_GO(CDET_F16, 4, 2, LDS_BIG);
+        else CDET_GO(CDET_F16, 2, 1, LDS_SMALL);
+    }
+#undef CDET_GO
+    CDET_LAUNCH_CHECK();
+    return 0;
+}
+static int launch_grads(const GradArgs& a, int dtype, bool big, hipStream_t s) {
+    const unsigned n = (unsigned)(a.ndw + a.ndx);
+#define CDET_GO(DT_, MT_, NT_, LDS_)                                                          \
+    do {                                                                                      \
+        static bool once = (allow_lds(class_grads_kernel<DT_, MT_, NT_>, LDS_), true);        \
+        (void)once;                                                                           \
+        class_grads_kernel<DT_, MT_, NT_><<<dim3(n), dim3(512), LDS_, s>>>(a);                \
+    } while (0)
+    if (dtype == CDET_BF16) {
+        if (big) CDET_GO(CDET_BF16, 4, 2, LDS_BIG);
+        else CDET_GO(CDET_BF16, 2, 1, LDS_SMALL);
+    } else {
+        if (big) CDET_GO(CDET_F16, 4, 2, LDS_BIG);
+        else CDET_GO(CDET_F16, 2, 1, LDS_SMALL);
+    }
+#undef CDET_GO
+    CDET_LAUNCH_CHECK();
+    return 0;
+}
+
+static LogitArgs logit_args(const cdet_linear_loss_desc* q) {
+    LogitArgs a = {};
+    a.x_ld = q->x_ld;
+    a.w_ld = q->w_ld;
+    a.c = q->scale / q->tau * kLog2e;
+    a.coff = kLog2e / q->tau;
+    a.N = q->N;
+    a.V = q->V;
+    a.d = q->d;
+    a.label64 = q->label64;
+    return a;
+}
+
+// logits' statistics -> lse (and, with labels, the loss)
+static int lin_forward(const cdet_linear_loss_desc* q, const LinPlan& p, const void* x, const void* w, const void* label, float* loss, float* lse, char* ws, hipStream_t s) {
+    LogitArgs a = logit_args(q);
+    a.x = (const uint16_t*)x;
+    a.w = (const uint16_t*)w;
+    a.off = q->offset;
+    a.label = label;
+    a.part = (float*)(ws + p.o_part);
+    a.zlab = (float*)(ws + p.o_zlab);
+    const int rc = launch_logits<false>(a, q->dtype, p.big_f, s);
+    if (rc) return rc;
+    class_lse_kernel<<<dim3(div_up(q->N, 64)), dim3(1024), 0, s>>>(a.part, p.nvb, q->N, q->V, label, q->label64, a.zlab, loss, lse);
+    CDET_LAUNCH_CHECK();
+    return 0;
+}
+
+static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const void* w, const void* label, const int32_t* idx, const float* saved, int k, const float* lse,
+                        int64_t lse_stride, const float* drow, int drow_stride, void* dx, int64_t dx_ld, void* dw, int64_t dw_ld, char* ws, hipStream_t s) {
+    const int N = q->N, V = q->V, d = q->d;
+    if (!dx && !dw) return 0;
+    if (N == 0) {
+        if (dw) {
+            class_zero_kernel<<<dim3(2048), dim3(256), 0, s>>>((uint16_t*)dw, V, dw_ld, d);
+            CDET_LAUNCH_CHECK();
+        }
+        return 0;
+    }
+    const LinPlan p = lin_plan(q, dx != nullptr);
+    float *lse2 = (float*)(ws + p.o_lse2), *coef = (float*)(ws + p.o_coef), *os = (float*)(ws + p.o_scale);
+    const float spread = q->dtype == CDET_F16 ? 4096.f : 1.f;
+    class_coef_kernel<<<dim3(1), dim3(1024), 0, s>>>(drow, drow_stride, label, q->label64, lse, lse_stride, N, V, q->scale * (idx ? q->tau : 1.f), spread, lse2, coef, os);
+    class_rows_kernel<<<dim3(std::min<int64_t>(2048, div_up((int64_t)p.rows32 * (d / 8), 256))), dim3(256), 0, s>>>((const uint16_t*)x, q->x_ld, lse2, N, p.rows32, d / 8,
+                                                                                                                  (u32x4*)(ws + p.o_x));
+    CDET_LAUNCH_CHECK();
+    const int bt = p.big_g ? 256 : 128;
+    for (int v0 = 0; v0 < V; v0 += p.piece) {
+        const int Vp = std::min(p.piece, V - v0);
+        LogitArgs a = logit_args(q);
+        a.x = (const uint16_t*)(ws + p.o_x);
+        a.x_ld = d;
+        a.w = (const uint16_t*)w + (int64_t)v0 * q->w_ld;
+        if (q->offset) {
+            class_weights_kernel<<<dim3(std::min<int64_t>(2048, div_up((int64_t)Vp * (d / 8), 256))), dim3(256), 0, s>>>(a.w, q->w_ld, q->offset + v0, Vp, d / 8,
+                                                                                                                        (u32x4*)(ws + p.o_w));
+            a.w = (const uint16_t*)(ws + p.o_w);
+            a.w_ld = d;
+            a.off = q->offset + v0;
+        }
+        a.V = Vp;
+        a.label = label;
+        a.v_first = v0;
+        a.lse2 = lse2;
+        a.coef = coef;
+        a.dz = (uint16_t*)(ws + p.o_dz);
+        a.dz_ld = p.piece;
+        a.dz_rows = p.rows32;
+        int rc = launch_logits<true>(a, q->dtype, p.big_f, s);
+        if (rc) return rc;
+        if (idx) {
+            const unsigned nb = (unsigned)div_up((int64_t)N * k, 256);
+            if (q->dtype == CDET_BF16) class_teacher_dz_kernel<CDET_BF16><<<dim3(nb), dim3(256), 0, s>>>(idx, saved, lse2, coef, k, N, v0, Vp, a.dz, a.dz_ld);
+            else class_teacher_dz_kernel<CDET_F16><<<dim3(nb), dim3(256), 0, s>>>(idx, saved, lse2, coef, k, N, v0, Vp, a.dz, a.dz_ld);
+            CDET_LAUNCH_CHECK();
+        }
+        GradArgs g = {};
+        g.x = a.x;
+        g.w = a.w;
+        g.dz = a.dz;
+        g.w_ld = a.w_ld;
+        g.dz_ld = a.dz_ld;
+        g.N = N;
+        g.rows32 = p.rows32;
+        g.d = d;
+        g.Vp = Vp;
+        g.vk = (int)up(Vp, p.big_f ? 256 : 128);
+        g.ntd = div_up(d, bt);
+        g.ndw = dw ? g.ntd * div_up(Vp, bt) : 0;
+        g.ntr = div_up(N, bt);
+        g.kper = p.kper;
+        g.splits = p.splits;
+        g.ndx = dx ? g.ntd * g.ntr * p.splits : 0;
+        g.dw = dw ? (uint16_t*)dw + (int64_t)v0 * dw_ld : nullptr;
+        g.dw_ld = dw_ld;
+        g.slab = (float*)(ws + p.o_slab);
+        g.add = v0 > 0;
+        g.outscale = os;
+        rc = launch_grads(g, q->dtype, p.big_g, s);
+        if (rc) return rc;
+    }
+    if (dx) {
+        const unsigned nb = (unsigned)std::min<int64_t>(4096, div_up((int64_t)N * (d / 4), 256));
+        if (q->dtype == CDET_BF16) class_dx_kernel<CDET_BF16><<<dim3(nb), dim3(256), 0, s>>>((const float*)(ws + p.o_slab), p.splits, N, d, os, (uint16_t*)dx, dx_ld);
+        else class_dx_kernel<CDET_F16><<<dim3(nb), dim3(256), 0, s>>>((const float*)(ws + p.o_slab), p.splits, N, d, os, (uint16_t*)dx, dx_ld);
+        CDET_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+}  // namespace cdet
+
+using namespace cdet;
+
+extern "C" int64_t cdet_linear_loss_ws_bytes(const cdet_linear_loss_desc* d, int32_t backward) {
+    if (!d || d->N <= 0 || d->V <= 0 || d->d <= 0) return 256;
+    const LinPlan p = lin_plan(d, true);
+    return backward ? p.bwd_bytes : p.fwd_bytes;
+}
+
+#define CDET_LIN_COMMON(who)                                                                                                                          \
+    if (int rc__ = lin_check(d, who)) return rc__;                                                                                                    \
+    CDET_CHECK_ARG(d->N == 0 || (x && al16(x)), who ": x must be given and 16-byte aligned");                                                           \
+    CDET_CHECK_ARG(w && al16(w), who ": w must be given and 16-byte aligned");                                                                          \
+    CDET_CHECK_ARG(d->x_ld == 0 || d->x_ld >= d->d, who ": x's row pitch %lld is below d", (long long)d->x_ld);                                         \
+    CDET_CHECK_ARG(d->w_ld == 0 || d->w_ld >= d->d, who ": w's row pitch %lld is below d", (long long)d->w_ld);                                         \
+    CDET_CHECK_ARG(d->N == 0 || (ws && al16(ws)), who ": the workspace must be given and 16-byte aligned");
+#define CDET_LIN_GRADS(who)                                                                                                                            \
+    CDET_CHECK_ARG((!dx || (al16(dx) && dx_ld >= d->d && dx_ld % 8 == 0)) && (!dw || (al16(dw) && dw_ld >= d->d && dw_ld % 8 == 0)),                     \
+                   who ": dx / dw must be 16-byte aligned with row pitches that are multiples of 8 and at least d");                                   \
+    CDET_CHECK_ARG(drow_stride == 0 || drow_stride == 1, who ": drow_stride must be 0 or 1");
+
+extern "C" int cdet_linear_ce_fwd(const cdet_linear_loss_desc* d, const void* x, const void* w, const void* labels, float* loss, float* lse, void* ws, void* stream) {
+    CDET_LIN_COMMON("cdet_linear_ce_fwd")
+    CDET_CHECK_ARG(d->tau == 1.f, "cdet_linear_ce_fwd: tau must be 1 (use scale)");
+    CDET_CHECK_ARG(d->N == 0 || (labels && loss && lse), "cdet_linear_ce_fwd: labels, loss and lse must be given");
+    if (d->N == 0) return 0;
+    return lin_forward(d, lin_plan(d, true), x, w, labels, loss, lse, (char*)ws, (hipStream_t)stream);
+}
+
+extern "C" int cdet_linear_ce_bwd(const cdet_linear_loss_desc* d, const void* x, const void* w, const void* labels, const float* lse, const float* drow, int32_t drow_stride,
+                                  void* dx, int64_t dx_ld, void* dw, int64_t dw_ld, void* ws, void* stream) {
+    CDET_LIN_COMMON("cdet_linear_ce_bwd")
+    CDET_LIN_GRADS("cdet_linear_ce_bwd")
+    CDET_CHECK_ARG(d->tau == 1.f, "cdet_linear_ce_bwd: tau must be 1 (use scale)");
+    CDET_CHECK_ARG(d->N == 0 || (labels && lse), "cdet_linear_ce_bwd: labels and lse must be given");
+    return lin_backward(d, x, w, labels, nullptr, nullptr, 0, lse, 1, drow, drow_stride, dx, dx_ld, dw, dw_ld, (char*)ws, (hipStream_t)stream);
+}
+
+extern "C" int cdet_linear_distill_fwd(const cdet_linear_loss_desc* d, const void* x, const void* w, int32_t k, const int32_t* idx, const void* val, int32_t val_dtype,
+                                       float* loss, float* saved, void* ws, void* stream) {
+    CDET_LIN_COMMON("cdet_linear_distill_fwd")
+    CDET_CHECK_ARG(k >= 1 && k <= 512, "cdet_linear_distill_fwd: k = %d (1 .. 512)", k);
+    CDET_CHECK_ARG(val_dtype == CDET_BF16 || val_dtype == CDET_F16 || val_dtype == CDET_F32, "cdet_linear_distill_fwd: val_dtype %d", val_dtype);
+    CDET_CHECK_ARG(d->N == 0 || (idx && val && loss && saved), "cdet_linear_distill_fwd: idx, val, loss and saved must be given");
+    if (d->N == 0) return 0;
+    const LinPlan p = lin_plan(d, true);
+    float* lse = (float*)((char*)ws + p.o_lse);
+    const int rc = lin_forward(d, p, x, w, nullptr, nullptr, lse, (char*)ws, (hipStream_t)stream);
+    if (rc) return rc;
+    const dim3 nb((unsigned)div_up(d->N, 4)), nt(256);
+    const LogitArgs a = logit_args(d);
+#define CDET_GO(DT_)                                                                                                                                        \
+    class_teacher_kernel<DT_><<<nb, nt, 0, (hipStream_t)stream>>>((const uint16_t*)x, d->x_ld, (const uint16_t*)w, d->w_ld, d->offset, a.c, a.coff, idx, val, val_dtype, \
+                                                                 k, 1.f / d->tau, d->tau * d->tau, d->N, d->V, d->d, lse, loss, saved)
+    if (d->dtype == CDET_BF16) CDET_GO(CDET_BF16);
+    else CDET_GO(CDET_F16);
+#undef CDET_GO
+    CDET_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int cdet_linear_distill_bwd(const cdet_linear_loss_desc* d, const void* x, const void* w, int32_t k, const int32_t* idx, const float* saved, const float* drow,
+                                       int32_t drow_stride, void* dx, int64_t dx_ld, void* dw, int64_t dw_ld, void* ws, void* stream) {
+    CDET_LIN_COMMON("cdet_linear_distill_bwd")
+    CDET_LIN_GRADS("cdet_linear_distill_bwd")
+    CDET_CHECK_ARG(k >= 1 && k <= 512, "cdet_linear_distill_bwd: k = %d (1 .. 512)", k);
+    CDET_CHECK_ARG(d->N == 0 || (idx && saved), "cdet_linear_distill_bwd: idx and saved must be given");
+    return lin_backward(d, x, w, nullptr, idx, saved, k, saved, 1 + 2 * (int64_t)k, drow, drow_stride, dx, dx_ld, dw, dw_ld, (char*)ws, (hipStream_t)stream);
+}

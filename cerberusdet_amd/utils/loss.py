@@ -79,3 +79,122 @@ class Loss:
         gt = pad_targets(batch, bs, imgsz, feats[0].device)
         scalar, items = _DetLossFn.apply(gt, self.nc[task], self.loss_weights[task], [float(s) for s in self.stride], *feats)
         return scalar, items.detach()
+
+
+# ---- losses over a long class list and from a teacher (csrc/class_loss.hip, csrc/topk_distill.hip) -----------------------------------------------------
+def _reduced(rows, counted, reduction):
+    if reduction == "none":
+        return rows
+    if reduction == "sum":
+        return rows.sum()
+    if reduction == "mean":  # over the rows that take part
+        return rows.sum() / counted.sum().clamp(min=1)
+    raise ValueError(f"reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
+
+
+class _LinearCeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, labels, offset, scale):
+        from .. import ops
+
+        loss, lse = ops.linear_ce_fwd(x, w, labels, offset=offset, scale=scale)
+        ctx.save_for_backward(x, w, labels, offset, lse)
+        ctx.scale = scale
+        ctx.mark_non_differentiable(lse)
+        return loss, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _):
+        from .. import ops
+
+        x, w, labels, offset, lse = ctx.saved_tensors
+        dx, dw = ops.linear_ce_bwd(x, w, labels, lse, g.float(), offset=offset, scale=ctx.scale, want_dx=ctx.needs_input_grad[0], want_dw=ctx.needs_input_grad[1])
+        return dx, dw, None, None, None
+
+
+class _LinearDistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, idx, val, tau, offset, scale):
+        from .. import ops
+
+        loss, saved = ops.linear_distill_fwd(x, w, idx, val, tau=tau, offset=offset, scale=scale)
+        ctx.save_for_backward(x, w, idx, offset, saved)
+        ctx.tau, ctx.scale = tau, scale
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        from .. import ops
+
+        x, w, idx, offset, saved = ctx.saved_tensors
+        dx, dw = ops.linear_distill_bwd(x, w, idx, saved, g.float(), tau=ctx.tau, offset=offset, scale=ctx.scale, want_dx=ctx.needs_input_grad[0],
+                                        want_dw=ctx.needs_input_grad[1])
+        return dx, dw, None, None, None, None, None
+
+
+class _TopkDistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, idx, val, tau):
+        from .. import ops
+
+        loss, ctx.dz = ops.topk_distill(logits, idx, val, tau=tau, want_grad=logits.requires_grad)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        return (ctx.dz * g[..., None]).to(ctx.dz.dtype), None, None, None
+
+
+def linear_cross_entropy(x, w, labels, offset=None, scale=1.0, reduction="mean"):
+    """Cross entropy of a linear classifier over a long class list, differentiable in x [N, d] and w [V, d] (bf16 / fp16); the N x V logits are never in
+    memory. Labels outside of 0 .. V-1 leave their row out; "mean" is over the rows that are left. See ops.linear_ce_fwd."""
+    loss, _ = _LinearCeFn.apply(x, w, labels, offset, float(scale))
+    return _reduced(loss, (labels >= 0) & (labels < w.shape[0]), reduction)
+
+
+def linear_distillation(x, w, idx, val, tau=1.0, offset=None, scale=1.0, reduction="mean"):
+    """Distillation of that classifier from a teacher's top k logits (idx [N, k] int32, val [N, k]), differentiable in x and w. See ops.linear_distill_fwd."""
+    loss = _LinearDistillFn.apply(x, w, idx, val, float(tau), offset, float(scale))
+    return _reduced(loss, ((idx >= 0) & (idx < w.shape[0])).any(1), reduction)
+
+
+def topk_distillation(logits, idx, val, tau=1.0, reduction="mean"):
+    """Distillation of logits [P, V] or [P, G, V] in memory from a teacher's top k, differentiable in the logits. See ops.topk_distill."""
+    loss = _TopkDistillFn.apply(logits, idx, val, float(tau))
+    return _reduced(loss, ((idx >= 0) & (idx < logits.shape[-1])).any(-1), reduction)
+
+
+class HeadDistillation:
+    """Distillation of a task's Detect head from a teacher's head maps of the same strides: `HeadDistillation(model, k, tau)(preds, teacher_preds, task)` ->
+    (scalar, items[2]), items = (box, cls). Box: the four reg_max-bin distributions of every pixel against the teacher's; cls: the class logits against the
+    teacher's k largest. Both are means over the pixels of all maps, weighted by `box` and `cls`. preds: three NCHW maps as Loss takes them (the model's NHWC
+    buffers are read in place)."""
+
+    def __init__(self, model, k=16, tau=2.0, box=1.0, cls=1.0):
+        self.k, self.tau, self.box, self.cls = int(k), float(tau), float(box), float(cls)
+        self.reg_max = {t: model.get_head(t).reg_max for t in model.heads}
+        self.nc = {t: model.get_head(t).nc for t in model.heads}
+
+    def __call__(self, preds, teacher_preds, task):
+        feats = preds[1] if isinstance(preds, tuple) else preds
+        teach = teacher_preds[1] if isinstance(teacher_preds, tuple) else teacher_preds
+        R, nc, items = self.reg_max[task], self.nc[task], []
+        for part in (0, 1):
+            total, count = 0.0, 0
+            for f, t in zip(feats, teach):
+                if f.shape != t.shape:
+                    raise ValueError(f"student and teacher maps differ: {tuple(f.shape)} and {tuple(t.shape)}")
+                fr, tr = (m.permute(0, 2, 3, 1) for m in (f, t.detach()))  # NHWC
+                n = fr.shape[0] * fr.shape[1] * fr.shape[2]
+                if part == 0:
+                    z, tz = (m[..., :4 * R].reshape(n, 4 * R).unflatten(1, (4, R)) for m in (fr, tr))
+                else:
+                    z, tz = (m[..., 4 * R:4 * R + nc].reshape(n, nc) for m in (fr, tr))
+                val, idx = tz.topk(R if part == 0 else min(self.k, nc), dim=-1)
+                total = total + topk_distillation(z, idx.int(), val, self.tau, reduction="sum")
+                count += idx[..., 0].numel()
+            items.append(total / count)
+        return self.box * items[0] + self.cls * items[1], torch.stack(items).detach()

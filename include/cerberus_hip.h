@@ -478,6 +478,58 @@ int cdet_det_loss(const cdet_loss_desc* d, const void* f0, const void* f1, const
                   int32_t* target_labels, float* target_bboxes, float* target_scores, void* ws, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Losses over a long class list (csrc/class_loss.hip, csrc/topk_distill.hip). The reference's classifier is one sigmoid per class on a short list
+ * (utils/loss.py:160-168); these are the softmax forms for open class lists and for learning from a teacher.
+ *
+ * Linear class projection fused with its loss; the N x V logits are never in memory:
+ *   z[r][v] = scale * <x_r, w_v> + offset[v],  p = softmax(z / tau)
+ *   linear_ce       loss_r = lse(z_r) - z[r][label_r]           (tau = 1)   dz[r][v] = g_r (p - [v == label_r])
+ *   linear_distill  loss_r = tau^2 sum_j q_rj (log q_rj - log p[r][idx_rj]) dz[r][v] = g_r tau (p - sum_{j: idx_rj == v} q_rj)
+ *   dx = scale * dz w, dw = scale * dz^T x
+ * x [N, d] and w [V, d]: bf16 / fp16, unit stride along d, row pitches in elements (multiples of 8; 0 repeats one row), 16-byte aligned, d % 8 == 0.
+ * Sums, softmax statistics and losses are fp32; dz is rounded to the 16-bit type once before it is multiplied with w and x.
+ *   offset  optional [V] fp32 (class priors); -inf leaves a class out, whatever its weights hold: p = 0, dw = 0. The
+ *           offset itself has no gradient.
+ *   labels  [N] int64 / int32; outside of 0 .. V-1 (-100, say): the row takes no part -- loss 0, gradient 0, whatever the row of x holds. A row
+ *           whose classes are all left out takes no part either; a label that is left out beside others that are not has loss +inf.
+ *   idx     [N, k] int32 classes of the teacher's largest logits, val [N, k] their values; outside of 0 .. V-1: an empty slot. A class may be named
+ *           twice (its slots count separately). q = softmax of val / tau over the filled slots; a row without any takes no part. k <= 512.
+ *   lse     [N] log-sum-exp of the row;  saved [N, 1 + 2 k] fp32: what linear_distill's backward needs (opaque)
+ *   drow    gradient of the rows' losses, fp32: [N] (drow_stride 1), one value (0), or NULL (ones)
+ *   dx, dw  16-bit like x and w, either may be NULL; whole [V, d] of dw is written, the pitches' tails are not touched
+ * ws: cdet_linear_loss_ws_bytes(d, backward) bytes, 16-byte aligned; contents need not survive between calls. N = 0 is allowed (dw = 0). */
+typedef struct {
+    int32_t N, V, d;
+    int32_t dtype;                 /* CDET_BF16 / CDET_F16                                           */
+    int64_t x_ld, w_ld;
+    float scale, tau;
+    const float* offset;
+    int32_t label64;               /* labels are int64 (1) or int32 (0)                              */
+} cdet_linear_loss_desc;
+int64_t cdet_linear_loss_ws_bytes(const cdet_linear_loss_desc* d, int32_t backward);
+int cdet_linear_ce_fwd(const cdet_linear_loss_desc* d, const void* x, const void* w, const void* labels, float* loss, float* lse, void* ws, void* stream);
+int cdet_linear_ce_bwd(const cdet_linear_loss_desc* d, const void* x, const void* w, const void* labels, const float* lse, const float* drow,
+                       int32_t drow_stride, void* dx, int64_t dx_ld, void* dw, int64_t dw_ld, void* ws, void* stream);
+int cdet_linear_distill_fwd(const cdet_linear_loss_desc* d, const void* x, const void* w, int32_t k, const int32_t* idx, const void* val, int32_t val_dtype,
+                            float* loss, float* saved, void* ws, void* stream);
+int cdet_linear_distill_bwd(const cdet_linear_loss_desc* d, const void* x, const void* w, int32_t k, const int32_t* idx, const float* saved,
+                            const float* drow, int32_t drow_stride, void* dx, int64_t dx_ld, void* dw, int64_t dw_ld, void* ws, void* stream);
+/* linear_distill's loss on logits that are in memory, loss AND gradient in one call (like cdet_det_loss): P pixels (rows) of G distributions of V
+ * logits each -- the class logits of a head map (G = 1), its four 16-bin box distributions (G = 4, V = 16). Distribution g of pixel p starts at
+ * logits + (p * ld + g * V) elements (pass the pointer of the first channel); its gradient, d(sum_r drow_r loss_r) / d logit * grad_scale, at
+ * dlogits + (p * grad_ld + g * V). idx / val [P * G, k], drow [P * G] or NULL (ones), loss [P * G]. Everything else in a pixel's pitch is left as it is.
+ * logits: fp32 / bf16 / fp16, any alignment of whole elements; -inf = a class left out. dlogits may be NULL (loss only) and may BE logits (same type
+ * and pitch). */
+typedef struct {
+    int32_t P, G, V, k;
+    int32_t dtype, val_dtype, grad_dtype;
+    int64_t ld, grad_ld;
+    float tau, grad_scale;
+} cdet_topk_distill_desc;
+int cdet_topk_distill(const cdet_topk_distill_desc* d, const void* logits, const int32_t* idx, const void* val, const float* drow, float* loss, void* dlogits,
+                      void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Batched NMS (utils/general.py:360-481 incl. torchvision.ops.nms at :464) for ALL images in one call.
  * pred: [N, 4+nc, A] (xywh + class scores), dtype. out_rows: [N, max_det, 6] fp32, out_count: [N] i32.
  * ---------------------------------------------------------------------------------------------- */

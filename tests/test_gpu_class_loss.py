@@ -1,0 +1,542 @@
+"""Losses over a long class list (csrc/class_loss.hip, csrc/topk_distill.hip) against their definitions in 64 bits.
+
+Tolerances, derived (u = 2^-24 a rounding to fp32, h = half a step of the 16-bit type, relative):
+  * a logit is a sum of d exact fp32 products (16-bit x 16-bit) in fp32: off by at most d u sum|x w|; scaling, offset, the log2 domain and the sums of
+    exponentials add a few roundings of quantities below |z| + |lse| + log2 e * 32: loss_tol() counts 16 of them. lse moves by at most what the logits do.
+  * dz is rounded once to 16 bits: h |dz|, and p is off by the factor exp(2 loss_tol) (fp16: the smallest step, relative to the largest row gradient, too).
+  * dx / dw: those errors times |w| / |x|, n u for the fp32 sum over n terms, and the rounding of the result."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _ops():
+    from cerberusdet_amd import ops
+
+    return ops
+
+
+def _rand(*shape, seed=0, dtype=F32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+
+
+def _randint(hi, shape, seed):
+    return torch.randint(hi, shape, generator=torch.Generator().manual_seed(seed)).to(DEV)
+
+
+def teacher(N, V, k, seed, empty=True, dup=True):
+    idx = _randint(V, (N, k), seed).int()
+    if not dup:
+        idx = torch.stack([torch.randperm(V, generator=torch.Generator().manual_seed(seed + r))[:k] for r in range(N)]).int().to(DEV)
+    if empty:
+        idx[::3, k // 2:] = -1
+        idx[::5] = -1
+        idx[1::7, 0] = V  # behind the list: empty as well
+    return idx, 3 * _rand(N, k, seed=seed + 1)
+
+
+def reference(x, w, labels=None, idx=None, val=None, tau=1.0, offset=None, scale=1.0, drow=None):
+    """Loss rows, dz, dx, dw in 64 bits, and the sums the tolerances need."""
+    X, W = x.double(), w.double()
+    z = scale * (X @ W.T) + (0 if offset is None else offset.double())
+    out_cls = torch.zeros(w.shape[0], dtype=torch.bool, device=DEV) if offset is None else offset == -math.inf
+    z = z.masked_fill(out_cls, -math.inf)
+    V = w.shape[0]
+    if idx is None:
+        idx, q = labels.long()[:, None], torch.ones(len(labels), 1, dtype=torch.float64, device=DEV)
+        q = q * ((idx >= 0) & (idx < V))
+        logq = torch.zeros_like(q)
+    else:
+        idx = idx.long()
+        ok = (idx >= 0) & (idx < V)
+        t = (val.double() / tau).masked_fill(~ok, -math.inf)
+        q = torch.softmax(t, 1).nan_to_num(0.0)
+        logq = torch.where(q > 0, torch.log(q.clamp(min=1e-300)), 0.0)
+    lse = torch.logsumexp(z / tau, 1)
+    live = (q.sum(1) > 0) & (lse > -math.inf)
+    at = idx.clamp(0, V - 1)
+    logp = (z / tau).gather(1, at) - lse[:, None]
+    loss = tau * tau * torch.where(q > 0, q * (logq - logp), 0.0).sum(1)
+    loss = torch.where(live, loss, 0.0)
+    g = torch.ones(len(x), dtype=torch.float64, device=DEV) if drow is None else drow.double().expand(len(x))
+    p = torch.softmax(z / tau, 1)
+    p[~live] = 0
+    dz = p.clone().scatter_add_(1, at, -torch.where(live[:, None], q, 0.0)) * (g * tau * scale)[:, None]
+    dz[~live] = 0
+    dz[:, out_cls] = 0
+    Xz = torch.where(live[:, None], X, 0.0)
+    Wz = torch.where(out_cls[:, None], 0.0, W)
+    mag = (X.abs() @ W.abs().T * abs(scale)).masked_fill(out_cls, 0.0).amax(1)
+    if offset is not None:
+        mag = mag + torch.where(out_cls, 0.0, offset.double().abs()).max()
+    return dict(loss=loss, lse=torch.logsumexp(z, 1), live=live, dz=dz, p=p * (g * tau * scale).abs()[:, None], dx=dz @ Wz, dw=dz.T @ Xz, X=Xz, W=Wz, mag=mag / tau, g=g)
+
+
+def loss_tol(ref, d):
+    mag = torch.where(ref["live"], ref["mag"], 0.0).nan_to_num(0.0)
+    return 2 * (d * U * mag + 16 * U * (2 * mag + 32 * 1.45))
+
+
+def check_rows(got, want, tol):
+    assert got.dtype == F32 and torch.equal(torch.isinf(got), torch.isinf(want)), "infinities"
+    fin = torch.isfinite(want)
+    err = (got.double() - want).abs()
+    assert torch.all(err[fin] <= tol[fin]), (err[fin] / tol[fin]).max().item()
+
+
+def check_grads(got_dx, got_dw, ref, x, scale=1.0, tau=1.0):
+    h = torch.finfo(x.dtype).eps / 2
+    tiny = torch.finfo(x.dtype).tiny * torch.finfo(x.dtype).eps  # smallest step of the type
+    d, V, N = x.shape[1], ref["W"].shape[0], x.shape[0]
+    dl = loss_tol(ref, d)
+    gmax = torch.where(ref["live"], ref["g"].abs(), 0.0).max() * tau * abs(scale)
+    edz = h * ref["dz"].abs() + ref["p"] * (2.2 * dl)[:, None] + gmax * 2 * tiny / (4096 if x.dtype == F16 else 1)
+    edz = torch.where(ref["live"][:, None], edz, 0.0)
+    for got, want, e, n, other in ((got_dx, ref["dx"], edz, V, ref["W"]), (got_dw, ref["dw"], edz.T, N, ref["X"])):
+        if got is None:
+            continue
+        a = ref["dz"].abs() if got is got_dx else ref["dz"].abs().T
+        tol = e @ other.abs() + (n + 8) * U * (a @ other.abs()) + 1.01 * h * want.abs() + tiny
+        assert got.dtype == x.dtype and got.shape == want.shape
+        err = (got.double() - want).abs()
+        assert torch.all(err <= tol), (err / tol).max().item()
+
+
+def run_ce(x, w, labels, offset=None, scale=1.0, drow=None, dx=True, dw=True):
+    ops = _ops()
+    loss, lse = ops.linear_ce_fwd(x, w, labels, offset=offset, scale=scale)
+    return loss, lse, *ops.linear_ce_bwd(x, w, labels, lse, drow, offset=offset, scale=scale, want_dx=dx, want_dw=dw)
+
+
+def ce_case(N, V, d, dtype, seed=0):
+    return _rand(N, d, seed=seed, dtype=dtype), (_rand(V, d, seed=seed + 1) * (2 / math.sqrt(d))).to(dtype), _randint(V, (N,), seed + 2)
+
+
+CE_SIZES = [(1, 1, 8), (1, 2, 8), (3, 5, 16), (1, 1000, 64), (64, 64, 64), (127, 129, 72), (130, 257, 104), (300, 1201, 320), (33, 9001, 264), (257, 128, 40),
+            (2600, 3900, 40),   # 256 x 256 tiles
+            (700, 21000, 24),   # the same with classes cut into slices for dx
+            (40000, 4500, 16)]  # several pieces of the class list
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("N,V,d", CE_SIZES)
+def test_linear_ce(N, V, d, dtype):
+    x, w, labels = ce_case(N, V, d, dtype)
+    if N > 2:
+        labels[::3] = -100
+        labels[1] = V  # behind the list: left out as well
+    drow = _rand(N, seed=9).abs() + 0.25
+    loss, lse, dx, dw = run_ce(x, w, labels, drow=drow)
+    ref = reference(x, w, labels, drow=drow)
+    check_rows(loss, ref["loss"], loss_tol(ref, d))
+    check_rows(lse, ref["lse"], 2 * (d * U * ref["mag"] + 16 * U * (2 * ref["mag"] + 46.4)))
+    check_grads(dx, dw, ref, x)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("N,V,d", [(5, 7, 8), (200, 700, 64), (2600, 3900, 40)])
+def test_linear_ce_offset_scale_label_types(N, V, d, dtype):
+    """Class offsets with left-out classes, a logit scale, int32 labels, one gradient for all rows, negative and zero row gradients."""
+    x, w, labels = ce_case(N, V, d, dtype, seed=3)
+    off = _rand(V, seed=4)
+    off[::4] = -math.inf
+    off[labels[2:]] = 0.5
+    labels[0] = 4  # a left-out class: loss inf, the gradient reaches the others only
+    off[4] = -math.inf
+    drow = _rand(N, seed=5)
+    drow[1] = 0
+    loss, lse, dx, dw = run_ce(x, w, labels.int(), offset=off, scale=1.7, drow=drow)
+    ref = reference(x, w, labels, offset=off, scale=1.7, drow=drow)
+    assert loss[0].item() == math.inf
+    check_rows(loss, ref["loss"], loss_tol(ref, d))
+    check_grads(dx, dw, ref, x, scale=1.7)
+    assert torch.all(dw[off == -math.inf] == 0)
+    one = torch.tensor([0.125], device=DEV)
+    _, _, dx1, dw1 = run_ce(x, w, labels, offset=off, scale=-0.4, drow=one)
+    check_grads(dx1, dw1, reference(x, w, labels, offset=off, scale=-0.4, drow=one), x, scale=-0.4)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_linear_ce_bad_values_in_left_out_places(dtype):
+    """NaN and infinities in ignored rows of x and in left-out classes of w reach nothing."""
+    x, w, labels = ce_case(150, 300, 64, dtype, seed=6)
+    off = torch.zeros(300, device=DEV)
+    off[::5] = -math.inf
+    labels[labels % 5 == 0] += 1
+    labels[::4] = -1
+    clean = run_ce(x, w, labels, offset=off)
+    xb, wb = x.clone(), w.clone()
+    xb[::8], xb[4::8] = math.nan, math.inf
+    wb[::10], wb[5::10] = math.nan, -math.inf
+    bad = run_ce(xb, wb, labels, offset=off)
+    live = labels >= 0
+    for a, b in zip(clean, bad):
+        if a.dim() == 1:
+            assert torch.equal(a[live], b[live])
+    assert torch.all(bad[0][~live] == 0)
+    for a, b in zip(clean[2:], bad[2:]):
+        assert torch.equal(a, b)
+    assert torch.all(bad[2][~live] == 0) and torch.all(bad[3][::5] == 0)
+
+
+def test_linear_ce_nothing_left():
+    """Every class left out, every row ignored, no rows at all: losses and gradients of 0."""
+    x, w, labels = ce_case(9, 20, 16, BF)
+    loss, lse, dx, dw = run_ce(x, w, labels, offset=torch.full((20,), -math.inf, device=DEV))
+    assert torch.all(loss == 0) and torch.all(lse == -math.inf) and torch.all(dx == 0) and torch.all(dw == 0)
+    loss, lse, dx, dw = run_ce(x, w, torch.full_like(labels, -100))
+    assert torch.all(loss == 0) and torch.all(dx == 0) and torch.all(dw == 0)
+    loss, lse, dx, dw = run_ce(x[:0], w, labels[:0])
+    assert loss.shape == (0,) and dx.shape == (0, 16) and torch.all(dw == 0)
+
+
+def test_linear_ce_far_logits():
+    """Logits of +-10^3: the running maximum keeps the sums finite."""
+    x, w, labels = ce_case(70, 400, 32, BF, seed=8)
+    loss, lse, dx, dw = run_ce(x, w, labels, scale=300.0)
+    ref = reference(x, w, labels, scale=300.0)
+    check_rows(loss, ref["loss"], loss_tol(ref, 32))
+    check_grads(dx, dw, ref, x, scale=300.0)
+
+
+def test_linear_ce_strides_and_alignment():
+    """Column slices of wider buffers, an odd pitch (copied), a repeated row, a misaligned start: same bits as contiguous inputs."""
+    N, V, d = 100, 333, 48
+    x, w, labels = ce_case(N, V, d, F16, seed=11)
+    want = run_ce(x, w, labels)
+
+    def within(t, pitch, lead):
+        buf = torch.full((t.shape[0], pitch), math.nan, dtype=t.dtype, device=DEV)
+        buf[:, lead:lead + t.shape[1]] = t
+        return buf[:, lead:lead + t.shape[1]]
+
+    for pitch, lead in ((64, 8), (51, 1), (56, 3)):
+        for a, b in zip(want, run_ce(within(x, pitch, lead), within(w, pitch, lead), labels)):
+            assert torch.equal(a, b)
+    for a, b in zip(want, run_ce(x.T.contiguous().T, w.T.contiguous().T, labels)):
+        assert torch.equal(a, b)
+    rep = x[:1].expand(N, d)
+    for a, b in zip(run_ce(rep.contiguous(), w, labels), run_ce(rep, w, labels)):
+        assert torch.equal(a, b)
+
+
+def test_linear_ce_parts_and_repeats():
+    """dx alone, dw alone and both agree to the bit; so do two calls."""
+    x, w, labels = ce_case(260, 1500, 80, BF, seed=12)
+    a, b = run_ce(x, w, labels), run_ce(x, w, labels)
+    for s, t in zip(a, b):
+        assert torch.equal(s, t)
+    assert torch.equal(run_ce(x, w, labels, dw=False)[2], a[2]) and run_ce(x, w, labels, dw=False)[3] is None
+    assert torch.equal(run_ce(x, w, labels, dx=False)[3], a[3]) and run_ce(x, w, labels, dx=False)[2] is None
+
+
+KD_SIZES = [(1, 1, 8, 1), (2, 9, 8, 3), (96, 365, 64, 16), (131, 1201, 72, 50), (5, 300, 16, 512), (2600, 3900, 40, 5), (40000, 4500, 16, 3)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("N,V,d,k", KD_SIZES)
+def test_linear_distill(N, V, d, k, dtype):
+    ops = _ops()
+    x, w, _ = ce_case(N, V, d, dtype, seed=20)
+    idx, val = teacher(N, V, k, 21, empty=N > 2)  # (drawn with repetition: classes are named twice)
+    drow = _rand(N, seed=23).abs() + 0.25
+    for tau, off in ((1.0, None), (2.5, _rand(V, seed=24))):
+        loss, saved = ops.linear_distill_fwd(x, w, idx, val, tau=tau, offset=off, scale=1.3)
+        dx, dw = ops.linear_distill_bwd(x, w, idx, saved, drow, tau=tau, offset=off, scale=1.3)
+        ref = reference(x, w, idx=idx, val=val, tau=tau, offset=off, scale=1.3, drow=drow)
+        # sum over slots of q times the error of log p and of log q (a teacher logit up to 16, a few roundings)
+        check_rows(loss, ref["loss"], tau * tau * (2 * loss_tol(ref, d) + 64 * U * 16))
+        check_grads(dx, dw, ref, x, scale=1.3, tau=tau)
+
+
+def test_linear_distill_types_and_infinities():
+    """16-bit teacher logits; -inf in a slot counts as nothing; a slot at a left-out class is loss inf; NaN in rows without a teacher reaches nothing."""
+    ops = _ops()
+    x, w, _ = ce_case(40, 90, 32, BF, seed=30)
+    idx, val = teacher(40, 90, 6, 31, empty=False, dup=False)
+    idx[3] = -1
+    val[5, 2:] = -math.inf
+    val[6] = -math.inf
+    xb = x.clone()
+    xb[3], xb[6] = math.nan, math.inf
+    for vt in (val.to(BF), val.to(F16), val):
+        loss, saved = ops.linear_distill_fwd(xb, w, idx, vt, tau=1.5)
+        dx, dw = ops.linear_distill_bwd(xb, w, idx, saved, tau=1.5)
+        ref = reference(x, w, idx=idx, val=vt, tau=1.5)
+        check_rows(loss, ref["loss"], 2.25 * (2 * loss_tol(ref, 32) + 64 * U * 16))
+        assert loss[3] == 0 and loss[6] == 0
+        check_grads(dx, dw, ref, x, tau=1.5)
+    off = torch.zeros(90, device=DEV)
+    off[idx[0, 0].long()] = -math.inf
+    loss, saved = ops.linear_distill_fwd(x, w, idx[:1].expand(40, 6), val[:1].expand(40, 6), offset=off)
+    assert torch.all(loss == math.inf)
+
+
+def test_ce_is_distillation_from_one_class():
+    """k = 1 is the cross entropy of that class."""
+    ops = _ops()
+    x, w, labels = ce_case(60, 200, 64, BF, seed=33)
+    loss, lse = ops.linear_ce_fwd(x, w, labels)
+    kd, _ = ops.linear_distill_fwd(x, w, labels.int()[:, None], torch.zeros(60, 1, device=DEV))
+    ref = reference(x, w, labels)
+    assert torch.all((loss - kd).abs().double() <= 2 * loss_tol(ref, 64))
+
+
+def map_reference(z, idx, val, tau, drow):
+    z, V = z.double(), z.shape[-1]
+    idx = idx.long()
+    ok = (idx >= 0) & (idx < V)
+    q = torch.softmax((val.double() / tau).masked_fill(~ok, -math.inf), -1).nan_to_num(0.0)
+    live = (q.sum(-1) > 0) & (z.amax(-1) > -math.inf)
+    q = q * live[..., None]
+    lp = torch.log_softmax(z / tau, -1)
+    at = idx.clamp(0, V - 1)
+    logq = torch.where(q > 0, torch.log(q.clamp(min=1e-300)), 0.0)
+    loss = tau * tau * torch.where(q > 0, q * (logq - lp.gather(-1, at)), 0.0).sum(-1)
+    g = (torch.ones_like(loss) if drow is None else drow.double().expand(loss.shape)) * tau
+    p = torch.where(live[..., None], lp.exp(), 0.0)
+    dz = p.clone().scatter_add_(-1, at, -q) * g[..., None]
+    return loss, dz, (p + p.clone().zero_().scatter_add_(-1, at, q)) * g.abs()[..., None]
+
+
+def check_map(got, z, idx, val, tau, drow):
+    loss, dz = got
+    wl, wd, mag = map_reference(z, idx, val, tau, drow)
+    V = z.shape[-1]
+    zm = torch.where(torch.isfinite(z), z.abs(), 0).double().amax(-1) / tau
+    # exponent (z - max) c: two roundings of it, exp2 / log2 to two; the sum of V terms in a tree over 16 per thread and lanes: 48 roundings at most
+    rel = U * (8 * zm + 64)
+    check_rows(loss, wl, tau * tau * 2 * (rel + U * 16 * (zm + 40)))
+    h = 0.0 if dz.dtype == F32 else torch.finfo(dz.dtype).eps / 2
+    tiny = torch.finfo(dz.dtype).tiny * torch.finfo(dz.dtype).eps
+    tol = 1.01 * (h * wd.abs() + (rel[..., None] + 64 * U) * mag) + 2 * tiny
+    err = (dz.double() - wd).abs()
+    assert torch.all(err <= tol), (err / tol).max().item()
+
+
+MAP_SIZES = [(1, 1, 1, 1), (1, 1, 2, 2), (7, 1, 16, 16), (33, 4, 16, 16), (50, 4, 13, 5), (20, 1, 64, 64), (20, 1, 65, 64), (9, 1, 64, 65), (40, 1, 80, 10),
+             (13, 1, 1203, 32), (6, 2, 2048, 100), (5, 1, 2049, 40), (3, 1, 8191, 512), (3, 1, 8193, 7), (2, 1, 32768, 64), (2, 1, 32769, 64), (2, 1, 100003, 30)]
+
+
+@pytest.mark.parametrize("dtype,gdt", [(F32, F32), (BF, BF), (F16, F16), (BF, F32), (F16, F32)])
+@pytest.mark.parametrize("P,G,V,k", MAP_SIZES)
+def test_topk_distill(P, G, V, k, dtype, gdt):
+    z = (2.5 * _rand(P, G, V, seed=40)).to(dtype)
+    idx, val = teacher(P * G, V, k, 41, empty=P > 2)
+    idx, val = idx.view(P, G, k), val.view(P, G, k)
+    drow = _rand(P, G, seed=42) + 1.5
+    got = _ops().topk_distill(z, idx, val, tau=2.0, drow=drow, grad_dtype=gdt)
+    assert got[1].dtype == gdt and got[1].shape == z.shape
+    check_map(got, z, idx, val, 2.0, drow)
+    if G == 1:
+        two = _ops().topk_distill(z[:, 0], idx[:, 0], val[:, 0], tau=2.0, drow=drow[:, 0], grad_dtype=gdt)
+        assert torch.equal(two[0], got[0][:, 0]) and torch.equal(two[1], got[1][:, 0])
+
+
+@pytest.mark.parametrize("V,k", [(40, 12), (1000, 20), (5000, 20), (9000, 20), (40000, 20)])
+def test_topk_distill_odd_values(V, k):
+    """The same class in many slots, -inf logits, rows of nothing but -inf, rows without a teacher that hold NaN, far logits."""
+    z = 2 * _rand(12, V, seed=50)
+    idx, val = teacher(12, V, k, 51, empty=False, dup=False)
+    idx[0, :] = 3
+    idx[1, ::2] = idx[1, 0].item()
+    z[2, ::2] = -math.inf
+    idx[2] = idx[2] | 1
+    z[3] = -math.inf
+    idx[4] = -1
+    z[4] = math.nan
+    z[5] *= 400
+    z[6, idx[6, 0].long()] = -math.inf  # the student rules out what the teacher names: loss inf, the gradient stays finite
+    got = _ops().topk_distill(z, idx, val, tau=1.0)
+    assert got[0][3] == 0 and got[0][4] == 0 and torch.all(got[1][3:5] == 0) and got[0][6] == math.inf
+    zr = z.clone()
+    zr[4] = 0
+    check_map(got, zr, idx, val, 1.0, None)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("G,V,lead,tail", [(4, 16, 0, 80), (1, 80, 64, 0), (1, 77, 3, 5), (1, 3001, 65, 6)])
+def test_topk_distill_on_a_slice_of_a_map(G, V, lead, tail, dtype):
+    """Channels of an NHWC map read in place, the gradient written into a slice of another map (and into the map itself), the neighbours untouched."""
+    ops = _ops()
+    P, k = 60, 8
+    full = (2 * _rand(P, lead + G * V + tail, seed=60)).to(dtype)
+    idx, val = teacher(P * G, V, k, 61)
+    idx, val = idx.view(P, G, k), val.view(P, G, k)
+
+    def part(t):
+        return t[:, lead:lead + G * V].unflatten(1, (G, V))
+
+    want = ops.topk_distill(part(full).contiguous(), idx, val, tau=2.0)
+    got = ops.topk_distill(part(full), idx, val, tau=2.0)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    grad = torch.full((P, lead + G * V + tail + 9), 7.0, dtype=dtype, device=DEV)
+    loss, out = ops.topk_distill(part(full), idx, val, tau=2.0, out=part(grad))
+    assert torch.equal(part(grad), want[1]) and out.data_ptr() == part(grad).data_ptr()
+    grad[:, lead:lead + G * V] = 7.0
+    assert torch.all(grad == 7.0)
+    same = full.clone()
+    loss, _ = ops.topk_distill(part(same), idx, val, tau=2.0, out=part(same))
+    assert torch.equal(loss, want[0]) and torch.equal(part(same), want[1])
+    same[:, lead:lead + G * V] = full[:, lead:lead + G * V]
+    assert torch.equal(same, full)
+    only, none = ops.topk_distill(part(full), idx, val, tau=2.0, want_grad=False)
+    assert none is None and torch.equal(only, want[0])
+
+
+def test_no_rows():
+    ops = _ops()
+    loss, dz = ops.topk_distill(torch.empty(0, 50, device=DEV), torch.empty(0, 4, dtype=torch.int32, device=DEV), torch.empty(0, 4, device=DEV))
+    assert loss.shape == (0,) and dz.shape == (0, 50)
+    w = _rand(30, 16, dtype=BF)
+    loss, saved = ops.linear_distill_fwd(w[:0], w, torch.empty(0, 4, dtype=torch.int32, device=DEV), torch.empty(0, 4, device=DEV))
+    dx, dw = ops.linear_distill_bwd(w[:0], w, torch.empty(0, 4, dtype=torch.int32, device=DEV), saved)
+    assert loss.shape == (0,) and dx.shape == (0, 16) and torch.all(dw == 0)
+
+
+def test_gradients_against_differences():
+    """dx and dw of the fused losses, and dlogits, against central differences of the 64-bit loss along random directions. The difference's own error is
+    (step^2 / 6) of a third derivative (below 1e-5 here); the kernels' is that of a 16-bit gradient, h sqrt(n) of sum |g_i u_i| at random signs -- 4 h of the
+    2-norms' product is asserted."""
+    from cerberusdet_amd.utils import loss as UL
+
+    x, w, labels = ce_case(24, 60, 32, BF, seed=70)
+    idx, val = teacher(24, 60, 8, 71)
+    drow = _rand(24, seed=72).abs()
+    cases = [("ce", lambda X, W: reference(X, W, labels)["loss"], lambda X, W: UL.linear_cross_entropy(X, W, labels, reduction="none")),
+             ("kd", lambda X, W: reference(X, W, idx=idx, val=val, tau=2.0)["loss"], lambda X, W: UL.linear_distillation(X, W, idx, val, tau=2.0, reduction="none"))]
+    for name, exact, fused in cases:
+        xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+        (fused(xl, wl) * drow).sum().backward()
+        for leaf, seed in ((xl, 73), (wl, 74)):
+            u = _rand(*leaf.shape, seed=seed).double()
+            step = 1e-4
+
+            def at(s):
+                X = x.double() + (s * u if leaf is xl else 0)
+                W = w.double() + (s * u if leaf is wl else 0)
+                return (exact(X, W) * drow.double()).sum()
+
+            num = (at(step) - at(-step)) / (2 * step)
+            ana = (leaf.grad.double() * u).sum()
+            assert abs(num - ana) <= 4 * (2.0 ** -8) * leaf.grad.double().norm() + 1e-4, (name, num, ana)
+    z = _rand(24, 60, seed=75).requires_grad_()
+    (UL.topk_distillation(z, idx, val, tau=2.0, reduction="none") * drow).sum().backward()
+    u = _rand(24, 60, seed=76).double()
+
+    def mat(s):
+        return (map_reference(z.detach().double() + s * u, idx, val, 2.0, None)[0] * drow.double()).sum()
+
+    assert abs((mat(1e-4) - mat(-1e-4)) / 2e-4 - (z.grad.double() * u).sum()) <= 1e-4
+
+
+def test_streams_and_captured_graphs():
+    """Calls on another stream, and forward + backward captured in two graphs that are replayed in turn with eager work between, give the eager result."""
+    ops = _ops()
+    data = []
+    for s in (80, 90):
+        x, w, labels = ce_case(150, 700, 64, BF, seed=s)
+        idx, val = teacher(150, 700, 12, s + 5)
+        z = 2 * _rand(40, 700, seed=s + 7)
+        data.append((x, w, labels, idx, val, z))
+
+    def all_of(x, w, labels, idx, val, z):
+        loss, lse = ops.linear_ce_fwd(x, w, labels)
+        kd, saved = ops.linear_distill_fwd(x, w, idx, val, tau=2.0)
+        return [loss, lse, *ops.linear_ce_bwd(x, w, labels, lse), kd, *ops.linear_distill_bwd(x, w, idx, saved, tau=2.0), *ops.topk_distill(z, idx[:40], val[:40])]
+
+    want = [all_of(*d) for d in data]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = all_of(*data[0])
+    side.synchronize()
+    for a, b in zip(want[0], got):
+        assert torch.equal(a, b)
+    graphs = []
+    for d in data:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = all_of(*d)
+        graphs.append((g, outs))
+    for _ in range(3):
+        for (g, outs), ref in zip(graphs, want):
+            for o in outs:
+                o.fill_(5)
+            g.replay()
+            eager = all_of(*data[0])
+            torch.cuda.synchronize()
+            for a, b in zip(ref, outs):
+                assert torch.equal(a, b)
+            for a, b in zip(want[0], eager):
+                assert torch.equal(a, b)
+
+
+def test_used_together():
+    """A student classifier learns from labels and from a teacher's top logits in one backward; the fused distillation is that of its own logits."""
+    from cerberusdet_amd.utils import loss as UL
+
+    ops = _ops()
+    N, V, d, k = 200, 900, 64, 20
+    x, w, labels = ce_case(N, V, d, BF, seed=100)
+    xt, wt = _rand(N, d, seed=101, dtype=BF), _rand(V, d, seed=102, dtype=BF)
+    val, idx = (xt.float() @ wt.float().T).topk(k, dim=1)
+    xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+    total = UL.linear_cross_entropy(xl, wl, labels) + 0.5 * UL.linear_distillation(xl, wl, idx.int(), val, tau=2.0)
+    total.backward()
+    m = torch.full((1,), 1 / N, device=DEV)
+    rc, rk = reference(x, w, labels, drow=m), reference(x, w, idx=idx, val=val, tau=2.0, drow=0.5 * m)
+    assert abs(total.item() - rc["loss"].mean().item() - 0.5 * rk["loss"].mean().item()) < 1e-4
+    # two 16-bit gradients, rounded and added in 16 bits: half a step each, and the errors of their dz (as much again)
+    for got, key in ((xl.grad, "dx"), (wl.grad, "dw")):
+        want = rc[key] + rk[key]
+        assert (got.double() - want).norm() <= 2.0 ** -8 * 2 * (rc[key].norm() + rk[key].norm())
+    z = x.double() @ w.double().T
+    on_logits, _ = ops.topk_distill(z.float(), idx.int(), val, tau=2.0)
+    fused, _ = ops.linear_distill_fwd(x, w, idx.int(), val, tau=2.0)
+    assert torch.all((on_logits - fused).abs().double() <= 4 * (2 * loss_tol(rk, d) + 64 * U * 16) * 2)
+
+
+def test_head_distillation_of_a_model():
+    """The Detect head's own maps: box bins and class logits of a model's output against a teacher's, and the gradient that reaches the maps."""
+    import copy
+    import sys
+
+    from util import load_golden
+
+    from cerberusdet_amd.models import CerberusDet
+    from cerberusdet_amd.utils.loss import HeadDistillation
+
+    _, meta = load_golden("model_tiny2")
+    m = CerberusDet(meta["tasks"], meta["nc"], cfg=copy.deepcopy(meta["cfg"]), verbose=False)
+    m.sequential_split(meta["cfg"]["cerber"], "cpu")
+    m = m.to(DEV).train()
+    task = meta["tasks"][0]
+    nc = m.get_head(task).nc
+    img = torch.rand(2, 3, 64, 64, generator=torch.Generator().manual_seed(3)).to(DEV)
+    feats = [f.detach().clone().requires_grad_() for f in m(img, task)]
+    teach = [f.detach() + _rand(*f.shape, seed=5 + i) for i, f in enumerate(feats)]
+    scalar, items = HeadDistillation(m, k=2, tau=2.0, box=0.5, cls=2.0)(feats, teach, task)
+    scalar.backward()
+    box = cls = 0.0
+    px = sum(f.shape[0] * f.shape[2] * f.shape[3] for f in feats)
+    leaves = [f.detach().double().requires_grad_() for f in feats]
+    for f, t in zip(leaves, teach):
+        fr, tr = f.permute(0, 2, 3, 1).reshape(-1, 64 + nc), t.double().permute(0, 2, 3, 1).reshape(-1, 64 + nc)
+        q = torch.softmax(tr[:, :64].view(-1, 4, 16) / 2, -1)
+        box = box + 4 * (q * (q.log() - torch.log_softmax(fr[:, :64].view(-1, 4, 16) / 2, -1))).sum()
+        val, idx = tr[:, 64:].topk(min(2, nc), dim=1)
+        q = torch.softmax(val / 2, -1)
+        cls = cls + 4 * (q * (q.log() - torch.log_softmax(fr[:, 64:] / 2, -1).gather(1, idx))).sum()
+    want = 0.5 * box / (4 * px) + 2 * cls / px
+    want.backward()
+    assert abs(scalar.item() - want.item()) <= 1e-5 * abs(want.item())
+    assert torch.allclose(items.double().cpu(), torch.stack([box / (4 * px), cls / px]).detach().cpu(), rtol=1e-5)
+    for f, l in zip(feats, leaves):
+        assert (f.grad.double() - l.grad).abs().max() <= 1e-5 * l.grad.abs().max()
