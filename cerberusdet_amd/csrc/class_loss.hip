@@ -7,7 +7,7 @@
 // Forward: one matrix product whose epilogue keeps, per row and per 128 (64) classes, the running maximum and the sum of exponentials; a second launch
 // joins those pairs per row in a fixed order. Backward: per piece of the class list the product is computed again, its epilogue turns the logits
 // into dz (16-bit, one [N, piece] buffer), and one launch computes the piece's dw and adds the piece to dx. dz is relative to the largest row gradient
-// (and, in fp16, times 2^12): p of a 10^5-class list times 1 / N is far below fp16's smallest number.
+// (class_prep_kernel): p of a 10^5-class list times 1 / N is far below fp16's smallest number.
 //
 // One product kernel for all three (gemm_tile): an 8-wave workgroup, 256 x 256 (or 128 x 128) outputs, K in steps of 32 through a ring of four LDS
 // stages filled by LDS-DMA. The two halves of the workgroup run half a step apart: while one multiplies, the other reads its fragments.
@@ -252,6 +252,20 @@ __device__ __forceinline__ void store_rows16(unsigned char* stg, const uint2 (&p
     __builtin_amdgcn_wave_barrier();
 }
 
+template <int DT, int MT, int NT>
+__device__ __forceinline__ void store_scaled(unsigned char* stg, const f32x16 (&acc)[MT][NT], int j, float os, int lane, uint16_t* dst, int64_t ld, int nrows,
+                                             int ncols) {
+    uint2 pk[MT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            pk[i][q].x = lpack2<DT>(acc[i][j][4 * q] * os, acc[i][j][4 * q + 1] * os);
+            pk[i][q].y = lpack2<DT>(acc[i][j][4 * q + 2] * os, acc[i][j][4 * q + 3] * os);
+        }
+    store_rows16<DT, MT>(stg, pk, lane, dst, ld, nrows, ncols);
+}
+
 template <int DT, int MT, int NT, bool BWD>
 __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_logits_kernel(const LogitArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -384,6 +398,8 @@ struct GradArgs {
     int ntr, splits, kper;// dx: row tiles, slices of the piece, classes per slice (a multiple of 32)
     uint16_t* dw;         // [Vp][dw_ld]
     int64_t dw_ld;
+    uint16_t* dx;         // one piece, one slice: dx itself; else null and
+    int64_t dx_ld;
     float* slab;          // [splits][N][d]
     int add;              // slabs hold earlier pieces
     const float* outscale;
@@ -405,16 +421,8 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_grads_kernel(const
         unsigned char* stg = smem + wave8 * (32 * (MT * 64 + 16));
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            uint2 pk[MT][4];
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    pk[i][q].x = lpack2<DT>(acc[i][j][4 * q] * os, acc[i][j][4 * q + 1] * os);
-                    pk[i][q].y = lpack2<DT>(acc[i][j][4 * q + 2] * os, acc[i][j][4 * q + 3] * os);
-                }
             const int v = v0 + (wave * NT + j) * 32, f = f0 + grp * MT * 32;
-            store_rows16<DT, MT>(stg, pk, lane, a.dw + (int64_t)v * a.dw_ld + f, a.dw_ld, a.Vp - v, a.d - f);
+            store_scaled<DT, MT>(stg, acc, j, os, lane, a.dw + (int64_t)v * a.dw_ld + f, a.dw_ld, a.Vp - v, a.d - f);
         }
         return;
     }
@@ -423,6 +431,16 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_grads_kernel(const
     const int k0 = s * a.kper, k = min(a.kper, a.Vp - k0);
     gemm_tile<DT, MT, NT, true, false>(smem, TileSrc{a.w + (int64_t)k0 * a.w_ld + f0, a.w_ld, a.d - f0},
                                        TileSrc{a.dz + (int64_t)r0 * a.dz_ld + k0, a.dz_ld, a.rows32 - r0}, k, acc);
+    if (a.dx) {
+        const float os = *a.outscale;
+        unsigned char* stg = smem + wave8 * (32 * (MT * 64 + 16));
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int r = r0 + (wave * NT + j) * 32, f = f0 + grp * MT * 32;
+            store_scaled<DT, MT>(stg, acc, j, os, lane, a.dx + (int64_t)r * a.dx_ld + f, a.dx_ld, a.N - r, a.d - f);
+        }
+        return;
+    }
     float* slab = a.slab + (int64_t)s * a.N * a.d;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -447,31 +465,50 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_grads_kernel(const
 }
 
 // ---- small launches ----------------------------------------------------------------------------------------------------------------------------------
-// rows' (maximum, sum) pairs -> lse; 64 rows a workgroup, 16 threads a row that take every 16th pair, joined in a fixed order
-__global__ __launch_bounds__(1024) void class_lse_kernel(const float* part, int nvb, int N, int V, const void* label, int label64, const float* zlab, float* loss,
+// rows' (maximum, sum) pairs -> lse: C rows a workgroup (a power of two), 1024 / C threads a row that take every (1024 / C)th pair, joined in a tree of
+// fixed order
+__device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2) {  // a sum of 0 has no maximum; one of inf or NaN stays
+    if (s2 == 0.f) return;
+    if (s == 0.f) {
+        m = m2;
+        s = s2;
+        return;
+    }
+    const float mn = fmaxf(m, m2);
+    s = s * __builtin_amdgcn_exp2f(m - mn) + s2 * __builtin_amdgcn_exp2f(m2 - mn);
+    m = mn;
+}
+__global__ __launch_bounds__(1024) void class_lse_kernel(const float* part, int nvb, int N, int V, int C, const void* label, int label64, const float* zlab, float* loss,
                                                          float* lse) {
-    __shared__ float sm[16][64], ss[16][64];
-    const int c = (int)threadIdx.x & 63, g = (int)threadIdx.x >> 6;
-    const int r = (int)blockIdx.x * 64 + c;
-    float m = -INFINITY, s = 0.f;
-    auto join = [](float& m, float& s, float m2, float s2) {  // a sum of 0 has no maximum; one of inf or NaN keeps it
-        if (s2 == 0.f) return;
-        if (s == 0.f) {
-            m = m2;
-            s = s2;
-            return;
+    __shared__ float sm[1024], ss[1024];
+    const int t = (int)threadIdx.x, c = t & (C - 1), G = 1024 / C, g = t / C;
+    const int r = (int)blockIdx.x * C + c;
+    float m = 0.f, s = 0.f;
+    if (r < N) {
+        const float *pm = part + r, *ps = part + (int64_t)nvb * N + r;
+        for (int b = g; b < nvb; b += 4 * G) {
+            float m4[4], s4[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool in = b + u * G < nvb;
+                m4[u] = in ? pm[(int64_t)(b + u * G) * N] : 0.f;
+                s4[u] = in ? ps[(int64_t)(b + u * G) * N] : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) lse_join(m, s, m4[u], s4[u]);
         }
-        const float mn = fmaxf(m, m2);
-        s = s * __builtin_amdgcn_exp2f(m - mn) + s2 * __builtin_amdgcn_exp2f(m2 - mn);
-        m = mn;
-    };
-    if (r < N)
-        for (int b = g; b < nvb; b += 16) join(m, s, part[(int64_t)b * N + r], part[((int64_t)nvb + b) * N + r]);
-    sm[g][c] = m;
-    ss[g][c] = s;
-    __syncthreads();
+    }
+    sm[t] = m;
+    ss[t] = s;
+    for (int o = G >> 1; o; o >>= 1) {
+        __syncthreads();
+        if (g < o) {
+            lse_join(m, s, sm[t + o * C], ss[t + o * C]);
+            sm[t] = m;
+            ss[t] = s;
+        }
+    }
     if (g || r >= N) return;
-    for (int k = 1; k < 16; ++k) join(m, s, sm[k][c], ss[k][c]);
     const float l2 = s == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(s);  // (v_log_f32: base 2)
     lse[r] = l2 * kLn2;
     if (loss) {
@@ -480,55 +517,85 @@ __global__ __launch_bounds__(1024) void class_lse_kernel(const float* part, int 
     }
 }
 
-// row coefficients of dz: g_r relative to the largest |g| (a power of two above it), so that dz uses the 16-bit type's range; outscale undoes it
-__global__ __launch_bounds__(1024) void class_coef_kernel(const float* drow, int drow_stride, const void* label, int label64, const float* lse, int64_t lse_stride,
-                                                          int N, int V, float gain, float spread, float* lse2, float* coef, float* outscale) {
+// The backward's inputs, in one launch: lse and coefficient of every row, x contiguous with the rows that take no part (and those behind the last)
+// zeroed, and, where classes can be left out, w with those zeroed -- so that 0 * inf and NaN stay out of the products.
+// A row's coefficient is g_r times what brings the largest |g| of the rows that take part to 1.984375 (fp16: times 2^12): the entries of dz that matter
+// most, g (p - 1) at the labels of rows with the largest weight (of all rows, under a mean), then lie at the top of a binade, where rounding to 16 bits
+// costs half of what it does at its bottom; and dz stays inside fp16's range. Every workgroup finds the maximum for itself (N up to 32768: 16 bytes a row
+// out of the L2), or is given it.
+struct PrepArgs {
+    const float* drow;
+    int drow_stride;
+    const void* label;
+    int label64;
+    const float* lse;
+    int64_t lse_stride;
+    int N, V, rows32, d8;
+    float gain, spread;
+    const float* gmax;          // null: find it
+    const uint16_t *x, *w;
+    int64_t x_ld, w_ld;
+    const float* off;           // of w's classes; w null: no copy
+    int Vp;
+    float *lse2, *coef, *outscale;
+    u32x4 *xo, *wo;
+};
+__device__ __forceinline__ bool prep_live(const PrepArgs& a, int r) {
+    const float l = a.lse[(int64_t)r * a.lse_stride];
+    if (!a.label) return l != INFINITY;  // (the teacher's mark)
+    if (l == -INFINITY) return false;
+    const int64_t lab = load_label(a.label, a.label64, r);
+    return lab >= 0 && lab < a.V;
+}
+__device__ __forceinline__ float prep_max(const PrepArgs& a) {  // 1024 threads
     __shared__ float red[16];
     const int t = (int)threadIdx.x;
-    auto live = [&](int r) {
-        const float l = lse[(int64_t)r * lse_stride];
-        if (l == INFINITY && !label) return false;
-        if (l == -INFINITY) return false;
-        if (!label) return true;
-        const int64_t lab = load_label(label, label64, r);
-        return lab >= 0 && lab < V;
-    };
     float m = 0.f;
-    for (int r = t; r < N; r += 1024)
-        if (live(r)) {
-            const float g = drow ? fabsf(drow[(int64_t)r * drow_stride]) : 1.f;
-            m = __builtin_isfinite(g) ? fmaxf(m, g) : m;
-        }
+    for (int r = t; r < a.N; r += 1024) {
+        const float g = a.drow ? fabsf(a.drow[(int64_t)r * a.drow_stride]) : 1.f;
+        if (g <= 3.4e38f && g > m && prep_live(a, r)) m = g;
+    }
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     if ((t & 63) == 0) red[t >> 6] = m;
     __syncthreads();
     m = red[0];
     for (int i = 1; i < 16; ++i) m = fmaxf(m, red[i]);
-    int e = 0;
-    if (m > 0.f) frexpf(m, &e);  // m < 2^e
-    e = max(-100, min(100, e));
-    const float down = ldexpf(1.f, -e);
-    for (int r = t; r < N; r += 1024) {
-        const bool on = live(r);
-        const float g = drow ? drow[(int64_t)r * drow_stride] : 1.f;
-        const float l = lse[(int64_t)r * lse_stride] * kLog2e;
-        lse2[r] = !on ? INFINITY : l == INFINITY ? NAN : l;  // +inf marks a row without a part; an infinite logit gives NaN gradients
-        coef[r] = on ? g * down * spread : 0.f;
-    }
-    if (t == 0) *outscale = ldexpf(gain, e) / spread;
+    return m;
 }
-
-// x -> [rows32][d] contiguous, rows without a part (and behind the last) zeroed: 0 * inf and NaN stay out of dw
-__global__ __launch_bounds__(256) void class_rows_kernel(const uint16_t* x, int64_t ld, const float* lse2, int N, int rows32, int d8, u32x4* out) {
-    const int64_t n = (int64_t)rows32 * d8;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int r = (int)(i / d8), c = (int)(i - (int64_t)r * d8);
+__global__ __launch_bounds__(1024) void class_max_kernel(const PrepArgs a, float* out) {
+    const float m = prep_max(a);
+    if (threadIdx.x == 0) *out = m;
+}
+__global__ __launch_bounds__(1024) void class_prep_kernel(const PrepArgs a) {
+    const int64_t t = (int64_t)blockIdx.x * 1024 + threadIdx.x, nt = (int64_t)gridDim.x * 1024;
+    float m = a.gmax ? *a.gmax : prep_max(a);
+    m = m > 0.f ? fminf(fmaxf(m, 1e-30f), 1e37f) : 1.f;
+    const float down = 1.984375f * a.spread / m;
+    for (int64_t r = t; r < a.N; r += nt) {
+        const bool on = prep_live(a, (int)r);
+        const float g = a.drow ? a.drow[r * a.drow_stride] : 1.f;
+        const float l = a.lse[r * a.lse_stride] * kLog2e;
+        a.lse2[r] = !on ? INFINITY : l == INFINITY ? NAN : l;  // +inf marks a row without a part; an infinite logit gives NaN gradients
+        a.coef[r] = on ? g * down : 0.f;
+    }
+    if (t == 0) *a.outscale = a.gain * m / (1.984375f * a.spread);
+    const int64_t nx = (int64_t)a.rows32 * a.d8;
+    for (int64_t i = t; i < nx; i += nt) {
+        const int r = (int)(i / a.d8), c = (int)(i - (int64_t)r * a.d8);
         u32x4 v = {0, 0, 0, 0};
-        if (r < N && lse2[r] != INFINITY) v = *reinterpret_cast<const u32x4*>(x + r * ld + c * 8);
-        out[i] = v;
+        if (r < a.N && prep_live(a, r)) v = *reinterpret_cast<const u32x4*>(a.x + r * a.x_ld + c * 8);
+        a.xo[i] = v;
+    }
+    if (!a.w) return;
+    const int64_t nw = (int64_t)a.Vp * a.d8;
+    for (int64_t i = t; i < nw; i += nt) {
+        const int r = (int)(i / a.d8), c = (int)(i - (int64_t)r * a.d8);
+        u32x4 v = {0, 0, 0, 0};
+        if (a.off[r] != -INFINITY) v = *reinterpret_cast<const u32x4*>(a.w + r * a.w_ld + c * 8);
+        a.wo[i] = v;
     }
 }
-// a piece's weights with the left-out classes zeroed: 0 * inf and NaN stay out of dx
+// a later piece's weights with the left-out classes zeroed
 __global__ __launch_bounds__(256) void class_weights_kernel(const uint16_t* w, int64_t ld, const float* off, int V, int d8, u32x4* out) {
     const int64_t n = (int64_t)V * d8;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
@@ -559,14 +626,17 @@ __global__ __launch_bounds__(256) void class_zero_kernel(uint16_t* p, int64_t ro
 
 // ---- distillation: the teacher's slots ---------------------------------------------------------------------------------------------------------------
 // One wave a row, 16 lanes a slot: the student's logits at the teacher's classes (dot products in fp32), the teacher's softmax over its filled slots, the
-// loss. saved: [N][1 + 2k] = lse of the row (+inf where the teacher says nothing), logits (log2 units), q.
+// loss. saved: [N][1 + 2k] = lse of the row (+inf where the teacher says nothing), logits (log2 units), q -- the first slot that names a class holds the
+// sum over all of its slots, the others -1.
 template <int DT>
 __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, int64_t x_ld, const uint16_t* w, int64_t w_ld, const float* off, float c, float coff,
                                                             const int32_t* idx, const void* val, int val_dtype, int k, float itau, float tau2, int N, int V, int d,
                                                             const float* lse, float* loss, float* saved) {
-    const int lane = (int)threadIdx.x & 63;
-    const int r = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
-    if (r >= N) return;
+    __shared__ int s_idx[4][512];
+    __shared__ float s_q[4][512];
+    const int lane = (int)threadIdx.x & 63, wv = (int)threadIdx.x >> 6;
+    const int r = (int)blockIdx.x * 4 + wv;
+    if (r >= N) return;  // (whole waves; no barrier of the workgroup follows)
     const int sub = lane >> 4, l = lane & 15;
     float* sv = saved + (int64_t)r * (1 + 2 * k);
     const int32_t* ir = idx + (int64_t)r * k;
@@ -621,8 +691,22 @@ __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, i
                 if (q != 0.f) sum += q * (lq - (z2 - l2) * kLn2);
             }
             sv[1 + j] = z2;
-            sv[1 + k + j] = q;
+            s_idx[wv][j] = on ? ir[j] : -1;
+            s_q[wv][j] = q;
         }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    for (int j = lane; j < k; j += 64) {
+        const int v = s_idx[wv][j];
+        float q = s_q[wv][j];
+        bool first = v >= 0;
+        for (int o = 0; o < k; ++o) {
+            const bool same = s_idx[wv][o] == v;
+            first = first && !(same && o < j);
+            q += same && o > j ? s_q[wv][o] : 0.f;
+        }
+        sv[1 + k + j] = first ? q : -1.f;
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -631,25 +715,19 @@ __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, i
         sv[0] = !some ? INFINITY : lse[r] == INFINITY ? NAN : lse[r];
     }
 }
-// dz at the teacher's classes of a piece: coef * (p - q), q summed over the slots that name the class; the slot that names it first writes
+// dz at the teacher's classes of a piece: coef * (p - q)
 template <int DT>
 __global__ __launch_bounds__(256) void class_teacher_dz_kernel(const int32_t* idx, const float* saved, const float* lse2, const float* coef, int k, int N, int v_first,
                                                                int Vp, uint16_t* dz, int64_t dz_ld) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= (int64_t)N * k) return;
+    const int v = idx[i];
+    if (v < v_first || v - v_first >= Vp) return;
     const int r = (int)(i / k), j = (int)(i - (int64_t)r * k);
-    const int32_t* ir = idx + (int64_t)r * k;
-    const int v = ir[j];
-    if (v < v_first || v - v_first >= Vp || lse2[r] == INFINITY) return;
     const float* sv = saved + (int64_t)r * (1 + 2 * k);
-    if (sv[1 + j] == -INFINITY) return;  // a left-out class gets no gradient
-    float q = sv[1 + k + j];
-    for (int o = 0; o < j; ++o)
-        if (ir[o] == v) return;
-    for (int o = j + 1; o < k; ++o)
-        if (ir[o] == v) q += sv[1 + k + o];
-    const float g = (__builtin_amdgcn_exp2f(sv[1 + j] - lse2[r]) - q) * coef[r];
-    dz[r * dz_ld + (v - v_first)] = Elem<DT>::from_f32(g);
+    const float q = sv[1 + k + j];
+    if (q == -1.f || lse2[r] == INFINITY || sv[1 + j] == -INFINITY) return;  // another slot's, or a row without a part, or a left-out class (no gradient)
+    dz[r * dz_ld + (v - v_first)] = Elem<DT>::from_f32((__builtin_amdgcn_exp2f(sv[1 + j] - lse2[r]) - q) * coef[r]);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------------------------------
@@ -658,7 +736,7 @@ static inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 static inline bool big_tiles(int64_t rows, int64_t cols) { return (up(rows, 256) / 256) * (up(cols, 256) / 256) >= 160; }
 
 struct LinPlan {
-    bool big_f, big_g;
+    bool big_f, big_g, direct;  // direct: dx comes out of the one product launch
     int nvb, rows32, piece, splits, kper;
     int64_t o_part, o_zlab, o_lse, fwd_bytes;
     int64_t o_lse2, o_coef, o_scale, o_x, o_w, o_dz, o_slab, bwd_bytes;
@@ -690,6 +768,7 @@ static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool want_dx) {
         const int64_t dxt = (up(N, bt) / bt) * (up(d, bt) / bt);
         int64_t n = std::min((piece + p.rows32 / 2) / p.rows32, (512 + dxt - 1) / dxt);
         n = std::max<int64_t>(1, std::min(n, piece / 128));
+        if (pieces == 1 && piece <= 2048) n = 1;  // 64 steps at most: shorter than a launch that adds slices up
         p.kper = (int)up(up(piece, n) / n, 32);
         p.splits = (int)(up(piece, p.kper) / p.kper);
         return dxt * p.splits + (piece / bt) * (up(d, bt) / bt);
@@ -698,11 +777,12 @@ static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool want_dx) {
     if (!p.big_g) cut(128);
     p.o_lse2 = take(N * 4);
     p.o_coef = take(N * 4);
-    p.o_scale = take(4);
+    p.o_scale = take(8);
     p.o_x = take((int64_t)p.rows32 * d * 2);
     p.o_w = q->offset ? take(piece * d * 2) : 0;
     p.o_dz = take((int64_t)p.rows32 * piece * 2);
-    p.o_slab = want_dx ? take((int64_t)p.splits * N * d * 4) : 0;
+    p.direct = pieces == 1 && p.splits == 1;
+    p.o_slab = want_dx && !p.direct ? take((int64_t)p.splits * N * d * 4) : 0;
     p.bwd_bytes = o;
     return p;
 }
@@ -793,7 +873,9 @@ static int lin_forward(const cdet_linear_loss_desc* q, const LinPlan& p, const v
     a.zlab = (float*)(ws + p.o_zlab);
     const int rc = launch_logits<false>(a, q->dtype, p.big_f, s);
     if (rc) return rc;
-    class_lse_kernel<<<dim3(div_up(q->N, 64)), dim3(1024), 0, s>>>(a.part, p.nvb, q->N, q->V, label, q->label64, a.zlab, loss, lse);
+    int C = 1;  // rows a workgroup: 64 keep the loads wide, fewer fill the chip
+    while (C < 64 && (C < 8 ? C < q->N : C * 256 <= q->N)) C *= 2;
+    class_lse_kernel<<<dim3(div_up(q->N, C)), dim3(1024), 0, s>>>(a.part, p.nvb, q->N, q->V, C, label, q->label64, a.zlab, loss, lse);
     CDET_LAUNCH_CHECK();
     return 0;
 }
@@ -812,9 +894,38 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
     const LinPlan p = lin_plan(q, dx != nullptr);
     float *lse2 = (float*)(ws + p.o_lse2), *coef = (float*)(ws + p.o_coef), *os = (float*)(ws + p.o_scale);
     const float spread = q->dtype == CDET_F16 ? 4096.f : 1.f;
-    class_coef_kernel<<<dim3(1), dim3(1024), 0, s>>>(drow, drow_stride, label, q->label64, lse, lse_stride, N, V, q->scale * (idx ? q->tau : 1.f), spread, lse2, coef, os);
-    class_rows_kernel<<<dim3(std::min<int64_t>(2048, div_up((int64_t)p.rows32 * (d / 8), 256))), dim3(256), 0, s>>>((const uint16_t*)x, q->x_ld, lse2, N, p.rows32, d / 8,
-                                                                                                                  (u32x4*)(ws + p.o_x));
+    PrepArgs pa = {};
+    pa.drow = drow;
+    pa.drow_stride = drow_stride;
+    pa.label = label;
+    pa.label64 = q->label64;
+    pa.lse = lse;
+    pa.lse_stride = lse_stride;
+    pa.N = N;
+    pa.V = V;
+    pa.rows32 = p.rows32;
+    pa.d8 = d / 8;
+    pa.gain = q->scale * (idx ? q->tau : 1.f);
+    pa.spread = spread;
+    pa.x = (const uint16_t*)x;
+    pa.x_ld = q->x_ld;
+    pa.lse2 = lse2;
+    pa.coef = coef;
+    pa.outscale = os;
+    pa.xo = (u32x4*)(ws + p.o_x);
+    if (q->offset) {
+        pa.w = (const uint16_t*)w;
+        pa.w_ld = q->w_ld;
+        pa.off = q->offset;
+        pa.Vp = std::min(V, p.piece);
+        pa.wo = (u32x4*)(ws + p.o_w);
+    }
+    if (N > 32768) {
+        class_max_kernel<<<dim3(1), dim3(1024), 0, s>>>(pa, os + 1);
+        CDET_LAUNCH_CHECK();
+        pa.gmax = os + 1;
+    }
+    class_prep_kernel<<<dim3((unsigned)std::min<int64_t>(N > 8192 ? 1024 : 256, div_up((int64_t)(p.rows32 + pa.Vp) * pa.d8, 1024))), dim3(1024), 0, s>>>(pa);
     CDET_LAUNCH_CHECK();
     const int bt = p.big_g ? 256 : 128;
     for (int v0 = 0; v0 < V; v0 += p.piece) {
@@ -824,8 +935,9 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         a.x_ld = d;
         a.w = (const uint16_t*)w + (int64_t)v0 * q->w_ld;
         if (q->offset) {
-            class_weights_kernel<<<dim3(std::min<int64_t>(2048, div_up((int64_t)Vp * (d / 8), 256))), dim3(256), 0, s>>>(a.w, q->w_ld, q->offset + v0, Vp, d / 8,
-                                                                                                                        (u32x4*)(ws + p.o_w));
+            if (v0)
+                class_weights_kernel<<<dim3(std::min<int64_t>(2048, div_up((int64_t)Vp * (d / 8), 256))), dim3(256), 0, s>>>(a.w, q->w_ld, q->offset + v0, Vp, d / 8,
+                                                                                                                            (u32x4*)(ws + p.o_w));
             a.w = (const uint16_t*)(ws + p.o_w);
             a.w_ld = d;
             a.off = q->offset + v0;
@@ -865,13 +977,15 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         g.ndx = dx ? g.ntd * g.ntr * p.splits : 0;
         g.dw = dw ? (uint16_t*)dw + (int64_t)v0 * dw_ld : nullptr;
         g.dw_ld = dw_ld;
+        g.dx = p.direct ? (uint16_t*)dx : nullptr;
+        g.dx_ld = dx_ld;
         g.slab = (float*)(ws + p.o_slab);
         g.add = v0 > 0;
         g.outscale = os;
         rc = launch_grads(g, q->dtype, p.big_g, s);
         if (rc) return rc;
     }
-    if (dx) {
+    if (dx && !p.direct) {
         const unsigned nb = (unsigned)std::min<int64_t>(4096, div_up((int64_t)N * (d / 4), 256));
         if (q->dtype == CDET_BF16) class_dx_kernel<CDET_BF16><<<dim3(nb), dim3(256), 0, s>>>((const float*)(ws + p.o_slab), p.splits, N, d, os, (uint16_t*)dx, dx_ld);
         else class_dx_kernel<CDET_F16><<<dim3(nb), dim3(256), 0, s>>>((const float*)(ws + p.o_slab), p.splits, N, d, os, (uint16_t*)dx, dx_ld);

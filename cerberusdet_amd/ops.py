@@ -387,65 +387,90 @@ def det_loss(feats, gt, nc, gains, strides, grad_scale=1.0, grad_dtype=None, wan
 
 
 # ---------------------------------------------------------------------------------------------------------------
-# Losses over a long class list (csrc/class_loss.hip, csrc/topk_distill.hip). Bad arguments raise ValueError before anything is launched.
-def _need(cond, msg):
-    if not cond:
-        raise ValueError(msg)
+# Losses over a long class list (csrc/class_loss.hip, csrc/topk_distill.hip). Bad arguments raise ValueError before anything is launched. The messages are
+# put together only when they are raised: for a single row these calls are as long as what the host does around the launch.
+def _bad(msg):
+    raise ValueError(msg)
 
 
-def _on(dev, **tensors):
-    """Every given tensor is a tensor on `dev`."""
-    for name, t in tensors.items():
-        if t is not None:
-            _need(isinstance(t, torch.Tensor) and t.device == dev, f"{name} must be a tensor on {dev}, got {getattr(t, 'device', type(t))}")
+class _Device:
+    """Context of a launch on `dev`: switches the current device where it is another one; `stream` = the device's current stream."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, dev):
+        self.index, self.before = dev.index, torch.cuda.current_device()
+
+    def __enter__(self):
+        if self.index != self.before:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.index != self.before:
+            torch.cuda.set_device(self.before)
+        return False
 
 
-def _feature_rows(t, what):
-    """[rows, d] as the kernels read it: unit stride along d, a row pitch of whole 16-byte pieces; anything else is copied once."""
-    if t.stride(1) == 1 and (t.stride(0) % 8 == 0 or t.shape[0] == 1) and 0 <= t.stride(0) < (1 << 22) and t.data_ptr() % 16 == 0:
-        return t, (t.stride(0) if t.shape[0] != 1 else t.shape[1])
+def _on(dev, name, t):
+    if not isinstance(t, torch.Tensor) or t.device != dev:
+        _bad(f"{name} must be a tensor on {dev}, got {getattr(t, 'device', type(t))}")
+
+
+def _feature_rows(t):
+    """[rows, d] as the kernels read it, and its row pitch: unit stride along d, a pitch of whole 16-byte pieces; anything else is copied once."""
+    ld, one = t.stride()
+    if one == 1 and t.data_ptr() % 16 == 0:
+        if t.shape[0] == 1:
+            return t, t.shape[1]
+        if ld % 8 == 0 and ld < (1 << 22) and (ld == 0 or ld >= t.shape[1]):
+            return t, ld
     t = t.contiguous()
     return (t if t.data_ptr() % 16 == 0 else t.clone()), t.shape[1]
 
 
 def _linear_loss_desc(x, w, offset, scale, tau, label64=0):
-    _need(isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor), "x and w must be tensors")
-    _need(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], f"x [N, d] and w [V, d] expected, got {tuple(x.shape)} and {tuple(w.shape)}")
-    _need(x.dtype == w.dtype and x.dtype in (torch.bfloat16, torch.float16), f"x and w must both be bf16 or fp16, got {x.dtype} and {w.dtype}")
-    _need(x.is_cuda, "x must be on the GPU (there is no CPU path)")
-    _on(x.device, w=w, offset=offset)
-    N, dim = x.shape
-    V = w.shape[0]
-    _need(dim >= 8 and dim % 8 == 0 and dim <= 65536, f"d = {dim} must be a multiple of 8 in 8 .. 65536")
-    _need(1 <= V <= 1 << 24 and N <= 1 << 24, f"1 .. 2^24 classes and at most 2^24 rows, got {V} and {N}")
+    """(descriptor, x and w as the kernels read them, offset)."""
+    if not isinstance(x, torch.Tensor) or not isinstance(w, torch.Tensor) or x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        _bad(f"x [N, d] and w [V, d] expected, got {getattr(x, 'shape', type(x))} and {getattr(w, 'shape', type(w))}")
+    if x.dtype != w.dtype or x.dtype not in (torch.bfloat16, torch.float16):
+        _bad(f"x and w must both be bf16 or fp16, got {x.dtype} and {w.dtype}")
+    if not x.is_cuda:
+        _bad("x must be on the GPU (there is no CPU path)")
+    _on(x.device, "w", w)
+    (N, dim), V = x.shape, w.shape[0]
+    if dim < 8 or dim % 8 or dim > 65536:
+        _bad(f"d = {dim} must be a multiple of 8 in 8 .. 65536")
+    if not 1 <= V <= 1 << 24 or N > 1 << 24:
+        _bad(f"1 .. 2^24 classes and at most 2^24 rows, got {V} and {N}")
     scale, tau = float(scale), float(tau)
-    _need(0.0 < tau < float("inf"), f"tau = {tau} must be positive")
-    _need(abs(scale) < float("inf"), f"scale = {scale} must be finite")
+    if not 0.0 < tau < float("inf") or not abs(scale) < float("inf"):
+        _bad(f"tau = {tau} must be positive, scale = {scale} finite")
     if offset is not None:
-        _need(offset.shape == (V,) and offset.dtype == torch.float32, f"offset must be [{V}] fp32, got {tuple(offset.shape)} {offset.dtype}")
+        _on(x.device, "offset", offset)
+        if offset.shape != (V,) or offset.dtype != torch.float32:
+            _bad(f"offset must be [{V}] fp32, got {tuple(offset.shape)} {offset.dtype}")
         offset = offset.contiguous()
-    xs, x_ld = _feature_rows(x, "x") if N else (x, dim)
-    ws_, w_ld = _feature_rows(w, "w")
-    d = L.LinearLossDesc()
-    d.N, d.V, d.d, d.dtype = N, V, dim, dt(x.dtype)
-    d.x_ld, d.w_ld, d.scale, d.tau, d.offset, d.label64 = x_ld, w_ld, scale, tau, ptr(offset), label64
-    return d, xs, ws_, offset
+    xs, x_ld = _feature_rows(x) if N else (x, dim)
+    wsrc, w_ld = _feature_rows(w)
+    return L.LinearLossDesc(N, V, dim, _DT[x.dtype], x_ld, w_ld, scale, tau, None if offset is None else offset.data_ptr(), label64), xs, wsrc, offset
 
 
 def _labels(labels, x):
-    _need(isinstance(labels, torch.Tensor) and labels.shape == (x.shape[0],) and labels.dtype in (torch.int64, torch.int32),
-          f"labels must be [{x.shape[0]}] int64 or int32")
-    _on(x.device, labels=labels)
+    if not isinstance(labels, torch.Tensor) or labels.shape != x.shape[:1] or labels.dtype not in (torch.int64, torch.int32):
+        _bad(f"labels must be [{x.shape[0]}] int64 or int32")
+    _on(x.device, "labels", labels)
     return labels.contiguous()
 
 
 def _teacher(idx, val, shape, dev):
-    _need(isinstance(idx, torch.Tensor) and idx.dtype == torch.int32 and idx.dim() == len(shape) + 1 and tuple(idx.shape[:-1]) == tuple(shape),
-          f"idx must be {list(shape)} + [k] int32")
-    _need(1 <= idx.shape[-1] <= 512, f"k = {idx.shape[-1]} (1 .. 512)")
-    _on(dev, idx=idx, val=val)
+    if not isinstance(idx, torch.Tensor) or idx.dtype != torch.int32 or idx.shape[:-1] != shape or not 1 <= idx.shape[-1] <= 512:
+        _bad(f"idx must be {list(shape)} + [k] int32 with k in 1 .. 512, got {getattr(idx, 'shape', type(idx))}")
+    _on(dev, "idx", idx)
     if val is not None:
-        _need(val.shape == idx.shape and val.dtype in (torch.float32, torch.bfloat16, torch.float16), f"val must be {list(idx.shape)} fp32, bf16 or fp16")
+        _on(dev, "val", val)
+        if val.shape != idx.shape or val.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            _bad(f"val must be {list(idx.shape)} fp32, bf16 or fp16, got {tuple(val.shape)} {val.dtype}")
         val = val.contiguous()
     return idx.contiguous(), val
 
@@ -454,48 +479,44 @@ def _row_grad(drow, shape, dev):
     """(tensor | None, stride): one value per row, one value for all, or None (ones)."""
     if drow is None:
         return None, 0
-    _on(dev, drow=drow)
-    _need(drow.dtype == torch.float32 and (drow.shape == shape or drow.numel() == 1), f"drow must be {list(shape)} (or one value) fp32, got {tuple(drow.shape)} {drow.dtype}")
+    _on(dev, "drow", drow)
+    if drow.dtype != torch.float32 or not (drow.shape == shape or drow.numel() == 1):
+        _bad(f"drow must be {list(shape)} (or one value) fp32, got {tuple(drow.shape)} {drow.dtype}")
     return drow.contiguous(), (1 if drow.numel() != 1 else 0)
-
-
-def _loss_ws(d, backward, dev):
-    return torch.empty(L.load().cdet_linear_loss_ws_bytes(C.byref(d), int(backward)), dtype=torch.uint8, device=dev)
-
-
-def _class_grads(x, w, want_dx, want_dw):
-    return (torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None), (torch.empty(w.shape, dtype=w.dtype, device=w.device) if want_dw else None)
 
 
 def linear_ce_fwd(x, w, labels, offset=None, scale=1.0):
     """Softmax cross entropy of z = scale * x @ w.T + offset without the logits in memory. x [N, d], w [V, d] bf16 / fp16; labels [N] int64 / int32, a label
     outside of 0 .. V-1 leaves its row out (loss 0); offset [V] fp32 (class priors, -inf = class left out). Returns (loss [N], lse [N]) fp32."""
-    lib = L.load()
+    lib, dev = L.load(), x.device if isinstance(x, torch.Tensor) else None
     d, xs, wsrc, off = _linear_loss_desc(x, w, offset, scale, 1.0)
     labels = _labels(labels, x)
     d.label64 = int(labels.dtype == torch.int64)
-    with torch.cuda.device(x.device):
-        loss = torch.empty(d.N, dtype=torch.float32, device=x.device)
-        lse = torch.empty(d.N, dtype=torch.float32, device=x.device)
-        ws = _loss_ws(d, False, x.device)
-        L.check(lib.cdet_linear_ce_fwd(C.byref(d), ptr(xs), ptr(wsrc), ptr(labels), ptr(loss), ptr(lse), ptr(ws), stream()), "cdet_linear_ce_fwd")
+    ref = C.byref(d)
+    with _Device(dev) as s:
+        loss, lse = torch.empty((2, d.N), dtype=torch.float32, device=dev)
+        ws = torch.empty(lib.cdet_linear_loss_ws_bytes(ref, 0), dtype=torch.uint8, device=dev)
+        L.check(lib.cdet_linear_ce_fwd(ref, xs.data_ptr(), wsrc.data_ptr(), labels.data_ptr(), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), s), "cdet_linear_ce_fwd")
     return loss, lse
 
 
 def linear_ce_bwd(x, w, labels, lse, drow=None, offset=None, scale=1.0, want_dx=True, want_dw=True):
     """Gradients of sum(drow * loss): (dx [N, d], dw [V, d]) in x's type (None where not wanted). lse: linear_ce_fwd's; drow: fp32 [N], one value, or None."""
-    lib = L.load()
+    lib, dev = L.load(), x.device if isinstance(x, torch.Tensor) else None
     d, xs, wsrc, off = _linear_loss_desc(x, w, offset, scale, 1.0)
     labels = _labels(labels, x)
     d.label64 = int(labels.dtype == torch.int64)
-    _on(x.device, lse=lse)
-    _need(lse is not None and lse.shape == (d.N,) and lse.dtype == torch.float32, f"lse must be [{d.N}] fp32")
+    _on(dev, "lse", lse)
+    if lse.shape != x.shape[:1] or lse.dtype != torch.float32:
+        _bad(f"lse must be [{d.N}] fp32")
     lse = lse.contiguous()
-    g, gs = _row_grad(drow, (d.N,), x.device)
-    with torch.cuda.device(x.device):
-        dx, dw = _class_grads(x, w, want_dx, want_dw)
-        ws = _loss_ws(d, True, x.device)
-        L.check(lib.cdet_linear_ce_bwd(C.byref(d), ptr(xs), ptr(wsrc), ptr(labels), ptr(lse), ptr(g), gs, ptr(dx), d.d, ptr(dw), d.d, ptr(ws), stream()),
+    g, gs = _row_grad(drow, x.shape[:1], dev)
+    ref = C.byref(d)
+    with _Device(dev) as s:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
+        dw = torch.empty(w.shape, dtype=x.dtype, device=dev) if want_dw else None
+        ws = torch.empty(lib.cdet_linear_loss_ws_bytes(ref, 1), dtype=torch.uint8, device=dev)
+        L.check(lib.cdet_linear_ce_bwd(ref, xs.data_ptr(), wsrc.data_ptr(), labels.data_ptr(), lse.data_ptr(), ptr(g), gs, ptr(dx), d.d, ptr(dw), d.d, ws.data_ptr(), s),
                 "cdet_linear_ce_bwd")
     return dx, dw
 
@@ -504,35 +525,47 @@ def linear_distill_fwd(x, w, idx, val, tau=1.0, offset=None, scale=1.0):
     """Distillation of the class projection z = scale * x @ w.T + offset from a teacher's top k logits, without the logits in memory:
     loss = tau^2 KL(softmax(val / tau) || softmax(z / tau) at idx) per row. idx [N, k] int32 (outside of 0 .. V-1: an empty slot; a row without any has loss 0),
     val [N, k] fp32 / bf16 / fp16. Returns (loss [N] fp32, saved [N, 1 + 2k] fp32 for linear_distill_bwd)."""
-    lib = L.load()
+    lib, dev = L.load(), x.device if isinstance(x, torch.Tensor) else None
     d, xs, wsrc, off = _linear_loss_desc(x, w, offset, scale, tau)
-    _need(val is not None, "val must be given")
-    idx, val = _teacher(idx, val, (d.N,), x.device)
+    if val is None:
+        _bad("val must be given")
+    idx, val = _teacher(idx, val, x.shape[:1], dev)
     k = idx.shape[1]
-    with torch.cuda.device(x.device):
-        loss = torch.empty(d.N, dtype=torch.float32, device=x.device)
-        saved = torch.empty((d.N, 1 + 2 * k), dtype=torch.float32, device=x.device)
-        ws = _loss_ws(d, False, x.device)
-        L.check(lib.cdet_linear_distill_fwd(C.byref(d), ptr(xs), ptr(wsrc), k, ptr(idx), ptr(val), dt(val), ptr(loss), ptr(saved), ptr(ws), stream()),
-                "cdet_linear_distill_fwd")
+    ref = C.byref(d)
+    with _Device(dev) as s:
+        loss = torch.empty(d.N, dtype=torch.float32, device=dev)
+        saved = torch.empty((d.N, 1 + 2 * k), dtype=torch.float32, device=dev)
+        ws = torch.empty(lib.cdet_linear_loss_ws_bytes(ref, 0), dtype=torch.uint8, device=dev)
+        L.check(lib.cdet_linear_distill_fwd(ref, xs.data_ptr(), wsrc.data_ptr(), k, idx.data_ptr(), val.data_ptr(), _DT[val.dtype], loss.data_ptr(), saved.data_ptr(),
+                                            ws.data_ptr(), s), "cdet_linear_distill_fwd")
     return loss, saved
 
 
 def linear_distill_bwd(x, w, idx, saved, drow=None, tau=1.0, offset=None, scale=1.0, want_dx=True, want_dw=True):
     """Gradients of sum(drow * loss) of linear_distill_fwd: (dx, dw) in x's type."""
-    lib = L.load()
+    lib, dev = L.load(), x.device if isinstance(x, torch.Tensor) else None
     d, xs, wsrc, off = _linear_loss_desc(x, w, offset, scale, tau)
-    idx, _ = _teacher(idx, None, (d.N,), x.device)
+    idx, _ = _teacher(idx, None, x.shape[:1], dev)
     k = idx.shape[1]
-    _on(x.device, saved=saved)
-    _need(saved is not None and saved.shape == (d.N, 1 + 2 * k) and saved.dtype == torch.float32 and saved.is_contiguous(), f"saved must be linear_distill_fwd's [{d.N}, {1 + 2 * k}]")
-    g, gs = _row_grad(drow, (d.N,), x.device)
-    with torch.cuda.device(x.device):
-        dx, dw = _class_grads(x, w, want_dx, want_dw)
-        ws = _loss_ws(d, True, x.device)
-        L.check(lib.cdet_linear_distill_bwd(C.byref(d), ptr(xs), ptr(wsrc), k, ptr(idx), ptr(saved), ptr(g), gs, ptr(dx), d.d, ptr(dw), d.d, ptr(ws), stream()),
-                "cdet_linear_distill_bwd")
+    _on(dev, "saved", saved)
+    if saved.shape != (d.N, 1 + 2 * k) or saved.dtype != torch.float32 or not saved.is_contiguous():
+        _bad(f"saved must be linear_distill_fwd's [{d.N}, {1 + 2 * k}]")
+    g, gs = _row_grad(drow, x.shape[:1], dev)
+    ref = C.byref(d)
+    with _Device(dev) as s:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
+        dw = torch.empty(w.shape, dtype=x.dtype, device=dev) if want_dw else None
+        ws = torch.empty(lib.cdet_linear_loss_ws_bytes(ref, 1), dtype=torch.uint8, device=dev)
+        L.check(lib.cdet_linear_distill_bwd(ref, xs.data_ptr(), wsrc.data_ptr(), k, idx.data_ptr(), saved.data_ptr(), ptr(g), gs, ptr(dx), d.d, ptr(dw), d.d,
+                                            ws.data_ptr(), s), "cdet_linear_distill_bwd")
     return dx, dw
+
+
+def _pixel_pitch(t, what, P, G, V):
+    st = t.stride()
+    if (V > 1 and st[-1] != 1) or (G > 1 and st[1] != V) or st[0] < 0:
+        _bad(f"{what}: unit stride along V and back-to-back distributions needed, strides {st}")
+    return st[0] if P > 1 else G * V
 
 
 def topk_distill(logits, idx, val, tau=1.0, drow=None, grad_scale=1.0, grad_dtype=None, want_grad=True, out=None):
@@ -541,43 +574,38 @@ def topk_distill(logits, idx, val, tau=1.0, drow=None, grad_scale=1.0, grad_dtyp
     as it lies, e.g. view.torch().flatten(0, 2). idx / val [.., k]; drow: weights of the rows. Returns (loss [..] fp32, dlogits | None): the gradient of
     sum(drow * loss) * grad_scale in grad_dtype (the logits' or fp32) -- in `out` if given (a slice of a gradient map, or the logits themselves)."""
     lib = L.load()
-    _need(isinstance(logits, torch.Tensor) and logits.dim() in (2, 3) and logits.dtype in (torch.float32, torch.bfloat16, torch.float16),
-          "logits must be [P, V] or [P, G, V] fp32, bf16 or fp16")
-    _need(logits.is_cuda, "logits must be on the GPU (there is no CPU path)")
-    dev, shape = logits.device, tuple(logits.shape)
+    if not isinstance(logits, torch.Tensor) or logits.dim() not in (2, 3) or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        _bad("logits must be [P, V] or [P, G, V] fp32, bf16 or fp16")
+    if not logits.is_cuda:
+        _bad("logits must be on the GPU (there is no CPU path)")
+    dev, shape = logits.device, logits.shape
     P, V, G = shape[0], shape[-1], (shape[1] if len(shape) == 3 else 1)
-    _need(V >= 1 and G >= 1 and V <= 1 << 24 and P * G < 1 << 31, f"logits {shape}")
-
-    def pitch(t, what):
-        _need((V == 1 or t.stride(-1) == 1) and (G == 1 or t.stride(1) == V) and t.stride(0) >= 0, f"{what}: unit stride along V and back-to-back distributions needed, strides {t.stride()}")
-        return t.stride(0) if P > 1 else G * V
-
-    ld = pitch(logits, "logits")
-    _need(val is not None, "val must be given")
+    if not 1 <= V <= 1 << 24 or G < 1 or P * G >= 1 << 31:
+        _bad(f"logits {tuple(shape)}")
+    ld = _pixel_pitch(logits, "logits", P, G, V)
+    if val is None:
+        _bad("val must be given")
     idx, val = _teacher(idx, val, shape[:-1], dev)
-    _need(0.0 < float(tau) < float("inf"), f"tau = {tau} must be positive")
-    grad_dtype = grad_dtype or (out.dtype if out is not None else logits.dtype)
-    _need(grad_dtype in (logits.dtype, torch.float32), f"grad_dtype must be {logits.dtype} or fp32")
+    tau = float(tau)
+    if not 0.0 < tau < float("inf"):
+        _bad(f"tau = {tau} must be positive")
+    grad_dtype = grad_dtype or (logits.dtype if out is None else out.dtype)
+    if grad_dtype is not logits.dtype and grad_dtype is not torch.float32:
+        _bad(f"grad_dtype must be {logits.dtype} or fp32")
     g, gs = _row_grad(drow, shape[:-1], dev)
-    if g is not None and gs == 0 and P * G != 1:
-        g = g.reshape(1).expand(P * G).contiguous()
-    with torch.cuda.device(dev):
+    with _Device(dev) as s:
+        if g is not None and gs == 0 and P * G != 1:
+            g = g.reshape(1).expand(P * G).contiguous()
         if out is not None:
-            _on(dev, out=out)
-            _need(tuple(out.shape) == shape and out.dtype == grad_dtype, f"out must be {shape} {grad_dtype}")
-            _need(P <= 1 or out.stride(0) >= G * V, "out: overlapping pixels")
+            _on(dev, "out", out)
+            if out.shape != shape or out.dtype != grad_dtype or (P > 1 and out.stride(0) < G * V):
+                _bad(f"out must be {tuple(shape)} {grad_dtype} without overlapping pixels")
         elif want_grad:
-            # rows of whole 16 bytes, so that every row's vectors are aligned
-            e = 16 // torch.empty(0, dtype=grad_dtype).element_size()
-            out = torch.empty((P, -(-G * V // e) * e), dtype=grad_dtype, device=dev)[:, :G * V]
-            out = out.unflatten(1, (G, V)) if len(shape) == 3 else out
-        d = L.TopkDistillDesc()
-        d.P, d.G, d.V, d.k = P, G, V, idx.shape[-1]
-        d.dtype, d.val_dtype, d.grad_dtype = dt(logits.dtype), dt(val.dtype), dt(grad_dtype)
-        d.ld, d.grad_ld = ld, (pitch(out, "out") if out is not None else 0)
-        d.tau, d.grad_scale = float(tau), float(grad_scale)
+            out = torch.empty(shape, dtype=grad_dtype, device=dev)
+        gld = _pixel_pitch(out, "out", P, G, V) if out is not None else 0
+        d = L.TopkDistillDesc(P, G, V, idx.shape[-1], _DT[logits.dtype], _DT[val.dtype], _DT[grad_dtype], ld, gld, tau, float(grad_scale))
         loss = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
-        L.check(lib.cdet_topk_distill(C.byref(d), ptr(logits), ptr(idx), ptr(val), ptr(g), ptr(loss), ptr(out), stream()), "cdet_topk_distill")
+        L.check(lib.cdet_topk_distill(C.byref(d), logits.data_ptr(), idx.data_ptr(), val.data_ptr(), ptr(g), loss.data_ptr(), ptr(out), s), "cdet_topk_distill")
     return loss, out
 
 
