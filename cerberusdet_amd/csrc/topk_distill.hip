@@ -1,10 +1,11 @@
 // Distillation from a teacher's top k logits on logits that are in memory: loss and gradient of every row in one launch.
 //   p = softmax(z / tau) over the row's V logits, q = softmax of the teacher's filled slots / tau
 //   loss = tau^2 sum_j q_j (log q_j - log p[idx_j]),   dz_v = drow * grad_scale * tau * (p_v - sum_{j: idx_j == v} q_j)
-// Bound by memory: logits once in, gradient once out. A row of up to 32768 logits stays in the registers of its 1, 4 or 16 waves (td_wide_kernel), so the
-// maximum, the sum and the gradient are taken from one read; a longer row is read again for its gradient (td_long_kernel: the second read comes out of
-// the 256 MiB cache). The gradient is written dense and then, behind a barrier, the k named entries are written again with their q. Rows of at most 64
-// logits (box distributions) take 16 lanes each and put q together in LDS first (td_narrow_kernel). p is exp2((z - max) c) / sum: its error does not
+// Bound by memory: logits once in, gradient once out. A row of up to 32768 logits stays in the registers of its 1, 4, 8 or 16 waves (td_wide_kernel), so the
+// maximum, the sum and the gradient are taken from one read (td_wave_kernel, td_wide_kernel); one of up to 256 KiB is held as it is stored
+// (td_held_kernel); a longer one is read again for its gradient (td_long_kernel). Above 2048 logits the gradient is written dense and then, behind a
+// barrier, the k named entries are written again with their q; shorter rows put q together in LDS first. Rows of at most 64 logits (box distributions)
+// take 16 lanes each (td_narrow_kernel). p is exp2((z - max) c) / sum: its error does not
 // grow with |z|.
 #include "common.h"
 
@@ -46,11 +47,55 @@ template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) 
     T v[N];
 };
 
-// sums / maxima over the workgroup's waves (NW = 1: inside the wave), the same value in every thread, in a fixed order
+// exponent of a logit relative to the row's maximum, log2 units. fp32: the difference first, so that the error does not grow with |z|; 16-bit logits and
+// gradients need no more than one fused rounding of z c (2^-24 |z c| against 2^-9)
+template <int DT>
+__device__ __forceinline__ float td_exp2(float z, float mu, float c, float muc) {
+    return __builtin_amdgcn_exp2f(DT == CDET_F32 ? (z - mu) * c : fmaf(z, c, -muc));
+}
+typedef __attribute__((ext_vector_type(2))) float tdf2;
+typedef __attribute__((ext_vector_type(2))) __bf16 tdb2;
+typedef __attribute__((ext_vector_type(2))) _Float16 tdh2;
+template <int GDT, int N>
+__device__ __forceinline__ void td_put(typename TdElem<GDT>::T* dst, const float (&v)[N]) {  // N consecutive elements, converted in pairs
+    if (GDT == CDET_F32) {
+        TdVec<float, N> o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o.v[e] = v[e];
+        *reinterpret_cast<TdVec<float, N>*>(dst) = o;
+    } else {
+        TdVec<uint16_t, N> o;
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const uint32_t p = GDT == CDET_BF16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(tdf2{v[e], v[e + 1]}, tdb2))
+                                                : __builtin_bit_cast(uint32_t, __builtin_convertvector(tdf2{v[e], v[e + 1]}, tdh2));
+            __builtin_memcpy(&o.v[e], &p, 4);
+        }
+        *reinterpret_cast<TdVec<uint16_t, N>*>(dst) = o;
+    }
+}
+
+// maximum / sum over the 16 lanes of a DPP row, then over the wave: the same value in every lane
+template <bool MAX>
+__device__ __forceinline__ float td_row16(float v) {
+#define CDET_DPP(ctrl)                                                                                                                              \
+    do {                                                                                                                                            \
+        const float u = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true)); \
+        v = MAX ? fmaxf(v, u) : v + u;                                                                                                              \
+    } while (0)
+    CDET_DPP(0xB1);   // quad_perm [1,0,3,2]
+    CDET_DPP(0x4E);   // quad_perm [2,3,0,1]
+    CDET_DPP(0x141);  // row_half_mirror
+    CDET_DPP(0x140);  // row_mirror
+#undef CDET_DPP
+    return v;
+}
+// maxima / sums over a row's waves (NW = 1: inside the wave), the same value in every thread, in a fixed order
 template <int NW, bool MAX>
 __device__ __forceinline__ float td_reduce(float v, float* scratch) {
+    v = td_row16<MAX>(v);
 #pragma unroll
-    for (int o = 32; o; o >>= 1) {
+    for (int o = 16; o < 64; o *= 2) {
         const float u = __shfl_xor(v, o);
         v = MAX ? fmaxf(v, u) : v + u;
     }
@@ -137,23 +182,169 @@ __device__ __forceinline__ void td_finish(const TdArgs& a, int64_t row, int t, b
 
 template <typename T, typename TG>
 __device__ __forceinline__ void td_row(const TdArgs& a, int64_t row, const T*& z, TG*& dz) {
-    const int64_t px = row / a.G, gr = row - px * a.G;
-    z = (const T*)a.z + px * a.ld + gr * a.V;
-    dz = a.dz ? (TG*)a.dz + px * a.gld + gr * a.V : nullptr;
+    const unsigned px = a.G == 1 ? (unsigned)row : (unsigned)row / (unsigned)a.G, gr = (unsigned)row - px * (unsigned)a.G;  // (rows < 2^31)
+    z = (const T*)a.z + (int64_t)px * a.ld + (int64_t)gr * a.V;
+    dz = a.dz ? (TG*)a.dz + (int64_t)px * a.gld + (int64_t)gr * a.V : nullptr;
 }
 
-// a row's logits in registers: up to NCH chunks of CH per thread, NW waves a row (NW = 1: four rows a workgroup)
+// V <= 2048: a wave a row, four rows a workgroup, the logits in registers and once in LDS: the slots find theirs there, and then leave their q there for the
+// dense gradient to take along -- no gather from and no second write to memory (67200 x 1203 fp32, k = 32 scattered classes: 134 us = 4.9 TB/s against 170 us with them)
+template <int DT, int GDT>
+__global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
+    typedef typename TdElem<DT>::T T;
+    typedef typename TdElem<GDT>::T TG;
+    constexpr int CH = 16 / sizeof(T), NCH = 32 / CH;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const int t = (int)threadIdx.x & 63, V = a.V, k = a.k;
+    const int64_t row = (int64_t)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
+    if (row >= a.rows) return;  // (whole waves, and no barrier of the workgroup follows)
+    float* const base = lds + ((int)threadIdx.x >> 6) * (4 * k + ((V + 7) & ~7));
+    const TdSlots sl(base, k);
+    float* const rb = base + 4 * k;
+    const T* z;
+    TG* dz;
+    td_row(a, row, z, dz);
+
+    int v0 = -1;
+    float x0 = 0.f;
+    if (t < k) {  // (in front of the logits: their wait does not take these along)
+        v0 = a.idx[row * k + t];
+        x0 = load_elem(a.val, row * k + t, a.vdt);
+    }
+    const float w = a.drow ? a.drow[row] : 1.f;
+    float v[NCH][CH];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int e0 = (i * 64 + t) * CH;
+        if (e0 + CH <= V) {
+            const TdVec<T, CH> x = *reinterpret_cast<const TdVec<T, CH>*>(z + e0);
+#pragma unroll
+            for (int e = 0; e < CH; ++e) v[i][e] = TdElem<DT>::get(x.v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < CH; ++e) v[i][e] = -INFINITY;
+            if (e0 < V)
+#pragma unroll
+                for (int e = 0; e < CH; ++e)
+                    if (e0 + e < V) v[i][e] = TdElem<DT>::get(z[e0 + e]);
+        }
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+        if (i * 64 * CH < V) {
+            const int e0 = (i * 64 + t) * CH;
+#pragma unroll
+            for (int e = 0; e < CH; e += 4) {
+                const f32x4 o = {v[i][e], v[i][e + 1], v[i][e + 2], v[i][e + 3]};
+                if (e0 < V) *reinterpret_cast<f32x4*>(rb + e0 + e) = o;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) m = fmaxf(m, o[u]);
+            }
+        }
+    td_sync<1>();
+    float tm = -INFINITY;
+    for (int j = t; j < k; j += 64) {
+        int c = j == t ? v0 : a.idx[row * k + j];
+        const float x = (j == t ? x0 : load_elem(a.val, row * k + j, a.vdt)) * a.itau;
+        if ((unsigned)c >= (unsigned)V) c = -1;
+        sl.v[j] = c;
+        sl.lq[j] = x;
+        if (c >= 0) {
+            sl.z[j] = rb[c];
+            tm = fmaxf(tm, x);
+        }
+    }
+    m = td_reduce<1, true>(m, nullptr);
+    tm = td_reduce<1, true>(tm, nullptr);
+    const bool on = m != -INFINITY && tm != -INFINITY;
+    const float mu = __builtin_isinf(m) ? 0.f : m, muc = mu * a.c;
+    float s = 0.f, ts = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+        if (i * 64 * CH < V)
+#pragma unroll
+            for (int e = 0; e < CH; ++e) {
+                v[i][e] = td_exp2<DT>(v[i][e], mu, a.c, muc);
+                s += v[i][e];
+            }
+    for (int j = t; j < k; j += 64)
+        if (sl.v[j] >= 0) ts += expf(sl.lq[j] - tm);
+    s = td_reduce<1, false>(s, nullptr);
+    ts = td_reduce<1, false>(ts, nullptr);
+    const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s), lts = logf(ts);
+    td_sync<1>();  // every slot has read its logit
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int e0 = (i * 64 + t) * CH;
+        if (e0 < V)
+#pragma unroll
+            for (int e = 0; e < CH; e += 4) *reinterpret_cast<f32x4*>(rb + e0 + e) = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float sum = 0.f;
+    for (int j = t; j < k; j += 64) {
+        const float lq = sl.lq[j] - tm - lts;
+        const float q = on && sl.v[j] >= 0 ? expf(lq) : 0.f;
+        sl.q[j] = q;
+        if (q != 0.f) sum += q * (lq - ((sl.z[j] - mu) * a.c - l2s) * kTdLn2);
+    }
+    sum = td_reduce<1, false>(sum, nullptr);
+    if (t == 0) a.loss[row] = on ? sum * a.tau2 : 0.f;
+    if (!dz) return;
+    td_sync<1>();
+    // a class named twice takes the q of all of its slots, in their order: found with one comparison a slot where the slots fit the lanes
+    bool alone = false;
+    if (k <= 64) {
+        const int c = t < k && sl.v[t] >= 0 ? sl.v[t] : -1 - t;
+        uint64_t twice = 0;
+        for (int o = 0; o < k; ++o) twice |= __ballot(c == __builtin_amdgcn_readlane(c, o)) & ~(1ull << o);
+        alone = twice == 0;
+    }
+    for (int j = t; j < k; j += 64) {
+        const int c = sl.v[j];
+        if (c < 0) continue;
+        float q = sl.q[j];
+        bool first = true;
+        if (!alone)
+            for (int o = 0; o < k; ++o) {
+                const bool same = sl.v[o] == c;
+                first = first && !(same && o < j);
+                q += same && o > j ? sl.q[o] : 0.f;
+            }
+        if (first) rb[c] = q;
+    }
+    td_sync<1>();
+    const float g = a.gs * w;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int e0 = (i * 64 + t) * CH;
+        if (e0 >= V) continue;
+        float o[CH];
+#pragma unroll
+        for (int e = 0; e < CH; e += 4) {
+            const f32x4 q = *reinterpret_cast<const f32x4*>(rb + e0 + e);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o[e + u] = on ? (v[i][e + u] * inv - q[u]) * g : 0.f;
+        }
+        if (e0 + CH <= V) td_put<GDT, CH>(dz + e0, o);
+        else
+#pragma unroll
+            for (int e = 0; e < CH; ++e)
+                if (e0 + e < V) dz[e0 + e] = TdElem<GDT>::put(o[e]);
+    }
+}
+
+// a row's logits in registers: up to NCH chunks of CH per thread, NW waves a row
 template <int DT, int GDT, int NW>
-__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void td_wide_kernel(const TdArgs a) {
+__global__ __launch_bounds__(NW * 64, NW == 16 ? 8 : 1) void td_wide_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
     typedef typename TdElem<GDT>::T TG;
     constexpr int NT = NW * 64, CH = 16 / sizeof(T), NCH = 32 / CH;
     extern __shared__ float lds[];
     __shared__ float scratch[16];
-    const int sub = NW == 1 ? (int)threadIdx.x >> 6 : 0, t = (int)threadIdx.x & (NT - 1), V = a.V;
-    const int64_t row = (int64_t)blockIdx.x * (NW == 1 ? 4 : 1) + sub;
-    if (row >= a.rows) return;  // (NW == 1: whole waves, and no barrier of the workgroup follows)
-    const TdSlots slots(lds + sub * 4 * a.k, a.k);
+    const int t = (int)threadIdx.x, V = a.V;
+    const int64_t row = blockIdx.x;
+    const TdSlots slots(lds, a.k);
     const T* z;
     TG* dz;
     td_row(a, row, z, dz);
@@ -184,35 +375,120 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void td_wide_kernel(const 
             for (int e = 0; e < CH; ++e) m = fmaxf(m, v[i][e]);
     m = td_reduce<NW, true>(m, scratch);
     on = on && m != -INFINITY;
-    const float mu = __builtin_isinf(m) ? 0.f : m;
+    const float mu = __builtin_isinf(m) ? 0.f : m, muc = mu * a.c;
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
         if (i * NT * CH < V)
 #pragma unroll
             for (int e = 0; e < CH; ++e) {
-                v[i][e] = __builtin_amdgcn_exp2f((v[i][e] - mu) * a.c);
+                v[i][e] = td_exp2<DT>(v[i][e], mu, a.c, muc);
                 s += v[i][e];
             }
     s = td_reduce<NW, false>(s, scratch);
     const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s);
-    const float g = a.gs * (a.drow ? a.drow[row] : 1.f);
+    const float g = a.gs * (a.drow ? a.drow[row] : 1.f), f = inv * g;
     if (dz) {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             const int e0 = (i * NT + t) * CH;
             if (e0 >= V) continue;
-            TdVec<TG, CH> o;
+            float o[CH];
 #pragma unroll
-            for (int e = 0; e < CH; ++e) o.v[e] = TdElem<GDT>::put(on ? v[i][e] * inv * g : 0.f);
-            if (e0 + CH <= V) *reinterpret_cast<TdVec<TG, CH>*>(dz + e0) = o;
+            for (int e = 0; e < CH; ++e) o[e] = on ? v[i][e] * f : 0.f;
+            if (e0 + CH <= V) td_put<GDT, CH>(dz + e0, o);
             else
 #pragma unroll
                 for (int e = 0; e < CH; ++e)
-                    if (e0 + e < V) dz[e0 + e] = o.v[e];
+                    if (e0 + e < V) dz[e0 + e] = TdElem<GDT>::put(o[e]);
         }
     }
     td_sync<NW>();  // the slots are complete, the dense gradient is written: the named entries may follow
+    td_finish<GDT, NW>(a, row, t, on, dz, mu, inv, l2s, g, slots, scratch);
+}
+
+// longer rows, as they are stored (16 waves a row, NCH chunks of 16 bytes a thread): two exponentials a logit instead of a second read
+template <int DT, int GDT, int NCH>
+__global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const TdArgs a) {
+    typedef typename TdElem<DT>::T T;
+    typedef typename TdElem<GDT>::T TG;
+    constexpr int NW = 16, NT = 1024, CH = 16 / sizeof(T);
+    extern __shared__ float lds[];
+    __shared__ float scratch[16];
+    const int t = (int)threadIdx.x, V = a.V;
+    const int64_t row = blockIdx.x;
+    const TdSlots slots(lds, a.k);
+    const T* z;
+    TG* dz;
+    td_row(a, row, z, dz);
+    const T ninf = TdElem<DT>::put(-INFINITY);
+    u32x4 v[NCH];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int e0 = (i * NT + t) * CH;
+        TdVec<T, CH> x;
+        if (e0 + CH <= V) x = *reinterpret_cast<const TdVec<T, CH>*>(z + e0);
+        else {
+#pragma unroll
+            for (int e = 0; e < CH; ++e) x.v[e] = ninf;
+            if (e0 < V)
+#pragma unroll
+                for (int e = 0; e < CH; ++e)
+                    if (e0 + e < V) x.v[e] = z[e0 + e];
+        }
+        __builtin_memcpy(&v[i], &x, 16);
+    }
+    auto logit = [&](int i, int e) {
+        if (DT == CDET_F32) return __uint_as_float(v[i][e]);
+        return TdElem<DT>::get((T)(v[i][(e >> 1) & 3] >> (16 * (e & 1))));
+    };
+    // each pass unpacks the chunks anew: without this the compiler keeps 128 fp32 values a thread from the first pass on
+    auto anew = [&](int i) { asm volatile("" : "+v"(v[i])); };
+    bool on = td_teacher<DT, NW>(a, row, t, z, slots, scratch);
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+        if (i * NT * CH < V) {
+            anew(i);
+#pragma unroll
+            for (int e = 0; e < CH; ++e) m = fmaxf(m, logit(i, e));
+        }
+    m = td_reduce<NW, true>(m, scratch);
+    on = on && m != -INFINITY;
+    const float mu = __builtin_isinf(m) ? 0.f : m, muc = mu * a.c;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+        if (i * NT * CH < V) {
+            anew(i);
+#pragma unroll
+            for (int e = 0; e < CH; ++e) s += td_exp2<DT>(logit(i, e), mu, a.c, muc);
+        }
+    s = td_reduce<NW, false>(s, scratch);
+    const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s);
+    const float g = a.gs * (a.drow ? a.drow[row] : 1.f), f = inv * g;
+    if (dz) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int e0 = (i * NT + t) * CH;
+            if (e0 >= V) continue;
+            anew(i);
+            float o[CH];
+            if (on) {  // (uniform)
+#pragma unroll
+                for (int e = 0; e < CH; ++e) o[e] = td_exp2<DT>(logit(i, e), mu, a.c, muc) * f;
+            } else {
+#pragma unroll
+                for (int e = 0; e < CH; ++e) o[e] = 0.f;
+            }
+            if (e0 + CH <= V) td_put<GDT, CH>(dz + e0, o);
+            else
+#pragma unroll
+                for (int e = 0; e < CH; ++e)
+                    if (e0 + e < V) dz[e0 + e] = TdElem<GDT>::put(o[e]);
+        }
+    }
+    td_sync<NW>();
     td_finish<GDT, NW>(a, row, t, on, dz, mu, inv, l2s, g, slots, scratch);
 }
 
@@ -260,155 +536,159 @@ __global__ __launch_bounds__(1024) void td_long_kernel(const TdArgs a) {
     }
     const float all = td_reduce<NW, true>(m, scratch);
     on = on && all != -INFINITY;
-    const float mu = __builtin_isinf(all) ? 0.f : all;
+    const float mu = __builtin_isinf(all) ? 0.f : all, muc = mu * a.c;
     s = s == 0.f ? 0.f : s * __builtin_amdgcn_exp2f(((__builtin_isinf(m) ? 0.f : m) - mu) * a.c);
     s = td_reduce<NW, false>(s, scratch);
     const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s);
-    const float g = a.gs * (a.drow ? a.drow[row] : 1.f);
+    const float g = a.gs * (a.drow ? a.drow[row] : 1.f), f = inv * g;
     if (dz) {
         for (int e0 = t * CH; e0 < V; e0 += NT * CH) {
             float v[CH];
             load(e0, v);
-            TdVec<TG, CH> o;
+            float o[CH];
 #pragma unroll
-            for (int e = 0; e < CH; ++e) o.v[e] = TdElem<GDT>::put(on ? __builtin_amdgcn_exp2f((v[e] - mu) * a.c) * inv * g : 0.f);
-            if (e0 + CH <= V) *reinterpret_cast<TdVec<TG, CH>*>(dz + e0) = o;
+            for (int e = 0; e < CH; ++e) o[e] = on ? td_exp2<DT>(v[e], mu, a.c, muc) * f : 0.f;
+            if (e0 + CH <= V) td_put<GDT, CH>(dz + e0, o);
             else
 #pragma unroll
                 for (int e = 0; e < CH; ++e)
-                    if (e0 + e < V) dz[e0 + e] = o.v[e];
+                    if (e0 + e < V) dz[e0 + e] = TdElem<GDT>::put(o[e]);
         }
     }
     td_sync<NW>();
     td_finish<GDT, NW>(a, row, t, on, dz, mu, inv, l2s, g, slots, scratch);
 }
 
-// V <= 64, k <= 64: 16 lanes a row, 16 rows a workgroup. Per row in LDS: the logits' log p, the q of every class, who named a class last
-template <int DT, int GDT>
+// V, k <= 16 E: 16 lanes a row, R rows of a lane at a time (their loads in flight together), 16 R rows a workgroup. A row's slots meet its classes in
+// LDS: log p of every class, and {q, slot} of the slot that named it last; as many owned classes as filled slots means that no class was named twice.
+template <int DT, int GDT, int E, int R>
 __global__ __launch_bounds__(256) void td_narrow_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
     typedef typename TdElem<GDT>::T TG;
-    constexpr int E = 4;
-    __shared__ float s_lp[16][64], s_q[16][64];
-    __shared__ int s_own[16][64];
-    const int l = (int)threadIdx.x & 15, r = (int)threadIdx.x >> 4, V = a.V, k = a.k;
-    const int64_t row = (int64_t)blockIdx.x * 16 + r;
-    const bool here = row < a.rows;
-    const T* z;
-    TG* dz;
-    td_row(a, here ? row : 0, z, dz);
-    auto gmax = [](float v) {
+    __shared__ float s_lp[R][16][16 * E];
+    __shared__ float2 s_q[R][16][16 * E];
+    const int lane = (int)threadIdx.x & 63, l = (int)threadIdx.x & 15, r = (int)threadIdx.x >> 4, V = a.V, k = a.k;
+    const uint64_t mine = 0xffffull << (lane & 48);
+    float v[R][E], tx[R][E], w[R];
+    int ti[R][E];
 #pragma unroll
-        for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-        return v;
-    };
-    auto gsum = [](float v) {
+    for (int i = 0; i < R; ++i) {
+        const int64_t row = ((int64_t)blockIdx.x * R + i) * 16 + r;
+        const bool here = row < a.rows;
+        const T* z;
+        TG* dz;
+        td_row(a, here ? row : 0, z, dz);
+        w[i] = a.drow && here ? a.drow[row] : 1.f;
 #pragma unroll
-        for (int o = 8; o; o >>= 1) v += __shfl_xor(v, o);
-        return v;
-    };
-    float v[E], tx[E];
-    int ti[E];
-    float m = -INFINITY, tm = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        v[e] = here && e * 16 + l < V ? TdElem<DT>::get(z[e * 16 + l]) : -INFINITY;
-        const int j = e * 16 + l;
-        ti[e] = -1;
-        tx[e] = -INFINITY;
-        if (here && j < k) {
-            const int c = a.idx[row * k + j];
-            ti[e] = (unsigned)c < (unsigned)V ? c : -1;
-            if (ti[e] >= 0) tx[e] = load_elem(a.val, row * k + j, a.vdt) * a.itau;
+        for (int e = 0; e < E; ++e) {
+            const int j = e * 16 + l;
+            v[i][e] = here && j < V ? TdElem<DT>::get(z[j]) : -INFINITY;
+            ti[i][e] = here && j < k ? a.idx[row * k + j] : -1;
+            tx[i][e] = here && j < k ? load_elem(a.val, row * k + j, a.vdt) : 0.f;
         }
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        m = fmaxf(m, v[e]);
-        tm = fmaxf(tm, tx[e]);
-    }
-    m = gmax(m);
-    tm = gmax(tm);
-    const float mu = __builtin_isinf(m) ? 0.f : m;
-    const bool on = tm != -INFINITY && m != -INFINITY;
-    float s = 0.f, ts = 0.f;
-    float p[E], lq[E];
+    for (int i = 0; i < R; ++i) {
+        float m = -INFINITY, tm = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        lq[e] = tx[e] - tm;
-        if (ti[e] >= 0) ts += expf(lq[e]);
-        v[e] = (v[e] - mu) * a.c;
-        p[e] = __builtin_amdgcn_exp2f(v[e]);
-        s += p[e];
-    }
-    s = gsum(s);
-    ts = gsum(ts);
-    const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s), lts = logf(ts);
-    float q[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        lq[e] -= lts;
-        q[e] = ti[e] >= 0 ? expf(lq[e]) : 0.f;
-        if (e * 16 < V) {
-            s_lp[r][e * 16 + l] = (v[e] - l2s) * kTdLn2;
-            s_q[r][e * 16 + l] = 0.f;
+        for (int e = 0; e < E; ++e) {
+            if ((unsigned)ti[i][e] >= (unsigned)V) ti[i][e] = -1;
+            tx[i][e] = ti[i][e] >= 0 ? tx[i][e] * a.itau : -INFINITY;
+            m = fmaxf(m, v[i][e]);
+            tm = fmaxf(tm, tx[i][e]);
         }
-    }
-    td_sync<1>();  // (a row's 16 lanes are in one wave)
-    float sum = 0.f;
-    bool twice = false;
+        m = td_row16<true>(m);
+        tm = td_row16<true>(tm);
+        const float mu = __builtin_isinf(m) ? 0.f : m;
+        const bool on = tm != -INFINITY && m != -INFINITY;
+        float s = 0.f, ts = 0.f, p[E], lq[E], q[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (ti[e] >= 0) {
-            if (q[e] != 0.f) sum += q[e] * (lq[e] - s_lp[r][ti[e]]);
-            s_own[r][ti[e]] = e * 16 + l;
-            s_q[r][ti[e]] = q[e];
+        for (int e = 0; e < E; ++e) {
+            lq[e] = (tx[i][e] - tm) * kTdLog2e;
+            q[e] = ti[i][e] >= 0 ? __builtin_amdgcn_exp2f(lq[e]) : 0.f;
+            ts += q[e];
+            v[i][e] = (v[i][e] - mu) * a.c;
+            p[e] = __builtin_amdgcn_exp2f(v[i][e]);
+            s += p[e];
         }
-    td_sync<1>();
+        s = td_row16<false>(s);
+        ts = td_row16<false>(ts);
+        const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s), itq = 1.f / ts, lts = __builtin_amdgcn_logf(ts);
+        int filled = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (ti[e] >= 0 && s_own[r][ti[e]] != e * 16 + l) twice = true;
-    sum = gsum(sum);
-    float qs[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) qs[e] = e * 16 < V ? s_q[r][e * 16 + l] : 0.f;
-    if (__ballot(twice)) {  // some class of these rows is named twice: add its slots up in their order
-#pragma unroll
-        for (int e = 0; e < E; ++e) qs[e] = 0.f;
-        for (int j = 0; j < k; ++j) {
-            const int src = ((int)threadIdx.x & 48) + (j & 15);
-            int c = -1;
-            float qj = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int ce = __shfl(ti[e], src);
-                const float qe = __shfl(q[e], src);
-                if (j >> 4 == e) {
-                    c = ce;
-                    qj = qe;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) qs[e] += c == e * 16 + l ? qj : 0.f;
+        for (int e = 0; e < E; ++e) {
+            lq[e] -= lts;
+            q[e] *= itq;
+            s_lp[i][r][e * 16 + l] = v[i][e] - l2s;
+            s_q[i][r][e * 16 + l] = float2{0.f, -1.f};
+            filled += __popcll(__ballot(ti[i][e] >= 0) & mine);
         }
-    }
-    if (!here) return;
-    const float g = a.gs * (a.drow ? a.drow[row] : 1.f);
-    if (dz) {
+        td_sync<1>();  // (a row's 16 lanes are in one wave)
+        float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            if (e * 16 + l < V) dz[e * 16 + l] = TdElem<GDT>::put(on ? (p[e] * inv - qs[e]) * g : 0.f);
+            if (ti[i][e] >= 0) {
+                if (q[e] != 0.f) sum += q[e] * (lq[e] - s_lp[i][r][ti[i][e]]);
+                s_q[i][r][ti[i][e]] = float2{q[e], (float)(e * 16 + l)};
+            }
+        td_sync<1>();
+        sum = td_row16<false>(sum) * kTdLn2;
+        float qs[E];
+        int owned = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float2 o = s_q[i][r][e * 16 + l];
+            qs[e] = o.x;
+            owned += __popcll(__ballot(o.y >= 0.f) & mine);
+        }
+        if (__ballot(owned != filled)) {  // some class of these rows is named twice: add its slots up in their order
+#pragma unroll
+            for (int e = 0; e < E; ++e) qs[e] = 0.f;
+            for (int j = 0; j < k; ++j) {
+                const int src = (lane & 48) + (j & 15);
+                int c = -1;
+                float qj = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int ce = __shfl(ti[i][e], src);
+                    const float qe = __shfl(q[e], src);
+                    if (j >> 4 == e) {
+                        c = ce;
+                        qj = qe;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) qs[e] += c == e * 16 + l ? qj : 0.f;
+            }
+        }
+        const int64_t row = ((int64_t)blockIdx.x * R + i) * 16 + r;
+        if (row < a.rows) {
+            const float g = a.gs * w[i];
+            const T* z;
+            TG* dz;
+            td_row(a, row, z, dz);
+            if (dz) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (e * 16 + l < V) dz[e * 16 + l] = TdElem<GDT>::put(on ? (p[e] * inv - qs[e]) * g : 0.f);
+            }
+            if (l == 0) a.loss[row] = on ? sum * a.tau2 : 0.f;
+        }
     }
-    if (l == 0) a.loss[row] = on ? sum * a.tau2 : 0.f;
 }
 
 template <int DT, int GDT>
 static int td_launch(const TdArgs& a, hipStream_t s) {
     const size_t lds = (size_t)a.k * 16;
-    if (a.V <= 64 && a.k <= 64) td_narrow_kernel<DT, GDT><<<dim3((unsigned)((a.rows + 15) / 16)), dim3(256), 0, s>>>(a);
-    else if (a.V <= 2048) td_wide_kernel<DT, GDT, 1><<<dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 4 * lds, s>>>(a);
+    const int narrow = a.V > a.k ? a.V : a.k;
+    if (narrow <= 16) td_narrow_kernel<DT, GDT, 1, 4><<<dim3((unsigned)((a.rows + 63) / 64)), dim3(256), 0, s>>>(a);
+    else if (narrow <= 64) td_narrow_kernel<DT, GDT, 4, 1><<<dim3((unsigned)((a.rows + 15) / 16)), dim3(256), 0, s>>>(a);
+    else if (a.V <= 2048) td_wave_kernel<DT, GDT><<<dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 4 * (lds + ((a.V + 7) & ~7) * 4), s>>>(a);
     else if (a.V <= 8192) td_wide_kernel<DT, GDT, 4><<<dim3((unsigned)a.rows), dim3(256), lds, s>>>(a);
+    else if (a.V <= 16384) td_wide_kernel<DT, GDT, 8><<<dim3((unsigned)a.rows), dim3(512), lds, s>>>(a);
     else if (a.V <= 32768) td_wide_kernel<DT, GDT, 16><<<dim3((unsigned)a.rows), dim3(1024), lds, s>>>(a);
+    else if (DT != CDET_F32 && a.V <= 65536) td_held_kernel<DT, GDT, 8><<<dim3((unsigned)a.rows), dim3(1024), lds, s>>>(a);
+    else if (a.V <= (DT == CDET_F32 ? 65536 : 131072)) td_held_kernel<DT, GDT, 16><<<dim3((unsigned)a.rows), dim3(1024), lds, s>>>(a);
     else td_long_kernel<DT, GDT><<<dim3((unsigned)a.rows), dim3(1024), lds, s>>>(a);
     CDET_LAUNCH_CHECK();
     return 0;

@@ -320,8 +320,8 @@ def check_map(got, z, idx, val, tau, drow):
     assert torch.all(err <= tol), (err / tol).max().item()
 
 
-MAP_SIZES = [(1, 1, 1, 1), (1, 1, 2, 2), (7, 1, 16, 16), (33, 4, 16, 16), (50, 4, 13, 5), (20, 1, 64, 64), (20, 1, 65, 64), (9, 1, 64, 65), (40, 1, 80, 10),
-             (13, 1, 1203, 32), (6, 2, 2048, 100), (5, 1, 2049, 40), (3, 1, 8191, 512), (3, 1, 8193, 7), (2, 1, 32768, 64), (2, 1, 32769, 64), (2, 1, 100003, 30)]
+MAP_SIZES = [(1, 1, 1, 1), (1, 1, 2, 2), (7, 1, 16, 16), (300, 4, 16, 9), (70, 1, 17, 5), (65, 1, 3, 17), (33, 4, 16, 16), (50, 4, 13, 5), (20, 1, 64, 64), (20, 1, 65, 64), (9, 1, 64, 65), (40, 1, 80, 10),
+             (13, 1, 1203, 32), (6, 2, 2048, 100), (5, 1, 2049, 40), (3, 1, 8191, 512), (3, 1, 8193, 7), (2, 1, 16385, 33), (2, 1, 32768, 64), (2, 1, 32769, 64), (2, 1, 65537, 64), (2, 1, 100003, 30), (2, 1, 131073, 9)]
 
 
 @pytest.mark.parametrize("dtype,gdt", [(F32, F32), (BF, BF), (F16, F16), (BF, F32), (F16, F32)])
@@ -339,7 +339,7 @@ def test_topk_distill(P, G, V, k, dtype, gdt):
         assert torch.equal(two[0], got[0][:, 0]) and torch.equal(two[1], got[1][:, 0])
 
 
-@pytest.mark.parametrize("V,k", [(40, 12), (1000, 20), (5000, 20), (9000, 20), (40000, 20)])
+@pytest.mark.parametrize("V,k", [(16, 12), (40, 12), (1000, 20), (1000, 100), (5000, 20), (9000, 20), (40000, 20), (140000, 20)])
 def test_topk_distill_odd_values(V, k):
     """The same class in many slots, -inf logits, rows of nothing but -inf, rows without a teacher that hold NaN, far logits."""
     z = 2 * _rand(12, V, seed=50)
