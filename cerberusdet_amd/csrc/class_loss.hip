@@ -9,7 +9,7 @@
 // into dz (16-bit, one [N, piece] buffer), and one launch computes the piece's dw and adds the piece to dx. dz is relative to the largest row gradient
 // (class_prep_kernel): p of a 10^5-class list times 1 / N is far below fp16's smallest number.
 //
-// One product kernel for all three (gemm_tile): an 8-wave workgroup, 256 x 256 (or 128 x 128) outputs, K in steps of 32 through a ring of four LDS
+// One product for all three (Pipe): an 8-wave workgroup, 256 x 256 (or 128 x 128) outputs, K in steps of 32 through a ring of four LDS
 // stages filled by LDS-DMA. The two halves of the workgroup run half a step apart: while one multiplies, the other reads its fragments.
 // Operand "A" (fragment rows) is what must come out contiguous: a lane ends up with four consecutive A rows of one B row. So A = classes in the first
 // product (a lane holds classes of ONE row of x: the softmax statistics are sums inside the lane), A = features in the other two. An operand whose
@@ -47,54 +47,71 @@ __device__ __forceinline__ int xcd_order(int b, int n) {  // consecutive logical
     return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + j;
 }
 
-// An operand of a tile: p points at the tile's first element. TR = false: rows of K-contiguous elements, [row][k]; TR = true: [k][row].
-struct TileSrc {
-    const uint16_t* p;
-    int64_t ld;
-    int rows;  // valid rows from p on (the rest reads as zero); a multiple of 8 when TR
-};
-
-// acc[mt][nt] += A B^T over K (any K; K % 8 == 0 for the K-contiguous operands). C row of register i: grp * MT*32 + mt*32 + 8*(i>>2) + 4*(lane>>5) + (i&3);
-// C column: wave * NT*32 + nt*32 + (lane&31). Ends with every wave past its last LDS access.
-template <int DT, int MT, int NT, bool ATR, bool BTR>
-__device__ __forceinline__ void gemm_tile(unsigned char* smem, TileSrc A, TileSrc B, int K, f32x16 (&acc)[MT][NT]) {
-    constexpr int ABYTES = MT * 64 * 64, BBYTES = NT * 128 * 64, STAGE = ABYTES + BBYTES;
-    constexpr int NA = MT / 2, NB = NT, NPW = NA + NB;  // DMA instructions (1 KiB) of a wave per step
-    const int tid = (int)threadIdx.x, lane = tid & 63;
-    const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int grp = wave8 >> 2, wave = wave8 & 3;
-    const int l31 = lane & 31, h = lane >> 5;
-    const int steps = (K + LBK - 1) / LBK;
-
-    // DMA sources. K-contiguous: piece `id` = rows 16 id .. +15, four lanes (64 B) a row, 16-byte slot s of row r stored at s ^ ((r >> 2) & 3): the 16
-    // lanes that one ds_read_b128 cycle serves then cover the 16 slots of 256 bytes. Transposed: piece `id` = 64 rows x 8 k, eight lanes (128 B) a k;
-    // slot s of k stored at s ^ (4 * ((k >> 1) & 1)): the four k of a transpose read, and its two 16-row halves, fall into different banks.
+// The staged stream of a workgroup's tiles and the multiplications on it. acc[mt][nt] = A B^T over K (any K; K % 8 == 0 for K-contiguous operands); C row of
+// register i: grp * MT*32 + mt*32 + 8*(i>>2) + 4*(lane>>5) + (i&3), C column: wave * NT*32 + nt*32 + (lane&31). The stream runs three stages ahead of the
+// multiplications, across the end of a tile: what `next` opens is fetched while the last tile is finished and its results are stored.
+// WALK = false: one tile only, without the branches of the crossing (a step of the small tile is short enough to feel them).
+template <int DT, int MT, int NT, bool ATR, bool BTR, bool WALK>
+struct Pipe {
+    static constexpr int ABYTES = MT * 64 * 64, BBYTES = NT * 128 * 64, STAGE = ABYTES + BBYTES;
+    static constexpr int NA = MT / 2, NB = NT, NPW = NA + NB;  // DMA instructions (1 KiB) of a wave per step
+    unsigned char* smem;
+    int lane, wave8, grp, wave, aoff, boff;
     unsigned va[NA], vb[NB];
     int ka[NA], kb[NB];  // the lane's first k of the piece
+    const uint16_t *ap, *bp;
+    int64_t astep, bstep;
+    int krem;            // K of the opened tile left to be fetched
+    int fslot, rslot;    // stages to be written / read next (byte offsets)
+    int sure;            // memory phases whose next stage is known to be there
+
+    __device__ __forceinline__ void init(unsigned char* s, int64_t a_ld, int64_t b_ld) {
+        smem = s;
+        const int tid = (int)threadIdx.x;
+        lane = tid & 63;
+        wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
+        grp = wave8 >> 2;
+        wave = wave8 & 3;
+        const int l31 = lane & 31, h = lane >> 5;
+        // DMA sources. K-contiguous: piece `id` = rows 16 id .. +15, four lanes (64 B) a row, 16-byte slot s of row r stored at s ^ ((r >> 2) & 3): the 16
+        // lanes that one ds_read_b128 cycle serves then cover the 16 slots of 256 bytes. Transposed: piece `id` = 64 rows x 8 k, eight lanes (128 B) a k;
+        // slot s of k stored at s ^ (4 * ((k >> 1) & 1)): the four k of a transpose read, and its two 16-row halves, fall into different banks.
 #pragma unroll
-    for (int i = 0; i < NA; ++i) {
-        const int id = wave8 + 8 * i;
-        const int k = ATR ? 8 * (id & 3) + (lane >> 3) : 8 * ((lane & 3) ^ ((lane >> 4) & 3));
-        const int row = ATR ? (id >> 2) * 64 + 8 * ((lane & 7) ^ (((lane >> 4) & 1) << 2)) : 16 * id + (lane >> 2);
-        ka[i] = row < A.rows ? k : 0x40000000;
-        va[i] = ATR ? (unsigned)(k * A.ld + row) * 2u : (unsigned)(row * A.ld + k) * 2u;
-    }
+        for (int i = 0; i < NA; ++i) va[i] = ATR ? (unsigned)(k_of(ATR, i) * a_ld + row_of(ATR, i)) * 2u : (unsigned)(row_of(ATR, i) * a_ld + k_of(ATR, i)) * 2u;
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        const int id = wave8 + 8 * i;
-        const int k = BTR ? 8 * (id & 3) + (lane >> 3) : 8 * ((lane & 3) ^ ((lane >> 4) & 3));
-        const int row = BTR ? (id >> 2) * 64 + 8 * ((lane & 7) ^ (((lane >> 4) & 1) << 2)) : 16 * id + (lane >> 2);
-        kb[i] = row < B.rows ? k : 0x40000000;
-        vb[i] = BTR ? (unsigned)(k * B.ld + row) * 2u : (unsigned)(row * B.ld + k) * 2u;
+        for (int i = 0; i < NB; ++i) vb[i] = BTR ? (unsigned)(k_of(BTR, i) * b_ld + row_of(BTR, i)) * 2u : (unsigned)(row_of(BTR, i) * b_ld + k_of(BTR, i)) * 2u;
+        astep = ATR ? LBK * a_ld : LBK;
+        bstep = BTR ? LBK * b_ld : LBK;
+        const int trl = (8 * h + ((lane & 15) >> 2)) * 128 + (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ (((lane >> 3) & 1) << 2)) << 4) + (lane & 1) * 8;
+        const int nrl = l31 * 64 + ((h ^ ((l31 >> 2) & 3)) << 4);
+        aoff = ATR ? trl + grp * (MT / 2) * 4096 : nrl + grp * MT * 2048;
+        boff = ABYTES + (BTR ? (trl ^ (((wave * NT) & 1) << 6)) + ((wave * NT) >> 1) * 4096 : nrl + wave * NT * 2048);
+        fslot = rslot = sure = 0;
     }
-    const int64_t astep = ATR ? LBK * A.ld : LBK, bstep = BTR ? LBK * B.ld : LBK;
-    const uint16_t *ap = A.p, *bp = B.p;
-    int krem = K;  // K left from the next step to be fetched on: <= 0 beyond the end, where every lane fetches zeros and the counts stay the same
-    int fslot = 0;
-    auto fetch = [&]() {
+    __device__ __forceinline__ int k_of(bool tr, int i) const {
+        const int id = wave8 + 8 * i;
+        return tr ? 8 * (id & 3) + (lane >> 3) : 8 * ((lane & 3) ^ ((lane >> 4) & 3));
+    }
+    __device__ __forceinline__ int row_of(bool tr, int i) const {
+        const int id = wave8 + 8 * i;
+        return tr ? (id >> 2) * 64 + 8 * ((lane & 7) ^ (((lane >> 4) & 1) << 2)) : 16 * id + (lane >> 2);
+    }
+    // the tile that is fetched from now on (rows beyond a_rows / b_rows, and everything beyond K, read as zero; a_rows 0: nothing is read)
+    __device__ __forceinline__ void open(const uint16_t* a, int a_rows, const uint16_t* b, int b_rows, int K) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) ka[i] = row_of(ATR, i) < a_rows ? k_of(ATR, i) : 0x40000000;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) kb[i] = row_of(BTR, i) < b_rows ? k_of(BTR, i) : 0x40000000;
+        ap = a;
+        bp = b;
+        krem = K;
+    }
+    template <class Next>
+    __device__ __forceinline__ void fetch(Next&& next) {
+        if (WALK && krem <= 0) next();
         const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)ap, 0, LCAP, 0x00020000);
         const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)bp, 0, LCAP, 0x00020000);
-        unsigned char* dst = smem + fslot * STAGE + wave8 * 1024;
+        unsigned char* dst = smem + fslot + wave8 * 1024;
 #pragma unroll
         for (int i = 0; i < NA; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(dst + i * 8192), 16, (int)(ka[i] < krem ? va[i] : LSENT), 0, 0, 0);
@@ -104,106 +121,123 @@ __device__ __forceinline__ void gemm_tile(unsigned char* smem, TileSrc A, TileSr
         ap += astep;
         bp += bstep;
         krem -= LBK;
-        fslot = (fslot + 1) & (LRING - 1);
-    };
-
-    // fragment addresses
-    const int trl = (8 * h + ((lane & 15) >> 2)) * 128 + (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ (((lane >> 3) & 1) << 2)) << 4) + (lane & 1) * 8;
-    const int nrl = l31 * 64 + ((h ^ ((l31 >> 2) & 3)) << 4);
-    const int aoff = ATR ? trl + grp * (MT / 2) * 4096 : nrl + grp * MT * 2048;
-    const int boff = ABYTES + (BTR ? (trl ^ (((wave * NT) & 1) << 6)) + ((wave * NT) >> 1) * 4096 : nrl + wave * NT * 2048);
-    auto frag_n = [&](int base, int t, int kk) { return *reinterpret_cast<const u32x4*>(smem + ((base + t * 2048) ^ (kk << 5))); };
-    // transpose reads are asm: in front of the builtin the compiler waits for every DMA in flight. Valid behind the phase's own wait (landed())
-    const int lds0 = (int)(unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
-    auto frag_t = [&](int base, int t, int kk, u32x2& lo, u32x2& hi) {
-        const int o = lds0 + (((base + (t >> 1) * 4096) ^ ((t & 1) << 6)) + kk * 2048);
-        asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(lo) : "v"(o));
-        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:512" : "=v"(hi) : "v"(o));
-    };
-
-    fetch();
-    fetch();
-    fetch();
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NPW) : "memory");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    if (grp == 1) {  // half a step behind from here to the end of the loop
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
+        fslot = fslot + STAGE == LRING * STAGE ? 0 : fslot + STAGE;
     }
-    int so = 0;
-    for (int st = 0; st < steps; ++st) {
-        u32x4 a[2][MT], b[2][NT];
-        u32x2 al[2][MT], ah[2][MT], bl[2][NT], bh[2][NT];
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                if (BTR) frag_t(so + boff, i, kk, bl[kk][i], bh[kk][i]);
-                else b[kk][i] = frag_n(so + boff, i, kk);
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                if (ATR) frag_t(so + aoff, i, kk, al[kk][i], ah[kk][i]);
-                else a[kk][i] = frag_n(so + aoff, i, kk);
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        // stage st + 3 goes where stage st - 1 was: its last reader, the other half in ITS memory phase of step st - 1, waited for its reads before the
-        // barrier that opened this phase
-        fetch();
-        so = so + STAGE == LRING * STAGE ? 0 : so + STAGE;
-        __builtin_amdgcn_sched_barrier(0);
-        // stage st + 1 has landed for this wave (two stages stay in flight); the fragments are in registers
+    template <class Next>
+    __device__ __forceinline__ void prime(Next&& next) {
+        fetch(next);
+        fetch(next);
+        fetch(next);
+    }
+    __device__ __forceinline__ void start() {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * NPW) : "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        // (the registers of the transpose reads become values here, behind the wait)
+    }
+    __device__ __forceinline__ u32x4 frag_n(int base, int t, int kk) const { return *reinterpret_cast<const u32x4*>(smem + ((base + t * 2048) ^ (kk << 5))); }
+    // transpose reads are asm: in front of the builtin the compiler waits for every DMA in flight. Their registers become values behind the phase's own wait
+    __device__ __forceinline__ void frag_t(int base, int t, int kk, u32x2& lo, u32x2& hi) const {
+        const int o = (int)(unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem + (((base + (t >> 1) * 4096) ^ ((t & 1) << 6)) + kk * 2048);
+        asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(lo) : "v"(o));
+        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:512" : "=v"(hi) : "v"(o));
+    }
+
+    // One tile. A step of a wave is a memory phase (fragment reads, one stage fetched) and a compute phase, each closed by a barrier; waves 4-7 run one phase
+    // behind waves 0-3. Every wave returns past its last read of the tile's last stage, whose slot, free(), nobody touches before the next fetch().
+    template <class Next>
+    __device__ __forceinline__ void run(int steps, f32x16 (&acc)[MT][NT], Next&& next) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            if (ATR) {
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    asm volatile("" : "+v"(al[kk][i]), "+v"(ah[kk][i]));
-                    a[kk][i] = u32x4{al[kk][i][0], al[kk][i][1], ah[kk][i][0], ah[kk][i][1]};
-                }
-            }
-            if (BTR) {
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        if (grp == 1) {
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        for (int st = 0; st < steps; ++st) {
+            u32x4 a[2][MT], b[2][NT];
+            u32x2 al[2][MT], ah[2][MT], bl[2][NT], bh[2][NT];
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    asm volatile("" : "+v"(bl[kk][i]), "+v"(bh[kk][i]));
-                    b[kk][i] = u32x4{bl[kk][i][0], bl[kk][i][1], bh[kk][i][0], bh[kk][i][1]};
+                    if (BTR) frag_t(rslot + boff, i, kk, bl[kk][i], bh[kk][i]);
+                    else b[kk][i] = frag_n(rslot + boff, i, kk);
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    if (ATR) frag_t(rslot + aoff, i, kk, al[kk][i], ah[kk][i]);
+                    else a[kk][i] = frag_n(rslot + aoff, i, kk);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            // stage st + 3 goes where stage st - 1 was: its last reader, the other half in ITS memory phase of step st - 1, waited for its reads before
+            // the barrier that opened this phase
+            fetch(next);
+            rslot = rslot + STAGE == LRING * STAGE ? 0 : rslot + STAGE;
+            __builtin_amdgcn_sched_barrier(0);
+            // stage st + 1 has landed for this wave (two stages stay in flight); the fragments are in registers
+            if (WALK && sure > 0) {
+                --sure;
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            } else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * NPW) : "memory");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                if (ATR) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        asm volatile("" : "+v"(al[kk][i]), "+v"(ah[kk][i]));
+                        a[kk][i] = u32x4{al[kk][i][0], al[kk][i][1], ah[kk][i][0], ah[kk][i][1]};
+                    }
+                }
+                if (BTR) {
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        asm volatile("" : "+v"(bl[kk][i]), "+v"(bh[kk][i]));
+                        b[kk][i] = u32x4{bl[kk][i][0], bl[kk][i][1], bh[kk][i][0], bh[kk][i][1]};
+                    }
+                }
+            }
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] = lmfma<DT>(a[kk][i], b[kk][j], acc[i][j]);
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (st + 1 < steps) {
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = lmfma<DT>(a[kk][i], b[kk][j], acc[i][j]);
-        __builtin_amdgcn_s_setprio(0);
-        __builtin_amdgcn_sched_barrier(0);
-        if (st + 1 < steps) {
+        if (grp == 0) {  // releases the other half into its last multiplication
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    if (grp == 0) {  // releases the other half into its last multiplication
+    __device__ __forceinline__ unsigned char* free_slot() const { return smem + (rslot == 0 ? (LRING - 1) * STAGE : rslot - STAGE); }
+    // before the tile's stores (they count like loads): the three stages in flight land, so that the next two memory phases need not wait behind the stores
+    __device__ __forceinline__ void settle() {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        sure = 2;
+    }
+    __device__ __forceinline__ void sync() {  // every wave is done with free_slot(), and with its share of the stages in flight
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the (empty) trailing fetches write zeros into the ring: done before anybody reuses it
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-}
+    __device__ __forceinline__ void drain() {  // after the last tile: the (empty) fetches in flight write zeros into the ring; then the LDS is free
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+};
 
 // ---- first product: logits of a tile of classes x rows ------------------------------------------------------------------------------------------
 struct LogitArgs {
@@ -231,159 +265,246 @@ __device__ __forceinline__ int64_t load_label(const void* p, int is64, int r) {
     return is64 ? reinterpret_cast<const int64_t*>(p)[r] : (int64_t)reinterpret_cast<const int32_t*>(p)[r];
 }
 
-// wave-private staging of 32 C columns x (MT*32) C rows of 16-bit values as whole rows of the destination
-template <int DT, int MT>
-__device__ __forceinline__ void store_rows16(unsigned char* stg, const uint2 (&pk)[MT][4], int lane, uint16_t* dst, int64_t ld, int nrows, int ncols) {
-    constexpr int RS = MT * 64 + 16, CH = MT * 4;  // +16: consecutive rows start in different banks
+// 32 C columns x (HT*32) C rows of 16-bit values through `stg` (wave-private, HT * 2 KiB) as whole rows of the destination: pk[i][q] = the lane's rows
+// 32 i + 8 q + 4 h .. +3 of column l31
+template <int HT>
+__device__ __forceinline__ void store_rows16(unsigned char* stg, const uint2 (&pk)[HT][4], int lane, uint16_t* dst, int64_t ld, int nrows, int ncols) {
+    constexpr int RS = HT * 64, CH = HT * 4;  // 16-byte chunk c of row r is kept at c ^ swz(r)
+    auto swz = [](int r) { return CH == 8 ? r & 7 : (r >> 1) & 3; };
     const int l31 = lane & 31, h = lane >> 5;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < HT; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) *reinterpret_cast<uint2*>(stg + l31 * RS + (i * 32 + q * 8 + h * 4) * 2) = pk[i][q];
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<uint2*>(stg + l31 * RS + (((i * 4 + q) ^ swz(l31)) << 4) + h * 8) = pk[i][q];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int it = 0; it < 32 * CH / 64; ++it) {
         const int id = it * 64 + lane, row = id / CH, ch = id % CH;
-        const u32x4 v = *reinterpret_cast<const u32x4*>(stg + row * RS + ch * 16);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(stg + row * RS + ((ch ^ swz(row)) << 4));
         if (row < nrows && ch * 8 < ncols) *reinterpret_cast<u32x4*>(dst + row * ld + ch * 8) = v;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
-
+// column tile j of the accumulators times f, in halves of MT / 2 row tiles
 template <int DT, int MT, int NT>
-__device__ __forceinline__ void store_scaled(unsigned char* stg, const f32x16 (&acc)[MT][NT], int j, float os, int lane, uint16_t* dst, int64_t ld, int nrows,
-                                             int ncols) {
-    uint2 pk[MT][4];
+__device__ __forceinline__ void store_scaled(unsigned char* stg, const f32x16 (&acc)[MT][NT], int j, float f, int lane, uint16_t* dst, int64_t ld, int nrows, int ncols) {
+    constexpr int HT = MT / 2;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int half = 0; half < 2; ++half) {
+        uint2 pk[HT][4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            pk[i][q].x = lpack2<DT>(acc[i][j][4 * q] * os, acc[i][j][4 * q + 1] * os);
-            pk[i][q].y = lpack2<DT>(acc[i][j][4 * q + 2] * os, acc[i][j][4 * q + 3] * os);
-        }
-    store_rows16<DT, MT>(stg, pk, lane, dst, ld, nrows, ncols);
+        for (int i = 0; i < HT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x16& c = acc[half * HT + i][j];
+                pk[i][q].x = lpack2<DT>(c[4 * q] * f, c[4 * q + 1] * f);
+                pk[i][q].y = lpack2<DT>(c[4 * q + 2] * f, c[4 * q + 3] * f);
+            }
+        store_rows16<HT>(stg, pk, lane, dst + half * HT * 32, ld, nrows, ncols - half * HT * 32);
+    }
 }
 
+// The large tile's workgroups are persistent, one a CU: each walks its tiles, the next tile's first stages in flight under the epilogue (4096 x 65536 x 640
+// bf16: 363 -> 327 us forward). A launch of the small tile has one tile a workgroup and skips that bookkeeping (96 x 365 x 320: 8.4 us with it, 6.3 without).
+// Panels of 8 row tiles; an XCD's workgroups take neighbouring tiles: together 8 row tiles x 4 class tiles at a time, whose operands its L2 hands out.
 template <int DT, int MT, int NT, bool BWD>
 __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_logits_kernel(const LogitArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr int BM = MT * 64, BN = NT * 128, GR = 8;
-    const int tid = (int)threadIdx.x, lane = tid & 63;
-    const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int grp = wave8 >> 2, wave = wave8 & 3, l31 = lane & 31, h = lane >> 5;
-    // panels of 8 row tiles: the 32 workgroups that an XCD runs at a time share 8 row tiles and 4 class tiles
-    const int L = xcd_order((int)blockIdx.x, (int)gridDim.x);
-    const int panel = L / (GR * a.ntv), pr0 = panel * GR, pw = min(GR, a.ntr - pr0), in = L - panel * GR * a.ntv;
-    const int tv = in / pw, tr = pr0 + in % pw;
-    const int v0 = tv * BM, r0 = tr * BN;
-
-    f32x16 acc[MT][NT];
-    gemm_tile<DT, MT, NT, false, false>(smem, TileSrc{a.w + (int64_t)v0 * a.w_ld, a.w_ld, a.V - v0}, TileSrc{a.x + (int64_t)r0 * a.x_ld, a.x_ld, a.N - r0}, a.d, acc);
-
-    // class offsets of the tile in LDS (log2 units; -inf: left out, or behind the last class)
-    float* offs = reinterpret_cast<float*>(smem);
-    int* any = reinterpret_cast<int*>(smem + BM * 4);
-    if (tid == 0) *any = 0;
-    __syncthreads();
-    if (tid < BM) {
-        const int v = v0 + tid;
-        float o = -INFINITY;
-        if (v < a.V) {
-            o = a.off ? a.off[v] * a.coff : 0.f;
-            if (o == -INFINITY) *any = 1;
+    constexpr bool WALK = MT == 4;
+    const int ntiles = a.ntv * a.ntr;
+    int L, end, per = 1;
+    if (WALK) {
+        const int nwg = (int)gridDim.x, xcd = (int)blockIdx.x & 7;
+        per = (nwg - xcd + 7) >> 3;  // workgroups of this XCD
+        const int q8 = ntiles >> 3, r8 = ntiles & 7;
+        const int first = xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8;
+        end = first + q8 + (xcd < r8 ? 1 : 0);
+        L = first + ((int)blockIdx.x >> 3);
+        if (L >= end) return;
+    } else {
+        L = xcd_order((int)blockIdx.x, (int)gridDim.x);
+        end = L + 1;
+    }
+    int v0, r0;                      // of the tile that is multiplied
+    auto place = [&](int t, int& v, int& r) {
+        const int panel = t / (GR * a.ntv), pr0 = panel * GR, pw = min(GR, a.ntr - pr0), in = t - panel * GR * a.ntv;
+        v = in / pw * BM;
+        r = (pr0 + in % pw) * BN;
+    };
+    place(L, v0, r0);
+    Pipe<DT, MT, NT, false, false, WALK> p;
+    p.init(smem, a.w_ld, a.x_ld);
+    int F = L;                       // the tile that is fetched
+    auto open = [&]() {
+        int v = v0, r = r0;
+        const bool more = F < end;
+        if (WALK && more && F != L) place(F, v, r);
+        p.open(a.w + (int64_t)v * a.w_ld, more ? a.V - v : 0, a.x + (int64_t)r * a.x_ld, more ? a.N - r : 0, a.d);
+        F += per;
+    };
+    // offsets of a tile's classes in log2 units, -inf for those left out or behind the last, and which of the writing waves met one. Walking: two tables behind
+    // the ring, the next tile's written a tile ahead; else one, in the ring when that has ended
+    constexpr int TABLE = BM + 4, STAGE = Pipe<DT, MT, NT, false, false, WALK>::STAGE;
+    float* table = reinterpret_cast<float*>(smem + LRING * STAGE);
+    const bool writer = a.off && (int)threadIdx.x < BM;
+    auto offset = [&](int t) {
+        int v = v0, r;
+        if (WALK && t != L) place(t, v, r);
+        v += (int)threadIdx.x;
+        return v < a.V ? a.off[v] : -INFINITY;
+    };
+    auto note = [&](float* dst, float o) {
+        o *= a.coff;
+        dst[threadIdx.x] = o;
+        const bool out = __ballot(o == -INFINITY) != 0;
+        if (p.lane == 0) reinterpret_cast<int*>(dst + BM)[p.wave8] = out;
+    };
+    int turn = 0;
+    open();
+    const float o_first = writer ? offset(L) : 0.f;
+    p.prime(open);
+    if (WALK && writer) note(table, o_first);
+    p.start();
+    const int lane = p.lane, l31 = lane & 31, h = lane >> 5, grp = p.grp, wave = p.wave, steps = (a.d + LBK - 1) / LBK;
+    for (;;) {
+        f32x16 acc[MT][NT];
+        p.run(steps, acc, open);
+        if (!WALK && a.off) {
+            p.drain();
+            table = reinterpret_cast<float*>(smem + p.rslot);  // (results are staged in free_slot())
+            if (writer) note(table, o_first);
+            p.sync();
         }
-        offs[tid] = o;
-    }
-    __syncthreads();
-    const float* offw = offs + grp * MT * 32 + 4 * h;
-    if (!BWD && *any) {  // a left-out class counts as nothing whatever its weights hold (0 * inf and NaN stay out)
+        const int vw = v0 + grp * MT * 32;               // the wave's first class
+        unsigned char* stg = p.free_slot() + p.wave8 * (MT * 1024);
+        const float* const offw = table + turn * TABLE + grp * MT * 32;
+        const int* const outs = reinterpret_cast<const int*>(table + turn * TABLE + BM);
+        turn ^= 1;
+        if (WALK && writer && L + per < end) note(table + turn * TABLE, offset(L + per));
+        // classes with an offset, or behind the last one: the logits themselves take the accumulators' place (the product's sign matters to the maximum)
+        float c = a.c;
+        if (a.off || v0 + BM > a.V || (!BWD && c <= 0.f)) {
+            bool out = v0 + BM > a.V;
+            if (a.off)
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const bool out = offw[i * 32 + 8 * (r >> 2) + (r & 3)] == -INFINITY;
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j][r] = out ? 0.f : acc[i][j][r];
-            }
-    }
-    unsigned char* stg = smem + 2048 + wave8 * (32 * (MT * 64 + 16));
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int r = r0 + (wave * NT + j) * 32 + l31;
-        int64_t lab = -1;
-        if (a.label && r < a.N) lab = load_label(a.label, a.label64, r) - a.v_first;
-        const int64_t local64 = lab - v0 - grp * MT * 32;
-        const int local = local64 >= 0 && local64 < MT * 32 ? (int)local64 : -1;
-        const bool mine = local >= 0 && ((local >> 2) & 1) == h;
-        const int slot = ((local >> 3) << 2) | (local & 3);  // (i, q, r & 3) of the lane that holds it
-        if (!BWD) {
-            float m = -INFINITY;
+                for (int i = 0; i < BM / 64; ++i) out = out || outs[i];
+            f32x4 o[MT][4];
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const f32x4 o = *reinterpret_cast<const f32x4*>(offw + i * 32 + q * 8);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float t = fmaf(acc[i][j][4 * q + e], a.c, o[e]);
-                        acc[i][j][4 * q + e] = t;
-                        m = fmaxf(m, t);
-                    }
-                }
-            m = fmaxf(m, __shfl_xor(m, 32));
-            const float mu = __builtin_isinf(m) ? 0.f : m;  // nothing left, or an infinite logit: exp2 of the values themselves
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(acc[i][j][e] - mu);
-            s += __shfl_xor(s, 32);
-            if (__ballot(mine)) {
-                float z = 0.f;
+                for (int q = 0; q < 4; ++q) o[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (a.off) {
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) z = slot == i * 16 + e ? acc[i][j][e] : z;
-                if (mine) a.zlab[r] = z;
+                    for (int q = 0; q < 4; ++q) o[i][q] = *reinterpret_cast<const f32x4*>(offw + i * 32 + q * 8 + h * 4);
             }
-            if (h == 0 && r < a.N) {
-                const int64_t vb = (int64_t)tv * 2 + grp, nvb = (int64_t)a.ntv * 2;
-                a.part[vb * a.N + r] = mu;
-                a.part[(nvb + vb) * a.N + r] = s;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) acc[i][j][4 * q + e] = fmaf(acc[i][j][4 * q + e], c, o[i][q][e]);
+            if (out) {  // -inf whatever the weights hold: 0 * inf and NaN stay out
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool gone = o[i][q][e] == -INFINITY || vw + i * 32 + q * 8 + h * 4 + e >= a.V;
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) acc[i][j][4 * q + e] = gone ? -INFINITY : acc[i][j][4 * q + e];
+                        }
+            }
+            c = 1.f;
+        }
+        if (!BWD) {
+            float mu[NT], s[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                float m = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
+                m = fmaxf(m, __shfl_xor(m, 32)) * c;
+                mu[j] = __builtin_isinf(m) ? 0.f : m;  // nothing left, or an infinite logit: exp2 of the values themselves
+                s[j] = 0.f;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[j] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, -mu[j]));
+                s[j] += __shfl_xor(s[j], 32);
+            }
+            float zl[NT];
+            bool mine[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int r = r0 + (wave * NT + j) * 32 + l31;
+                const int64_t at = a.label && r < a.N ? load_label(a.label, a.label64, r) - vw : -1;
+                mine[j] = at >= 0 && at < MT * 32 && (((int)at >> 2) & 1) == h;
+                zl[j] = 0.f;
+                if (__ballot(mine[j])) {
+                    const int slot = (((int)at >> 3) << 2) | ((int)at & 3);  // (i, q, e) of the lane that holds it
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) zl[j] = slot == i * 16 + e ? acc[i][j][e] : zl[j];
+                }
+            }
+            p.settle();
+            const int64_t vb = (int64_t)(vw / (MT * 32)), nvb = (int64_t)a.ntv * 2;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int r = r0 + (wave * NT + j) * 32 + l31;
+                if (mine[j]) a.zlab[r] = zl[j] * c;
+                if (h == 0 && r < a.N) {
+                    a.part[vb * a.N + r] = mu[j];
+                    a.part[(nvb + vb) * a.N + r] = s[j];
+                }
             }
         } else {
-            const bool live = r < a.N;
-            const float l2 = live ? a.lse2[r] : INFINITY;
-            const float g = live ? a.coef[r] : 0.f;
+            float g[NT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const f32x4 o = *reinterpret_cast<const f32x4*>(offw + i * 32 + q * 8);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * q + e], a.c, o[e]) - l2);
-                }
-            const bool named = mine && offs[grp * MT * 32 + local] != -INFINITY;  // (a left-out class gets no gradient)
-            if (__ballot(named)) {
+            for (int j = 0; j < NT; ++j) {
+                const int r = r0 + (wave * NT + j) * 32 + l31;
+                const bool live = r < a.N;
+                const float l2 = live ? a.lse2[r] : INFINITY;
+                g[j] = live ? a.coef[r] : 0.f;
+                const int64_t at = a.label && live ? load_label(a.label, a.label64, r) - a.v_first - vw : -1;
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[i][j][e] -= named && slot == i * 16 + e ? 1.f : 0.f;
-            }
-            uint2 pk[MT][4];
+                    for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, -l2));
+                bool mine = at >= 0 && at < MT * 32 && vw + at < a.V && (((int)at >> 2) & 1) == h;
+                if (a.off && mine) mine = offw[(int)at] != -INFINITY;  // (a left-out class gets no gradient)
+                if (__ballot(mine)) {
+                    const int slot = (((int)at >> 3) << 2) | ((int)at & 3);
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+                    for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    pk[i][q].x = lpack2<DT>(acc[i][j][4 * q] * g, acc[i][j][4 * q + 1] * g);
-                    pk[i][q].y = lpack2<DT>(acc[i][j][4 * q + 2] * g, acc[i][j][4 * q + 3] * g);
+                        for (int e = 0; e < 16; ++e) acc[i][j][e] -= mine && slot == i * 16 + e ? 1.f : 0.f;
                 }
-            const int rr = r0 + (wave * NT + j) * 32;
-            store_rows16<DT, MT>(stg, pk, lane, a.dz + (int64_t)rr * a.dz_ld + v0 + grp * MT * 32, a.dz_ld, a.dz_rows - rr, MT * 32);
+            }
+            p.settle();
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int rr = r0 + (wave * NT + j) * 32;
+                store_scaled<DT, MT, NT>(stg, acc, j, g[j], lane, a.dz + (int64_t)rr * a.dz_ld + vw, a.dz_ld, a.dz_rows - rr, MT * 32);
+            }
         }
+        L += per;
+        if (!WALK || L >= end) break;
+        p.sync();
+        place(L, v0, r0);
     }
+    p.drain();
 }
 
 // ---- second product of the backward: a piece's dw tiles and dx tiles in one launch -----------------------------------------------------------------
@@ -413,31 +534,45 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_grads_kernel(const
     const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = wave8 >> 2, wave = wave8 & 3, l31 = lane & 31, h = lane >> 5;
     int L = xcd_order((int)blockIdx.x, (int)gridDim.x);
+    unsigned char* stg = smem + wave8 * (MT * 1024);
     f32x16 acc[MT][NT];
     if (L < a.ndw) {  // dw[v][f] = sum_r dz[r][v] x[r][f]
         const int f0 = (L % a.ntd) * BM, v0 = (L / a.ntd) * BN;
-        gemm_tile<DT, MT, NT, true, true>(smem, TileSrc{a.x + f0, a.d, a.d - f0}, TileSrc{a.dz + v0, a.dz_ld, a.vk - v0}, a.rows32, acc);
+        Pipe<DT, MT, NT, true, true, false> p;
+        auto none = []() {};
+        p.init(smem, a.d, a.dz_ld);
+        p.open(a.x + f0, a.d - f0, a.dz + v0, a.vk - v0, a.rows32);
+        p.prime(none);
+        p.start();
+        p.run(a.rows32 / LBK, acc, none);
+        p.drain();
         const float os = *a.outscale;
-        unsigned char* stg = smem + wave8 * (32 * (MT * 64 + 16));
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int v = v0 + (wave * NT + j) * 32, f = f0 + grp * MT * 32;
-            store_scaled<DT, MT>(stg, acc, j, os, lane, a.dw + (int64_t)v * a.dw_ld + f, a.dw_ld, a.Vp - v, a.d - f);
+            store_scaled<DT, MT, NT>(stg, acc, j, os, lane, a.dw + (int64_t)v * a.dw_ld + f, a.dw_ld, a.Vp - v, a.d - f);
         }
         return;
     }
     L -= a.ndw;  // dx[r][f] += sum over the slice's classes of dz[r][v] w[v][f]
     const int f0 = (L % a.ntd) * BM, r0 = (L / a.ntd % a.ntr) * BN, s = L / a.ntd / a.ntr;
-    const int k0 = s * a.kper, k = min(a.kper, a.Vp - k0);
-    gemm_tile<DT, MT, NT, true, false>(smem, TileSrc{a.w + (int64_t)k0 * a.w_ld + f0, a.w_ld, a.d - f0},
-                                       TileSrc{a.dz + (int64_t)r0 * a.dz_ld + k0, a.dz_ld, a.rows32 - r0}, k, acc);
+    const int k0 = s * a.kper, k = max(0, min(a.kper, a.Vp - k0));
+    {
+        Pipe<DT, MT, NT, true, false, false> p;
+        auto none = []() {};
+        p.init(smem, a.w_ld, a.dz_ld);
+        p.open(a.w + (int64_t)k0 * a.w_ld + f0, a.d - f0, a.dz + (int64_t)r0 * a.dz_ld + k0, a.rows32 - r0, k);
+        p.prime(none);
+        p.start();
+        p.run((k + LBK - 1) / LBK, acc, none);
+        p.drain();
+    }
     if (a.dx) {
         const float os = *a.outscale;
-        unsigned char* stg = smem + wave8 * (32 * (MT * 64 + 16));
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int r = r0 + (wave * NT + j) * 32, f = f0 + grp * MT * 32;
-            store_scaled<DT, MT>(stg, acc, j, os, lane, a.dx + (int64_t)r * a.dx_ld + f, a.dx_ld, a.N - r, a.d - f);
+            store_scaled<DT, MT, NT>(stg, acc, j, os, lane, a.dx + (int64_t)r * a.dx_ld + f, a.dx_ld, a.N - r, a.d - f);
         }
         return;
     }
@@ -812,11 +947,12 @@ static int launch_logits(LogitArgs a, int dtype, bool big, hipStream_t s) {
     a.ntr = div_up(a.N, bt);
     const int64_t n = (int64_t)a.ntv * a.ntr;
     CDET_CHECK_ARG(n < ((int64_t)1 << 31), "linear loss: too many tiles");
-#define CDET_GO(DT_, MT_, NT_, LDS_)                                                                       \
+#define CDET_GO(DT_, MT_, NT_, RING_)                                                                      \
     do {                                                                                                   \
+        constexpr size_t LDS_ = RING_ + (MT_ == 4 ? 2 * (MT_ * 64 + 4) * 4 : 0);                                                  \
         static bool once = (allow_lds(class_logits_kernel<DT_, MT_, NT_, BWD>, LDS_), true);               \
         (void)once;                                                                                        \
-        class_logits_kernel<DT_, MT_, NT_, BWD><<<dim3((unsigned)n), dim3(512), LDS_, s>>>(a);             \
+        class_logits_kernel<DT_, MT_, NT_, BWD><<<dim3((unsigned)MT_ == 4 ? std::min<int64_t>(n, 256) : n), dim3(512), LDS_, s>>>(a); \
     } while (0)
     if (dtype == CDET_BF16) {
         if (big) CDET_GO(CDET_BF16, 4, 2, LDS_BIG);
