@@ -15,6 +15,7 @@
 // product (a lane holds classes of ONE row of x: the softmax statistics are sums inside the lane), A = features in the other two. An operand whose
 // memory runs along the output index instead of K is staged as it lies and transposed by ds_read_b64_tr_b16 on the way to the registers.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -50,7 +51,7 @@ __device__ __forceinline__ int xcd_order(int b, int n) {  // consecutive logical
 // The staged stream of a workgroup's tiles and the multiplications on it. acc[mt][nt] = A B^T over K (any K; K % 8 == 0 for K-contiguous operands); C row of
 // register i: grp * MT*32 + mt*32 + 8*(i>>2) + 4*(lane>>5) + (i&3), C column: wave * NT*32 + nt*32 + (lane&31). The stream runs three stages ahead of the
 // multiplications, across the end of a tile: what `next` opens is fetched while the last tile is finished and its results are stored.
-// WALK = false: one tile only, without the branches of the crossing (a step of the small tile is short enough to feel them).
+// WALK = false: one tile only, without the branches of the crossing.
 template <int DT, int MT, int NT, bool ATR, bool BTR, bool WALK>
 struct Pipe {
     static constexpr int ABYTES = MT * 64 * 64, BBYTES = NT * 128 * 64, STAGE = ABYTES + BBYTES;
@@ -239,6 +240,196 @@ struct Pipe {
     }
 };
 
+// The small tile, for launches that leave most of the chip idle: what counts is how long ONE workgroup takes for a step. Four waves (2 x 2) of MT x NT row
+// tiles, no phases: a wave multiplies one half of a step while it reads the next half's fragments, one barrier a step, RING - 1 stages ahead. (As phases of
+// 8 waves, like the large tile, the two products of 997 x 1201 x 320's gradients took 16.1 us, so 13.7; a deeper ring does not help.) Same interface as Pipe; column = wave * NT*32 + nt*32 + (lane&31),
+// wave = 0, 1; run() leaves the LDS free.
+template <int DT, int MT, int NT, bool ATR, bool BTR, int RING>
+struct Quad {
+    static constexpr int ABYTES = MT * 64 * 64, BBYTES = NT * 64 * 64, STAGE = ABYTES + BBYTES;
+    static constexpr int NA = MT, NB = NT, NPW = NA + NB;
+    unsigned char* smem;
+    int lane, wave8, grp, wave, aoff, boff;
+    unsigned va[NA], vb[NB];
+    int ka[NA], kb[NB];
+    const uint16_t *ap, *bp;
+    int64_t astep, bstep;
+    int krem, fslot;
+
+    __device__ __forceinline__ int k_of(bool tr, int i) const {
+        const int id = wave8 + 4 * i;
+        return tr ? 8 * (id & 3) + (lane >> 3) : 8 * ((lane & 3) ^ ((lane >> 4) & 3));
+    }
+    __device__ __forceinline__ int row_of(bool tr, int i) const {
+        const int id = wave8 + 4 * i;
+        return tr ? (id >> 2) * 64 + 8 * ((lane & 7) ^ (((lane >> 4) & 1) << 2)) : 16 * id + (lane >> 2);
+    }
+    __device__ __forceinline__ void init(unsigned char* s, int64_t a_ld, int64_t b_ld) {
+        smem = s;
+        const int tid = (int)threadIdx.x;
+        lane = tid & 63;
+        wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
+        grp = wave8 >> 1;
+        wave = wave8 & 1;
+        const int l31 = lane & 31, h = lane >> 5;
+#pragma unroll
+        for (int i = 0; i < NA; ++i) va[i] = ATR ? (unsigned)(k_of(ATR, i) * a_ld + row_of(ATR, i)) * 2u : (unsigned)(row_of(ATR, i) * a_ld + k_of(ATR, i)) * 2u;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) vb[i] = BTR ? (unsigned)(k_of(BTR, i) * b_ld + row_of(BTR, i)) * 2u : (unsigned)(row_of(BTR, i) * b_ld + k_of(BTR, i)) * 2u;
+        astep = ATR ? LBK * a_ld : LBK;
+        bstep = BTR ? LBK * b_ld : LBK;
+        const int trl = (8 * h + ((lane & 15) >> 2)) * 128 + (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ (((lane >> 3) & 1) << 2)) << 4) + (lane & 1) * 8;
+        const int nrl = l31 * 64 + ((h ^ ((l31 >> 2) & 3)) << 4);
+        const int lds0 = (int)(unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+        aoff = lds0 + (ATR ? trl + ((grp * MT) >> 1) * 4096 : nrl + grp * MT * 2048);
+        boff = lds0 + ABYTES + (BTR ? trl + ((wave * NT) >> 1) * 4096 : nrl + wave * NT * 2048);
+        fslot = 0;
+    }
+    __device__ __forceinline__ void open(const uint16_t* a, int a_rows, const uint16_t* b, int b_rows, int K) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) ka[i] = row_of(ATR, i) < a_rows ? k_of(ATR, i) : 0x40000000;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) kb[i] = row_of(BTR, i) < b_rows ? k_of(BTR, i) : 0x40000000;
+        ap = a;
+        bp = b;
+        krem = K;
+    }
+    __device__ __forceinline__ void fetch_a(int i) {
+        const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)ap, 0, LCAP, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(smem + fslot + wave8 * 1024 + i * 4096), 16,
+                                                 (int)(ka[i] < krem ? va[i] : LSENT), 0, 0, 0);
+    }
+    __device__ __forceinline__ void fetch_b(int i) {
+        const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)bp, 0, LCAP, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void*)(smem + fslot + ABYTES + wave8 * 1024 + i * 4096), 16,
+                                                 (int)(kb[i] < krem ? vb[i] : LSENT), 0, 0, 0);
+    }
+    __device__ __forceinline__ void fetched() {
+        ap += astep;
+        bp += bstep;
+        krem -= LBK;
+        fslot = fslot + STAGE == RING * STAGE ? 0 : fslot + STAGE;
+    }
+    template <class Next>
+    __device__ __forceinline__ void prime(Next&&) {
+#pragma unroll
+        for (int f = 0; f < RING - 1; ++f) {
+#pragma unroll
+            for (int i = 0; i < NA; ++i) fetch_a(i);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) fetch_b(i);
+            fetched();
+        }
+    }
+    __device__ __forceinline__ void start() {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 2) * NPW) : "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // tile t (32 rows) of the wave's, half kk; asm, so that the compiler waits for no DMA in front of it: the registers become values behind a wait
+    template <bool TR>
+    __device__ __forceinline__ void read(u32x4& r, u32x2& lo, u32x2& hi, int base, int t, int kk) const {
+        if (TR) {
+            const int o = (base ^ ((t & 1) << 6)) + (t >> 1) * 4096 + kk * 2048;
+            asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(lo) : "v"(o));
+            asm volatile("ds_read_b64_tr_b16 %0, %1 offset:512" : "=v"(hi) : "v"(o));
+        } else {
+            const int o = (base ^ (kk << 5)) + t * 2048;
+            asm volatile("ds_read_b128 %0, %1" : "=v"(r) : "v"(o));
+        }
+    }
+    template <bool TR>
+    static __device__ __forceinline__ void value(u32x4& r, u32x2& lo, u32x2& hi) {
+        if (TR) {
+            asm volatile("" : "+v"(lo), "+v"(hi));
+            r = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        } else asm volatile("" : "+v"(r));
+    }
+    template <class Next>
+    __device__ __forceinline__ void run(int steps, f32x16 (&acc)[MT][NT], Next&&) {
+        u32x4 a[2][MT], b[2][NT];
+        u32x2 al[2][MT], ah[2][MT], bl[2][NT], bh[2][NT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        int so = 0;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) read<BTR>(b[0][i], bl[0][i], bh[0][i], boff, i, 0);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) read<ATR>(a[0][i], al[0][i], ah[0][i], aoff, i, 0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < NT; ++i) value<BTR>(b[0][i], bl[0][i], bh[0][i]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) value<ATR>(a[0][i], al[0][i], ah[0][i]);
+        for (int st = 0; st < steps; ++st) {
+            const int ab = aoff + so, bb = boff + so;
+            so = so + STAGE == RING * STAGE ? 0 : so + STAGE;
+            const int an = aoff + so, bn = boff + so;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) read<BTR>(b[1][i], bl[1][i], bh[1][i], bb, i, 1);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) read<ATR>(a[1][i], al[1][i], ah[1][i], ab, i, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            // multiply half 0; fetch stage st + RING - 1, into the slot whose last reads ended before the barrier of step st - 1
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                fetch_a(i);
+                if (i < NB) fetch_b(i);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = lmfma<DT>(a[0][i], b[0][j], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            fetched();
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 2) * NPW) : "memory");  // stage st + 1, and this stage's last fragments
+#pragma unroll
+            for (int i = 0; i < NT; ++i) value<BTR>(b[1][i], bl[1][i], bh[1][i]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) value<ATR>(a[1][i], al[1][i], ah[1][i]);
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            // multiply half 1; read half 0 of the next stage
+#pragma unroll
+            for (int i = 0; i < NT; ++i) read<BTR>(b[0][i], bl[0][i], bh[0][i], bn, i, 0);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) read<ATR>(a[0][i], al[0][i], ah[0][i], an, i, 0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = lmfma<DT>(a[1][i], b[1][j], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < NT; ++i) value<BTR>(b[0][i], bl[0][i], bh[0][i]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) value<ATR>(a[0][i], al[0][i], ah[0][i]);
+        }
+        drain();
+    }
+    __device__ __forceinline__ unsigned char* free_slot() const { return smem; }
+    __device__ __forceinline__ void settle() {}
+    __device__ __forceinline__ void sync() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __device__ __forceinline__ void drain() {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+};
+constexpr int QRING = 4;
+template <int DT, int MT, int NT, bool ATR, bool BTR, bool WALK>
+using Product = std::conditional_t<MT == 4, Pipe<DT, MT, NT, ATR, BTR, WALK>, Quad<DT, MT, NT, ATR, BTR, QRING>>;
+template <int MT> constexpr int kLinThreads = MT == 4 ? 512 : 256;
+template <int MT, int NT> constexpr int kLinCols = MT == 4 ? NT * 128 : NT * 64;  // B rows of a tile (A rows: MT * 64)
+
 // ---- first product: logits of a tile of classes x rows ------------------------------------------------------------------------------------------
 struct LogitArgs {
     const uint16_t* x;
@@ -310,9 +501,9 @@ __device__ __forceinline__ void store_scaled(unsigned char* stg, const f32x16 (&
 // bf16: 363 -> 327 us forward). A launch of the small tile has one tile a workgroup and skips that bookkeeping (96 x 365 x 320: 8.4 us with it, 6.3 without).
 // Panels of 8 row tiles; an XCD's workgroups take neighbouring tiles: together 8 row tiles x 4 class tiles at a time, whose operands its L2 hands out.
 template <int DT, int MT, int NT, bool BWD>
-__global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_logits_kernel(const LogitArgs a) {
+__global__ __launch_bounds__(kLinThreads<MT>, 2) void class_logits_kernel(const LogitArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    constexpr int BM = MT * 64, BN = NT * 128, GR = 8;
+    constexpr int BM = MT * 64, BN = kLinCols<MT, NT>, GR = 8;
     constexpr bool WALK = MT == 4;
     const int ntiles = a.ntv * a.ntr;
     int L, end, per = 1;
@@ -335,7 +526,7 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_logits_kernel(cons
         r = (pr0 + in % pw) * BN;
     };
     place(L, v0, r0);
-    Pipe<DT, MT, NT, false, false, WALK> p;
+    Product<DT, MT, NT, false, false, WALK> p;
     p.init(smem, a.w_ld, a.x_ld);
     int F = L;                       // the tile that is fetched
     auto open = [&]() {
@@ -347,7 +538,7 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_logits_kernel(cons
     };
     // offsets of a tile's classes in log2 units, -inf for those left out or behind the last, and which of the writing waves met one. Walking: two tables behind
     // the ring, the next tile's written a tile ahead; else one, in the ring when that has ended
-    constexpr int TABLE = BM + 4, STAGE = Pipe<DT, MT, NT, false, false, WALK>::STAGE;
+    constexpr int TABLE = BM + 4, STAGE = Product<DT, MT, NT, false, false, WALK>::STAGE;
     float* table = reinterpret_cast<float*>(smem + LRING * STAGE);
     const bool writer = a.off && (int)threadIdx.x < BM;
     auto offset = [&](int t) {
@@ -373,8 +564,7 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_logits_kernel(cons
         f32x16 acc[MT][NT];
         p.run(steps, acc, open);
         if (!WALK && a.off) {
-            p.drain();
-            table = reinterpret_cast<float*>(smem + p.rslot);  // (results are staged in free_slot())
+            table = reinterpret_cast<float*>(smem + STAGE);  // (results are staged in free_slot())
             if (writer) note(table, o_first);
             p.sync();
         }
@@ -527,18 +717,19 @@ struct GradArgs {
 };
 
 template <int DT, int MT, int NT>
-__global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_grads_kernel(const GradArgs a) {
+__global__ __launch_bounds__(kLinThreads<MT>, 2) void class_grads_kernel(const GradArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    constexpr int BM = MT * 64, BN = NT * 128;
+    constexpr int BM = MT * 64, BN = kLinCols<MT, NT>;
     const int tid = (int)threadIdx.x, lane = tid & 63;
     const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int grp = wave8 >> 2, wave = wave8 & 3, l31 = lane & 31, h = lane >> 5;
+    constexpr int WN = MT == 4 ? 4 : 2;  // waves along the tile's columns
+    const int grp = wave8 / WN, wave = wave8 % WN, l31 = lane & 31, h = lane >> 5;
     int L = xcd_order((int)blockIdx.x, (int)gridDim.x);
     unsigned char* stg = smem + wave8 * (MT * 1024);
     f32x16 acc[MT][NT];
     if (L < a.ndw) {  // dw[v][f] = sum_r dz[r][v] x[r][f]
         const int f0 = (L % a.ntd) * BM, v0 = (L / a.ntd) * BN;
-        Pipe<DT, MT, NT, true, true, false> p;
+        Product<DT, MT, NT, true, true, false> p;
         auto none = []() {};
         p.init(smem, a.d, a.dz_ld);
         p.open(a.x + f0, a.d - f0, a.dz + v0, a.vk - v0, a.rows32);
@@ -558,7 +749,7 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void class_grads_kernel(const
     const int f0 = (L % a.ntd) * BM, r0 = (L / a.ntd % a.ntr) * BN, s = L / a.ntd / a.ntr;
     const int k0 = s * a.kper, k = max(0, min(a.kper, a.Vp - k0));
     {
-        Pipe<DT, MT, NT, true, false, false> p;
+        Product<DT, MT, NT, true, false, false> p;
         auto none = []() {};
         p.init(smem, a.w_ld, a.dz_ld);
         p.open(a.w + (int64_t)k0 * a.w_ld + f0, a.d - f0, a.dz + (int64_t)r0 * a.dz_ld + k0, a.rows32 - r0, k);
@@ -775,79 +966,99 @@ __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, i
     const int sub = lane >> 4, l = lane & 15;
     float* sv = saved + (int64_t)r * (1 + 2 * k);
     const int32_t* ir = idx + (int64_t)r * k;
-    auto slot_on = [&](int j) { return j < k && (unsigned)ir[j] < (unsigned)V; };
-    auto teach = [&](int j) { return load_elem(val, (int64_t)r * k + j, val_dtype) * itau; };
-    // the teacher's maximum and sum
+    // the slots in LDS: class (-1: empty) and the teacher's logit, later q; its maximum and sum
     float m = -INFINITY;
-    bool some = false;
-    for (int j = lane; j < k; j += 64)
-        if (slot_on(j)) {
-            const float t = teach(j);
-            m = t != t ? t : fmaxf(m, t);
-            some = true;
-        }
+    for (int j = lane; j < k; j += 64) {
+        const int v = ir[j];
+        const float t = load_elem(val, (int64_t)r * k + j, val_dtype) * itau;
+        const bool on = (unsigned)v < (unsigned)V;
+        s_idx[wv][j] = on ? v : -1;
+        s_q[wv][j] = t;
+        if (on) m = m != m || t != t ? NAN : fmaxf(m, t);
+    }
     for (int o = 32; o; o >>= 1) {
         const float m2 = __shfl_xor(m, o);
-        m = (m != m || m2 != m2) ? NAN : fmaxf(m, m2);
+        m = m != m || m2 != m2 ? NAN : fmaxf(m, m2);
     }
-    some = __ballot(some) != 0 && m != -INFINITY;
+    const float lse_r = lse[r], l2 = lse_r * kLog2e;
+    const bool some = m != -INFINITY && l2 != -INFINITY;  // (no filled slot, or nothing but -inf in them, or no class left)
     float s = 0.f;
     for (int j = lane; j < k; j += 64)
-        if (slot_on(j)) s += expf(teach(j) - m);
+        if (s_idx[wv][j] >= 0) s += expf(s_q[wv][j] - m);
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
     const float ls = logf(s);
-    const float l2 = lse[r] * kLog2e;
-    some = some && l2 != -INFINITY;
-    float sum = 0.f;
-    for (int j0 = 0; j0 < k; j0 += 4) {
-        const int j = j0 + sub;
-        const bool on = some && slot_on(j);
-        float z = 0.f;
-        if (on) {
-            const int v = ir[j];
-            const uint16_t *xr = x + r * x_ld, *wr = w + v * w_ld;
-            for (int f = l * 8; f < d; f += 128) {
-                const u32x4 xv = *reinterpret_cast<const u32x4*>(xr + f), wv = *reinterpret_cast<const u32x4*>(wr + f);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    z = fmaf(Elem<DT>::to_f32((uint16_t)(xv[e] & 0xffff)), Elem<DT>::to_f32((uint16_t)(wv[e] & 0xffff)), z);
-                    z = fmaf(Elem<DT>::to_f32((uint16_t)(xv[e] >> 16)), Elem<DT>::to_f32((uint16_t)(wv[e] >> 16)), z);
-                }
-            }
-        }
-        for (int o = 8; o; o >>= 1) z += __shfl_xor(z, o);
-        if (j < k && l == 0) {
-            float z2 = -INFINITY, q = 0.f;
-            if (on) {
-                const float ov = off ? off[ir[j]] : 0.f;
-                z2 = ov == -INFINITY ? -INFINITY : fmaf(z, c, ov * coff);
-                const float lq = teach(j) - m - ls;
-                q = expf(lq);
-                if (q != 0.f) sum += q * (lq - (z2 - l2) * kLn2);
-            }
-            sv[1 + j] = z2;
-            s_idx[wv][j] = on ? ir[j] : -1;
-            s_q[wv][j] = q;
-        }
-    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    for (int j = lane; j < k; j += 64) {
-        const int v = s_idx[wv][j];
-        float q = s_q[wv][j];
-        bool first = v >= 0;
-        for (int o = 0; o < k; ++o) {
-            const bool same = s_idx[wv][o] == v;
-            first = first && !(same && o < j);
-            q += same && o > j ? s_q[wv][o] : 0.f;
+    float sum = 0.f;
+    constexpr int U = 4;  // rows of w in flight per 16 lanes
+    const uint16_t* xr = x + r * x_ld;
+    for (int j0 = 0; j0 < k; j0 += 4 * U) {
+        float z[U];
+        int v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * 4 + sub;
+            v[u] = some && j < k ? s_idx[wv][j] : -1;
+            z[u] = 0.f;
         }
-        sv[1 + k + j] = first ? q : -1.f;
+        for (int f = l * 8; f < d; f += 128) {
+            const u32x4 xv = *reinterpret_cast<const u32x4*>(xr + f);
+            u32x4 wr[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) wr[u] = v[u] >= 0 ? *reinterpret_cast<const u32x4*>(w + v[u] * w_ld + f) : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    z[u] = fmaf(Elem<DT>::to_f32((uint16_t)(xv[e] & 0xffff)), Elem<DT>::to_f32((uint16_t)(wr[u][e] & 0xffff)), z[u]);
+                    z[u] = fmaf(Elem<DT>::to_f32((uint16_t)(xv[e] >> 16)), Elem<DT>::to_f32((uint16_t)(wr[u][e] >> 16)), z[u]);
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * 4 + sub;
+            for (int o = 8; o; o >>= 1) z[u] += __shfl_xor(z[u], o);
+            if (j < k && l == 0) {
+                float z2 = -INFINITY, q = 0.f;
+                if (v[u] >= 0) {
+                    const float ov = off ? off[v[u]] : 0.f;
+                    z2 = ov == -INFINITY ? -INFINITY : fmaf(z[u], c, ov * coff);
+                    const float lq = s_q[wv][j] - m - ls;
+                    q = expf(lq);
+                    if (q != 0.f) sum += q * (lq - (z2 - l2) * kLn2);
+                }
+                sv[1 + j] = z2;
+                s_q[wv][j] = q;
+            }
+        }
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
     if (lane == 0) {
         loss[r] = some ? sum * tau2 : 0.f;
-        sv[0] = !some ? INFINITY : lse[r] == INFINITY ? NAN : lse[r];
+        sv[0] = !some ? INFINITY : lse_r == INFINITY ? NAN : lse_r;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    // is a class named twice: one comparison a slot where the slots fit the lanes
+    bool alone = false;
+    if (k <= 64) {
+        const int v = lane < k && s_idx[wv][lane] >= 0 ? s_idx[wv][lane] : -1 - lane;
+        uint64_t twice = 0;
+        for (int o = 0; o < k; ++o) twice |= __ballot(v == __builtin_amdgcn_readlane(v, o)) & ~(1ull << o);
+        alone = twice == 0;
+    }
+    for (int j = lane; j < k; j += 64) {
+        const int v = s_idx[wv][j];
+        float q = s_q[wv][j];
+        bool first = some && v >= 0;
+        if (!alone)
+            for (int o = 0; o < k; ++o) {
+                const bool same = s_idx[wv][o] == v;
+                first = first && !(same && o < j);
+                q += same && o > j ? s_q[wv][o] : 0.f;
+            }
+        sv[1 + k + j] = first ? q : -1.f;
     }
 }
 // dz at the teacher's classes of a piece: coef * (p - q)
@@ -938,7 +1149,7 @@ template <typename K>
 static void allow_lds(K kernel, size_t bytes) {
     (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
-constexpr size_t LDS_BIG = 4 * 32768, LDS_SMALL = 4 * 16384;
+constexpr size_t LDS_BIG = 4 * 32768, LDS_SMALL = QRING * 16384;
 
 template <bool BWD>
 static int launch_logits(LogitArgs a, int dtype, bool big, hipStream_t s) {
@@ -952,14 +1163,14 @@ static int launch_logits(LogitArgs a, int dtype, bool big, hipStream_t s) {
         constexpr size_t LDS_ = RING_ + (MT_ == 4 ? 2 * (MT_ * 64 + 4) * 4 : 0);                                                  \
         static bool once = (allow_lds(class_logits_kernel<DT_, MT_, NT_, BWD>, LDS_), true);               \
         (void)once;                                                                                        \
-        class_logits_kernel<DT_, MT_, NT_, BWD><<<dim3((unsigned)MT_ == 4 ? std::min<int64_t>(n, 256) : n), dim3(512), LDS_, s>>>(a); \
+        class_logits_kernel<DT_, MT_, NT_, BWD><<<dim3((unsigned)MT_ == 4 ? std::min<int64_t>(n, 256) : n), dim3(kLinThreads<MT_>), LDS_, s>>>(a); \
     } while (0)
     if (dtype == CDET_BF16) {
         if (big) CDET_GO(CDET_BF16, 4, 2, LDS_BIG);
-        else CDET_GO(CDET_BF16, 2, 1, LDS_SMALL);
+        else CDET_GO(CDET_BF16, 2, 2, LDS_SMALL);
     } else {
         if (big) CDET_GO(CDET_F16, 4, 2, LDS_BIG);
-        else CDET_GO(CDET_F16, 2, 1, LDS_SMALL);
+        else CDET_GO(CDET_F16, 2, 2, LDS_SMALL);
     }
 #undef CDET_GO
     CDET_LAUNCH_CHECK();
@@ -971,14 +1182,14 @@ static int launch_grads(const GradArgs& a, int dtype, bool big, hipStream_t s) {
     do {                                                                                      \
         static bool once = (allow_lds(class_grads_kernel<DT_, MT_, NT_>, LDS_), true);        \
         (void)once;                                                                           \
-        class_grads_kernel<DT_, MT_, NT_><<<dim3(n), dim3(512), LDS_, s>>>(a);                \
+        class_grads_kernel<DT_, MT_, NT_><<<dim3(n), dim3(kLinThreads<MT_>), LDS_, s>>>(a);   \
     } while (0)
     if (dtype == CDET_BF16) {
         if (big) CDET_GO(CDET_BF16, 4, 2, LDS_BIG);
-        else CDET_GO(CDET_BF16, 2, 1, LDS_SMALL);
+        else CDET_GO(CDET_BF16, 2, 2, LDS_SMALL);
     } else {
         if (big) CDET_GO(CDET_F16, 4, 2, LDS_BIG);
-        else CDET_GO(CDET_F16, 2, 1, LDS_SMALL);
+        else CDET_GO(CDET_F16, 2, 2, LDS_SMALL);
     }
 #undef CDET_GO
     CDET_LAUNCH_CHECK();
