@@ -450,10 +450,22 @@ struct LogitArgs {
     uint16_t* dz;         // [rows][dz_ld]
     int64_t dz_ld;
     int dz_rows;          // rows to be written (N rounded up to 32)
+    const int32_t* idx;   // small tile only: the teacher's slots (patch_teacher), or null
+    const float* saved;
+    int k;
 };
 
 __device__ __forceinline__ int64_t load_label(const void* p, int is64, int r) {
     return is64 ? reinterpret_cast<const int64_t*>(p)[r] : (int64_t)reinterpret_cast<const int32_t*>(p)[r];
+}
+
+// dz at a class that slot i = (row r, j) of the teacher names: coef * (p - q)
+template <int DT>
+__device__ __forceinline__ void patch_teacher(const float* saved, const float* lse2, const float* coef, int k, int r, int j, uint16_t* at) {
+    const float* sv = saved + (int64_t)r * (1 + 2 * k);
+    const float q = sv[1 + k + j];
+    if (q == -1.f || lse2[r] == INFINITY || sv[1 + j] == -INFINITY) return;  // another slot's, or a row without a part, or a left-out class (no gradient)
+    *at = Elem<DT>::from_f32((__builtin_amdgcn_exp2f(sv[1 + j] - lse2[r]) - q) * coef[r]);
 }
 
 // 32 C columns x (HT*32) C rows of 16-bit values through `stg` (wave-private, HT * 2 KiB) as whole rows of the destination: pk[i][q] = the lane's rows
@@ -687,6 +699,14 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_logits_kernel(const 
             for (int j = 0; j < NT; ++j) {
                 const int rr = r0 + (wave * NT + j) * 32;
                 store_scaled<DT, MT, NT>(stg, acc, j, g[j], lane, a.dz + (int64_t)rr * a.dz_ld + vw, a.dz_ld, a.dz_rows - rr, MT * 32);
+            }
+        }
+        if (!WALK && BWD && a.idx) {
+            __syncthreads();  // the tile is written: the entries that the teacher names may follow
+            const int rows = min(BN, a.N - r0), V = min(BM, a.V - v0);
+            for (int i = (int)threadIdx.x; i < rows * a.k; i += kLinThreads<MT>) {
+                const int r = r0 + i / a.k, j = i % a.k, v = a.idx[(int64_t)r0 * a.k + i] - a.v_first - v0;
+                if ((unsigned)v < (unsigned)V) patch_teacher<DT>(a.saved, a.lse2, a.coef, a.k, r, j, a.dz + r * a.dz_ld + v0 + v);
             }
         }
         L += per;
@@ -957,7 +977,7 @@ __global__ __launch_bounds__(256) void class_zero_kernel(uint16_t* p, int64_t ro
 template <int DT>
 __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, int64_t x_ld, const uint16_t* w, int64_t w_ld, const float* off, float c, float coff,
                                                             const int32_t* idx, const void* val, int val_dtype, int k, float itau, float tau2, int N, int V, int d,
-                                                            const float* lse, float* loss, float* saved) {
+                                                            const float* lse, const float* part, int nvb, float* loss, float* saved) {
     __shared__ int s_idx[4][512];
     __shared__ float s_q[4][512];
     const int lane = (int)threadIdx.x & 63, wv = (int)threadIdx.x >> 6;
@@ -980,7 +1000,24 @@ __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, i
         const float m2 = __shfl_xor(m, o);
         m = m != m || m2 != m2 ? NAN : fmaxf(m, m2);
     }
-    const float lse_r = lse[r], l2 = lse_r * kLog2e;
+    float lse_r;
+    if (part) {  // few pairs a row: joined here instead of in a launch of their own
+        float pm = 0.f, ps = 0.f;
+        if (lane < nvb) {
+            pm = part[(int64_t)lane * N + r];
+            ps = part[((int64_t)nvb + lane) * N + r];
+        }
+        for (int o = 1; o < 64; o *= 2) {
+            const float m2 = __shfl_xor(pm, o), s2 = __shfl_xor(ps, o);
+            const bool up = lane & o;  // (the same order in every lane: the lower lane's pair first)
+            float a0 = up ? m2 : pm, b0 = up ? s2 : ps;
+            lse_join(a0, b0, up ? pm : m2, up ? ps : s2);
+            pm = a0;
+            ps = b0;
+        }
+        lse_r = ps == 0.f ? -INFINITY : (pm + __builtin_amdgcn_logf(ps)) * kLn2;
+    } else lse_r = lse[r];
+    const float l2 = lse_r * kLog2e;
     const bool some = m != -INFINITY && l2 != -INFINITY;  // (no filled slot, or nothing but -inf in them, or no class left)
     float s = 0.f;
     for (int j = lane; j < k; j += 64)
@@ -1061,7 +1098,7 @@ __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, i
         sv[1 + k + j] = first ? q : -1.f;
     }
 }
-// dz at the teacher's classes of a piece: coef * (p - q)
+// dz at the teacher's classes of a piece (the small tile's launch does it by itself)
 template <int DT>
 __global__ __launch_bounds__(256) void class_teacher_dz_kernel(const int32_t* idx, const float* saved, const float* lse2, const float* coef, int k, int N, int v_first,
                                                                int Vp, uint16_t* dz, int64_t dz_ld) {
@@ -1070,10 +1107,7 @@ __global__ __launch_bounds__(256) void class_teacher_dz_kernel(const int32_t* id
     const int v = idx[i];
     if (v < v_first || v - v_first >= Vp) return;
     const int r = (int)(i / k), j = (int)(i - (int64_t)r * k);
-    const float* sv = saved + (int64_t)r * (1 + 2 * k);
-    const float q = sv[1 + k + j];
-    if (q == -1.f || lse2[r] == INFINITY || sv[1 + j] == -INFINITY) return;  // another slot's, or a row without a part, or a left-out class (no gradient)
-    dz[r * dz_ld + (v - v_first)] = Elem<DT>::from_f32((__builtin_amdgcn_exp2f(sv[1 + j] - lse2[r]) - q) * coef[r]);
+    patch_teacher<DT>(saved, lse2, coef, k, r, j, dz + r * dz_ld + (v - v_first));
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------------------------------
@@ -1209,7 +1243,7 @@ static LogitArgs logit_args(const cdet_linear_loss_desc* q) {
     return a;
 }
 
-// logits' statistics -> lse (and, with labels, the loss)
+// logits' statistics -> lse (and, with labels, the loss); lse null: the statistics only
 static int lin_forward(const cdet_linear_loss_desc* q, const LinPlan& p, const void* x, const void* w, const void* label, float* loss, float* lse, char* ws, hipStream_t s) {
     LogitArgs a = logit_args(q);
     a.x = (const uint16_t*)x;
@@ -1219,7 +1253,7 @@ static int lin_forward(const cdet_linear_loss_desc* q, const LinPlan& p, const v
     a.part = (float*)(ws + p.o_part);
     a.zlab = (float*)(ws + p.o_zlab);
     const int rc = launch_logits<false>(a, q->dtype, p.big_f, s);
-    if (rc) return rc;
+    if (rc || !lse) return rc;
     int C = 1;  // rows a workgroup: 64 keep the loads wide, fewer fill the chip
     while (C < 64 && (C < 8 ? C < q->N : C * 256 <= q->N)) C *= 2;
     class_lse_kernel<<<dim3(div_up(q->N, C)), dim3(1024), 0, s>>>(a.part, p.nvb, q->N, q->V, C, label, q->label64, a.zlab, loss, lse);
@@ -1297,9 +1331,12 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         a.dz = (uint16_t*)(ws + p.o_dz);
         a.dz_ld = p.piece;
         a.dz_rows = p.rows32;
+        a.idx = p.big_f ? nullptr : idx;
+        a.saved = saved;
+        a.k = k;
         int rc = launch_logits<true>(a, q->dtype, p.big_f, s);
         if (rc) return rc;
-        if (idx) {
+        if (idx && p.big_f) {
             const unsigned nb = (unsigned)div_up((int64_t)N * k, 256);
             if (q->dtype == CDET_BF16) class_teacher_dz_kernel<CDET_BF16><<<dim3(nb), dim3(256), 0, s>>>(idx, saved, lse2, coef, k, N, v0, Vp, a.dz, a.dz_ld);
             else class_teacher_dz_kernel<CDET_F16><<<dim3(nb), dim3(256), 0, s>>>(idx, saved, lse2, coef, k, N, v0, Vp, a.dz, a.dz_ld);
@@ -1388,14 +1425,16 @@ extern "C" int cdet_linear_distill_fwd(const cdet_linear_loss_desc* d, const voi
     CDET_CHECK_ARG(d->N == 0 || (idx && val && loss && saved), "cdet_linear_distill_fwd: idx, val, loss and saved must be given");
     if (d->N == 0) return 0;
     const LinPlan p = lin_plan(d, true);
-    float* lse = (float*)((char*)ws + p.o_lse);
+    const bool few = p.nvb <= 64;  // (class_teacher_kernel joins them)
+    float* lse = few ? nullptr : (float*)((char*)ws + p.o_lse);
+    const float* part = few ? (const float*)((char*)ws + p.o_part) : nullptr;
     const int rc = lin_forward(d, p, x, w, nullptr, nullptr, lse, (char*)ws, (hipStream_t)stream);
     if (rc) return rc;
     const dim3 nb((unsigned)div_up(d->N, 4)), nt(256);
     const LogitArgs a = logit_args(d);
 #define CDET_GO(DT_)                                                                                                                                        \
     class_teacher_kernel<DT_><<<nb, nt, 0, (hipStream_t)stream>>>((const uint16_t*)x, d->x_ld, (const uint16_t*)w, d->w_ld, d->offset, a.c, a.coff, idx, val, val_dtype, \
-                                                                 k, 1.f / d->tau, d->tau * d->tau, d->N, d->V, d->d, lse, loss, saved)
+                                                                 k, 1.f / d->tau, d->tau * d->tau, d->N, d->V, d->d, lse, part, p.nvb, loss, saved)
     if (d->dtype == CDET_BF16) CDET_GO(CDET_BF16);
     else CDET_GO(CDET_F16);
 #undef CDET_GO

@@ -394,12 +394,12 @@ def _bad(msg):
 
 
 class _Device:
-    """Context of a launch on `dev`: switches the current device where it is another one; `stream` = the device's current stream."""
+    """Context of a launch on GPU `index`: switches the current device where it is another one; yields the device's current stream."""
 
     __slots__ = ("index", "before")
 
-    def __init__(self, dev):
-        self.index, self.before = dev.index, torch.cuda.current_device()
+    def __init__(self, index):
+        self.index, self.before = index, torch._C._cuda_getDevice()
 
     def __enter__(self):
         if self.index != self.before:
@@ -412,9 +412,9 @@ class _Device:
         return False
 
 
-def _on(dev, name, t):
-    if not isinstance(t, torch.Tensor) or t.device != dev:
-        _bad(f"{name} must be a tensor on {dev}, got {getattr(t, 'device', type(t))}")
+def _on(index, name, t):
+    if not isinstance(t, torch.Tensor) or t.get_device() != index:
+        _bad(f"{name} must be a tensor on cuda:{index}, got {getattr(t, 'device', type(t))}")
 
 
 def _feature_rows(t):
@@ -435,9 +435,10 @@ def _linear_loss_desc(x, w, offset, scale, tau, label64=0):
         _bad(f"x [N, d] and w [V, d] expected, got {getattr(x, 'shape', type(x))} and {getattr(w, 'shape', type(w))}")
     if x.dtype != w.dtype or x.dtype not in (torch.bfloat16, torch.float16):
         _bad(f"x and w must both be bf16 or fp16, got {x.dtype} and {w.dtype}")
-    if not x.is_cuda:
+    gpu = x.get_device()
+    if gpu < 0:
         _bad("x must be on the GPU (there is no CPU path)")
-    _on(x.device, "w", w)
+    _on(gpu, "w", w)
     (N, dim), V = x.shape, w.shape[0]
     if dim < 8 or dim % 8 or dim > 65536:
         _bad(f"d = {dim} must be a multiple of 8 in 8 .. 65536")
@@ -447,7 +448,7 @@ def _linear_loss_desc(x, w, offset, scale, tau, label64=0):
     if not 0.0 < tau < float("inf") or not abs(scale) < float("inf"):
         _bad(f"tau = {tau} must be positive, scale = {scale} finite")
     if offset is not None:
-        _on(x.device, "offset", offset)
+        _on(gpu, "offset", offset)
         if offset.shape != (V,) or offset.dtype != torch.float32:
             _bad(f"offset must be [{V}] fp32, got {tuple(offset.shape)} {offset.dtype}")
         offset = offset.contiguous()
@@ -459,27 +460,27 @@ def _linear_loss_desc(x, w, offset, scale, tau, label64=0):
 def _labels(labels, x):
     if not isinstance(labels, torch.Tensor) or labels.shape != x.shape[:1] or labels.dtype not in (torch.int64, torch.int32):
         _bad(f"labels must be [{x.shape[0]}] int64 or int32")
-    _on(x.device, "labels", labels)
+    _on(x.get_device(), "labels", labels)
     return labels.contiguous()
 
 
-def _teacher(idx, val, shape, dev):
+def _teacher(idx, val, shape, gpu):
     if not isinstance(idx, torch.Tensor) or idx.dtype != torch.int32 or idx.shape[:-1] != shape or not 1 <= idx.shape[-1] <= 512:
         _bad(f"idx must be {list(shape)} + [k] int32 with k in 1 .. 512, got {getattr(idx, 'shape', type(idx))}")
-    _on(dev, "idx", idx)
+    _on(gpu, "idx", idx)
     if val is not None:
-        _on(dev, "val", val)
+        _on(gpu, "val", val)
         if val.shape != idx.shape or val.dtype not in (torch.float32, torch.bfloat16, torch.float16):
             _bad(f"val must be {list(idx.shape)} fp32, bf16 or fp16, got {tuple(val.shape)} {val.dtype}")
         val = val.contiguous()
     return idx.contiguous(), val
 
 
-def _row_grad(drow, shape, dev):
+def _row_grad(drow, shape, gpu):
     """(tensor | None, stride): one value per row, one value for all, or None (ones)."""
     if drow is None:
         return None, 0
-    _on(dev, "drow", drow)
+    _on(gpu, "drow", drow)
     if drow.dtype != torch.float32 or not (drow.shape == shape or drow.numel() == 1):
         _bad(f"drow must be {list(shape)} (or one value) fp32, got {tuple(drow.shape)} {drow.dtype}")
     return drow.contiguous(), (1 if drow.numel() != 1 else 0)
@@ -488,13 +489,15 @@ def _row_grad(drow, shape, dev):
 def linear_ce_fwd(x, w, labels, offset=None, scale=1.0):
     """Softmax cross entropy of z = scale * x @ w.T + offset without the logits in memory. x [N, d], w [V, d] bf16 / fp16; labels [N] int64 / int32, a label
     outside of 0 .. V-1 leaves its row out (loss 0); offset [V] fp32 (class priors, -inf = class left out). Returns (loss [N], lse [N]) fp32."""
-    lib, dev = L.load(), x.device if isinstance(x, torch.Tensor) else None
+    lib = L.load()
     d, xs, wsrc, off = _linear_loss_desc(x, w, offset, scale, 1.0)
     labels = _labels(labels, x)
     d.label64 = int(labels.dtype == torch.int64)
     ref = C.byref(d)
-    with _Device(dev) as s:
-        loss, lse = torch.empty((2, d.N), dtype=torch.float32, device=dev)
+    dev = x.device
+    with _Device(dev.index) as s:
+        loss = torch.empty(d.N, dtype=torch.float32, device=dev)
+        lse = torch.empty(d.N, dtype=torch.float32, device=dev)
         ws = torch.empty(lib.cdet_linear_loss_ws_bytes(ref, 0), dtype=torch.uint8, device=dev)
         L.check(lib.cdet_linear_ce_fwd(ref, xs.data_ptr(), wsrc.data_ptr(), labels.data_ptr(), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), s), "cdet_linear_ce_fwd")
     return loss, lse
@@ -502,17 +505,18 @@ def linear_ce_fwd(x, w, labels, offset=None, scale=1.0):
 
 def linear_ce_bwd(x, w, labels, lse, drow=None, offset=None, scale=1.0, want_dx=True, want_dw=True):
     """Gradients of sum(drow * loss): (dx [N, d], dw [V, d]) in x's type (None where not wanted). lse: linear_ce_fwd's; drow: fp32 [N], one value, or None."""
-    lib, dev = L.load(), x.device if isinstance(x, torch.Tensor) else None
+    lib = L.load()
     d, xs, wsrc, off = _linear_loss_desc(x, w, offset, scale, 1.0)
     labels = _labels(labels, x)
     d.label64 = int(labels.dtype == torch.int64)
-    _on(dev, "lse", lse)
+    _on(x.get_device(), "lse", lse)
     if lse.shape != x.shape[:1] or lse.dtype != torch.float32:
         _bad(f"lse must be [{d.N}] fp32")
     lse = lse.contiguous()
-    g, gs = _row_grad(drow, x.shape[:1], dev)
+    g, gs = _row_grad(drow, x.shape[:1], x.get_device())
     ref = C.byref(d)
-    with _Device(dev) as s:
+    dev = x.device
+    with _Device(dev.index) as s:
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
         dw = torch.empty(w.shape, dtype=x.dtype, device=dev) if want_dw else None
         ws = torch.empty(lib.cdet_linear_loss_ws_bytes(ref, 1), dtype=torch.uint8, device=dev)
@@ -525,14 +529,15 @@ def linear_distill_fwd(x, w, idx, val, tau=1.0, offset=None, scale=1.0):
     """Distillation of the class projection z = scale * x @ w.T + offset from a teacher's top k logits, without the logits in memory:
     loss = tau^2 KL(softmax(val / tau) || softmax(z / tau) at idx) per row. idx [N, k] int32 (outside of 0 .. V-1: an empty slot; a row without any has loss 0),
     val [N, k] fp32 / bf16 / fp16. Returns (loss [N] fp32, saved [N, 1 + 2k] fp32 for linear_distill_bwd)."""
-    lib, dev = L.load(), x.device if isinstance(x, torch.Tensor) else None
+    lib = L.load()
     d, xs, wsrc, off = _linear_loss_desc(x, w, offset, scale, tau)
     if val is None:
         _bad("val must be given")
-    idx, val = _teacher(idx, val, x.shape[:1], dev)
+    idx, val = _teacher(idx, val, x.shape[:1], x.get_device())
     k = idx.shape[1]
     ref = C.byref(d)
-    with _Device(dev) as s:
+    dev = x.device
+    with _Device(dev.index) as s:
         loss = torch.empty(d.N, dtype=torch.float32, device=dev)
         saved = torch.empty((d.N, 1 + 2 * k), dtype=torch.float32, device=dev)
         ws = torch.empty(lib.cdet_linear_loss_ws_bytes(ref, 0), dtype=torch.uint8, device=dev)
@@ -543,16 +548,17 @@ def linear_distill_fwd(x, w, idx, val, tau=1.0, offset=None, scale=1.0):
 
 def linear_distill_bwd(x, w, idx, saved, drow=None, tau=1.0, offset=None, scale=1.0, want_dx=True, want_dw=True):
     """Gradients of sum(drow * loss) of linear_distill_fwd: (dx, dw) in x's type."""
-    lib, dev = L.load(), x.device if isinstance(x, torch.Tensor) else None
+    lib = L.load()
     d, xs, wsrc, off = _linear_loss_desc(x, w, offset, scale, tau)
-    idx, _ = _teacher(idx, None, x.shape[:1], dev)
+    idx, _ = _teacher(idx, None, x.shape[:1], x.get_device())
     k = idx.shape[1]
-    _on(dev, "saved", saved)
+    _on(x.get_device(), "saved", saved)
     if saved.shape != (d.N, 1 + 2 * k) or saved.dtype != torch.float32 or not saved.is_contiguous():
         _bad(f"saved must be linear_distill_fwd's [{d.N}, {1 + 2 * k}]")
-    g, gs = _row_grad(drow, x.shape[:1], dev)
+    g, gs = _row_grad(drow, x.shape[:1], x.get_device())
     ref = C.byref(d)
-    with _Device(dev) as s:
+    dev = x.device
+    with _Device(dev.index) as s:
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
         dw = torch.empty(w.shape, dtype=x.dtype, device=dev) if want_dw else None
         ws = torch.empty(lib.cdet_linear_loss_ws_bytes(ref, 1), dtype=torch.uint8, device=dev)
@@ -576,35 +582,37 @@ def topk_distill(logits, idx, val, tau=1.0, drow=None, grad_scale=1.0, grad_dtyp
     lib = L.load()
     if not isinstance(logits, torch.Tensor) or logits.dim() not in (2, 3) or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         _bad("logits must be [P, V] or [P, G, V] fp32, bf16 or fp16")
-    if not logits.is_cuda:
+    gpu, shape = logits.get_device(), logits.shape
+    if gpu < 0:
         _bad("logits must be on the GPU (there is no CPU path)")
-    dev, shape = logits.device, logits.shape
     P, V, G = shape[0], shape[-1], (shape[1] if len(shape) == 3 else 1)
     if not 1 <= V <= 1 << 24 or G < 1 or P * G >= 1 << 31:
         _bad(f"logits {tuple(shape)}")
     ld = _pixel_pitch(logits, "logits", P, G, V)
     if val is None:
         _bad("val must be given")
-    idx, val = _teacher(idx, val, shape[:-1], dev)
+    rows = shape[:-1]
+    idx, val = _teacher(idx, val, rows, gpu)
     tau = float(tau)
     if not 0.0 < tau < float("inf"):
         _bad(f"tau = {tau} must be positive")
     grad_dtype = grad_dtype or (logits.dtype if out is None else out.dtype)
     if grad_dtype is not logits.dtype and grad_dtype is not torch.float32:
         _bad(f"grad_dtype must be {logits.dtype} or fp32")
-    g, gs = _row_grad(drow, shape[:-1], dev)
-    with _Device(dev) as s:
+    g, gs = _row_grad(drow, rows, gpu)
+    dev = logits.device
+    with _Device(gpu) as s:
         if g is not None and gs == 0 and P * G != 1:
             g = g.reshape(1).expand(P * G).contiguous()
         if out is not None:
-            _on(dev, "out", out)
+            _on(gpu, "out", out)
             if out.shape != shape or out.dtype != grad_dtype or (P > 1 and out.stride(0) < G * V):
                 _bad(f"out must be {tuple(shape)} {grad_dtype} without overlapping pixels")
         elif want_grad:
             out = torch.empty(shape, dtype=grad_dtype, device=dev)
         gld = _pixel_pitch(out, "out", P, G, V) if out is not None else 0
         d = L.TopkDistillDesc(P, G, V, idx.shape[-1], _DT[logits.dtype], _DT[val.dtype], _DT[grad_dtype], ld, gld, tau, float(grad_scale))
-        loss = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+        loss = torch.empty(rows, dtype=torch.float32, device=dev)
         L.check(lib.cdet_topk_distill(C.byref(d), logits.data_ptr(), idx.data_ptr(), val.data_ptr(), ptr(g), loss.data_ptr(), ptr(out), s), "cdet_topk_distill")
     return loss, out
 
