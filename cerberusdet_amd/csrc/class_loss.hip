@@ -726,6 +726,7 @@ struct GradArgs {
     int N, rows32, d, Vp; // Vp: classes of the piece
     int vk;               // columns of dz that hold numbers (Vp rounded up to the tile)
     int ntd, ndw, ndx;    // tiles along d; dw tiles, dx tiles
+    int dx_first;
     int ntr, splits, kper;// dx: row tiles, slices of the piece, classes per slice (a multiple of 32)
     uint16_t* dw;         // [Vp][dw_ld]
     int64_t dw_ld;
@@ -744,10 +745,19 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_grads_kernel(const G
     const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
     constexpr int WN = MT == 4 ? 4 : 2;  // waves along the tile's columns
     const int grp = wave8 / WN, wave = wave8 % WN, l31 = lane & 31, h = lane >> 5;
-    int L = xcd_order((int)blockIdx.x, (int)gridDim.x);
+    // every XCD gets its even share of the dw tiles and of the dx tiles (neighbouring ones), the longer kind first
+    int L;
+    bool is_dw;
+    {
+        const int xcd = (int)blockIdx.x & 7, j = (int)blockIdx.x >> 3, n = (int)gridDim.x;
+        auto start = [&](int count) { return (count >> 3) * xcd + min(xcd, count & 7); };  // of this XCD's share of `count`
+        const int dw0 = start(a.ndw), dwn = (a.ndw >> 3) + (xcd < (a.ndw & 7) ? 1 : 0), dx0 = start(n) - dw0, dxn = (n >> 3) + (xcd < (n & 7) ? 1 : 0) - dwn;
+        is_dw = a.dx_first ? j >= dxn : j < dwn;
+        L = is_dw ? dw0 + (a.dx_first ? j - dxn : j) : dx0 + (a.dx_first ? j : j - dwn);
+    }
     unsigned char* stg = smem + wave8 * (MT * 1024);
     f32x16 acc[MT][NT];
-    if (L < a.ndw) {  // dw[v][f] = sum_r dz[r][v] x[r][f]
+    if (is_dw) {  // dw[v][f] = sum_r dz[r][v] x[r][f]
         const int f0 = (L % a.ntd) * BM, v0 = (L / a.ntd) * BN;
         Product<DT, MT, NT, true, true, false> p;
         auto none = []() {};
@@ -765,7 +775,7 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_grads_kernel(const G
         }
         return;
     }
-    L -= a.ndw;  // dx[r][f] += sum over the slice's classes of dz[r][v] w[v][f]
+    // dx[r][f] += sum over the slice's classes of dz[r][v] w[v][f]
     const int f0 = (L % a.ntd) * BM, r0 = (L / a.ntd % a.ntr) * BN, s = L / a.ntd / a.ntr;
     const int k0 = s * a.kper, k = max(0, min(a.kper, a.Vp - k0));
     {
@@ -1115,14 +1125,61 @@ static inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 // 256 x 256 tiles read 131 FLOP per byte staged, 128 x 128 tiles half of that, so the large ones are taken wherever they fill most of the 256 CUs
 static inline bool big_tiles(int64_t rows, int64_t cols) { return (up(rows, 256) / 256) * (up(cols, 256) / 256) >= 160; }
 
+// The backward's shape: how many pieces the class list is cut into, and each piece's classes into how many slices for dx (whose tiles, rows x features, are
+// few). Costs in steps of the large tile (0.86 us): a tile of K costs K / 32 + 6; a launch is as long as the busiest of an XCD's 32 CUs, longer kind of
+// tile first, and 5 more; a slice's fp32 slab is written (and read, from the second piece on) at 3.5 MB a step. dz of a piece stays within 192 MiB, so that
+// it lives in the 256 MiB cache between its three uses. 4096 x 65536 x 640: 4 pieces of 4 slices, by equal lengths, took 4 x 219 us for the products,
+// 3 pieces of 5 take 3 x 244.
+struct GradShape {
+    int piece, pieces, splits, kper, tiles, dx_first;
+};
+static GradShape grad_shape(int64_t N, int64_t V, int64_t d, int64_t rows32, bool want_dx, bool want_dw) {
+    const int64_t ntd = up(d, 256) / 256, ntr = up(N, 256) / 256, Vt = up(V, 256) / 256;
+    const int64_t most = std::max<int64_t>(8, ((int64_t)96 << 20) / rows32 / 256);  // class tiles of a piece
+    GradShape best = {};
+    double least = 1e30;
+    const int64_t n0 = up(Vt, most) / most;
+    for (int64_t n = n0; n <= 2 * n0 + 2 && n <= Vt; ++n) {
+        const int64_t pt = up(Vt, n) / n;  // class tiles of a piece
+        const double t_dw = rows32 / 32 + 6, logits = (double)(up(pt * ntr, 256) / 256) * (double)(d / 32 + 7);
+        for (int64_t s = 1; s <= 64 && s <= pt * 2; ++s) {
+            const int64_t kper = up(up(pt * 256, s) / s, 32);
+            if (s > 1 && (s - 1) * kper >= pt * 256) continue;
+            const double t_dx = kper / 32 + 6;
+            // one XCD: a tiles of length ta, then b of tb on 32 CUs
+            int64_t na = want_dw ? up(pt * ntd, 8) / 8 : 0, nb = want_dx ? up(ntd * ntr * s, 8) / 8 : 0;
+            double ta = t_dw, tb = t_dx;
+            const bool swap = tb > ta;
+            if (swap) {
+                std::swap(na, nb);
+                std::swap(ta, tb);
+            }
+            const int64_t full = na / 32, rest = na % 32;                // rest CUs are busy until t1, the others from t0 on free
+            const double t0 = full * ta, t1 = rest ? t0 + ta : t0;
+            const int64_t gap = rest ? (int64_t)(ta / tb) * (32 - rest) : 0;  // shorter tiles that fit beside the last long ones
+            double span = t1;
+            if (nb > gap) span = t1 + (double)(up(nb - gap, 32) / 32) * tb;
+            else if (nb) span = std::max(t1, t0 + (double)(up(nb, 32 - rest) / (32 - rest)) * tb);
+            const double slab = want_dx && (n > 1 || s > 1) ? (double)s * N * d * 4 / 3.5e6 : 0.;
+            const double cost = n * (logits + span + 10 + slab * (n > 1 ? 2 : 1)) + (slab > 0 ? slab + 5 : 0.);
+            if (cost < least) {
+                least = cost;
+                best = GradShape{(int)(pt * 256), (int)n, (int)s, (int)kper, (int)(8 * (na + nb)), swap ? 1 : 0};
+            }
+            if (!want_dx) break;
+        }
+    }
+    return best;
+}
+
 struct LinPlan {
     bool big_f, big_g, direct;  // direct: dx comes out of the one product launch
-    int nvb, rows32, piece, splits, kper;
+    int nvb, rows32, piece, splits, kper, dx_first;
     int64_t o_part, o_zlab, o_lse, fwd_bytes;
     int64_t o_lse2, o_coef, o_scale, o_x, o_w, o_dz, o_slab, bwd_bytes;
 };
-static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool want_dx) {
-    LinPlan p;
+static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool backward) {
+    LinPlan p = {};
     const int64_t N = q->N, V = q->V, d = q->d;
     p.big_f = big_tiles(N, V);
     p.nvb = (int)(up(V, p.big_f ? 256 : 128) / (p.big_f ? 128 : 64));
@@ -1136,33 +1193,40 @@ static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool want_dx) {
     p.o_zlab = take(N * 4);
     p.o_lse = take(N * 4);
     p.fwd_bytes = o;
+    if (!backward) return p;
     o = 0;
     p.rows32 = (int)up(N, 32);
-    // dz of a piece stays within 128 MiB (written once, read by two products: it should live in the 256 MiB cache), but never below 2048 classes
-    int64_t piece = std::max<int64_t>(2048, ((int64_t)64 << 20) / p.rows32 / 256 * 256);
-    const int64_t pieces = up(V, piece) / piece;
-    piece = up(up(V, pieces) / pieces, 256);  // equal pieces
-    p.piece = (int)piece;
-    // dx tiles are few (rows x features): the piece's classes are cut into slices of about the dw tiles' length (rows), as long as tiles are missing
-    auto cut = [&](int64_t bt) {
-        const int64_t dxt = (up(N, bt) / bt) * (up(d, bt) / bt);
-        int64_t n = std::min((piece + p.rows32 / 2) / p.rows32, (512 + dxt - 1) / dxt);
-        n = std::max<int64_t>(1, std::min(n, piece / 128));
-        if (pieces == 1 && piece <= 2048) n = 1;  // 64 steps at most: shorter than a launch that adds slices up
-        p.kper = (int)up(up(piece, n) / n, 32);
-        p.splits = (int)(up(piece, p.kper) / p.kper);
-        return dxt * p.splits + (piece / bt) * (up(d, bt) / bt);
-    };
-    p.big_g = cut(256) >= 160;
-    if (!p.big_g) cut(128);
+    // (the plan of the last call is kept, by its sizes: the search takes longer than a launch)
+    static thread_local int64_t last[3] = {-1, -1, -1};
+    static thread_local GradShape shape;
+    if (last[0] != N || last[1] != V || last[2] != d) {
+        shape = grad_shape(N, V, d, p.rows32, true, true);
+        last[0] = N;
+        last[1] = V;
+        last[2] = d;
+    }
+    p.piece = shape.piece;
+    p.splits = shape.splits;
+    p.kper = shape.kper;
+    p.dx_first = shape.dx_first;
+    p.big_g = shape.tiles >= 160;
+    if (!p.big_g) {  // few tiles: one piece; slices of dx about as long as the dw tiles (rows), none where that is 64 steps at most -- less than their addition
+        p.piece = (int)up(V, 256);
+        const int64_t dxt = (up(N, 128) / 128) * (up(d, 128) / 128);
+        int64_t n = std::min<int64_t>((p.piece + p.rows32 / 2) / p.rows32, (512 + dxt - 1) / dxt);
+        n = p.piece <= 2048 ? 1 : std::max<int64_t>(1, std::min<int64_t>(n, p.piece / 128));
+        p.kper = (int)up(up(p.piece, n) / n, 32);
+        p.splits = (int)(up(p.piece, p.kper) / p.kper);
+        p.dx_first = p.kper > p.rows32;
+    }
+    p.direct = p.piece >= V && p.splits == 1;
     p.o_lse2 = take(N * 4);
     p.o_coef = take(N * 4);
     p.o_scale = take(8);
     p.o_x = take((int64_t)p.rows32 * d * 2);
-    p.o_w = q->offset ? take(piece * d * 2) : 0;
-    p.o_dz = take((int64_t)p.rows32 * piece * 2);
-    p.direct = pieces == 1 && p.splits == 1;
-    p.o_slab = want_dx && !p.direct ? take((int64_t)p.splits * N * d * 4) : 0;
+    p.o_w = q->offset ? take((int64_t)p.piece * d * 2) : 0;
+    p.o_dz = take((int64_t)p.rows32 * p.piece * 2);
+    p.o_slab = p.direct ? 0 : take((int64_t)p.splits * N * d * 4);
     p.bwd_bytes = o;
     return p;
 }
@@ -1272,7 +1336,7 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         }
         return 0;
     }
-    const LinPlan p = lin_plan(q, dx != nullptr);
+    const LinPlan p = lin_plan(q, true);
     float *lse2 = (float*)(ws + p.o_lse2), *coef = (float*)(ws + p.o_coef), *os = (float*)(ws + p.o_scale);
     const float spread = q->dtype == CDET_F16 ? 4096.f : 1.f;
     PrepArgs pa = {};
@@ -1355,6 +1419,7 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         g.vk = (int)up(Vp, p.big_f ? 256 : 128);
         g.ntd = div_up(d, bt);
         g.ndw = dw ? g.ntd * div_up(Vp, bt) : 0;
+        g.dx_first = p.dx_first;
         g.ntr = div_up(N, bt);
         g.kper = p.kper;
         g.splits = p.splits;
@@ -1384,7 +1449,7 @@ using namespace cdet;
 
 extern "C" int64_t cdet_linear_loss_ws_bytes(const cdet_linear_loss_desc* d, int32_t backward) {
     if (!d || d->N <= 0 || d->V <= 0 || d->d <= 0) return 256;
-    const LinPlan p = lin_plan(d, true);
+    const LinPlan p = lin_plan(d, backward != 0);
     return backward ? p.bwd_bytes : p.fwd_bytes;
 }
 
@@ -1405,7 +1470,7 @@ extern "C" int cdet_linear_ce_fwd(const cdet_linear_loss_desc* d, const void* x,
     CDET_CHECK_ARG(d->tau == 1.f, "cdet_linear_ce_fwd: tau must be 1 (use scale)");
     CDET_CHECK_ARG(d->N == 0 || (labels && loss && lse), "cdet_linear_ce_fwd: labels, loss and lse must be given");
     if (d->N == 0) return 0;
-    return lin_forward(d, lin_plan(d, true), x, w, labels, loss, lse, (char*)ws, (hipStream_t)stream);
+    return lin_forward(d, lin_plan(d, false), x, w, labels, loss, lse, (char*)ws, (hipStream_t)stream);
 }
 
 extern "C" int cdet_linear_ce_bwd(const cdet_linear_loss_desc* d, const void* x, const void* w, const void* labels, const float* lse, const float* drow, int32_t drow_stride,
@@ -1424,7 +1489,7 @@ extern "C" int cdet_linear_distill_fwd(const cdet_linear_loss_desc* d, const voi
     CDET_CHECK_ARG(val_dtype == CDET_BF16 || val_dtype == CDET_F16 || val_dtype == CDET_F32, "cdet_linear_distill_fwd: val_dtype %d", val_dtype);
     CDET_CHECK_ARG(d->N == 0 || (idx && val && loss && saved), "cdet_linear_distill_fwd: idx, val, loss and saved must be given");
     if (d->N == 0) return 0;
-    const LinPlan p = lin_plan(d, true);
+    const LinPlan p = lin_plan(d, false);
     const bool few = p.nvb <= 64;  // (class_teacher_kernel joins them)
     float* lse = few ? nullptr : (float*)((char*)ws + p.o_lse);
     const float* part = few ? (const float*)((char*)ws + p.o_part) : nullptr;

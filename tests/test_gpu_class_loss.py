@@ -120,7 +120,7 @@ def ce_case(N, V, d, dtype, seed=0):
 
 CE_SIZES = [(1, 1, 8), (1, 2, 8), (3, 5, 16), (1, 1000, 64), (64, 64, 64), (127, 129, 72), (130, 257, 104), (300, 1201, 320), (33, 9001, 264), (257, 128, 40),
             (2600, 3900, 40),   # 256 x 256 tiles
-            (700, 21000, 24),   # the same with classes cut into slices for dx
+            (700, 21000, 24), (1100, 30000, 264),  # the same with classes cut into slices for dx
             (40000, 4500, 16)]  # several pieces of the class list
 
 
