@@ -33,6 +33,10 @@ constexpr unsigned LSENT = 0xE0000000u;   // offset beyond every buffer: the DMA
 constexpr int LCAP = (int)0xD0000000u;    // extent of every buffer descriptor (offsets are at most 256 rows or 32 rows of < 4 M elements)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// bit masks (which rows take part, which classes are not left out), read through the scalar cache: they do not count with the DMA
+typedef const __attribute__((address_space(4))) uint32_t* mask_t;
+__device__ __forceinline__ mask_t as_mask(const uint32_t* p) { return (mask_t)(uintptr_t)p; }
+
 template <int DT>
 __device__ __forceinline__ f32x16 lmfma(const u32x4& a, const u32x4& b, const f32x16& c) {
     if (DT == CDET_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -243,8 +247,9 @@ struct Pipe {
 // The small tile, for launches that leave most of the chip idle: what counts is how long ONE workgroup takes for a step. Four waves (2 x 2) of MT x NT row
 // tiles, no phases: a wave multiplies one half of a step while it reads the next half's fragments, one barrier a step, RING - 1 stages ahead. (As phases of
 // 8 waves, like the large tile, the two products of 997 x 1201 x 320's gradients took 16.1 us, so 13.7; a deeper ring does not help.) Same interface as Pipe; column = wave * NT*32 + nt*32 + (lane&31),
-// wave = 0, 1; run() leaves the LDS free.
-template <int DT, int MT, int NT, bool ATR, bool BTR, int RING>
+// wave = 0, 1; run() leaves the LDS free. Rows and classes that take no part are not read: open() takes a bit per row of B, and (KM) per k of A -- a launch
+// less than copies without them, which the large tile is given instead: in its loop the test costs 3 % of the gradients' products.
+template <int DT, int MT, int NT, bool ATR, bool BTR, int RING, bool KM>
 struct Quad {
     static constexpr int ABYTES = MT * 64 * 64, BBYTES = NT * 64 * 64, STAGE = ABYTES + BBYTES;
     static constexpr int NA = MT, NB = NT, NPW = NA + NB;
@@ -255,6 +260,8 @@ struct Quad {
     const uint16_t *ap, *bp;
     int64_t astep, bstep;
     int krem, fslot;
+    mask_t km;     // k mask: word of the fourth stage from now; w[]: of the next three
+    uint32_t w[3];
 
     __device__ __forceinline__ int k_of(bool tr, int i) const {
         const int id = wave8 + 4 * i;
@@ -285,29 +292,54 @@ struct Quad {
         boff = lds0 + ABYTES + (BTR ? trl + ((wave * NT) >> 1) * 4096 : nrl + wave * NT * 2048);
         fslot = 0;
     }
-    __device__ __forceinline__ void open(const uint16_t* a, int a_rows, const uint16_t* b, int b_rows, int K) {
+    __device__ __forceinline__ void open(const uint16_t* a, int a_rows, const uint16_t* b, int b_rows, int K, const uint32_t* k_mask = nullptr,
+                                         const uint32_t* b_mask = nullptr) {
 #pragma unroll
-        for (int i = 0; i < NA; ++i) ka[i] = row_of(ATR, i) < a_rows ? k_of(ATR, i) : 0x40000000;
+        for (int i = 0; i < NA; ++i) ka[i] = KM ? (row_of(ATR, i) < a_rows ? 1 << k_of(ATR, i) : 0) : row_of(ATR, i) < a_rows ? k_of(ATR, i) : 0x40000000;
 #pragma unroll
-        for (int i = 0; i < NB; ++i) kb[i] = row_of(BTR, i) < b_rows ? k_of(BTR, i) : 0x40000000;
+        for (int i = 0; i < NB; ++i) {
+            bool ok = row_of(BTR, i) < b_rows;
+            if (!BTR && b_mask) {  // (a piece is 16 rows: half a word)
+                const int id = wave8 + 4 * i;
+                ok = ok && ((as_mask(b_mask)[id >> 1] >> ((id & 1) * 16 + (lane >> 2))) & 1);
+            }
+            kb[i] = ok ? k_of(BTR, i) : 0x40000000;
+        }
         ap = a;
         bp = b;
         krem = K;
+        if (KM) {
+            km = as_mask(k_mask);
+            w[0] = km[0];
+            w[1] = km[1];
+            w[2] = km[2];
+            km += 3;
+        }
+    }
+    // KM: ka is the bit of the lane's k, and the stage's word says which k there are
+    __device__ __forceinline__ uint32_t a_word() const { return krem >= LBK ? w[0] : krem > 0 ? w[0] & ((1u << krem) - 1) : 0u; }
+    __device__ __forceinline__ bool a_ok(int i, uint32_t word) const { return KM ? (ka[i] & (int)word) != 0 : ka[i] < krem; }
+    __device__ __forceinline__ uint32_t read_word() { return KM ? *km++ : 0u; }  // (the masks are longer than their numbers by what is read ahead)
+    __device__ __forceinline__ void push_word(uint32_t word) {
+        w[0] = w[1];
+        w[1] = w[2];
+        w[2] = word;
     }
     __device__ __forceinline__ void fetch_a(int i) {
         const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)ap, 0, LCAP, 0x00020000);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(smem + fslot + wave8 * 1024 + i * 4096), 16,
-                                                 (int)(ka[i] < krem ? va[i] : LSENT), 0, 0, 0);
+                                                 (int)(a_ok(i, a_word()) ? va[i] : LSENT), 0, 0, 0);
     }
     __device__ __forceinline__ void fetch_b(int i) {
         const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)bp, 0, LCAP, 0x00020000);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void*)(smem + fslot + ABYTES + wave8 * 1024 + i * 4096), 16,
                                                  (int)(kb[i] < krem ? vb[i] : LSENT), 0, 0, 0);
     }
-    __device__ __forceinline__ void fetched() {
+    __device__ __forceinline__ void fetched(uint32_t word) {
         ap += astep;
         bp += bstep;
         krem -= LBK;
+        if (KM) push_word(word);
         fslot = fslot + STAGE == RING * STAGE ? 0 : fslot + STAGE;
     }
     template <class Next>
@@ -318,7 +350,7 @@ struct Quad {
             for (int i = 0; i < NA; ++i) fetch_a(i);
 #pragma unroll
             for (int i = 0; i < NB; ++i) fetch_b(i);
-            fetched();
+            fetched(read_word());
         }
     }
     __device__ __forceinline__ void start() {
@@ -369,6 +401,8 @@ struct Quad {
             const int ab = aoff + so, bb = boff + so;
             so = so + STAGE == RING * STAGE ? 0 : so + STAGE;
             const int an = aoff + so, bn = boff + so;
+            if (KM) asm volatile("" : "+s"(w[0]), "+s"(w[1]), "+s"(w[2]));
+            const uint32_t word = read_word();
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < NT; ++i) read<BTR>(b[1][i], bl[1][i], bh[1][i], bb, i, 1);
@@ -384,7 +418,7 @@ struct Quad {
                 for (int j = 0; j < NT; ++j) acc[i][j] = lmfma<DT>(a[0][i], b[0][j], acc[i][j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            fetched();
+            fetched(word);
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 2) * NPW) : "memory");  // stage st + 1, and this stage's last fragments
 #pragma unroll
             for (int i = 0; i < NT; ++i) value<BTR>(b[1][i], bl[1][i], bh[1][i]);
@@ -425,8 +459,8 @@ struct Quad {
     }
 };
 constexpr int QRING = 4;
-template <int DT, int MT, int NT, bool ATR, bool BTR, bool WALK>
-using Product = std::conditional_t<MT == 4, Pipe<DT, MT, NT, ATR, BTR, WALK>, Quad<DT, MT, NT, ATR, BTR, QRING>>;
+template <int DT, int MT, int NT, bool ATR, bool BTR, bool WALK, bool KM>
+using Product = std::conditional_t<MT == 4, Pipe<DT, MT, NT, ATR, BTR, WALK>, Quad<DT, MT, NT, ATR, BTR, QRING, KM>>;
 template <int MT> constexpr int kLinThreads = MT == 4 ? 512 : 256;
 template <int MT, int NT> constexpr int kLinCols = MT == 4 ? NT * 128 : NT * 64;  // B rows of a tile (A rows: MT * 64)
 
@@ -447,10 +481,11 @@ struct LogitArgs {
     // backward
     const float* lse2;    // [N] (+inf: the row takes no part)
     const float* coef;    // [N]
+    const uint32_t* live; // small tile: bit per row, takes part (the others' features are not read: 0 * inf and NaN stay out)
     uint16_t* dz;         // [rows][dz_ld]
     int64_t dz_ld;
     int dz_rows;          // rows to be written (N rounded up to 32)
-    const int32_t* idx;   // small tile only: the teacher's slots (patch_teacher), or null
+    const int32_t* idx;   // small tile only: the teacher's slots, or null
     const float* saved;
     int k;
 };
@@ -459,14 +494,22 @@ __device__ __forceinline__ int64_t load_label(const void* p, int is64, int r) {
     return is64 ? reinterpret_cast<const int64_t*>(p)[r] : (int64_t)reinterpret_cast<const int32_t*>(p)[r];
 }
 
-// dz at a class that slot i = (row r, j) of the teacher names: coef * (p - q)
-template <int DT>
-__device__ __forceinline__ void patch_teacher(const float* saved, const float* lse2, const float* coef, int k, int r, int j, uint16_t* at) {
-    const float* sv = saved + (int64_t)r * (1 + 2 * k);
-    const float q = sv[1 + k + j];
-    if (q == -1.f || lse2[r] == INFINITY || sv[1 + j] == -INFINITY) return;  // another slot's, or a row without a part, or a left-out class (no gradient)
-    *at = Elem<DT>::from_f32((__builtin_amdgcn_exp2f(sv[1 + j] - lse2[r]) - q) * coef[r]);
-}
+// dz at the class that slot j of row r names: coef * (p - q)
+struct TeacherDz {
+    float z2, q, l2, g;
+    __device__ __forceinline__ void load(const float* saved, const float* lse2, const float* coef, int k, int r, int j) {
+        const float* sv = saved + (int64_t)r * (1 + 2 * k);
+        z2 = sv[1 + j];
+        q = sv[1 + k + j];
+        l2 = lse2[r];
+        g = coef[r];
+    }
+    template <int DT>
+    __device__ __forceinline__ void store(uint16_t* at) const {
+        if (q == -1.f || l2 == INFINITY || z2 == -INFINITY) return;  // another slot's, or a row without a part, or a left-out class (no gradient)
+        *at = Elem<DT>::from_f32((__builtin_amdgcn_exp2f(z2 - l2) - q) * g);
+    }
+};
 
 // 32 C columns x (HT*32) C rows of 16-bit values through `stg` (wave-private, HT * 2 KiB) as whole rows of the destination: pk[i][q] = the lane's rows
 // 32 i + 8 q + 4 h .. +3 of column l31
@@ -481,17 +524,22 @@ __device__ __forceinline__ void store_rows16(unsigned char* stg, const uint2 (&p
         for (int q = 0; q < 4; ++q) *reinterpret_cast<uint2*>(stg + l31 * RS + (((i * 4 + q) ^ swz(l31)) << 4) + h * 8) = pk[i][q];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    u32x4 v[32 * CH / 64];
 #pragma unroll
     for (int it = 0; it < 32 * CH / 64; ++it) {
         const int id = it * 64 + lane, row = id / CH, ch = id % CH;
-        const u32x4 v = *reinterpret_cast<const u32x4*>(stg + row * RS + ((ch ^ swz(row)) << 4));
-        if (row < nrows && ch * 8 < ncols) *reinterpret_cast<u32x4*>(dst + row * ld + ch * 8) = v;
+        v[it] = *reinterpret_cast<const u32x4*>(stg + row * RS + ((ch ^ swz(row)) << 4));
+    }
+#pragma unroll
+    for (int it = 0; it < 32 * CH / 64; ++it) {
+        const int id = it * 64 + lane, row = id / CH, ch = id % CH;
+        if (row < nrows && ch * 8 < ncols) *reinterpret_cast<u32x4*>(dst + row * ld + ch * 8) = v[it];
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
-// column tile j of the accumulators times f, in halves of MT / 2 row tiles
-template <int DT, int MT, int NT>
+// column tile j of the accumulators (TIMES: times f), in halves of MT / 2 row tiles
+template <int DT, bool TIMES, int MT, int NT>
 __device__ __forceinline__ void store_scaled(unsigned char* stg, const f32x16 (&acc)[MT][NT], int j, float f, int lane, uint16_t* dst, int64_t ld, int nrows, int ncols) {
     constexpr int HT = MT / 2;
 #pragma unroll
@@ -502,8 +550,8 @@ __device__ __forceinline__ void store_scaled(unsigned char* stg, const f32x16 (&
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const f32x16& c = acc[half * HT + i][j];
-                pk[i][q].x = lpack2<DT>(c[4 * q] * f, c[4 * q + 1] * f);
-                pk[i][q].y = lpack2<DT>(c[4 * q + 2] * f, c[4 * q + 3] * f);
+                pk[i][q].x = TIMES ? lpack2<DT>(c[4 * q] * f, c[4 * q + 1] * f) : lpack2<DT>(c[4 * q], c[4 * q + 1]);
+                pk[i][q].y = TIMES ? lpack2<DT>(c[4 * q + 2] * f, c[4 * q + 3] * f) : lpack2<DT>(c[4 * q + 2], c[4 * q + 3]);
             }
         store_rows16<HT>(stg, pk, lane, dst + half * HT * 32, ld, nrows, ncols - half * HT * 32);
     }
@@ -538,19 +586,21 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_logits_kernel(const 
         r = (pr0 + in % pw) * BN;
     };
     place(L, v0, r0);
-    Product<DT, MT, NT, false, false, WALK> p;
+    Product<DT, MT, NT, false, false, WALK, false> p;
     p.init(smem, a.w_ld, a.x_ld);
     int F = L;                       // the tile that is fetched
     auto open = [&]() {
         int v = v0, r = r0;
         const bool more = F < end;
         if (WALK && more && F != L) place(F, v, r);
-        p.open(a.w + (int64_t)v * a.w_ld, more ? a.V - v : 0, a.x + (int64_t)r * a.x_ld, more ? a.N - r : 0, a.d);
+        const uint16_t *w = a.w + (int64_t)v * a.w_ld, *x = a.x + (int64_t)r * a.x_ld;
+        if constexpr (WALK) p.open(w, more ? a.V - v : 0, x, more ? a.N - r : 0, a.d);
+        else p.open(w, a.V - v, x, a.N - r, a.d, nullptr, BWD ? a.live + (r >> 5) : nullptr);
         F += per;
     };
     // offsets of a tile's classes in log2 units, -inf for those left out or behind the last, and which of the writing waves met one. Walking: two tables behind
     // the ring, the next tile's written a tile ahead; else one, in the ring when that has ended
-    constexpr int TABLE = BM + 4, STAGE = Product<DT, MT, NT, false, false, WALK>::STAGE;
+    constexpr int TABLE = BM + 4, STAGE = Product<DT, MT, NT, false, false, WALK, false>::STAGE;
     float* table = reinterpret_cast<float*>(smem + LRING * STAGE);
     const bool writer = a.off && (int)threadIdx.x < BM;
     auto offset = [&](int t) {
@@ -672,18 +722,17 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_logits_kernel(const 
                 }
             }
         } else {
-            float g[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const int r = r0 + (wave * NT + j) * 32 + l31;
                 const bool live = r < a.N;
-                const float l2 = live ? a.lse2[r] : INFINITY;
-                g[j] = live ? a.coef[r] : 0.f;
+                const float l2 = live ? a.lse2[r] : INFINITY, g = live ? a.coef[r] : 0.f, mag = fabsf(g);
                 const int64_t at = a.label && live ? load_label(a.label, a.label64, r) - a.v_first - vw : -1;
+                const float l2g = l2 - __builtin_amdgcn_logf(mag);  // |g| p = exp2(t - lse + log2 |g|): nothing for g = 0
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, -l2));
+                    for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, -l2g));
                 bool mine = at >= 0 && at < MT * 32 && vw + at < a.V && (((int)at >> 2) & 1) == h;
                 if (a.off && mine) mine = offw[(int)at] != -INFINITY;  // (a left-out class gets no gradient)
                 if (__ballot(mine)) {
@@ -691,22 +740,42 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_logits_kernel(const 
 #pragma unroll
                     for (int i = 0; i < MT; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) acc[i][j][e] -= mine && slot == i * 16 + e ? 1.f : 0.f;
+                        for (int e = 0; e < 16; ++e) acc[i][j][e] -= mine && slot == i * 16 + e ? mag : 0.f;
+                }
+                if (__ballot(g < 0.f)) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[i][j][e] = g < 0.f ? -acc[i][j][e] : acc[i][j][e];
                 }
             }
             p.settle();
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const int rr = r0 + (wave * NT + j) * 32;
-                store_scaled<DT, MT, NT>(stg, acc, j, g[j], lane, a.dz + (int64_t)rr * a.dz_ld + vw, a.dz_ld, a.dz_rows - rr, MT * 32);
+                store_scaled<DT, false>(stg, acc, j, 1.f, lane, a.dz + (int64_t)rr * a.dz_ld + vw, a.dz_ld, a.dz_rows - rr, MT * 32);
             }
         }
         if (!WALK && BWD && a.idx) {
             __syncthreads();  // the tile is written: the entries that the teacher names may follow
             const int rows = min(BN, a.N - r0), V = min(BM, a.V - v0);
-            for (int i = (int)threadIdx.x; i < rows * a.k; i += kLinThreads<MT>) {
-                const int r = r0 + i / a.k, j = i % a.k, v = a.idx[(int64_t)r0 * a.k + i] - a.v_first - v0;
-                if ((unsigned)v < (unsigned)V) patch_teacher<DT>(a.saved, a.lse2, a.coef, a.k, r, j, a.dz + r * a.dz_ld + v0 + v);
+            constexpr int U = 8;  // slots of a thread in flight
+            const int n = rows * a.k;
+            for (int i0 = (int)threadIdx.x; i0 < n; i0 += U * kLinThreads<MT>) {
+                int v[U], r[U];
+                TeacherDz t[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int i = i0 + u * kLinThreads<MT>;
+                    v[u] = -1;
+                    if (i >= n) continue;
+                    r[u] = r0 + i / a.k;
+                    v[u] = a.idx[(int64_t)r0 * a.k + i] - a.v_first - v0;
+                    t[u].load(a.saved, a.lse2, a.coef, a.k, r[u], i % a.k);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if ((unsigned)v[u] < (unsigned)V) t[u].template store<DT>(a.dz + r[u] * a.dz_ld + v0 + v[u]);
             }
         }
         L += per;
@@ -719,10 +788,11 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_logits_kernel(const 
 
 // ---- second product of the backward: a piece's dw tiles and dx tiles in one launch -----------------------------------------------------------------
 struct GradArgs {
-    const uint16_t* x;    // [rows32][d], rows without a part zeroed
-    const uint16_t* w;    // [Vp][w_ld], first class of the piece
+    const uint16_t* x;    // [N][x_ld]; large tile: with zeros in the rows that take no part
+    const uint16_t* w;    // [Vp][w_ld], first class of the piece; large tile: with zeros in left-out classes
     const uint16_t* dz;   // [rows32][dz_ld]
-    int64_t w_ld, dz_ld;
+    const uint32_t *live, *kept;  // small tile: bit per row, takes part; per class of the piece, not left out. The others are not read: 0 * inf and NaN stay out
+    int64_t x_ld, w_ld, dz_ld;
     int N, rows32, d, Vp; // Vp: classes of the piece
     int vk;               // columns of dz that hold numbers (Vp rounded up to the tile)
     int ntd, ndw, ndx;    // tiles along d; dw tiles, dx tiles
@@ -759,10 +829,11 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_grads_kernel(const G
     f32x16 acc[MT][NT];
     if (is_dw) {  // dw[v][f] = sum_r dz[r][v] x[r][f]
         const int f0 = (L % a.ntd) * BM, v0 = (L / a.ntd) * BN;
-        Product<DT, MT, NT, true, true, false> p;
+        Product<DT, MT, NT, true, true, false, MT == 2> p;
         auto none = []() {};
-        p.init(smem, a.d, a.dz_ld);
-        p.open(a.x + f0, a.d - f0, a.dz + v0, a.vk - v0, a.rows32);
+        p.init(smem, a.x_ld, a.dz_ld);
+        if constexpr (MT == 4) p.open(a.x + f0, a.d - f0, a.dz + v0, a.vk - v0, a.N);
+        else p.open(a.x + f0, a.d - f0, a.dz + v0, a.vk - v0, a.N, a.live);
         p.prime(none);
         p.start();
         p.run(a.rows32 / LBK, acc, none);
@@ -771,18 +842,20 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_grads_kernel(const G
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int v = v0 + (wave * NT + j) * 32, f = f0 + grp * MT * 32;
-            store_scaled<DT, MT, NT>(stg, acc, j, os, lane, a.dw + (int64_t)v * a.dw_ld + f, a.dw_ld, a.Vp - v, a.d - f);
+            store_scaled<DT, true>(stg, acc, j, os, lane, a.dw + (int64_t)v * a.dw_ld + f, a.dw_ld, a.Vp - v, a.d - f);
         }
         return;
     }
     // dx[r][f] += sum over the slice's classes of dz[r][v] w[v][f]
     const int f0 = (L % a.ntd) * BM, r0 = (L / a.ntd % a.ntr) * BN, s = L / a.ntd / a.ntr;
-    const int k0 = s * a.kper, k = max(0, min(a.kper, a.Vp - k0));
+    const int k0 = min(s * a.kper, a.Vp), k = min(a.kper, a.Vp - k0);
     {
-        Product<DT, MT, NT, true, false, false> p;
+        Product<DT, MT, NT, true, false, false, MT == 2> p;
         auto none = []() {};
         p.init(smem, a.w_ld, a.dz_ld);
-        p.open(a.w + (int64_t)k0 * a.w_ld + f0, a.d - f0, a.dz + (int64_t)r0 * a.dz_ld + k0, a.rows32 - r0, k);
+        const uint16_t *w = a.w + (int64_t)k0 * a.w_ld + f0, *dz = a.dz + (int64_t)r0 * a.dz_ld + k0;
+        if constexpr (MT == 4) p.open(w, a.d - f0, dz, a.rows32 - r0, k);
+        else p.open(w, a.d - f0, dz, a.rows32 - r0, k, a.kept + (k0 >> 5));
         p.prime(none);
         p.start();
         p.run((k + LBK - 1) / LBK, acc, none);
@@ -793,7 +866,7 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_grads_kernel(const G
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int r = r0 + (wave * NT + j) * 32, f = f0 + grp * MT * 32;
-            store_scaled<DT, MT, NT>(stg, acc, j, os, lane, a.dx + (int64_t)r * a.dx_ld + f, a.dx_ld, a.N - r, a.d - f);
+            store_scaled<DT, true>(stg, acc, j, os, lane, a.dx + (int64_t)r * a.dx_ld + f, a.dx_ld, a.N - r, a.d - f);
         }
         return;
     }
@@ -873,8 +946,8 @@ __global__ __launch_bounds__(1024) void class_lse_kernel(const float* part, int 
     }
 }
 
-// The backward's inputs, in one launch: lse and coefficient of every row, x contiguous with the rows that take no part (and those behind the last)
-// zeroed, and, where classes can be left out, w with those zeroed -- so that 0 * inf and NaN stay out of the products.
+// What the backward needs of every row -- lse, coefficient, whether it takes part -- and which classes are not left out; and, for the large tile, x with
+// zeros in the rows that take no part and, where classes can be left out, w of the first piece with zeros in those (0 * inf and NaN stay out).
 // A row's coefficient is g_r times what brings the largest |g| of the rows that take part to 1.984375 (fp16: times 2^12): the entries of dz that matter
 // most, g (p - 1) at the labels of rows with the largest weight (of all rows, under a mean), then lie at the top of a binade, where rounding to 16 bits
 // costs half of what it does at its bottom; and dz stays inside fp16's range. Every workgroup finds the maximum for itself (N up to 32768: 16 bytes a row
@@ -886,18 +959,19 @@ struct PrepArgs {
     int label64;
     const float* lse;
     int64_t lse_stride;
-    int N, V, rows32, d8;
+    int N, V;
     float gain, spread;
     const float* gmax;          // null: find it
-    const uint16_t *x, *w;
-    int64_t x_ld, w_ld;
-    const float* off;           // of w's classes; w null: no copy
-    int Vp;
+    const float* off;           // [V] or null
     float *lse2, *coef, *outscale;
+    uint32_t *live, *kept;
+    const uint16_t *x, *w;      // null: no copy
+    int64_t x_ld, w_ld;
+    int d8, Vp;
     u32x4 *xo, *wo;
 };
-__device__ __forceinline__ bool prep_live(const PrepArgs& a, int r) {
-    const float l = a.lse[(int64_t)r * a.lse_stride];
+__device__ __forceinline__ bool prep_live(const PrepArgs& a, int64_t r) {
+    const float l = a.lse[r * a.lse_stride];
     if (!a.label) return l != INFINITY;  // (the teacher's mark)
     if (l == -INFINITY) return false;
     const int64_t lab = load_label(a.label, a.label64, r);
@@ -927,38 +1001,37 @@ __global__ __launch_bounds__(1024) void class_prep_kernel(const PrepArgs a) {
     float m = a.gmax ? *a.gmax : prep_max(a);
     m = m > 0.f ? fminf(fmaxf(m, 1e-30f), 1e37f) : 1.f;
     const float down = 1.984375f * a.spread / m;
-    for (int64_t r = t; r < a.N; r += nt) {
-        const bool on = prep_live(a, (int)r);
+    for (int64_t r = t; r - (t & 63) < a.N; r += nt) {  // (whole waves: a wave writes 64 bits)
+        const bool on = r < a.N && prep_live(a, r);
+        const uint64_t bits = __ballot(on);
+        if ((t & 63) == 0) *reinterpret_cast<uint64_t*>(a.live + (r >> 5)) = bits;
+        if (r >= a.N) continue;
         const float g = a.drow ? a.drow[r * a.drow_stride] : 1.f;
         const float l = a.lse[r * a.lse_stride] * kLog2e;
         a.lse2[r] = !on ? INFINITY : l == INFINITY ? NAN : l;  // +inf marks a row without a part; an infinite logit gives NaN gradients
         a.coef[r] = on ? g * down : 0.f;
     }
+    for (int64_t v = t; v - (t & 63) < a.V; v += nt) {
+        const uint64_t bits = __ballot(v < a.V && (!a.off || a.off[v] != -INFINITY));
+        if ((t & 63) == 0) *reinterpret_cast<uint64_t*>(a.kept + (v >> 5)) = bits;
+    }
     if (t == 0) *a.outscale = a.gain * m / (1.984375f * a.spread);
-    const int64_t nx = (int64_t)a.rows32 * a.d8;
-    for (int64_t i = t; i < nx; i += nt) {
-        const int r = (int)(i / a.d8), c = (int)(i - (int64_t)r * a.d8);
-        u32x4 v = {0, 0, 0, 0};
-        if (r < a.N && prep_live(a, r)) v = *reinterpret_cast<const u32x4*>(a.x + r * a.x_ld + c * 8);
-        a.xo[i] = v;
-    }
-    if (!a.w) return;
-    const int64_t nw = (int64_t)a.Vp * a.d8;
-    for (int64_t i = t; i < nw; i += nt) {
-        const int r = (int)(i / a.d8), c = (int)(i - (int64_t)r * a.d8);
-        u32x4 v = {0, 0, 0, 0};
-        if (a.off[r] != -INFINITY) v = *reinterpret_cast<const u32x4*>(a.w + r * a.w_ld + c * 8);
-        a.wo[i] = v;
-    }
+    if (a.x)
+        for (int64_t i = t; i < (int64_t)a.N * a.d8; i += nt) {
+            const int64_t r = i / a.d8, c = i - r * a.d8;
+            a.xo[i] = prep_live(a, r) ? *reinterpret_cast<const u32x4*>(a.x + r * a.x_ld + c * 8) : u32x4{0, 0, 0, 0};
+        }
+    if (a.w)
+        for (int64_t i = t; i < (int64_t)a.Vp * a.d8; i += nt) {
+            const int64_t v = i / a.d8, c = i - v * a.d8;
+            a.wo[i] = a.off[v] != -INFINITY ? *reinterpret_cast<const u32x4*>(a.w + v * a.w_ld + c * 8) : u32x4{0, 0, 0, 0};
+        }
 }
-// a later piece's weights with the left-out classes zeroed
+// a later piece's weights with zeros in the left-out classes
 __global__ __launch_bounds__(256) void class_weights_kernel(const uint16_t* w, int64_t ld, const float* off, int V, int d8, u32x4* out) {
-    const int64_t n = (int64_t)V * d8;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int r = (int)(i / d8), c = (int)(i - (int64_t)r * d8);
-        u32x4 v = {0, 0, 0, 0};
-        if (off[r] != -INFINITY) v = *reinterpret_cast<const u32x4*>(w + r * ld + c * 8);
-        out[i] = v;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)V * d8; i += (int64_t)gridDim.x * 256) {
+        const int64_t v = i / d8, c = i - v * d8;
+        out[i] = off[v] != -INFINITY ? *reinterpret_cast<const u32x4*>(w + v * ld + c * 8) : u32x4{0, 0, 0, 0};
     }
 }
 template <int DT>
@@ -1117,7 +1190,9 @@ __global__ __launch_bounds__(256) void class_teacher_dz_kernel(const int32_t* id
     const int v = idx[i];
     if (v < v_first || v - v_first >= Vp) return;
     const int r = (int)(i / k), j = (int)(i - (int64_t)r * k);
-    patch_teacher<DT>(saved, lse2, coef, k, r, j, dz + r * dz_ld + (v - v_first));
+    TeacherDz t;
+    t.load(saved, lse2, coef, k, r, j);
+    t.store<DT>(dz + r * dz_ld + (v - v_first));
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------------------------------
@@ -1176,7 +1251,7 @@ struct LinPlan {
     bool big_f, big_g, direct;  // direct: dx comes out of the one product launch
     int nvb, rows32, piece, splits, kper, dx_first;
     int64_t o_part, o_zlab, o_lse, fwd_bytes;
-    int64_t o_lse2, o_coef, o_scale, o_x, o_w, o_dz, o_slab, bwd_bytes;
+    int64_t o_lse2, o_coef, o_scale, o_live, o_kept, o_x, o_w, o_dz, o_slab, bwd_bytes;
 };
 static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool backward) {
     LinPlan p = {};
@@ -1223,8 +1298,10 @@ static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool backward) {
     p.o_lse2 = take(N * 4);
     p.o_coef = take(N * 4);
     p.o_scale = take(8);
-    p.o_x = take((int64_t)p.rows32 * d * 2);
-    p.o_w = q->offset ? take((int64_t)p.piece * d * 2) : 0;
+    p.o_live = take(up(N, 256) / 8 + 64);  // (bits; 64 bytes more than they need are read)
+    p.o_kept = take(up(V, 256) / 8 + 64);
+    p.o_x = p.big_f || p.big_g ? take(N * d * 2) : 0;
+    p.o_w = (p.big_f || p.big_g) && q->offset ? take((int64_t)p.piece * d * 2) : 0;
     p.o_dz = take((int64_t)p.rows32 * p.piece * 2);
     p.o_slab = p.direct ? 0 : take((int64_t)p.splits * N * d * 4);
     p.bwd_bytes = o;
@@ -1348,20 +1425,24 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
     pa.lse_stride = lse_stride;
     pa.N = N;
     pa.V = V;
-    pa.rows32 = p.rows32;
-    pa.d8 = d / 8;
     pa.gain = q->scale * (idx ? q->tau : 1.f);
     pa.spread = spread;
-    pa.x = (const uint16_t*)x;
-    pa.x_ld = q->x_ld;
+    pa.off = q->offset;
     pa.lse2 = lse2;
     pa.coef = coef;
     pa.outscale = os;
-    pa.xo = (u32x4*)(ws + p.o_x);
-    if (q->offset) {
+    pa.live = (uint32_t*)(ws + p.o_live);
+    pa.kept = (uint32_t*)(ws + p.o_kept);
+    pa.x_ld = q->x_ld;
+    pa.w_ld = q->w_ld;
+    pa.d8 = d / 8;
+    const bool copy_x = p.big_f || p.big_g, copy_w = copy_x && q->offset;
+    if (copy_x) {
+        pa.x = (const uint16_t*)x;
+        pa.xo = (u32x4*)(ws + p.o_x);
+    }
+    if (copy_w) {
         pa.w = (const uint16_t*)w;
-        pa.w_ld = q->w_ld;
-        pa.off = q->offset;
         pa.Vp = std::min(V, p.piece);
         pa.wo = (u32x4*)(ws + p.o_w);
     }
@@ -1370,22 +1451,26 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         CDET_LAUNCH_CHECK();
         pa.gmax = os + 1;
     }
-    class_prep_kernel<<<dim3((unsigned)std::min<int64_t>(N > 8192 ? 1024 : 256, div_up((int64_t)(p.rows32 + pa.Vp) * pa.d8, 1024))), dim3(1024), 0, s>>>(pa);
+    const int64_t most = std::max<int64_t>(std::max(N, V), copy_x ? ((int64_t)N + pa.Vp) * (d / 8) : 0);
+    class_prep_kernel<<<dim3((unsigned)std::min<int64_t>(N > 8192 ? 1024 : 256, div_up(most, 1024))), dim3(1024), 0, s>>>(pa);
     CDET_LAUNCH_CHECK();
     const int bt = p.big_g ? 256 : 128;
     for (int v0 = 0; v0 < V; v0 += p.piece) {
         const int Vp = std::min(p.piece, V - v0);
         LogitArgs a = logit_args(q);
-        a.x = (const uint16_t*)(ws + p.o_x);
-        a.x_ld = d;
+        a.x = copy_x ? (const uint16_t*)(ws + p.o_x) : (const uint16_t*)x;
+        a.x_ld = copy_x ? d : q->x_ld;
         a.w = (const uint16_t*)w + (int64_t)v0 * q->w_ld;
-        if (q->offset) {
-            if (v0)
-                class_weights_kernel<<<dim3(std::min<int64_t>(2048, div_up((int64_t)Vp * (d / 8), 256))), dim3(256), 0, s>>>(a.w, q->w_ld, q->offset + v0, Vp, d / 8,
-                                                                                                                            (u32x4*)(ws + p.o_w));
+        a.off = q->offset ? q->offset + v0 : nullptr;
+        a.live = pa.live;
+        if (copy_w) {
+            if (v0) {
+                class_weights_kernel<<<dim3((unsigned)std::min<int64_t>(2048, div_up((int64_t)Vp * (d / 8), 256))), dim3(256), 0, s>>>(a.w, q->w_ld, a.off, Vp, d / 8,
+                                                                                                                                  (u32x4*)(ws + p.o_w));
+                CDET_LAUNCH_CHECK();
+            }
             a.w = (const uint16_t*)(ws + p.o_w);
             a.w_ld = d;
-            a.off = q->offset + v0;
         }
         a.V = Vp;
         a.label = label;
@@ -1410,6 +1495,9 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         g.x = a.x;
         g.w = a.w;
         g.dz = a.dz;
+        g.live = pa.live;
+        g.kept = pa.kept + (v0 >> 5);
+        g.x_ld = a.x_ld;
         g.w_ld = a.w_ld;
         g.dz_ld = a.dz_ld;
         g.N = N;
