@@ -797,13 +797,15 @@ struct GradArgs {
     int vk;               // columns of dz that hold numbers (Vp rounded up to the tile)
     int ntd, ndw, ndx;    // tiles along d; dw tiles, dx tiles
     int dx_first;
-    int ntr, splits, kper;// dx: row tiles, slices of the piece, classes per slice (a multiple of 32)
+    int ntr, kper;        // dx: row tiles, classes per slice of the piece (a multiple of 32)
+    int wsplits, rper;    // dw: slices of the rows, rows per slice (a multiple of 32)
     uint16_t* dw;         // [Vp][dw_ld]
     int64_t dw_ld;
     uint16_t* dx;         // one piece, one slice: dx itself; else null and
     int64_t dx_ld;
-    float* slab;          // [splits][N][d]
-    int add;              // slabs hold earlier pieces
+    float* slab;          // dx [slices][N][d], and
+    int add;              // whether it holds earlier pieces
+    float* wslab;         // more than one slice of the rows: [slices][Vp][d]
     const float* outscale;
 };
 
@@ -827,17 +829,44 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_grads_kernel(const G
     }
     unsigned char* stg = smem + wave8 * (MT * 1024);
     f32x16 acc[MT][NT];
-    if (is_dw) {  // dw[v][f] = sum_r dz[r][v] x[r][f]
-        const int f0 = (L % a.ntd) * BM, v0 = (L / a.ntd) * BN;
+    // column tile j of the accumulators onto rows of a slab
+    auto onto = [&](float* slab, int j, int row0, int rows, int f0, bool add) {
+        const int r = row0 + (wave * NT + j) * 32 + l31;
+        if (r >= rows) return;
+        f32x4 *p = reinterpret_cast<f32x4*>(slab + (int64_t)r * a.d), old[MT][4];
+        const int c0 = f0 + grp * MT * 32 + h * 4;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                old[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (add && c0 + i * 32 + q * 8 < a.d) old[i][q] = p[(c0 + i * 32 + q * 8) >> 2];
+            }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c0 + i * 32 + q * 8 < a.d)
+                    p[(c0 + i * 32 + q * 8) >> 2] = old[i][q] + f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    };
+    if (is_dw) {  // dw[v][f] = sum over the slice's rows of dz[r][v] x[r][f]
+        const int nvt = a.ndw / (a.ntd * a.wsplits), f0 = (L % a.ntd) * BM, v0 = (L / a.ntd % nvt) * BN, s = L / a.ntd / nvt;
+        const int k0 = min(s * a.rper, a.N), k = min(a.rper, a.N - k0);
         Product<DT, MT, NT, true, true, false, MT == 2> p;
         auto none = []() {};
         p.init(smem, a.x_ld, a.dz_ld);
-        if constexpr (MT == 4) p.open(a.x + f0, a.d - f0, a.dz + v0, a.vk - v0, a.N);
-        else p.open(a.x + f0, a.d - f0, a.dz + v0, a.vk - v0, a.N, a.live);
+        const uint16_t *x = a.x + (int64_t)k0 * a.x_ld + f0, *dz = a.dz + (int64_t)k0 * a.dz_ld + v0;
+        if constexpr (MT == 4) p.open(x, a.d - f0, dz, a.vk - v0, k);
+        else p.open(x, a.d - f0, dz, a.vk - v0, k, a.live + (k0 >> 5));
         p.prime(none);
         p.start();
-        p.run(a.rows32 / LBK, acc, none);
+        p.run((k + LBK - 1) / LBK, acc, none);
         p.drain();
+        if (a.wsplits > 1) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) onto(a.wslab + (int64_t)s * a.Vp * a.d, j, v0, a.Vp, f0, false);
+            return;
+        }
         const float os = *a.outscale;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -870,27 +899,8 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_grads_kernel(const G
         }
         return;
     }
-    float* slab = a.slab + (int64_t)s * a.N * a.d;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int r = r0 + (wave * NT + j) * 32 + l31;
-        if (r >= a.N) continue;
-        f32x4 *p = reinterpret_cast<f32x4*>(slab + (int64_t)r * a.d), old[MT][4];
-        const int c0 = f0 + grp * MT * 32 + h * 4;
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                old[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (a.add && c0 + i * 32 + q * 8 < a.d) old[i][q] = p[(c0 + i * 32 + q * 8) >> 2];
-            }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (c0 + i * 32 + q * 8 < a.d)
-                    p[(c0 + i * 32 + q * 8) >> 2] = old[i][q] + f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-    }
+    for (int j = 0; j < NT; ++j) onto(a.slab + (int64_t)s * a.N * a.d, j, r0, a.N, f0, a.add);
 }
 
 // ---- small launches ----------------------------------------------------------------------------------------------------------------------------------
@@ -1034,19 +1044,30 @@ __global__ __launch_bounds__(256) void class_weights_kernel(const uint16_t* w, i
         out[i] = off[v] != -INFINITY ? *reinterpret_cast<const u32x4*>(w + v * ld + c * 8) : u32x4{0, 0, 0, 0};
     }
 }
+// slices' slabs -> 16-bit, in a fixed order; blockIdx.y: which of two
+struct SumArgs {
+    const float* slab[2];
+    uint16_t* out[2];
+    int64_t ld[2];
+    int rows[2], slices[2];
+    int d;
+    const float* outscale;
+};
 template <int DT>
-__global__ __launch_bounds__(256) void class_dx_kernel(const float* slab, int splits, int N, int d, const float* outscale, uint16_t* dx, int64_t ld) {
-    const int d4 = d >> 2;
-    const int64_t n = (int64_t)N * d4;
-    const float os = *outscale;
+__global__ __launch_bounds__(256) void class_sum_kernel(const SumArgs a) {
+    const int w = (int)blockIdx.y, d4 = a.d >> 2, slices = a.slices[w];
+    const int64_t n = (int64_t)a.rows[w] * d4, ld = a.ld[w];
+    const f32x4* slab = reinterpret_cast<const f32x4*>(a.slab[w]);
+    uint16_t* out = a.out[w];
+    const float os = *a.outscale;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        f32x4 v = reinterpret_cast<const f32x4*>(slab)[i];
-        for (int s = 1; s < splits; ++s) v += reinterpret_cast<const f32x4*>(slab)[(int64_t)s * n + i];
+        f32x4 v = slab[i];
+        for (int s = 1; s < slices; ++s) v += slab[(int64_t)s * n + i];
         const int64_t r = i / d4;
         uint2 o;
         o.x = lpack2<DT>(v[0] * os, v[1] * os);
         o.y = lpack2<DT>(v[2] * os, v[3] * os);
-        *reinterpret_cast<uint2*>(dx + r * ld + (i - r * d4) * 4) = o;
+        *reinterpret_cast<uint2*>(out + r * ld + (i - r * d4) * 4) = o;
     }
 }
 __global__ __launch_bounds__(256) void class_zero_kernel(uint16_t* p, int64_t rows, int64_t ld, int d) {
@@ -1198,60 +1219,77 @@ __global__ __launch_bounds__(256) void class_teacher_dz_kernel(const int32_t* id
 // ---- host --------------------------------------------------------------------------------------------------------------------------------------------
 static inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 // 256 x 256 tiles read 131 FLOP per byte staged, 128 x 128 tiles half of that, so the large ones are taken wherever they fill most of the 256 CUs
-static inline bool big_tiles(int64_t rows, int64_t cols) { return (up(rows, 256) / 256) * (up(cols, 256) / 256) >= 160; }
+// (130 x 65536 x 1024 forward 34 us against 42) and the rows more than half of one (1 x 131072 x 1024: 50 against 43)
+static inline bool big_tiles(int64_t rows, int64_t cols) { return rows > 128 && (up(rows, 256) / 256) * (up(cols, 256) / 256) >= 160; }
 
-// The backward's shape: how many pieces the class list is cut into, and each piece's classes into how many slices for dx (whose tiles, rows x features, are
-// few). Costs in steps of the large tile (0.86 us): a tile of K costs K / 32 + 6; a launch is as long as the busiest of an XCD's 32 CUs, longer kind of
-// tile first, and 5 more; a slice's fp32 slab is written (and read, from the second piece on) at 3.5 MB a step. dz of a piece stays within 192 MiB, so that
-// it lives in the 256 MiB cache between its three uses. 4096 x 65536 x 640: 4 pieces of 4 slices, by equal lengths, took 4 x 219 us for the products,
-// 3 pieces of 5 take 3 x 244.
+// The backward's shape: tile, pieces that the class list is cut into, and slices of a piece's classes for dx and of the rows for dw, whose tiles may be few
+// (dx: rows x features; dw: classes x features). Times in us, measured: a step of the large tile 0.86, of the small one 0.3 alone on its CU and 0.62 as one of
+// two; a tile 6 (8, 5) steps more than its K / 32 (the large one 12 where the two are compared: the estimate is short where
+// its tiles are short); a launch is as long as the busiest of an XCD's 32 CUs (64 places), the longer kind of tile first, and 4
+// more; slabs of slices move at 4 MB/us.
+// dz of a piece stays within 192 MiB, so that it lives in the 256 MiB cache between its three uses.
+// 4096 x 65536 x 640: 4 pieces of 4 slices, by equal lengths, took 4 x 219 us for the products, 3 pieces of 5 take 3 x 242; 8400 x 1203 x 1024: @
 struct GradShape {
-    int piece, pieces, splits, kper, tiles, dx_first;
+    int big, piece, pieces, splits, kper, wsplits, rper, dx_first;
 };
-static GradShape grad_shape(int64_t N, int64_t V, int64_t d, int64_t rows32, bool want_dx, bool want_dw) {
-    const int64_t ntd = up(d, 256) / 256, ntr = up(N, 256) / 256, Vt = up(V, 256) / 256;
-    const int64_t most = std::max<int64_t>(8, ((int64_t)96 << 20) / rows32 / 256);  // class tiles of a piece
-    GradShape best = {};
-    double least = 1e30;
-    const int64_t n0 = up(Vt, most) / most;
-    for (int64_t n = n0; n <= 2 * n0 + 2 && n <= Vt; ++n) {
-        const int64_t pt = up(Vt, n) / n;  // class tiles of a piece
-        const double t_dw = rows32 / 32 + 6, logits = (double)(up(pt * ntr, 256) / 256) * (double)(d / 32 + 7);
-        for (int64_t s = 1; s <= 64 && s <= pt * 2; ++s) {
-            const int64_t kper = up(up(pt * 256, s) / s, 32);
-            if (s > 1 && (s - 1) * kper >= pt * 256) continue;
-            const double t_dx = kper / 32 + 6;
-            // one XCD: a tiles of length ta, then b of tb on 32 CUs
-            int64_t na = want_dw ? up(pt * ntd, 8) / 8 : 0, nb = want_dx ? up(ntd * ntr * s, 8) / 8 : 0;
-            double ta = t_dw, tb = t_dx;
-            const bool swap = tb > ta;
-            if (swap) {
-                std::swap(na, nb);
-                std::swap(ta, tb);
+static double grad_span(int64_t na, double ta, int64_t nb, double tb, int64_t places) {  // a tiles of ta, then b of tb <= ta
+    const int64_t full = na / places, rest = na % places;
+    const double t0 = full * ta, t1 = rest ? t0 + ta : t0;  // `rest` places are busy until t1, the others free from t0 on
+    if (!nb) return t1;
+    const int64_t gap = rest ? (int64_t)(ta / tb) * (places - rest) : 0;
+    if (nb > gap) return t1 + (double)((nb - gap + places - 1) / places) * tb;
+    return std::max(t1, t0 + (double)((nb + places - rest - 1) / (places - rest)) * tb);
+}
+static GradShape grad_shape(int64_t N, int64_t V, int64_t d) {
+    static const int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 14, 16, 20, 24, 32, 48, 64};
+    const int64_t rows32 = up(N, 32);
+    GradShape best = {}, of_big = {};
+    double least = 1e30, least_big = 1e30, more = 0.;  // more: what 6 steps a tile add to of_big
+    for (int big = 0; big < 2; ++big) {
+        const int64_t bt = big ? 256 : 128;
+        const int64_t ntd = up(d, bt) / bt, ntr = up(N, bt) / bt, Vt = up(V, 256) / 256;
+        const int64_t most = std::max<int64_t>(8, ((int64_t)96 << 20) / rows32 / 256), n0 = up(Vt, most) / most;  // 256-class tiles of a piece; pieces
+        for (int64_t n = n0; n <= 2 * n0 + 2 && n <= Vt; ++n) {
+            if (!big && n > 1) break;
+            const int64_t pc = up(Vt, n) / n * 256;
+            const double logits = n > 1 ? (double)(up(pc / 256 * up(N, 256) / 256, 256) / 256) * (double)(d / 32 + 7) * 0.86 : 0.;
+            for (int sw : kCuts) {
+                const int64_t rper = up(up(rows32, sw) / sw, 32);
+                if (sw > 1 && (rper < 256 || (sw - 1) * rper >= rows32)) break;
+                for (int sx : kCuts) {
+                    const int64_t kper = up(up(pc, sx) / sx, 32);
+                    if (sx > 1 && (kper < 256 || (sx - 1) * kper >= pc)) break;
+                    int64_t na = up(pc / bt * ntd * sw, 8) / 8, nb = up(ntr * ntd * sx, 8) / 8;
+                    const bool pairs = !big && na + nb > 32;
+                    const double step = big ? 0.86 : pairs ? 0.3 + 0.01 * std::min<int64_t>(na + nb - 32, 32) : 0.3, fixed = big ? 6 : pairs ? 5 : 8;
+                    const int64_t places = pairs ? 64 : 32;
+                    double ta = (rper / 32 + fixed) * step, tb = (kper / 32 + fixed) * step;
+                    const bool swap = tb > ta;
+                    if (swap) {
+                        std::swap(na, nb);
+                        std::swap(ta, tb);
+                    }
+                    const double xslab = n > 1 || sx > 1 ? (double)sx * N * d * 4 / 4e6 : 0., wslab = sw > 1 ? (double)sw * pc * d * 4 / 4e6 : 0.;
+                    const double cost = n * (logits + grad_span(na, ta, nb, tb, places) + 4 + xslab * (n > 1 ? 2 : 1) + wslab * 2) + xslab +
+                                        (n > 1 ? n * (wslab > 0 ? 4 : 0) + (xslab > 0 ? 4 : 0) : xslab + wslab > 0 ? 4 : 0);
+                    if (cost < (big ? least_big : least)) {
+                        (big ? least_big : least) = cost;
+                        (big ? of_big : best) = GradShape{big, (int)pc, (int)n, sx, (int)kper, sw, (int)rper, swap ? 1 : 0};
+                        if (big) more = (double)n * ((na + nb + 31) / 32) * 6 * 0.86;
+                    }
+                }
             }
-            const int64_t full = na / 32, rest = na % 32;                // rest CUs are busy until t1, the others from t0 on free
-            const double t0 = full * ta, t1 = rest ? t0 + ta : t0;
-            const int64_t gap = rest ? (int64_t)(ta / tb) * (32 - rest) : 0;  // shorter tiles that fit beside the last long ones
-            double span = t1;
-            if (nb > gap) span = t1 + (double)(up(nb - gap, 32) / 32) * tb;
-            else if (nb) span = std::max(t1, t0 + (double)(up(nb, 32 - rest) / (32 - rest)) * tb);
-            const double slab = want_dx && (n > 1 || s > 1) ? (double)s * N * d * 4 / 3.5e6 : 0.;
-            const double cost = n * (logits + span + 10 + slab * (n > 1 ? 2 : 1)) + (slab > 0 ? slab + 5 : 0.);
-            if (cost < least) {
-                least = cost;
-                best = GradShape{(int)(pt * 256), (int)n, (int)s, (int)kper, (int)(8 * (na + nb)), swap ? 1 : 0};
-            }
-            if (!want_dx) break;
         }
     }
-    return best;
+    return least_big + more < least ? of_big : best;
 }
 
 struct LinPlan {
-    bool big_f, big_g, direct;  // direct: dx comes out of the one product launch
-    int nvb, rows32, piece, splits, kper, dx_first;
+    bool big_f, direct;  // direct: dx comes out of the one product launch
+    int nvb, rows32;
+    GradShape g;
     int64_t o_part, o_zlab, o_lse, fwd_bytes;
-    int64_t o_lse2, o_coef, o_scale, o_live, o_kept, o_x, o_w, o_dz, o_slab, bwd_bytes;
+    int64_t o_lse2, o_coef, o_scale, o_live, o_kept, o_x, o_w, o_dz, o_slab, o_wslab, bwd_bytes;
 };
 static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool backward) {
     LinPlan p = {};
@@ -1271,39 +1309,27 @@ static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool backward) {
     if (!backward) return p;
     o = 0;
     p.rows32 = (int)up(N, 32);
-    // (the plan of the last call is kept, by its sizes: the search takes longer than a launch)
+    // (the last call's shape is kept, by its sizes: the search takes longer than a launch)
     static thread_local int64_t last[3] = {-1, -1, -1};
     static thread_local GradShape shape;
     if (last[0] != N || last[1] != V || last[2] != d) {
-        shape = grad_shape(N, V, d, p.rows32, true, true);
+        shape = grad_shape(N, V, d);
         last[0] = N;
         last[1] = V;
         last[2] = d;
     }
-    p.piece = shape.piece;
-    p.splits = shape.splits;
-    p.kper = shape.kper;
-    p.dx_first = shape.dx_first;
-    p.big_g = shape.tiles >= 160;
-    if (!p.big_g) {  // few tiles: one piece; slices of dx about as long as the dw tiles (rows), none where that is 64 steps at most -- less than their addition
-        p.piece = (int)up(V, 256);
-        const int64_t dxt = (up(N, 128) / 128) * (up(d, 128) / 128);
-        int64_t n = std::min<int64_t>((p.piece + p.rows32 / 2) / p.rows32, (512 + dxt - 1) / dxt);
-        n = p.piece <= 2048 ? 1 : std::max<int64_t>(1, std::min<int64_t>(n, p.piece / 128));
-        p.kper = (int)up(up(p.piece, n) / n, 32);
-        p.splits = (int)(up(p.piece, p.kper) / p.kper);
-        p.dx_first = p.kper > p.rows32;
-    }
-    p.direct = p.piece >= V && p.splits == 1;
+    p.g = shape;
+    p.direct = shape.pieces == 1 && shape.splits == 1;
     p.o_lse2 = take(N * 4);
     p.o_coef = take(N * 4);
     p.o_scale = take(8);
     p.o_live = take(up(N, 256) / 8 + 64);  // (bits; 64 bytes more than they need are read)
     p.o_kept = take(up(V, 256) / 8 + 64);
-    p.o_x = p.big_f || p.big_g ? take(N * d * 2) : 0;
-    p.o_w = (p.big_f || p.big_g) && q->offset ? take((int64_t)p.piece * d * 2) : 0;
-    p.o_dz = take((int64_t)p.rows32 * p.piece * 2);
-    p.o_slab = p.direct ? 0 : take((int64_t)p.splits * N * d * 4);
+    p.o_x = p.big_f || shape.big ? take(N * d * 2) : 0;
+    p.o_w = (p.big_f || shape.big) && q->offset ? take((int64_t)shape.piece * d * 2) : 0;
+    p.o_dz = take((int64_t)p.rows32 * shape.piece * 2);
+    p.o_slab = p.direct ? 0 : take((int64_t)shape.splits * N * d * 4);
+    p.o_wslab = shape.wsplits > 1 ? take((int64_t)shape.wsplits * shape.piece * d * 4) : 0;
     p.bwd_bytes = o;
     return p;
 }
@@ -1436,14 +1462,14 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
     pa.x_ld = q->x_ld;
     pa.w_ld = q->w_ld;
     pa.d8 = d / 8;
-    const bool copy_x = p.big_f || p.big_g, copy_w = copy_x && q->offset;
+    const bool copy_x = p.big_f || p.g.big, copy_w = copy_x && q->offset;
     if (copy_x) {
         pa.x = (const uint16_t*)x;
         pa.xo = (u32x4*)(ws + p.o_x);
     }
     if (copy_w) {
         pa.w = (const uint16_t*)w;
-        pa.Vp = std::min(V, p.piece);
+        pa.Vp = std::min(V, p.g.piece);
         pa.wo = (u32x4*)(ws + p.o_w);
     }
     if (N > 32768) {
@@ -1454,9 +1480,34 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
     const int64_t most = std::max<int64_t>(std::max(N, V), copy_x ? ((int64_t)N + pa.Vp) * (d / 8) : 0);
     class_prep_kernel<<<dim3((unsigned)std::min<int64_t>(N > 8192 ? 1024 : 256, div_up(most, 1024))), dim3(1024), 0, s>>>(pa);
     CDET_LAUNCH_CHECK();
-    const int bt = p.big_g ? 256 : 128;
-    for (int v0 = 0; v0 < V; v0 += p.piece) {
-        const int Vp = std::min(p.piece, V - v0);
+    const int bt = p.g.big ? 256 : 128;
+    SumArgs sum = {};
+    sum.d = d;
+    sum.outscale = os;
+    auto launch_sum = [&](bool sum_dx, bool sum_dw) {
+        SumArgs a = sum;
+        if (!sum_dx) {  // (the one job comes first)
+            a.slab[0] = a.slab[1];
+            a.out[0] = a.out[1];
+            a.ld[0] = a.ld[1];
+            a.rows[0] = a.rows[1];
+            a.slices[0] = a.slices[1];
+        }
+        const int jobs = (sum_dx ? 1 : 0) + (sum_dw ? 1 : 0), rows = jobs == 2 ? std::max(a.rows[0], a.rows[1]) : a.rows[0];
+        const dim3 nb((unsigned)std::min<int64_t>(4096, div_up((int64_t)rows * (d / 4), 256)), (unsigned)jobs);
+        if (q->dtype == CDET_BF16) class_sum_kernel<CDET_BF16><<<nb, dim3(256), 0, s>>>(a);
+        else class_sum_kernel<CDET_F16><<<nb, dim3(256), 0, s>>>(a);
+        CDET_LAUNCH_CHECK();
+        return 0;
+    };
+    const bool sum_dx = dx && !p.direct, sum_dw = dw && p.g.wsplits > 1;
+    sum.slab[0] = (const float*)(ws + p.o_slab);
+    sum.out[0] = (uint16_t*)dx;
+    sum.ld[0] = dx_ld;
+    sum.rows[0] = N;
+    sum.slices[0] = p.g.splits;
+    for (int v0 = 0; v0 < V; v0 += p.g.piece) {
+        const int Vp = std::min(p.g.piece, V - v0);
         LogitArgs a = logit_args(q);
         a.x = copy_x ? (const uint16_t*)(ws + p.o_x) : (const uint16_t*)x;
         a.x_ld = copy_x ? d : q->x_ld;
@@ -1478,7 +1529,7 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         a.lse2 = lse2;
         a.coef = coef;
         a.dz = (uint16_t*)(ws + p.o_dz);
-        a.dz_ld = p.piece;
+        a.dz_ld = p.g.piece;
         a.dz_rows = p.rows32;
         a.idx = p.big_f ? nullptr : idx;
         a.saved = saved;
@@ -1506,12 +1557,14 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         g.Vp = Vp;
         g.vk = (int)up(Vp, p.big_f ? 256 : 128);
         g.ntd = div_up(d, bt);
-        g.ndw = dw ? g.ntd * div_up(Vp, bt) : 0;
-        g.dx_first = p.dx_first;
+        g.wsplits = p.g.wsplits;
+        g.rper = p.g.rper;
+        g.wslab = (float*)(ws + p.o_wslab);
+        g.ndw = dw ? g.ntd * div_up(Vp, bt) * g.wsplits : 0;
+        g.dx_first = p.g.dx_first;
         g.ntr = div_up(N, bt);
-        g.kper = p.kper;
-        g.splits = p.splits;
-        g.ndx = dx ? g.ntd * g.ntr * p.splits : 0;
+        g.kper = p.g.kper;
+        g.ndx = dx ? g.ntd * g.ntr * p.g.splits : 0;
         g.dw = dw ? (uint16_t*)dw + (int64_t)v0 * dw_ld : nullptr;
         g.dw_ld = dw_ld;
         g.dx = p.direct ? (uint16_t*)dx : nullptr;
@@ -1519,14 +1572,16 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         g.slab = (float*)(ws + p.o_slab);
         g.add = v0 > 0;
         g.outscale = os;
-        rc = launch_grads(g, q->dtype, p.big_g, s);
+        rc = launch_grads(g, q->dtype, p.g.big != 0, s);
         if (rc) return rc;
-    }
-    if (dx && !p.direct) {
-        const unsigned nb = (unsigned)std::min<int64_t>(4096, div_up((int64_t)N * (d / 4), 256));
-        if (q->dtype == CDET_BF16) class_dx_kernel<CDET_BF16><<<dim3(nb), dim3(256), 0, s>>>((const float*)(ws + p.o_slab), p.splits, N, d, os, (uint16_t*)dx, dx_ld);
-        else class_dx_kernel<CDET_F16><<<dim3(nb), dim3(256), 0, s>>>((const float*)(ws + p.o_slab), p.splits, N, d, os, (uint16_t*)dx, dx_ld);
-        CDET_LAUNCH_CHECK();
+        const bool ends = v0 + Vp >= V;
+        sum.slab[1] = g.wslab;
+        sum.out[1] = g.dw;
+        sum.ld[1] = dw_ld;
+        sum.rows[1] = Vp;
+        sum.slices[1] = g.wsplits;
+        if (sum_dw || (ends && sum_dx)) rc = launch_sum(ends && sum_dx, sum_dw);
+        if (rc) return rc;
     }
     return 0;
 }

@@ -4,8 +4,8 @@
 // Bound by memory: logits once in, gradient once out. A row of up to 32768 logits stays in the registers of its 1, 4, 8 or 16 waves (td_wide_kernel), so the
 // maximum, the sum and the gradient are taken from one read (td_wave_kernel, td_wide_kernel); one of up to 256 KiB is held as it is stored
 // (td_held_kernel); a longer one is read again for its gradient (td_long_kernel). Above 2048 logits the gradient is written dense and then, behind a
-// barrier, the k named entries are written again with their q; shorter rows put q together in LDS first. Rows of at most 64 logits (box distributions)
-// take 16 lanes each (td_narrow_kernel). p is exp2((z - max) c) / sum: its error does not
+// barrier, the k named entries are written again with their q; shorter rows put q together in LDS first. Rows of at most 128 logits (box distributions,
+// ordinary class lists) take 16 lanes each (td_narrow_kernel). p is exp2((z - max) c) / sum: its error does not
 // grow with |z|.
 #include "common.h"
 
@@ -273,13 +273,14 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
     s = td_reduce<1, false>(s, nullptr);
     ts = td_reduce<1, false>(ts, nullptr);
     const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s), lts = logf(ts);
-    td_sync<1>();  // every slot has read its logit
+    td_sync<1>();  // every slot has read its logit: from here on the row says which slot names a class (-1: none; of several, one of them)
+    int* const own = reinterpret_cast<int*>(rb);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int e0 = (i * 64 + t) * CH;
         if (e0 < V)
 #pragma unroll
-            for (int e = 0; e < CH; e += 4) *reinterpret_cast<f32x4*>(rb + e0 + e) = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int e = 0; e < CH; e += 4) *reinterpret_cast<u32x4*>(rb + e0 + e) = u32x4{~0u, ~0u, ~0u, ~0u};
     }
     float sum = 0.f;
     for (int j = t; j < k; j += 64) {
@@ -292,28 +293,24 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
     if (t == 0) a.loss[row] = on ? sum * a.tau2 : 0.f;
     if (!dz) return;
     td_sync<1>();
-    // a class named twice takes the q of all of its slots, in their order: found with one comparison a slot where the slots fit the lanes
-    bool alone = false;
-    if (k <= 64) {
-        const int c = t < k && sl.v[t] >= 0 ? sl.v[t] : -1 - t;
-        uint64_t twice = 0;
-        for (int o = 0; o < k; ++o) twice |= __ballot(c == __builtin_amdgcn_readlane(c, o)) & ~(1ull << o);
-        alone = twice == 0;
-    }
-    for (int j = t; j < k; j += 64) {
-        const int c = sl.v[j];
-        if (c < 0) continue;
-        float q = sl.q[j];
-        bool first = true;
-        if (!alone)
-            for (int o = 0; o < k; ++o) {
-                const bool same = sl.v[o] == c;
-                first = first && !(same && o < j);
-                q += same && o > j ? sl.q[o] : 0.f;
-            }
-        if (first) rb[c] = q;
-    }
+    for (int j = t; j < k; j += 64)
+        if (sl.v[j] >= 0) own[sl.v[j]] = j;
     td_sync<1>();
+    bool lost = false;  // another slot names this one's class
+    for (int j = t; j < k; j += 64) lost = lost || (sl.v[j] >= 0 && own[sl.v[j]] != j);
+    if (__ballot(lost)) {  // a class named twice takes the q of all of its slots, in their order
+        for (int j = t; j < k; j += 64) {
+            const int c = sl.v[j];
+            if (c < 0 || own[c] != j) continue;
+            float q = 0.f;
+            for (int o = 0; o < k; ++o) q += sl.v[o] == c ? sl.q[o] : 0.f;
+            sl.z[j] = q;
+        }
+        td_sync<1>();
+        for (int j = t; j < k; j += 64)
+            if (sl.v[j] >= 0 && own[sl.v[j]] == j) sl.q[j] = sl.z[j];
+        td_sync<1>();
+    }
     const float g = a.gs * w;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
@@ -322,9 +319,13 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
         float o[CH];
 #pragma unroll
         for (int e = 0; e < CH; e += 4) {
-            const f32x4 q = *reinterpret_cast<const f32x4*>(rb + e0 + e);
+            const u32x4 by = *reinterpret_cast<const u32x4*>(rb + e0 + e);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) o[e + u] = on ? (v[i][e + u] * inv - q[u]) * g : 0.f;
+            for (int u = 0; u < 4; ++u) {
+                float p = v[i][e + u] * inv;
+                if ((int)by[u] >= 0) p -= sl.q[by[u]];
+                o[e + u] = on ? p * g : 0.f;
+            }
         }
         if (e0 + CH <= V) td_put<GDT, CH>(dz + e0, o);
         else
@@ -682,7 +683,9 @@ static int td_launch(const TdArgs& a, hipStream_t s) {
     const size_t lds = (size_t)a.k * 16;
     const int narrow = a.V > a.k ? a.V : a.k;
     if (narrow <= 16) td_narrow_kernel<DT, GDT, 1, 4><<<dim3((unsigned)((a.rows + 63) / 64)), dim3(256), 0, s>>>(a);
+    else if (narrow <= 32) td_narrow_kernel<DT, GDT, 2, 2><<<dim3((unsigned)((a.rows + 31) / 32)), dim3(256), 0, s>>>(a);
     else if (narrow <= 64) td_narrow_kernel<DT, GDT, 4, 1><<<dim3((unsigned)((a.rows + 15) / 16)), dim3(256), 0, s>>>(a);
+    else if (narrow <= 128) td_narrow_kernel<DT, GDT, 8, 1><<<dim3((unsigned)((a.rows + 15) / 16)), dim3(256), 0, s>>>(a);
     else if (a.V <= 2048) td_wave_kernel<DT, GDT><<<dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 4 * (lds + ((a.V + 7) & ~7) * 4), s>>>(a);
     else if (a.V <= 8192) td_wide_kernel<DT, GDT, 4><<<dim3((unsigned)a.rows), dim3(256), lds, s>>>(a);
     else if (a.V <= 16384) td_wide_kernel<DT, GDT, 8><<<dim3((unsigned)a.rows), dim3(512), lds, s>>>(a);

@@ -121,7 +121,8 @@ def ce_case(N, V, d, dtype, seed=0):
 CE_SIZES = [(1, 1, 8), (1, 2, 8), (3, 5, 16), (1, 1000, 64), (64, 64, 64), (127, 129, 72), (130, 257, 104), (300, 1201, 320), (33, 9001, 264), (257, 128, 40),
             (2600, 3900, 40),   # 256 x 256 tiles
             (700, 21000, 24), (1100, 30000, 264),  # the same with classes cut into slices for dx
-            (40000, 4500, 16)]  # several pieces of the class list
+            (40000, 4500, 16),  # several pieces of the class list
+            (9000, 300, 72), (5000, 130, 520)]  # rows cut into slices for dw
 
 
 @pytest.mark.parametrize("dtype", [BF, F16])
@@ -320,7 +321,7 @@ def check_map(got, z, idx, val, tau, drow):
     assert torch.all(err <= tol), (err / tol).max().item()
 
 
-MAP_SIZES = [(1, 1, 1, 1), (1, 1, 2, 2), (7, 1, 16, 16), (300, 4, 16, 9), (70, 1, 17, 5), (65, 1, 3, 17), (33, 4, 16, 16), (50, 4, 13, 5), (20, 1, 64, 64), (20, 1, 65, 64), (9, 1, 64, 65), (40, 1, 80, 10),
+MAP_SIZES = [(1, 1, 1, 1), (1, 1, 2, 2), (7, 1, 16, 16), (300, 4, 16, 9), (70, 1, 17, 5), (65, 1, 3, 17), (90, 1, 74, 74), (40, 2, 128, 33), (40, 1, 129, 128), (33, 4, 16, 16), (50, 4, 13, 5), (20, 1, 64, 64), (20, 1, 65, 64), (9, 1, 64, 65), (40, 1, 80, 10),
              (13, 1, 1203, 32), (6, 2, 2048, 100), (5, 1, 2049, 40), (3, 1, 8191, 512), (3, 1, 8193, 7), (2, 1, 16385, 33), (2, 1, 32768, 64), (2, 1, 32769, 64), (2, 1, 65537, 64), (2, 1, 100003, 30), (2, 1, 131073, 9)]
 
 
@@ -339,7 +340,7 @@ def test_topk_distill(P, G, V, k, dtype, gdt):
         assert torch.equal(two[0], got[0][:, 0]) and torch.equal(two[1], got[1][:, 0])
 
 
-@pytest.mark.parametrize("V,k", [(16, 12), (40, 12), (1000, 20), (1000, 100), (5000, 20), (9000, 20), (40000, 20), (140000, 20)])
+@pytest.mark.parametrize("V,k", [(16, 12), (30, 12), (40, 12), (100, 70), (1000, 20), (1000, 100), (5000, 20), (9000, 20), (40000, 20), (140000, 20)])
 def test_topk_distill_odd_values(V, k):
     """The same class in many slots, -inf logits, rows of nothing but -inf, rows without a teacher that hold NaN, far logits."""
     z = 2 * _rand(12, V, seed=50)
