@@ -493,7 +493,8 @@ int cdet_det_loss(const cdet_loss_desc* d, const void* f0, const void* f1, const
  *   labels  [N] int64 / int32; outside of 0 .. V-1 (-100, say): the row takes no part -- loss 0, gradient 0, whatever the row of x holds. A row
  *           whose classes are all left out takes no part either; a label that is left out beside others that are not has loss +inf.
  *   idx     [N, k] int32 classes of the teacher's largest logits, val [N, k] their values; outside of 0 .. V-1: an empty slot. A class may be named
- *           twice (its slots count separately). q = softmax of val / tau over the filled slots; a row without any takes no part. k <= 512.
+ *           twice (its slots count separately). q = softmax of val / tau over the filled slots; a row without any takes no part; one that
+ *           names a left-out class beside others has loss +inf (and that class no gradient). k <= 512.
  *   lse     [N] log-sum-exp of the row;  saved [N, 1 + 2 k] fp32: what linear_distill's backward needs (opaque)
  *   drow    gradient of the rows' losses, fp32: [N] (drow_stride 1), one value (0), or NULL (ones)
  *   dx, dw  16-bit like x and w, either may be NULL; whole [V, d] of dw is written, the pitches' tails are not touched

@@ -479,6 +479,109 @@ def test_streams_and_captured_graphs():
                 assert torch.equal(a, b)
 
 
+def test_captured_training_step():
+    """The differentiable losses with their means and a backward pass, captured once and replayed with new data in the same buffers: each replay is the eager
+    step on that data. (The leaves' gradients are taken with autograd.grad; no eager graph of the same leaves lives during the capture.)"""
+    from cerberusdet_amd.utils import loss as UL
+
+    N, V, d, k = 5000, 700, 64, 10
+    x, w, labels = ce_case(N, V, d, BF, seed=120)
+    idx, val = teacher(N, V, k, 121)
+    z = 2 * _rand(N, 50, seed=122)
+    zi, zv = teacher(N, 50, k, 123)
+
+    def step(x, w, z, labels, idx, val, zi, zv):
+        x, w, z = (t.detach().requires_grad_() for t in (x, w, z))
+        total = UL.linear_cross_entropy(x, w, labels) + 0.5 * UL.linear_distillation(x, w, idx, val, tau=2.0) + UL.topk_distillation(z, zi, zv, tau=2.0)
+        return [total.detach(), *torch.autograd.grad(total, (x, w, z))]
+
+    data = (x, w, z, labels, idx, val, zi, zv)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*data)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(*data)
+    for turn in range(4):
+        x.copy_(_rand(N, d, seed=130 + turn, dtype=BF))
+        z.copy_(_rand(N, 50, seed=140 + turn))
+        labels.copy_(_randint(V, (N,), 150 + turn))
+        for o in outs:
+            o.fill_(3)
+        graph.replay()
+        got = [o.clone() for o in outs]
+        want = step(*data)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), turn
+
+
+def test_two_threads_two_streams():
+    """Calls of different sizes from two host threads on streams of their own."""
+    import threading
+
+    cases = [ce_case(n, v, d, BF, seed=160 + n) for n, v, d in ((300, 2000, 64), (1100, 30000, 264))]
+    want = [run_ce(*c) for c in cases]
+    torch.cuda.synchronize()
+    got, streams = [None, None], [torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(10):
+                got[i] = run_ce(*cases[i])
+        streams[i].synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(want, got):
+        for s, t in zip(a, b):
+            assert torch.equal(s, t)
+
+
+def test_gradients_leave_pitch_tails_alone():
+    """Through the C interface: dx and dw with pitches above d; what lies behind a row stays."""
+    import ctypes as C
+
+    from cerberusdet_amd import _lib as L
+
+    ops, N, V, d = _ops(), 200, 700, 64
+    x, w, labels = ce_case(N, V, d, BF, seed=170)
+    loss, lse, dx, dw = run_ce(x, w, labels)
+    lib = L.load()
+    desc = L.LinearLossDesc(N, V, d, L.BF16, d, d, 1.0, 1.0, None, 1)
+    bx, bw = torch.full((N, d + 24), 9.0, dtype=BF, device=DEV), torch.full((V, d + 8), 9.0, dtype=BF, device=DEV)
+    ws = torch.empty(lib.cdet_linear_loss_ws_bytes(C.byref(desc), 1), dtype=torch.uint8, device=DEV).fill_(255)  # (contents do not matter)
+    L.check(lib.cdet_linear_ce_bwd(C.byref(desc), x.data_ptr(), w.data_ptr(), labels.data_ptr(), lse.data_ptr(), None, 0, bx.data_ptr(), d + 24, bw.data_ptr(), d + 8,
+                                   ws.data_ptr(), ops.stream()))
+    assert torch.equal(bx[:, :d], dx) and torch.equal(bw[:, :d], dw) and torch.all(bx[:, d:] == 9) and torch.all(bw[:, d:] == 9)
+
+
+def test_offsets_beyond_32_bits():
+    """Rows more than 2^31 elements apart from the first: x and w with the largest pitch, logits of 2.6e9 elements."""
+    ops, ld = _ops(), (1 << 22) - 8
+    x, w, labels = ce_case(700, 600, 64, BF, seed=180)
+    want = run_ce(x, w, labels)
+    big = torch.empty(700, ld, dtype=BF, device=DEV)
+    big[:, :64], big[:600, 128:192] = x, w
+    for a, b in zip(want, run_ce(big[:, :64], big[:600, 128:192], labels)):
+        assert torch.equal(a, b)
+    del big
+    P, V = 40000, 65536
+    z = torch.empty(P, V, dtype=BF, device=DEV)
+    z[:] = _rand(1, V, seed=181).to(BF)
+    z[P - 3:] = _rand(3, V, seed=182).to(BF)
+    idx, val = teacher(P, V, 4, 183)
+    loss, dz = ops.topk_distill(z, idx, val)
+    few = ops.topk_distill(z[P - 3:].clone(), idx[P - 3:], val[P - 3:])
+    assert torch.equal(loss[P - 3:], few[0]) and torch.equal(dz[P - 3:], few[1])
+
+
 def test_used_together():
     """A student classifier learns from labels and from a teacher's top logits in one backward; the fused distillation is that of its own logits."""
     from cerberusdet_amd.utils import loss as UL
