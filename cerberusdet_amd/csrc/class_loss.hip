@@ -1078,34 +1078,25 @@ __global__ __launch_bounds__(256) void class_zero_kernel(uint16_t* p, int64_t ro
 }
 
 // ---- distillation: the teacher's slots ---------------------------------------------------------------------------------------------------------------
-// One wave a row, 16 lanes a slot: the student's logits at the teacher's classes (dot products in fp32), the teacher's softmax over its filled slots, the
-// loss. saved: [N][1 + 2k] = lse of the row (+inf where the teacher says nothing), logits (log2 units), q -- the first slot that names a class holds the
-// sum over all of its slots, the others -1.
+// A workgroup a row, 16 lanes a slot: the student's logits at the teacher's classes (dot products in fp32), the teacher's softmax over its filled slots, the
+// loss. Rows of w are fetched from all over the list: 64 of them in flight a workgroup (1021 x 50 x 512: 16 us, with one wave a row 22).
+// saved: [N][1 + 2k] = lse of the row (+inf where the teacher says nothing), logits (log2 units), q -- the first slot that names a class holds the sum over
+// all of its slots, the others -1.
 template <int DT>
 __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, int64_t x_ld, const uint16_t* w, int64_t w_ld, const float* off, float c, float coff,
                                                             const int32_t* idx, const void* val, int val_dtype, int k, float itau, float tau2, int N, int V, int d,
                                                             const float* lse, const float* part, int nvb, float* loss, float* saved) {
-    __shared__ int s_idx[4][512];
-    __shared__ float s_q[4][512];
-    const int lane = (int)threadIdx.x & 63, wv = (int)threadIdx.x >> 6;
-    const int r = (int)blockIdx.x * 4 + wv;
-    if (r >= N) return;  // (whole waves; no barrier of the workgroup follows)
-    const int sub = lane >> 4, l = lane & 15;
+    __shared__ int s_idx[512];
+    __shared__ float s_t[512], s_q[512], s_sum[4];
+    const int t = (int)threadIdx.x, lane = t & 63, wv = t >> 6, r = (int)blockIdx.x;
+    const int sub = t >> 4, l = t & 15;
     float* sv = saved + (int64_t)r * (1 + 2 * k);
     const int32_t* ir = idx + (int64_t)r * k;
-    // the slots in LDS: class (-1: empty) and the teacher's logit, later q; its maximum and sum
-    float m = -INFINITY;
-    for (int j = lane; j < k; j += 64) {
+    // the slots in LDS: class (-1: empty) and the teacher's logit
+    for (int j = t; j < k; j += 256) {
         const int v = ir[j];
-        const float t = load_elem(val, (int64_t)r * k + j, val_dtype) * itau;
-        const bool on = (unsigned)v < (unsigned)V;
-        s_idx[wv][j] = on ? v : -1;
-        s_q[wv][j] = t;
-        if (on) m = m != m || t != t ? NAN : fmaxf(m, t);
-    }
-    for (int o = 32; o; o >>= 1) {
-        const float m2 = __shfl_xor(m, o);
-        m = m != m || m2 != m2 ? NAN : fmaxf(m, m2);
+        s_idx[j] = (unsigned)v < (unsigned)V ? v : -1;
+        s_t[j] = load_elem(val, (int64_t)r * k + j, val_dtype) * itau;
     }
     float lse_r;
     if (part) {  // few pairs a row: joined here instead of in a launch of their own
@@ -1125,24 +1116,30 @@ __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, i
         lse_r = ps == 0.f ? -INFINITY : (pm + __builtin_amdgcn_logf(ps)) * kLn2;
     } else lse_r = lse[r];
     const float l2 = lse_r * kLog2e;
-    const bool some = m != -INFINITY && l2 != -INFINITY;  // (no filled slot, or nothing but -inf in them, or no class left)
-    float s = 0.f;
+    __syncthreads();
+    // the teacher's maximum and sum, by every wave for itself
+    float m = -INFINITY, s = 0.f;
     for (int j = lane; j < k; j += 64)
-        if (s_idx[wv][j] >= 0) s += expf(s_q[wv][j] - m);
+        if (s_idx[j] >= 0) m = m != m || s_t[j] != s_t[j] ? NAN : fmaxf(m, s_t[j]);
+    for (int o = 32; o; o >>= 1) {
+        const float m2 = __shfl_xor(m, o);
+        m = m != m || m2 != m2 ? NAN : fmaxf(m, m2);
+    }
+    const bool some = m != -INFINITY && l2 != -INFINITY;  // (no filled slot, or nothing but -inf in them, or no class left)
+    for (int j = lane; j < k; j += 64)
+        if (s_idx[j] >= 0) s += expf(s_t[j] - m);
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
     const float ls = logf(s);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
     float sum = 0.f;
-    constexpr int U = 4;  // rows of w in flight per 16 lanes
+    constexpr int U = 4;  // slots of 16 lanes in flight
     const uint16_t* xr = x + r * x_ld;
-    for (int j0 = 0; j0 < k; j0 += 4 * U) {
+    for (int j0 = 0; j0 < k; j0 += 16 * U) {
         float z[U];
         int v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * 4 + sub;
-            v[u] = some && j < k ? s_idx[wv][j] : -1;
+            const int j = j0 + u * 16 + sub;
+            v[u] = some && j < k ? s_idx[j] : -1;
             z[u] = 0.f;
         }
         for (int f = l * 8; f < d; f += 128) {
@@ -1160,48 +1157,39 @@ __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, i
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * 4 + sub;
+            const int j = j0 + u * 16 + sub;
             for (int o = 8; o; o >>= 1) z[u] += __shfl_xor(z[u], o);
             if (j < k && l == 0) {
                 float z2 = -INFINITY, q = 0.f;
                 if (v[u] >= 0) {
                     const float ov = off ? off[v[u]] : 0.f;
                     z2 = ov == -INFINITY ? -INFINITY : fmaf(z[u], c, ov * coff);
-                    const float lq = s_q[wv][j] - m - ls;
+                    const float lq = s_t[j] - m - ls;
                     q = expf(lq);
                     if (q != 0.f) sum += q * (lq - (z2 - l2) * kLn2);
                 }
                 sv[1 + j] = z2;
-                s_q[wv][j] = q;
+                s_q[j] = q;
             }
         }
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    if (lane == 0) {
-        loss[r] = some ? sum * tau2 : 0.f;
+    if (lane == 0) s_sum[wv] = sum;
+    __syncthreads();
+    if (t == 0) {
+        loss[r] = some ? (s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) * tau2 : 0.f;
         sv[0] = !some ? INFINITY : lse_r == INFINITY ? NAN : lse_r;
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    // is a class named twice: one comparison a slot where the slots fit the lanes
-    bool alone = false;
-    if (k <= 64) {
-        const int v = lane < k && s_idx[wv][lane] >= 0 ? s_idx[wv][lane] : -1 - lane;
-        uint64_t twice = 0;
-        for (int o = 0; o < k; ++o) twice |= __ballot(v == __builtin_amdgcn_readlane(v, o)) & ~(1ull << o);
-        alone = twice == 0;
-    }
-    for (int j = lane; j < k; j += 64) {
-        const int v = s_idx[wv][j];
-        float q = s_q[wv][j];
+    for (int j = t; j < k; j += 256) {
+        const int v = s_idx[j];
+        float q = s_q[j];
         bool first = some && v >= 0;
-        if (!alone)
-            for (int o = 0; o < k; ++o) {
-                const bool same = s_idx[wv][o] == v;
-                first = first && !(same && o < j);
-                q += same && o > j ? s_q[wv][o] : 0.f;
-            }
+        for (int o = 0; o < k; ++o) {
+            const bool same = s_idx[o] == v;
+            first = first && !(same && o < j);
+            q += same && o > j ? s_q[o] : 0.f;
+        }
         sv[1 + k + j] = first ? q : -1.f;
     }
 }
@@ -1648,7 +1636,7 @@ extern "C" int cdet_linear_distill_fwd(const cdet_linear_loss_desc* d, const voi
     const float* part = few ? (const float*)((char*)ws + p.o_part) : nullptr;
     const int rc = lin_forward(d, p, x, w, nullptr, nullptr, lse, (char*)ws, (hipStream_t)stream);
     if (rc) return rc;
-    const dim3 nb((unsigned)div_up(d->N, 4)), nt(256);
+    const dim3 nb((unsigned)d->N), nt(256);
     const LogitArgs a = logit_args(d);
 #define CDET_GO(DT_)                                                                                                                                        \
     class_teacher_kernel<DT_><<<nb, nt, 0, (hipStream_t)stream>>>((const uint16_t*)x, d->x_ld, (const uint16_t*)w, d->w_ld, d->offset, a.c, a.coff, idx, val, val_dtype, \
