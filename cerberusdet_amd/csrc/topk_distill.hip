@@ -5,7 +5,7 @@
 // maximum, the sum and the gradient are taken from one read (td_wave_kernel, td_wide_kernel); one of up to 256 KiB is held as it is stored
 // (td_held_kernel); a longer one is read again for its gradient (td_long_kernel). Above 2048 logits the gradient is written dense and then, behind a
 // barrier, the k named entries are written again with their q; shorter rows put q together in LDS first. Rows of at most 128 logits (box distributions,
-// ordinary class lists) take 16 lanes each (td_narrow_kernel). p is exp2((z - max) c) / sum: its error does not
+// ordinary class lists) take 4, 8 or 16 lanes each (td_narrow_kernel). p is exp2((z - max) c) / sum: its error does not
 // grow with |z|.
 #include "common.h"
 
@@ -75,9 +75,9 @@ __device__ __forceinline__ void td_put(typename TdElem<GDT>::T* dst, const float
     }
 }
 
-// maximum / sum over the 16 lanes of a DPP row, then over the wave: the same value in every lane
-template <bool MAX>
-__device__ __forceinline__ float td_row16(float v) {
+// maximum / sum over 4, 8 or 16 neighbouring lanes: the same value in each of them
+template <int L, bool MAX>
+__device__ __forceinline__ float td_lanes(float v) {
 #define CDET_DPP(ctrl)                                                                                                                              \
     do {                                                                                                                                            \
         const float u = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true)); \
@@ -85,15 +85,15 @@ __device__ __forceinline__ float td_row16(float v) {
     } while (0)
     CDET_DPP(0xB1);   // quad_perm [1,0,3,2]
     CDET_DPP(0x4E);   // quad_perm [2,3,0,1]
-    CDET_DPP(0x141);  // row_half_mirror
-    CDET_DPP(0x140);  // row_mirror
+    if (L > 4) CDET_DPP(0x141);  // row_half_mirror
+    if (L > 8) CDET_DPP(0x140);  // row_mirror
 #undef CDET_DPP
     return v;
 }
 // maxima / sums over a row's waves (NW = 1: inside the wave), the same value in every thread, in a fixed order
 template <int NW, bool MAX>
 __device__ __forceinline__ float td_reduce(float v, float* scratch) {
-    v = td_row16<MAX>(v);
+    v = td_lanes<16, MAX>(v);
 #pragma unroll
     for (int o = 16; o < 64; o *= 2) {
         const float u = __shfl_xor(v, o);
@@ -187,13 +187,15 @@ __device__ __forceinline__ void td_row(const TdArgs& a, int64_t row, const T*& z
     dz = a.dz ? (TG*)a.dz + (int64_t)px * a.gld + (int64_t)gr * a.V : nullptr;
 }
 
-// V <= 2048: a wave a row, four rows a workgroup, the logits in registers and once in LDS: the slots find theirs there, and then leave their q there for the
-// dense gradient to take along -- no gather from and no second write to memory (67200 x 1203 fp32, k = 32 scattered classes: 134 us = 4.9 TB/s against 170 us with them)
-template <int DT, int GDT>
+// V <= 2048: a wave a row, four rows a workgroup, the logits in registers (up to PER a lane) and once in LDS: the slots find theirs there, and then leave their
+// q there for the dense gradient to take along -- no gather from and no second write to memory (67200 x 1203 fp32, k = 32 scattered classes: 123 us = 5.4 TB/s,
+// with them 170). What a row holds behind its last whole 16 bytes goes a logit a lane (as a partial chunk 134 us). PER = 32 for
+// all lengths: 67200 x 365 fp32 55 us, with 8 44.
+template <int DT, int GDT, int PER>
 __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
     typedef typename TdElem<GDT>::T TG;
-    constexpr int CH = 16 / sizeof(T), NCH = 32 / CH;
+    constexpr int CH = 16 / sizeof(T), NCH = PER / CH;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int t = (int)threadIdx.x & 63, V = a.V, k = a.k;
     const int64_t row = (int64_t)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
@@ -223,13 +225,12 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
         } else {
 #pragma unroll
             for (int e = 0; e < CH; ++e) v[i][e] = -INFINITY;
-            if (e0 < V)
-#pragma unroll
-                for (int e = 0; e < CH; ++e)
-                    if (e0 + e < V) v[i][e] = TdElem<DT>::get(z[e0 + e]);
         }
     }
-    float m = -INFINITY;
+    const int et = V - V % CH + t;  // what is left behind the last whole chunk, a logit a lane
+    float vt = et < V ? TdElem<DT>::get(z[et]) : -INFINITY;
+    float m = vt;
+    if (et < V) rb[et] = vt;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
         if (i * 64 * CH < V) {
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
 #pragma unroll
             for (int e = 0; e < CH; e += 4) {
                 const f32x4 o = {v[i][e], v[i][e + 1], v[i][e + 2], v[i][e + 3]};
-                if (e0 < V) *reinterpret_cast<f32x4*>(rb + e0 + e) = o;
+                if (e0 + CH <= V) *reinterpret_cast<f32x4*>(rb + e0 + e) = o;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) m = fmaxf(m, o[u]);
             }
@@ -268,6 +269,8 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
                 v[i][e] = td_exp2<DT>(v[i][e], mu, a.c, muc);
                 s += v[i][e];
             }
+    vt = td_exp2<DT>(vt, mu, a.c, muc);
+    s += vt;
     for (int j = t; j < k; j += 64)
         if (sl.v[j] >= 0) ts += expf(sl.lq[j] - tm);
     s = td_reduce<1, false>(s, nullptr);
@@ -278,10 +281,11 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int e0 = (i * 64 + t) * CH;
-        if (e0 < V)
+        if (e0 + CH <= V)
 #pragma unroll
             for (int e = 0; e < CH; e += 4) *reinterpret_cast<u32x4*>(rb + e0 + e) = u32x4{~0u, ~0u, ~0u, ~0u};
     }
+    if (et < V) own[et] = -1;
     float sum = 0.f;
     for (int j = t; j < k; j += 64) {
         const float lq = sl.lq[j] - tm - lts;
@@ -315,7 +319,7 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int e0 = (i * 64 + t) * CH;
-        if (e0 >= V) continue;
+        if (e0 + CH > V) continue;
         float o[CH];
 #pragma unroll
         for (int e = 0; e < CH; e += 4) {
@@ -327,15 +331,16 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
                 o[e + u] = on ? p * g : 0.f;
             }
         }
-        if (e0 + CH <= V) td_put<GDT, CH>(dz + e0, o);
-        else
-#pragma unroll
-            for (int e = 0; e < CH; ++e)
-                if (e0 + e < V) dz[e0 + e] = TdElem<GDT>::put(o[e]);
+        td_put<GDT, CH>(dz + e0, o);
+    }
+    if (et < V) {
+        const int by = own[et];
+        dz[et] = TdElem<GDT>::put(on ? (vt * inv - (by >= 0 ? sl.q[by] : 0.f)) * g : 0.f);
     }
 }
 
-// a row's logits in registers: up to NCH chunks of CH per thread, NW waves a row
+// V <= 32768: a row's logits in registers, up to NCH chunks of CH per thread, NW waves a row; loss, maximum and sum from one read. Bound by memory:
+// 16800 x 8192 fp32 212 us = 5.2 TB/s, 4200 x 32768 210 us.
 template <int DT, int GDT, int NW>
 __global__ __launch_bounds__(NW * 64, NW == 16 ? 8 : 1) void td_wide_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
@@ -408,7 +413,8 @@ __global__ __launch_bounds__(NW * 64, NW == 16 ? 8 : 1) void td_wide_kernel(cons
     td_finish<GDT, NW>(a, row, t, on, dz, mu, inv, l2s, g, slots, scratch);
 }
 
-// longer rows, as they are stored (16 waves a row, NCH chunks of 16 bytes a thread): two exponentials a logit instead of a second read
+// longer rows, as they are stored (16 waves a row, NCH chunks of 16 bytes a thread): two exponentials a logit instead of a second read.
+// 8192 x 65536 bf16 396 us = 5.4 TB/s; NCH = 16 leaves one row a CU, whose loads and stores take turns: 4096 x 131072 bf16 475 us = 4.5 TB/s.
 template <int DT, int GDT, int NCH>
 __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
@@ -494,6 +500,7 @@ __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const T
 }
 
 // rows that do not fit the registers: one pass for a running maximum and sum, a second one for the gradient; 16 waves a row
+// (1024 x 131072 fp32 312 us = 5.2 TB/s over its three passes)
 template <int DT, int GDT>
 __global__ __launch_bounds__(1024) void td_long_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
@@ -560,133 +567,164 @@ __global__ __launch_bounds__(1024) void td_long_kernel(const TdArgs a) {
     td_finish<GDT, NW>(a, row, t, on, dz, mu, inv, l2s, g, slots, scratch);
 }
 
-// V, k <= 16 E: 16 lanes a row, R rows of a lane at a time (their loads in flight together), 16 R rows a workgroup. A row's slots meet its classes in
-// LDS: log p of every class, and {q, slot} of the slot that named it last; as many owned classes as filled slots means that no class was named twice.
-template <int DT, int GDT, int E, int R>
+// N consecutive elements of which the first n exist, as fp32; the others `none`
+template <int DT, int N>
+__device__ __forceinline__ void td_get(const void* base, int64_t at, int n, float none, float (&v)[N]) {
+    typedef typename TdElem<DT>::T T;
+    const T* p = (const T*)base + at;
+    if (n >= N) {
+        const TdVec<T, N> u = *reinterpret_cast<const TdVec<T, N>*>(p);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = TdElem<DT>::get(u.v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = e < n ? TdElem<DT>::get(p[e]) : none;
+    }
+}
+
+// V <= L E, k <= L S: L lanes a row, E neighbouring classes and S slots a lane. A row's slots meet its classes in LDS: log p of every class, and {q, 1} of the slot
+// that named it last; as many owned classes as filled slots means that no class was named twice. Few elements a lane leave it bound by its instructions, so a
+// lane takes four neighbours (6, 8 in longer rows) and, where k <= L, one slot: 268800 x 4 x 16 fp32, k = 16: 56 us = 5.1 TB/s, with a class and a slot a lane
+// and 16 lanes a row 82; 268800 x 80, k = 10: 31 us, with eight slots on each of two lanes 50.
+template <int DT, int GDT, int L, int E, int S>
 __global__ __launch_bounds__(256) void td_narrow_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
     typedef typename TdElem<GDT>::T TG;
-    __shared__ float s_lp[R][16][16 * E];
-    __shared__ float2 s_q[R][16][16 * E];
-    const int lane = (int)threadIdx.x & 63, l = (int)threadIdx.x & 15, r = (int)threadIdx.x >> 4, V = a.V, k = a.k;
-    const uint64_t mine = 0xffffull << (lane & 48);
-    float v[R][E], tx[R][E], w[R];
-    int ti[R][E];
+    constexpr int ROWS = 256 / L, W = L * E + 4;  // (4: rows start in different banks)
+    __shared__ __attribute__((aligned(16))) float s_lp[ROWS][W];
+    __shared__ __attribute__((aligned(16))) float s_q[ROWS][2 * W];
+    const int lane = (int)threadIdx.x & 63, l = (int)threadIdx.x & (L - 1), r = (int)threadIdx.x / L, V = a.V, k = a.k;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + r;
+    const bool here = row < a.rows;
+    const T* z;
+    TG* dz;
+    td_row(a, here ? row : 0, z, dz);
+    const float w = a.drow && here ? a.drow[row] : 1.f;
+    const int nv = here ? V - l * E : 0, nk = here ? k - l * S : 0;
+    float v[E], tx[S];
+    int ti[S];
+    td_get<DT, E>(z, l * E, nv, -INFINITY, v);
+    const int64_t at = (here ? row : 0) * k + l * S;
+    if (a.vdt == CDET_F32) td_get<CDET_F32, S>(a.val, at, nk, 0.f, tx);
+    else if (a.vdt == CDET_BF16) td_get<CDET_BF16, S>(a.val, at, nk, 0.f, tx);
+    else td_get<CDET_F16, S>(a.val, at, nk, 0.f, tx);
+    if (nk >= S) {
+        const TdVec<int, S> u = *reinterpret_cast<const TdVec<int, S>*>(a.idx + at);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int64_t row = ((int64_t)blockIdx.x * R + i) * 16 + r;
-        const bool here = row < a.rows;
-        const T* z;
-        TG* dz;
-        td_row(a, here ? row : 0, z, dz);
-        w[i] = a.drow && here ? a.drow[row] : 1.f;
+        for (int j = 0; j < S; ++j) ti[j] = u.v[j];
+    } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int j = e * 16 + l;
-            v[i][e] = here && j < V ? TdElem<DT>::get(z[j]) : -INFINITY;
-            ti[i][e] = here && j < k ? a.idx[row * k + j] : -1;
-            tx[i][e] = here && j < k ? load_elem(a.val, row * k + j, a.vdt) : 0.f;
-        }
+        for (int j = 0; j < S; ++j) ti[j] = j < nk ? a.idx[at + j] : -1;
+    }
+    float m = -INFINITY, tm = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+        if ((unsigned)ti[j] >= (unsigned)V) ti[j] = -1;
+        tx[j] = ti[j] >= 0 ? tx[j] * a.itau : -INFINITY;
+        tm = fmaxf(tm, tx[j]);
+    }
+    m = td_lanes<L, true>(m);
+    tm = td_lanes<L, true>(tm);
+    const float mu = __builtin_isinf(m) ? 0.f : m;
+    const bool on = tm != -INFINITY && m != -INFINITY;
+    float s = 0.f, ts = 0.f, p[E], lq[S], q[S];
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+        lq[j] = (tx[j] - tm) * kTdLog2e;
+        q[j] = ti[j] >= 0 ? __builtin_amdgcn_exp2f(lq[j]) : 0.f;
+        ts += q[j];
     }
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        float m = -INFINITY, tm = -INFINITY;
+    for (int e = 0; e < E; ++e) {
+        v[e] = (v[e] - mu) * a.c;
+        p[e] = __builtin_amdgcn_exp2f(v[e]);
+        s += p[e];
+    }
+    s = td_lanes<L, false>(s);
+    ts = td_lanes<L, false>(ts);
+    const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s), itq = 1.f / ts, lts = __builtin_amdgcn_logf(ts);
+    float *lp = s_lp[r], *sq = s_q[r];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if ((unsigned)ti[i][e] >= (unsigned)V) ti[i][e] = -1;
-            tx[i][e] = ti[i][e] >= 0 ? tx[i][e] * a.itau : -INFINITY;
-            m = fmaxf(m, v[i][e]);
-            tm = fmaxf(tm, tx[i][e]);
+    for (int e = 0; e < E; e += 2) {
+        *reinterpret_cast<float2*>(lp + l * E + e) = float2{v[e] - l2s, v[e + 1] - l2s};
+        *reinterpret_cast<f32x4*>(sq + 2 * (l * E + e)) = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    td_sync<1>();  // (a row's lanes are in one wave)
+    float sum = 0.f, more = 0.f;  // more: filled slots that own no class
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+        if (ti[j] >= 0) {
+            lq[j] -= lts;
+            q[j] *= itq;
+            if (q[j] != 0.f) sum += q[j] * (lq[j] - lp[ti[j]]);
+            *reinterpret_cast<float2*>(sq + 2 * ti[j]) = float2{q[j], 1.f};
+            more += 1.f;
         }
-        m = td_row16<true>(m);
-        tm = td_row16<true>(tm);
-        const float mu = __builtin_isinf(m) ? 0.f : m;
-        const bool on = tm != -INFINITY && m != -INFINITY;
-        float s = 0.f, ts = 0.f, p[E], lq[E], q[E];
+    td_sync<1>();
+    sum = td_lanes<L, false>(sum) * kTdLn2;
+    float qs[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            lq[e] = (tx[i][e] - tm) * kTdLog2e;
-            q[e] = ti[i][e] >= 0 ? __builtin_amdgcn_exp2f(lq[e]) : 0.f;
-            ts += q[e];
-            v[i][e] = (v[i][e] - mu) * a.c;
-            p[e] = __builtin_amdgcn_exp2f(v[i][e]);
-            s += p[e];
-        }
-        s = td_row16<false>(s);
-        ts = td_row16<false>(ts);
-        const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s), itq = 1.f / ts, lts = __builtin_amdgcn_logf(ts);
-        int filled = 0;
+    for (int e = 0; e < E; e += 2) {
+        const f32x4 o = *reinterpret_cast<const f32x4*>(sq + 2 * (l * E + e));
+        qs[e] = o[0];
+        qs[e + 1] = o[2];
+        more -= o[1] + o[3];
+    }
+    more = td_lanes<L, false>(more);
+    if (__ballot(more != 0.f)) {  // some class of these rows is named twice: add its slots up in their order
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            lq[e] -= lts;
-            q[e] *= itq;
-            s_lp[i][r][e * 16 + l] = v[i][e] - l2s;
-            s_q[i][r][e * 16 + l] = float2{0.f, -1.f};
-            filled += __popcll(__ballot(ti[i][e] >= 0) & mine);
-        }
-        td_sync<1>();  // (a row's 16 lanes are in one wave)
-        float sum = 0.f;
+        for (int e = 0; e < E; ++e) qs[e] = 0.f;
+        for (int j = 0; j * S < k; ++j) {
+            const int src = (lane & (64 - L)) + j;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (ti[i][e] >= 0) {
-                if (q[e] != 0.f) sum += q[e] * (lq[e] - s_lp[i][r][ti[i][e]]);
-                s_q[i][r][ti[i][e]] = float2{q[e], (float)(e * 16 + l)};
+            for (int o = 0; o < S; ++o) {
+                const int c = __shfl(ti[o], src) - l * E;
+                const float qj = __shfl(q[o], src);
+#pragma unroll
+                for (int e = 0; e < E; ++e) qs[e] += c == e ? qj : 0.f;
             }
-        td_sync<1>();
-        sum = td_row16<false>(sum) * kTdLn2;
-        float qs[E];
-        int owned = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float2 o = s_q[i][r][e * 16 + l];
-            qs[e] = o.x;
-            owned += __popcll(__ballot(o.y >= 0.f) & mine);
-        }
-        if (__ballot(owned != filled)) {  // some class of these rows is named twice: add its slots up in their order
-#pragma unroll
-            for (int e = 0; e < E; ++e) qs[e] = 0.f;
-            for (int j = 0; j < k; ++j) {
-                const int src = (lane & 48) + (j & 15);
-                int c = -1;
-                float qj = 0.f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const int ce = __shfl(ti[i][e], src);
-                    const float qe = __shfl(q[e], src);
-                    if (j >> 4 == e) {
-                        c = ce;
-                        qj = qe;
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < E; ++e) qs[e] += c == e * 16 + l ? qj : 0.f;
-            }
-        }
-        const int64_t row = ((int64_t)blockIdx.x * R + i) * 16 + r;
-        if (row < a.rows) {
-            const float g = a.gs * w[i];
-            const T* z;
-            TG* dz;
-            td_row(a, row, z, dz);
-            if (dz) {
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (e * 16 + l < V) dz[e * 16 + l] = TdElem<GDT>::put(on ? (p[e] * inv - qs[e]) * g : 0.f);
-            }
-            if (l == 0) a.loss[row] = on ? sum * a.tau2 : 0.f;
         }
     }
+    if (!here) return;
+    if (dz) {
+        const float g = a.gs * w;
+        float o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = on ? (p[e] * inv - qs[e]) * g : 0.f;
+        if (nv >= E) td_put<GDT, E>(dz + l * E, o);
+        else
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e < nv) dz[l * E + e] = TdElem<GDT>::put(o[e]);
+    }
+    if (l == 0) a.loss[row] = on ? sum * a.tau2 : 0.f;
 }
 
 template <int DT, int GDT>
 static int td_launch(const TdArgs& a, hipStream_t s) {
     const size_t lds = (size_t)a.k * 16;
+#define CDET_NARROW(L, E)                                                                                          \
+    do {                                                                                                           \
+        const dim3 grid((unsigned)((a.rows + 256 / L - 1) / (256 / L)));                                           \
+        if (a.k <= L) td_narrow_kernel<DT, GDT, L, E, 1><<<grid, dim3(256), 0, s>>>(a);                            \
+        else td_narrow_kernel<DT, GDT, L, E, E><<<grid, dim3(256), 0, s>>>(a);                                     \
+    } while (0)
     const int narrow = a.V > a.k ? a.V : a.k;
-    if (narrow <= 16) td_narrow_kernel<DT, GDT, 1, 4><<<dim3((unsigned)((a.rows + 63) / 64)), dim3(256), 0, s>>>(a);
-    else if (narrow <= 32) td_narrow_kernel<DT, GDT, 2, 2><<<dim3((unsigned)((a.rows + 31) / 32)), dim3(256), 0, s>>>(a);
-    else if (narrow <= 64) td_narrow_kernel<DT, GDT, 4, 1><<<dim3((unsigned)((a.rows + 15) / 16)), dim3(256), 0, s>>>(a);
-    else if (narrow <= 128) td_narrow_kernel<DT, GDT, 8, 1><<<dim3((unsigned)((a.rows + 15) / 16)), dim3(256), 0, s>>>(a);
-    else if (a.V <= 2048) td_wave_kernel<DT, GDT><<<dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 4 * (lds + ((a.V + 7) & ~7) * 4), s>>>(a);
+    if (narrow <= 16) CDET_NARROW(4, 4);
+    else if (narrow <= 32) CDET_NARROW(8, 4);
+    else if (narrow <= 64) CDET_NARROW(16, 4);
+    else if (narrow <= 96) CDET_NARROW(16, 6);
+    else if (narrow <= 128) CDET_NARROW(16, 8);
+#undef CDET_NARROW
+    else if (a.V <= 2048) {
+        const dim3 grid((unsigned)((a.rows + 3) / 4));
+        const size_t row = lds + ((a.V + 7) & ~7) * 4;
+        if (a.V <= 512) td_wave_kernel<DT, GDT, 8><<<grid, dim3(256), 4 * row, s>>>(a);
+        else if (a.V <= 1024) td_wave_kernel<DT, GDT, 16><<<grid, dim3(256), 4 * row, s>>>(a);
+        else td_wave_kernel<DT, GDT, 32><<<grid, dim3(256), 4 * row, s>>>(a);
+    }
     else if (a.V <= 8192) td_wide_kernel<DT, GDT, 4><<<dim3((unsigned)a.rows), dim3(256), lds, s>>>(a);
     else if (a.V <= 16384) td_wide_kernel<DT, GDT, 8><<<dim3((unsigned)a.rows), dim3(512), lds, s>>>(a);
     else if (a.V <= 32768) td_wide_kernel<DT, GDT, 16><<<dim3((unsigned)a.rows), dim3(1024), lds, s>>>(a);

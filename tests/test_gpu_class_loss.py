@@ -340,6 +340,44 @@ def test_topk_distill(P, G, V, k, dtype, gdt):
         assert torch.equal(two[0], got[0][:, 0]) and torch.equal(two[1], got[1][:, 0])
 
 
+# both numbers of slots a lane of every narrow form, tails inside a lane's classes and slots, rows that do not fill a workgroup
+NARROW = [(129, 3, 16, 4), (65, 2, 10, 3), (90, 1, 4, 16), (90, 1, 32, 8), (67, 1, 31, 9), (70, 1, 6, 29), (70, 1, 64, 16), (33, 2, 50, 17), (70, 1, 96, 16), (35, 1, 95, 17), (31, 1, 12, 90),
+          (70, 1, 128, 16), (33, 1, 97, 128), (17, 1, 127, 99)]
+
+
+@pytest.mark.parametrize("dtype,vdt", [(F32, F32), (BF, F32), (BF, BF), (F16, F16), (F32, BF)])
+@pytest.mark.parametrize("P,G,V,k", NARROW)
+def test_topk_distill_narrow_rows(P, G, V, k, dtype, vdt):
+    z = (2.5 * _rand(P, G, V, seed=43)).to(dtype)
+    for dup in (True, False):
+        if not dup and k > V:
+            continue
+        idx, val = teacher(P * G, V, k, 44, dup=dup)
+        idx, val = idx.view(P, G, k), val.view(P, G, k).to(vdt)
+        check_map(_ops().topk_distill(z, idx, val, tau=1.5), z, idx, val, 1.5, None)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("V", [130, 133, 255, 503, 511, 512, 513, 519, 1017, 1024, 1026, 1033, 2041, 2046, 2047])
+def test_topk_distill_row_tails(V, dtype):
+    """What is left of a row behind its last whole 16 bytes, and the ends of the forms by length."""
+    z = (2.5 * _rand(9, V, seed=45)).to(dtype)
+    idx, val = teacher(9, V, 70, 46)
+    idx[:, 5] = V - 1
+    idx[1, 6:9] = V - 2
+    got = _ops().topk_distill(z, idx, val, tau=1.5)
+    check_map(got, z, idx, val, 1.5, None)
+    same = torch.cat([z, z], 1)  # in place, every row at another alignment
+    part = same[:, V:]
+    loss, _ = _ops().topk_distill(part, idx, val, tau=1.5, out=part)
+    assert torch.equal(loss, got[0]) and torch.equal(part, got[1]) and torch.equal(same[:, :V], z)
+
+
+@pytest.mark.parametrize("V,k", [(16, 4), (30, 8), (64, 16), (80, 10), (90, 80), (128, 16)])
+def test_topk_distill_narrow_odd_values(V, k):
+    test_topk_distill_odd_values(V, k)
+
+
 @pytest.mark.parametrize("V,k", [(16, 12), (30, 12), (40, 12), (100, 70), (1000, 20), (1000, 100), (5000, 20), (9000, 20), (40000, 20), (140000, 20)])
 def test_topk_distill_odd_values(V, k):
     """The same class in many slots, -inf logits, rows of nothing but -inf, rows without a teacher that hold NaN, far logits."""
