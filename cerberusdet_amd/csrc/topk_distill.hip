@@ -94,11 +94,10 @@ __device__ __forceinline__ float td_lanes(float v) {
 template <int NW, bool MAX>
 __device__ __forceinline__ float td_reduce(float v, float* scratch) {
     v = td_lanes<16, MAX>(v);
+    float u[4];  // (v_readlane: no LDS crossbar)
 #pragma unroll
-    for (int o = 16; o < 64; o *= 2) {
-        const float u = __shfl_xor(v, o);
-        v = MAX ? fmaxf(v, u) : v + u;
-    }
+    for (int i = 0; i < 4; ++i) u[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 16 * i));
+    v = MAX ? fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])) : (u[0] + u[1]) + (u[2] + u[3]);
     if (NW > 1) {
         const int w = (int)threadIdx.x >> 6;
         __syncthreads();
@@ -187,10 +186,16 @@ __device__ __forceinline__ void td_row(const TdArgs& a, int64_t row, const T*& z
     dz = a.dz ? (TG*)a.dz + (int64_t)px * a.gld + (int64_t)gr * a.V : nullptr;
 }
 
-// V <= 2048: a wave a row, four rows a workgroup, the logits in registers (up to PER a lane) and once in LDS: the slots find theirs there, and then leave their
-// q there for the dense gradient to take along -- no gather from and no second write to memory (67200 x 1203 fp32, k = 32 scattered classes: 123 us = 5.4 TB/s,
-// with them 170). What a row holds behind its last whole 16 bytes goes a logit a lane (as a partial chunk 134 us). PER = 32 for
-// all lengths: 67200 x 365 fp32 55 us, with 8 44.
+// V <= 2048: a wave a row, four rows a workgroup, the logits in registers (up to PER a lane) and, as they are stored, in LDS: the slots find theirs there, and
+// then leave their numbers (16 bits) there for the dense gradient to take their q along -- no gather from and no second write to memory (67200 x 1203 fp32,
+// k = 32 scattered classes: 123 us = 5.4 TB/s, with them 170). LDS of 32 bits an element leaves 16-bit rows half of the waves (67200 x 2048 bf16: 101 us =
+// 5.4 TB/s, so 144). What a row holds behind its last whole 16 bytes goes a logit a lane (67200 x 1203: as a partial chunk 134 us). PER = 32 for all
+// lengths: 67200 x 365 fp32 55 us, with 8 44. 16-bit rows of odd lengths pay for addresses off by 2 bytes: 67200 x 1203 bf16 85 us, x 1204 67.
+__host__ __device__ constexpr int td_wave_slots(int k) { return (14 * k + 4 + 15) & ~15; }  // bytes of a row: q (k + 1), log q, the student's logits, classes,
+template <typename T>
+__host__ __device__ constexpr int td_wave_lds(int k, int V) {  // and the logits as they are stored (16 KiB at most)
+    return td_wave_slots(k) + ((V * (int)sizeof(T) + 15) & ~15);
+}
 template <int DT, int GDT, int PER>
 __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
@@ -200,9 +205,10 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
     const int t = (int)threadIdx.x & 63, V = a.V, k = a.k;
     const int64_t row = (int64_t)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
     if (row >= a.rows) return;  // (whole waves, and no barrier of the workgroup follows)
-    float* const base = lds + ((int)threadIdx.x >> 6) * (4 * k + ((V + 7) & ~7));
-    const TdSlots sl(base, k);
-    float* const rb = base + 4 * k;
+    float* const base = lds + ((int)threadIdx.x >> 6) * (td_wave_lds<T>(k, V) / 4);
+    float *const sq = base, *const slq = base + k + 1, *const sz = slq + k;  // (sq[k] = 0: what a class takes that no slot names)
+    int16_t* const sv = reinterpret_cast<int16_t*>(sz + k);
+    T* const rb = reinterpret_cast<T*>(base + td_wave_slots(k) / 4);
     const T* z;
     TG* dz;
     td_row(a, row, z, dz);
@@ -214,45 +220,43 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
         x0 = load_elem(a.val, row * k + t, a.vdt);
     }
     const float w = a.drow ? a.drow[row] : 1.f;
-    float v[NCH][CH];
+    TdVec<T, CH> raw[NCH];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+        if ((i * 64 + t) * CH + CH <= V) raw[i] = *reinterpret_cast<const TdVec<T, CH>*>(z + (i * 64 + t) * CH);
+    const int et = V - V % CH + t;  // what is left behind the last whole chunk, a logit a lane
+    const T zt = et < V ? z[et] : T(0);
+    float v[NCH][CH], m = -INFINITY, vt = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int e0 = (i * 64 + t) * CH;
         if (e0 + CH <= V) {
-            const TdVec<T, CH> x = *reinterpret_cast<const TdVec<T, CH>*>(z + e0);
+            *reinterpret_cast<u32x4*>(rb + e0) = __builtin_bit_cast(u32x4, raw[i]);
 #pragma unroll
-            for (int e = 0; e < CH; ++e) v[i][e] = TdElem<DT>::get(x.v[e]);
+            for (int e = 0; e < CH; ++e) v[i][e] = TdElem<DT>::get(raw[i].v[e]);
         } else {
 #pragma unroll
             for (int e = 0; e < CH; ++e) v[i][e] = -INFINITY;
         }
+#pragma unroll
+        for (int e = 0; e < CH; ++e) m = fmaxf(m, v[i][e]);
     }
-    const int et = V - V % CH + t;  // what is left behind the last whole chunk, a logit a lane
-    float vt = et < V ? TdElem<DT>::get(z[et]) : -INFINITY;
-    float m = vt;
-    if (et < V) rb[et] = vt;
-#pragma unroll
-    for (int i = 0; i < NCH; ++i)
-        if (i * 64 * CH < V) {
-            const int e0 = (i * 64 + t) * CH;
-#pragma unroll
-            for (int e = 0; e < CH; e += 4) {
-                const f32x4 o = {v[i][e], v[i][e + 1], v[i][e + 2], v[i][e + 3]};
-                if (e0 + CH <= V) *reinterpret_cast<f32x4*>(rb + e0 + e) = o;
-#pragma unroll
-                for (int u = 0; u < 4; ++u) m = fmaxf(m, o[u]);
-            }
-        }
+    if (et < V) {
+        rb[et] = zt;
+        vt = TdElem<DT>::get(zt);
+        m = fmaxf(m, vt);
+    }
+    if (t == 0) sq[k] = 0.f;
     td_sync<1>();
     float tm = -INFINITY;
     for (int j = t; j < k; j += 64) {
         int c = j == t ? v0 : a.idx[row * k + j];
         const float x = (j == t ? x0 : load_elem(a.val, row * k + j, a.vdt)) * a.itau;
         if ((unsigned)c >= (unsigned)V) c = -1;
-        sl.v[j] = c;
-        sl.lq[j] = x;
+        sv[j] = (int16_t)c;
+        slq[j] = x;
         if (c >= 0) {
-            sl.z[j] = rb[c];
+            sz[j] = TdElem<DT>::get(rb[c]);
             tm = fmaxf(tm, x);
         }
     }
@@ -272,47 +276,52 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
     vt = td_exp2<DT>(vt, mu, a.c, muc);
     s += vt;
     for (int j = t; j < k; j += 64)
-        if (sl.v[j] >= 0) ts += expf(sl.lq[j] - tm);
+        if (sv[j] >= 0) {
+            const float lq = (slq[j] - tm) * kTdLog2e, q = __builtin_amdgcn_exp2f(lq);
+            slq[j] = lq;
+            sq[j] = q;
+            ts += q;
+        }
     s = td_reduce<1, false>(s, nullptr);
     ts = td_reduce<1, false>(ts, nullptr);
-    const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s), lts = logf(ts);
-    td_sync<1>();  // every slot has read its logit: from here on the row says which slot names a class (-1: none; of several, one of them)
-    int* const own = reinterpret_cast<int*>(rb);
+    const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s), its = 1.f / ts, lts = __builtin_amdgcn_logf(ts);
+    td_sync<1>();  // every slot has read its logit: from here on the row says which slot names a class (k: none; of several, one of them)
+    uint16_t* const own = reinterpret_cast<uint16_t*>(rb);
+    const uint32_t none = (uint32_t)k * 0x10001u;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int e0 = (i * 64 + t) * CH;
         if (e0 + CH <= V)
 #pragma unroll
-            for (int e = 0; e < CH; e += 4) *reinterpret_cast<u32x4*>(rb + e0 + e) = u32x4{~0u, ~0u, ~0u, ~0u};
+            for (int e = 0; e < CH; e += 4) *reinterpret_cast<uint2*>(own + e0 + e) = uint2{none, none};
     }
-    if (et < V) own[et] = -1;
+    if (et < V) own[et] = (uint16_t)k;
     float sum = 0.f;
     for (int j = t; j < k; j += 64) {
-        const float lq = sl.lq[j] - tm - lts;
-        const float q = on && sl.v[j] >= 0 ? expf(lq) : 0.f;
-        sl.q[j] = q;
-        if (q != 0.f) sum += q * (lq - ((sl.z[j] - mu) * a.c - l2s) * kTdLn2);
+        const float q = on && sv[j] >= 0 ? sq[j] * its : 0.f;
+        sq[j] = q;
+        if (q != 0.f) sum += q * (slq[j] - lts - (sz[j] - mu) * a.c + l2s);
     }
-    sum = td_reduce<1, false>(sum, nullptr);
+    sum = td_reduce<1, false>(sum, nullptr) * kTdLn2;
     if (t == 0) a.loss[row] = on ? sum * a.tau2 : 0.f;
     if (!dz) return;
     td_sync<1>();
     for (int j = t; j < k; j += 64)
-        if (sl.v[j] >= 0) own[sl.v[j]] = j;
+        if (sv[j] >= 0) own[sv[j]] = (uint16_t)j;
     td_sync<1>();
     bool lost = false;  // another slot names this one's class
-    for (int j = t; j < k; j += 64) lost = lost || (sl.v[j] >= 0 && own[sl.v[j]] != j);
+    for (int j = t; j < k; j += 64) lost = lost || (sv[j] >= 0 && own[sv[j]] != j);
     if (__ballot(lost)) {  // a class named twice takes the q of all of its slots, in their order
         for (int j = t; j < k; j += 64) {
-            const int c = sl.v[j];
+            const int c = sv[j];
             if (c < 0 || own[c] != j) continue;
             float q = 0.f;
-            for (int o = 0; o < k; ++o) q += sl.v[o] == c ? sl.q[o] : 0.f;
-            sl.z[j] = q;
+            for (int o = 0; o < k; ++o) q += sv[o] == c ? sq[o] : 0.f;
+            sz[j] = q;
         }
         td_sync<1>();
         for (int j = t; j < k; j += 64)
-            if (sl.v[j] >= 0 && own[sl.v[j]] == j) sl.q[j] = sl.z[j];
+            if (sv[j] >= 0 && own[sv[j]] == j) sq[j] = sz[j];
         td_sync<1>();
     }
     const float g = a.gs * w;
@@ -322,21 +331,22 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
         if (e0 + CH > V) continue;
         float o[CH];
 #pragma unroll
-        for (int e = 0; e < CH; e += 4) {
-            const u32x4 by = *reinterpret_cast<const u32x4*>(rb + e0 + e);
+        for (int e = 0; e < CH; ++e) o[e] = v[i][e] * inv;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                float p = v[i][e + u] * inv;
-                if ((int)by[u] >= 0) p -= sl.q[by[u]];
-                o[e + u] = on ? p * g : 0.f;
+        for (int e = 0; e < CH; e += 4) {
+            const uint2 by = *reinterpret_cast<const uint2*>(own + e0 + e);
+            if (((by.x ^ none) | (by.y ^ none)) != 0u) {
+                o[e] -= sq[by.x & 0xffffu];
+                o[e + 1] -= sq[by.x >> 16];
+                o[e + 2] -= sq[by.y & 0xffffu];
+                o[e + 3] -= sq[by.y >> 16];
             }
         }
+#pragma unroll
+        for (int e = 0; e < CH; ++e) o[e] = on ? o[e] * g : 0.f;
         td_put<GDT, CH>(dz + e0, o);
     }
-    if (et < V) {
-        const int by = own[et];
-        dz[et] = TdElem<GDT>::put(on ? (vt * inv - (by >= 0 ? sl.q[by] : 0.f)) * g : 0.f);
-    }
+    if (et < V) dz[et] = TdElem<GDT>::put(on ? (vt * inv - sq[own[et]]) * g : 0.f);
 }
 
 // V <= 32768: a row's logits in registers, up to NCH chunks of CH per thread, NW waves a row; loss, maximum and sum from one read. Bound by memory:
@@ -720,7 +730,7 @@ static int td_launch(const TdArgs& a, hipStream_t s) {
 #undef CDET_NARROW
     else if (a.V <= 2048) {
         const dim3 grid((unsigned)((a.rows + 3) / 4));
-        const size_t row = lds + ((a.V + 7) & ~7) * 4;
+        const size_t row = td_wave_lds<typename TdElem<DT>::T>(a.k, a.V);
         if (a.V <= 512) td_wave_kernel<DT, GDT, 8><<<grid, dim3(256), 4 * row, s>>>(a);
         else if (a.V <= 1024) td_wave_kernel<DT, GDT, 16><<<grid, dim3(256), 4 * row, s>>>(a);
         else td_wave_kernel<DT, GDT, 32><<<grid, dim3(256), 4 * row, s>>>(a);
