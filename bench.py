@@ -707,11 +707,12 @@ def main():
             dist.init_process_group(backend="nccl", device_id=device)
 
     from cerberusdet_amd.trainers import Averaging
+    from cerberusdet_amd.trainers.averaging import on_group
 
     model, cfg = build_model(args.cfg, device)
     if use_dist:  # every rank starts from rank 0's weights (what DDP's constructor broadcast does in the reference, train.py:184)
         for t in list(model.state_dict().values()):
-            dist.broadcast(t, src=0)
+            on_group(dist.broadcast, t, src=0)
     trainer = Averaging(device, model, HYP, TASKS, epochs=100, nb=1000, rank=rank if use_dist else -1, world_size=world, sync_bn=args.sync_bn)
     n_iter = args.warmup + args.steps
     n_distinct = min(n_iter, 4)  # a few distinct synthetic batches, resident in HBM, cycled
@@ -753,7 +754,7 @@ def main():
     dt = time.perf_counter() - t0
     if use_dist:
         tt = torch.tensor([dt], device=device, dtype=torch.float64)
-        dist.all_reduce(tt, op=dist.ReduceOp.MAX)
+        on_group(dist.all_reduce, tt, op=dist.ReduceOp.MAX)
         dt = float(tt)
     comm_exposed = None
     if comm_timer is not None:

@@ -249,7 +249,7 @@ class Plan:
         plans of the same tasks (frozen / unfrozen trunk, another batch shape) reuse their slots (peer_exchange.PeerExchange.make_call)."""
         import torch.distributed as dist
 
-        from .trainers.averaging import comm_span
+        from .trainers.averaging import comm_span, on_group
 
         model = self.model
         px = getattr(self.model, "_peer_xchg", None)
@@ -265,7 +265,7 @@ class Plan:
 
         def call(st, t=t):
             with comm_span(model, "syncbn"):
-                dist.all_reduce(t, op=dist.ReduceOp.SUM)
+                on_group(dist.all_reduce, t, op=dist.ReduceOp.SUM)
 
         call.__name__ = "all_reduce"
         return call

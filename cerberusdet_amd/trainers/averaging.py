@@ -121,6 +121,24 @@ def _block_of(key: str) -> int:
     return int(parts[1]) if len(parts) > 2 and parts[0] == "blocks" and parts[1].isdigit() else -1
 
 
+class _Done:
+    """The handle of a collective that has ended."""
+
+    def wait(self):
+        return True
+
+
+def on_group(collective, t: torch.Tensor, group=None, async_op: bool = False, **kw):
+    """`collective` (dist.all_reduce, dist.broadcast) of `t` in place, on the current stream's order. A gloo group is given host memory -- a synchronous copy there
+    and back: its collectives on device tensors hang now and then where several ranks share one GPU (the only place where gloo meets GPU tensors)."""
+    if t.is_cuda and dist.is_initialized() and dist.get_backend(group) == "gloo":
+        host = t.cpu()
+        collective(host, group=group, **kw)
+        t.copy_(host)
+        return _Done() if async_op else None
+    return collective(t, group=group, async_op=async_op, **kw)
+
+
 class GradReducer:
     """Bucketed gradient all-reduce keyed on the block DAG. One flat fp32 bucket per block, sent as REDUCTION UNITS: the slices that become
     final at one point of the backward -- every backbone row of block 0, every other block as a whole. A unit is reduced (SUM, async) when the
@@ -158,7 +176,7 @@ class GradReducer:
         current stream's order. The trainer calls it the moment the slice is final (Averaging._unit_done)."""
         if not self.enabled or (block_idx is not None and block_idx in self.skip_blocks):
             return
-        self.handles.append(dist.all_reduce(t, op=dist.ReduceOp.SUM, group=self.group, async_op=True))
+        self.handles.append(on_group(dist.all_reduce, t, group=self.group, async_op=True, op=dist.ReduceOp.SUM))
         self.reduced_bytes += t.numel() * t.element_size()
 
     def wait(self):
