@@ -373,6 +373,14 @@ def test_topk_distill_row_tails(V, dtype):
     assert torch.equal(loss, got[0]) and torch.equal(part, got[1]) and torch.equal(same[:, :V], z)
 
 
+@pytest.mark.parametrize("P,V,k", [(9, 100, 300), (5, 1, 200), (6, 2048, 512), (3, 2040, 511)])
+def test_topk_distill_more_slots_than_classes_and_the_most(P, V, k):
+    z = 2.5 * _rand(P, V, seed=47)
+    idx, val = teacher(P, V, k, 48)
+    check_map(_ops().topk_distill(z, idx, val, tau=2.0), z, idx, val, 2.0, None)
+    check_map(_ops().topk_distill(z.bfloat16(), idx, val, tau=2.0), z.bfloat16(), idx, val, 2.0, None)
+
+
 @pytest.mark.parametrize("V,k", [(16, 4), (30, 8), (64, 16), (80, 10), (90, 80), (128, 16)])
 def test_topk_distill_narrow_odd_values(V, k):
     test_topk_distill_odd_values(V, k)
