@@ -145,7 +145,7 @@ class _TopkDistillFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        return (ctx.dz * g[..., None]).to(ctx.dz.dtype), None, None, None
+        return (ctx.dz * g[..., None]).to(ctx.dz.dtype), None, None, None  # (16-bit logits: rounded to their type as dz, and once more times g)
 
 
 def linear_cross_entropy(x, w, labels, offset=None, scale=1.0, reduction="mean"):
