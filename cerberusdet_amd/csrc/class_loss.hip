@@ -18,6 +18,7 @@
 // memory runs along the output index instead of K is staged as it lies and transposed by ds_read_b64_tr_b16 on the way to the registers.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -1077,6 +1078,281 @@ __global__ __launch_bounds__(256) void class_zero_kernel(uint16_t* p, int64_t ro
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * d; i += (int64_t)gridDim.x * 256) p[i / d * ld + i % d] = 0;
 }
 
+// ---- backward of few rows ------------------------------------------------------------------------------------------------------------------------------
+// At most 128 rows: the class list is what there is to read, so one launch does with one read of it what the tiles above do with two and four launches.
+// A workgroup holds x in LDS and walks over blocks of 32 classes, the next block's weights on the way to registers under this one's products:
+//   z [classes][rows] = w x^T, K = d shared out to the waves and joined in LDS;  dz, 16-bit, in both orders -- up to 64 rows as two such numbers, the
+//   second what the first one's rounding leaves: a row's few large entries average no roundings, and the products wait for memory (from 65 rows on they
+//   do not: 128 x 131072 x 320 87 us with one, 110 with two);
+//   dw block = dz x, written out;  dx += dz w, in registers until the end: one fp32 slice a workgroup (class_few_sum_kernel adds them in their order).
+// A wave owns FT tiles of 32 features in the last two; RT tiles of 32 rows. Bound by memory for long lists, w in and dw out: backward of 1 x 131072 x 960
+// 113 us = 4.5 TB/s (by tiles of 128 x 128: 183), 32 x 131072 x 512 72 us (98), 128 x 131072 x 320 87 us (100); of short ones by three waits for LDS and
+// one for memory: 96 x 365 x 320 15 + 4 us of kernels (21).
+struct FewArgs {
+    const uint16_t *x, *w;
+    int64_t x_ld, w_ld;
+    const float* off;
+    float c, coff;
+    int N, V, d;
+    const void* label;
+    int label64;
+    const int32_t* idx;   // the teacher's slots (at most kFewSlots * 512), or null
+    const float* saved;
+    int k;
+    const float* lse;
+    int64_t lse_stride;
+    const float* drow;
+    int drow_stride;
+    float gain, spread;   // as PrepArgs
+    uint16_t* dw;         // or null
+    int64_t dw_ld;
+    float* slab;          // dx [workgroups][N][d], or null
+    float* outscale;
+};
+constexpr int kFewSlots = 8;
+static inline int few_lds(int RT, int d) {
+    const int S = (d + 31) / 32 * 64 + 16;
+    return (RT * 32 + 32) * S + 32768 + RT * 32 * 80 + 32 * (RT * 64 + 16) + (RT * 32 * 4 + 64) * 4;
+}
+__device__ __forceinline__ u32x4 few_row(const unsigned char* p) { return *reinterpret_cast<const u32x4*>(p); }
+// features f0 .. +31 as fragment rows, K = lines k0 .. +15 of S bytes
+__device__ __forceinline__ u32x4 few_tr(const unsigned char* base, int S, int k0, int f0, int lane) {
+    typedef s16x4 __attribute__((address_space(3))) * lds_t;
+    const unsigned char* p = base + (k0 + 8 * (lane >> 5) + ((lane & 15) >> 2)) * S + (f0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
+    const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)p)),
+                hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p + 4 * S)));
+    return u32x4{lo.x, lo.y, hi.x, hi.y};
+}
+__device__ __forceinline__ void few_sync() {  // LDS only: loads in flight stay in flight
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+}
+template <int DT, int RT, int FT>
+__global__ __launch_bounds__(512, 2) void class_few_kernel(const FewArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    constexpr int KP = 8 / RT, CS = RT * 64 + 16, WP = FT * 2;
+    constexpr bool TWO = RT <= 2;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, h = lane >> 5;
+    const int nft = (a.d + 31) >> 5, S = nft * 64 + 16, nch = (a.V + 31) >> 5, step = (int)gridDim.x;
+    unsigned char *xs = smem, *ws = xs + RT * 32 * S, *red = ws + 32 * S, *dzr = red + 32768, *dzc = dzr + RT * 32 * 80, *lor = red, *loc = red + RT * 32 * 80;
+    float *l2s = reinterpret_cast<float*>(dzc + 32 * CS), *gs = l2s + RT * 32, *gm = gs + RT * 32, *offs = gm + RT * 32;
+    int* labs = reinterpret_cast<int*>(offs + 64);
+    int ch = (int)blockIdx.x;
+    // a block's weights, the wave's own features of them; offsets (-inf: left out, or behind the last class)
+    u32x4 wr[WP];
+    float on = 0.f;
+    auto fetch = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < WP; ++i) {
+            const int p = lane + 64 * i, v = b * 32 + p / (FT * 4), col = (wave * FT * 4 + p % (FT * 4)) * 8;
+            wr[i] = v < a.V && col < a.d ? *reinterpret_cast<const u32x4*>(a.w + v * a.w_ld + col) : u32x4{0, 0, 0, 0};
+        }
+        if (tid < 32) on = b * 32 + tid >= a.V ? -INFINITY : a.off ? a.off[b * 32 + tid] : 0.f;
+    };
+    fetch(ch);
+    int sv[kFewSlots];
+#pragma unroll
+    for (int u = 0; u < kFewSlots; ++u) sv[u] = a.idx && tid + 512 * u < a.N * a.k ? a.idx[tid + 512 * u] : -1;
+    if (tid < RT * 32) {  // the rows, as class_prep_kernel has them
+        const int r = tid;
+        float l = r < a.N ? a.lse[r * a.lse_stride] : 0.f, g = r < a.N ? (a.drow ? a.drow[(int64_t)r * a.drow_stride] : 1.f) : 0.f;
+        const int64_t lab = a.label && r < a.N ? load_label(a.label, a.label64, r) : -1;
+        const bool live = r < a.N && (a.label ? l != -INFINITY && lab >= 0 && lab < a.V : l != INFINITY);
+        l *= kLog2e;
+        l2s[r] = !live ? INFINITY : l == INFINITY ? NAN : l;
+        gs[r] = live ? g : 0.f;
+        gm[r] = live && fabsf(g) <= 3.4e38f ? fabsf(g) : 0.f;
+        labs[r] = live ? (int)lab : -1;
+    }
+    if (tid < 32) offs[tid] = on;
+    __syncthreads();
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < (RT + 1) / 2; ++i) m = fmaxf(m, gm[(lane + 64 * i) & (RT * 32 - 1)]);
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    m = m > 0.f ? fminf(fmaxf(m, 1e-30f), 1e37f) : 1.f;
+    const float down = 1.984375f * a.spread / m, os = a.gain * m / (1.984375f * a.spread);
+    if (blockIdx.x == 0 && tid == 0) *a.outscale = os;
+#pragma unroll 1
+    for (int p = lane; p < nft * 4; p += 64) {  // x, zeros in the rows that take no part and behind the last feature
+        u32x4 xv[RT * 4];
+#pragma unroll
+        for (int i = 0; i < RT * 4; ++i) {
+            const int r = wave + 8 * i;
+            xv[i] = p * 8 < a.d && l2s[r] != INFINITY ? *reinterpret_cast<const u32x4*>(a.x + r * a.x_ld + p * 8) : u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < RT * 4; ++i) *reinterpret_cast<u32x4*>(xs + (wave + 8 * i) * S + p * 16) = xv[i];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    f32x16 acc[RT][FT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int i = 0; i < FT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[t][i][e] = 0.f;
+    const int t0 = wave % RT, kp = wave / RT;
+    for (int buf = 0; ch < nch; ch += step, buf ^= 32) {
+        int ln = (int)threadIdx.x & 63;
+        asm volatile("" : "+v"(ln));  // (addresses are computed anew for every block: kept across the loop they cost more registers than there are)
+        const int lane = ln, l31 = lane & 31, h = lane >> 5, tid = wave * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < WP; ++i) {
+            const int p = lane + 64 * i, row = p / (FT * 4), at = wave * FT * 4 + p % (FT * 4);
+            if (at < nft * 4) *reinterpret_cast<u32x4*>(ws + row * S + at * 16) = offs[buf + row] == -INFINITY ? u32x4{0, 0, 0, 0} : wr[i];
+        }
+        if (ch + step < nch) fetch(ch + step);
+        few_sync();
+        f32x16 z;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[e] = 0.f;
+        const unsigned char *wz = ws + l31 * S + h * 16, *xz = xs + (t0 * 32 + l31) * S + h * 16;
+#pragma unroll 4
+        for (int s = kp; s < 2 * nft; s += KP) z = lmfma<DT>(few_row(wz + s * 32), few_row(xz + s * 32), z);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f32x4*>(red + (wave * 32 + l31) * 128 + (((2 * q + h) ^ (l31 & 7)) << 4)) = f32x4{z[4 * q], z[4 * q + 1], z[4 * q + 2], z[4 * q + 3]};
+        if (tid < 32) offs[(buf ^ 32) + tid] = on;
+        few_sync();
+        // two classes of RT rows a thread
+        const int r31 = tid >> 4, cp = tid & 15;
+        const float2 o = *reinterpret_cast<const float2*>(offs + buf + 2 * cp);
+        float2 sums[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            sums[t] = float2{0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < KP; ++j) {
+                const float2 u = *reinterpret_cast<const float2*>(red + ((j * RT + t) * 32 + r31) * 128 + (((cp >> 1) ^ (r31 & 7)) << 4) + (cp & 1) * 8);
+                sums[t].x += u.x;
+                sums[t].y += u.y;
+            }
+        }
+        if (TWO) few_sync();  // (the rests take the place of the sums)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const float2 s = sums[t];
+            const int r = t * 32 + r31, at = labs[r] - ch * 32 - 2 * cp;
+            const float l2 = l2s[r], g = gs[r] * down, mag = fabsf(g), l2g = l2 - __builtin_amdgcn_logf(mag);
+            float d0 = __builtin_amdgcn_exp2f(fmaf(s.x, a.c, o.x * a.coff) - l2g), d1 = __builtin_amdgcn_exp2f(fmaf(s.y, a.c, o.y * a.coff) - l2g);
+            d0 -= at == 0 ? mag : 0.f;
+            d1 -= at == 1 ? mag : 0.f;
+            d0 = o.x == -INFINITY || l2 == INFINITY ? 0.f : g < 0.f ? -d0 : d0;
+            d1 = o.y == -INFINITY || l2 == INFINITY ? 0.f : g < 0.f ? -d1 : d1;
+            const uint32_t pk = lpack2<DT>(d0, d1);
+            *reinterpret_cast<uint32_t*>(dzr + r * 80 + cp * 4) = pk;
+            *reinterpret_cast<uint16_t*>(dzc + 2 * cp * CS + r * 2) = (uint16_t)pk;
+            *reinterpret_cast<uint16_t*>(dzc + (2 * cp + 1) * CS + r * 2) = (uint16_t)(pk >> 16);
+            if (TWO) {
+                const uint32_t rest = lpack2<DT>(d0 - Elem<DT>::to_f32((uint16_t)pk), d1 - Elem<DT>::to_f32((uint16_t)(pk >> 16)));
+                *reinterpret_cast<uint32_t*>(lor + r * 80 + cp * 4) = rest;
+                *reinterpret_cast<uint16_t*>(loc + 2 * cp * CS + r * 2) = (uint16_t)rest;
+                *reinterpret_cast<uint16_t*>(loc + (2 * cp + 1) * CS + r * 2) = (uint16_t)(rest >> 16);
+            }
+        }
+        few_sync();
+        if (a.idx) {  // the classes that the teacher names
+#pragma unroll
+            for (int u = 0; u < kFewSlots; ++u) {
+                const unsigned v = (unsigned)sv[u] - (unsigned)ch * 32u;
+                if (v >= 32u) continue;
+                const int i = tid + 512 * u, r = i / a.k, j = i - r * a.k;
+                const float z2 = a.saved[(int64_t)r * (1 + 2 * a.k) + 1 + j], q = a.saved[(int64_t)r * (1 + 2 * a.k) + 1 + a.k + j], l2 = l2s[r];
+                if (q == -1.f || l2 == INFINITY || z2 == -INFINITY) continue;  // (TeacherDz)
+                const float dz = (__builtin_amdgcn_exp2f(z2 - l2) - q) * (gs[r] * down);
+                const uint16_t b = Elem<DT>::from_f32(dz);
+                *reinterpret_cast<uint16_t*>(dzr + r * 80 + v * 2) = b;
+                *reinterpret_cast<uint16_t*>(dzc + v * CS + r * 2) = b;
+                if (TWO) {
+                    const uint16_t rest = Elem<DT>::from_f32(dz - Elem<DT>::to_f32(b));
+                    *reinterpret_cast<uint16_t*>(lor + r * 80 + v * 2) = rest;
+                    *reinterpret_cast<uint16_t*>(loc + v * CS + r * 2) = rest;
+                }
+            }
+            few_sync();
+        }
+#pragma unroll
+        for (int i = 0; i < FT; ++i) {
+            const int f0 = (wave * FT + i) * 32;
+            if (f0 >= a.d) break;
+            if (a.slab) {
+                const u32x4 w0 = few_tr(ws, S, 0, f0, lane), w1 = few_tr(ws, S, 16, f0, lane);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    const int b = (t * 32 + l31) * 80 + h * 16;
+                    acc[t][i] = lmfma<DT>(w0, few_row(dzr + b), acc[t][i]);
+                    acc[t][i] = lmfma<DT>(w1, few_row(dzr + b + 32), acc[t][i]);
+                    if (TWO) {
+                        acc[t][i] = lmfma<DT>(w0, few_row(lor + b), acc[t][i]);
+                        acc[t][i] = lmfma<DT>(w1, few_row(lor + b + 32), acc[t][i]);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (a.dw) {  // onto the block's weights, which nobody reads any more
+                f32x16 o16;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o16[e] = 0.f;
+#pragma unroll
+                for (int t = 0; t < 2 * RT; ++t) {
+                    const u32x4 xt = few_tr(xs, S, t * 16, f0, lane);
+                    o16 = lmfma<DT>(xt, few_row(dzc + l31 * CS + t * 32 + h * 16), o16);
+                    if (TWO) o16 = lmfma<DT>(xt, few_row(loc + l31 * CS + t * 32 + h * 16), o16);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<uint2*>(ws + l31 * S + (f0 + 8 * q + 4 * h) * 2) =
+                        uint2{lpack2<DT>(o16[4 * q] * os, o16[4 * q + 1] * os), lpack2<DT>(o16[4 * q + 2] * os, o16[4 * q + 3] * os)};
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (a.dw) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < WP; ++i) {
+                const int p = lane + 64 * i, v = ch * 32 + p / (FT * 4), at = wave * FT * 4 + p % (FT * 4);
+                if (v < a.V && at * 8 < a.d) *reinterpret_cast<u32x4*>(a.dw + v * a.dw_ld + at * 8) = few_row(ws + (p / (FT * 4)) * S + at * 16);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    if (!a.slab) return;
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int i = 0; i < FT; ++i) {
+            const int r = t * 32 + l31, f0 = (wave * FT + i) * 32 + 4 * h;
+            if (r >= a.N) continue;
+            float* dst = a.slab + ((int64_t)blockIdx.x * a.N + r) * a.d;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (f0 + 8 * q < a.d)
+                    *reinterpret_cast<f32x4*>(dst + f0 + 8 * q) = f32x4{acc[t][i][4 * q], acc[t][i][4 * q + 1], acc[t][i][4 * q + 2], acc[t][i][4 * q + 3]};
+        }
+}
+// the slices of dx: 8 threads a column of four, every eighth slice each
+template <int DT>
+__global__ __launch_bounds__(256) void class_few_sum_kernel(const float* slab, int slices, int N, int d, uint16_t* out, int64_t ld, const float* outscale) {
+    __shared__ f32x4 sm[8][32];
+    const int c = (int)threadIdx.x & 31, g = (int)threadIdx.x >> 5, n4 = N * (d / 4), at = (int)blockIdx.x * 32 + c;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (at < n4)
+#pragma unroll 4
+        for (int s = g; s < slices; s += 8) v += reinterpret_cast<const f32x4*>(slab)[(int64_t)s * n4 + at];
+    sm[g][c] = v;
+    __syncthreads();
+    if (g || at >= n4) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v += sm[i][c];
+    const float os = *outscale;
+    const int r = at / (d / 4), f = (at - r * (d / 4)) * 4;
+    *reinterpret_cast<uint2*>(out + r * ld + f) = uint2{lpack2<DT>(v[0] * os, v[1] * os), lpack2<DT>(v[2] * os, v[3] * os)};
+}
+
 // ---- distillation: the teacher's slots ---------------------------------------------------------------------------------------------------------------
 // A workgroup a row, 16 lanes a slot: the student's logits at the teacher's classes (dot products in fp32), the teacher's softmax over its filled slots, the
 // loss. Rows of w are fetched from all over the list: 64 of them in flight a workgroup (1021 x 50 x 512: 16 us, with one wave a row 22).
@@ -1282,7 +1558,9 @@ struct LinPlan {
     GradShape g;
     int64_t o_part, o_zlab, o_lse, fwd_bytes;
     int64_t o_lse2, o_coef, o_scale, o_live, o_kept, o_x, o_w, o_dz, o_slab, o_wslab, bwd_bytes;
+    int few, few_wgs;  // backward of few rows: 0, or row tiles of class_few_kernel; its workgroups (workspace: the scale, 256 bytes, and their slices)
 };
+static const int kFewRows = 128;
 static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool backward) {
     LinPlan p = {};
     const int64_t N = q->N, V = q->V, d = q->d;
@@ -1323,6 +1601,15 @@ static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool backward) {
     p.o_slab = p.direct ? 0 : take((int64_t)shape.splits * N * d * 4);
     p.o_wslab = shape.wsplits > 1 ? take((int64_t)shape.wsplits * shape.piece * d * 4) : 0;
     p.bwd_bytes = o;
+    if (N <= kFewRows) {
+        const int rt = N <= 32 ? 1 : N <= 64 ? 2 : 4, ft = (int)up(up(d, 32) / 32, 8) / 8;
+        if (rt * ft <= (rt == 2 ? 6 : rt == 1 ? 4 : 8) && few_lds(rt, (int)d) <= 160 * 1024) {
+            p.few = rt;
+            const double nch = (double)(up(V, 32) / 32);
+            p.few_wgs = (int)std::max(1., std::min(std::min(nch, 256.), std::sqrt(nch * 1.9e6 / (double)(N * d))));
+            p.bwd_bytes = std::max(p.bwd_bytes, 256 + (int64_t)p.few_wgs * N * d * 4);
+        }
+    }
     return p;
 }
 
@@ -1395,6 +1682,42 @@ static int launch_grads(const GradArgs& a, int dtype, bool big, hipStream_t s) {
     return 0;
 }
 
+static int launch_few(const FewArgs& a, int dtype, int rt, int wgs, uint16_t* dx, int64_t dx_ld, hipStream_t s) {
+    const size_t lds = (size_t)few_lds(rt, a.d);
+    const int nft = (a.d + 31) / 32;
+#define CDET_GO(DT_, RT_, FT_)                                                                        \
+    do {                                                                                              \
+        static std::atomic<uint64_t> seen{0};                                                         \
+        allow_lds(seen, class_few_kernel<DT_, RT_, FT_>, 160 * 1024);                                 \
+        class_few_kernel<DT_, RT_, FT_><<<dim3((unsigned)wgs), dim3(512), lds, s>>>(a);               \
+    } while (0)
+#define CDET_FEW(DT_)                                                                                 \
+    do {                                                                                              \
+        if (rt == 1) {                                                                                \
+            if (nft <= 8) CDET_GO(DT_, 1, 1);                                                         \
+            else if (nft <= 16) CDET_GO(DT_, 1, 2);                                                   \
+            else CDET_GO(DT_, 1, 4);                                                                  \
+        } else if (rt == 2) {                                                                         \
+            if (nft <= 8) CDET_GO(DT_, 2, 1);                                                         \
+            else CDET_GO(DT_, 2, 3);                                                                  \
+        } else {                                                                                      \
+            if (nft <= 8) CDET_GO(DT_, 4, 1);                                                         \
+            else CDET_GO(DT_, 4, 2);                                                                  \
+        }                                                                                             \
+    } while (0)
+    if (dtype == CDET_BF16) CDET_FEW(CDET_BF16);
+    else CDET_FEW(CDET_F16);
+#undef CDET_FEW
+#undef CDET_GO
+    CDET_LAUNCH_CHECK();
+    if (!dx) return 0;
+    const unsigned nb = (unsigned)div_up((int64_t)a.N * (a.d / 4), 32);
+    if (dtype == CDET_BF16) class_few_sum_kernel<CDET_BF16><<<dim3(nb), dim3(256), 0, s>>>(a.slab, wgs, a.N, a.d, dx, dx_ld, a.outscale);
+    else class_few_sum_kernel<CDET_F16><<<dim3(nb), dim3(256), 0, s>>>(a.slab, wgs, a.N, a.d, dx, dx_ld, a.outscale);
+    CDET_LAUNCH_CHECK();
+    return 0;
+}
+
 static LogitArgs logit_args(const cdet_linear_loss_desc* q) {
     LogitArgs a = {};
     a.x_ld = q->x_ld;
@@ -1438,6 +1761,35 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         return 0;
     }
     const LinPlan p = lin_plan(q, true);
+    if (p.few && (!idx || N * (int64_t)k <= kFewSlots * 512)) {
+        FewArgs a = {};
+        a.x = (const uint16_t*)x;
+        a.w = (const uint16_t*)w;
+        a.x_ld = q->x_ld;
+        a.w_ld = q->w_ld;
+        a.off = q->offset;
+        a.c = q->scale / q->tau * kLog2e;
+        a.coff = kLog2e / q->tau;
+        a.N = N;
+        a.V = V;
+        a.d = d;
+        a.label = label;
+        a.label64 = q->label64;
+        a.idx = idx;
+        a.saved = saved;
+        a.k = k;
+        a.lse = lse;
+        a.lse_stride = lse_stride;
+        a.drow = drow;
+        a.drow_stride = drow_stride;
+        a.gain = q->scale * (idx ? q->tau : 1.f);
+        a.spread = q->dtype == CDET_F16 ? 4096.f : 1.f;
+        a.dw = (uint16_t*)dw;
+        a.dw_ld = dw_ld;
+        a.slab = dx ? (float*)(ws + 256) : nullptr;
+        a.outscale = (float*)ws;
+        return launch_few(a, q->dtype, p.few, p.few_wgs, (uint16_t*)dx, dx_ld, s);
+    }
     float *lse2 = (float*)(ws + p.o_lse2), *coef = (float*)(ws + p.o_coef), *os = (float*)(ws + p.o_scale);
     const float spread = q->dtype == CDET_F16 ? 4096.f : 1.f;
     PrepArgs pa = {};

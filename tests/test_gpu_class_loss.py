@@ -256,6 +256,57 @@ def test_linear_distill(N, V, d, k, dtype):
         check_grads(dx, dw, ref, x, scale=1.3, tau=tau)
 
 
+FEW = [(1, 33, 8), (2, 32, 256), (31, 31, 264), (32, 97, 960), (32, 9001, 512), (33, 64, 608), (64, 700, 40), (60, 20000, 264), (65, 65, 320), (128, 1000, 256), (97, 12000, 304), (1, 40000, 520),
+       (33, 70, 616), (70, 70, 328), (32, 70, 968)]  # (the last three: a row of features more than the few rows' kernel holds)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("N,V,d", FEW)
+def test_few_rows(N, V, d, dtype):
+    """The ends of the backward of few rows, with every kind of row and class: ignored rows and left-out classes that hold NaN, negative and zero gradients."""
+    ops = _ops()
+    x, w, labels = ce_case(N, V, d, dtype, seed=60)
+    off = _rand(V, seed=61)
+    drow = _rand(N, seed=62)
+    xb, wb = x.clone(), w.clone()
+    if N > 2:
+        labels[::5] = -1
+        xb[::5] = math.nan
+        drow[1] = 0
+    if V > 32:
+        off[::7] = -math.inf
+        wb[::7] = math.inf
+        off[labels[labels >= 0]] = 0.25
+    wb = torch.where((off == -math.inf)[:, None], wb, w)
+    loss, lse, dx, dw = run_ce(xb, wb, labels, offset=off, scale=0.8, drow=drow)
+    ref = reference(x, w, labels, offset=off, scale=0.8, drow=drow)
+    check_rows(loss, ref["loss"], loss_tol(ref, d))
+    check_grads(dx, dw, ref, x, scale=0.8)
+    again = run_ce(xb, wb, labels, offset=off, scale=0.8, drow=drow)
+    assert torch.equal(dx, again[2]) and torch.equal(dw, again[3])
+    assert torch.equal(run_ce(xb, wb, labels, offset=off, scale=0.8, drow=drow, dw=False)[2], dx)
+    assert torch.equal(run_ce(xb, wb, labels, offset=off, scale=0.8, drow=drow, dx=False)[3], dw)
+    k = min(V, 11)
+    idx, val = teacher(N, V, k, 63, empty=N > 2)
+    loss, saved = ops.linear_distill_fwd(x, w, idx, val, tau=2.0)
+    dx, dw = ops.linear_distill_bwd(x, w, idx, saved, drow, tau=2.0)
+    ref = reference(x, w, idx=idx, val=val, tau=2.0, drow=drow)
+    check_rows(loss, ref["loss"], 4 * (2 * loss_tol(ref, d) + 64 * U * 16))
+    check_grads(dx, dw, ref, x, tau=2.0)
+
+
+@pytest.mark.parametrize("N,k", [(8, 512), (9, 512), (128, 32), (128, 33)])
+def test_few_rows_slots(N, k):
+    """As many slots as the few rows' kernel takes, and one row or slot more."""
+    ops = _ops()
+    x, w, _ = ce_case(N, 900, 64, BF, seed=65)
+    idx, val = teacher(N, 900, k, 66)
+    loss, saved = ops.linear_distill_fwd(x, w, idx, val, tau=1.5)
+    ref = reference(x, w, idx=idx, val=val, tau=1.5)
+    check_rows(loss, ref["loss"], 2.25 * (2 * loss_tol(ref, 64) + 64 * U * 16))
+    check_grads(*ops.linear_distill_bwd(x, w, idx, saved, tau=1.5), ref, x, tau=1.5)
+
+
 def test_linear_distill_types_and_infinities():
     """16-bit teacher logits; -inf in a slot counts as nothing; a slot at a left-out class is loss inf; NaN in rows without a teacher reaches nothing."""
     ops = _ops()
