@@ -1129,7 +1129,7 @@ __device__ __forceinline__ void few_sync() {  // LDS only: loads in flight stay 
     __builtin_amdgcn_sched_barrier(0);
 }
 template <int DT, int RT, int FT>
-__global__ __launch_bounds__(512, 2) void class_few_kernel(const FewArgs a) {
+__global__ __launch_bounds__(512, RT * FT <= 2 ? 4 : 2) void class_few_kernel(const FewArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr int KP = 8 / RT, CS = RT * 64 + 16, WP = FT * 2;
     constexpr bool TWO = RT <= 2;
@@ -1334,91 +1334,75 @@ __global__ __launch_bounds__(512, 2) void class_few_kernel(const FewArgs a) {
                     *reinterpret_cast<f32x4*>(dst + f0 + 8 * q) = f32x4{acc[t][i][4 * q], acc[t][i][4 * q + 1], acc[t][i][4 * q + 2], acc[t][i][4 * q + 3]};
         }
 }
-// the slices of dx: 8 threads a column of four, every eighth slice each
+// the slices of dx: 32 threads a column of four, every 32nd slice each (with 8 threads the 512 slices of 4 x 21675 x 232 took 7.9 us, so 4.0)
 template <int DT>
 __global__ __launch_bounds__(256) void class_few_sum_kernel(const float* slab, int slices, int N, int d, uint16_t* out, int64_t ld, const float* outscale) {
-    __shared__ f32x4 sm[8][32];
-    const int c = (int)threadIdx.x & 31, g = (int)threadIdx.x >> 5, n4 = N * (d / 4), at = (int)blockIdx.x * 32 + c;
+    __shared__ f32x4 sm[32][8];
+    const int c = (int)threadIdx.x & 7, g = (int)threadIdx.x >> 3, n4 = N * (d / 4), at = (int)blockIdx.x * 8 + c;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (at < n4)
-#pragma unroll 4
-        for (int s = g; s < slices; s += 8) v += reinterpret_cast<const f32x4*>(slab)[(int64_t)s * n4 + at];
+#pragma unroll 8
+        for (int s = g; s < slices; s += 32) v += reinterpret_cast<const f32x4*>(slab)[(int64_t)s * n4 + at];
     sm[g][c] = v;
     __syncthreads();
     if (g || at >= n4) return;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) v += sm[i][c];
+    for (int i = 1; i < 32; ++i) v += sm[i][c];
     const float os = *outscale;
     const int r = at / (d / 4), f = (at - r * (d / 4)) * 4;
     *reinterpret_cast<uint2*>(out + r * ld + f) = uint2{lpack2<DT>(v[0] * os, v[1] * os), lpack2<DT>(v[2] * os, v[3] * os)};
 }
 
 // ---- distillation: the teacher's slots ---------------------------------------------------------------------------------------------------------------
-// A workgroup a row, 16 lanes a slot: the student's logits at the teacher's classes (dot products in fp32), the teacher's softmax over its filled slots, the
-// loss. Rows of w are fetched from all over the list: 64 of them in flight a workgroup (1021 x 50 x 512: 16 us, with one wave a row 22).
+// A workgroup a row, LS lanes a slot (16; 64 for up to 16 slots, whose features would be read one after the other): the student's logits at the teacher's
+// classes (dot products in fp32), the teacher's softmax over its filled slots, the loss. Rows of w are fetched from all over the list: 64 (16) of them in
+// flight a workgroup, before anything that waits for the row's statistics (1021 x 50 x 512: 13.3 us, behind them 16; 449 x 3 x 920: 7.2, with 16 lanes 9.4).
 // saved: [N][1 + 2k] = lse of the row (+inf where the teacher says nothing), logits (log2 units), q -- the first slot that names a class holds the sum over
 // all of its slots, the others -1.
-template <int DT>
+__device__ __forceinline__ float row16_sum(float v) {
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xf, 0xf, true));   // quad_perm [1,0,3,2]
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xf, 0xf, true));   // quad_perm [2,3,0,1]
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xf, 0xf, true));  // row_half_mirror
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xf, 0xf, true));  // row_mirror
+}
+template <int DT, int LS>
 __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, int64_t x_ld, const uint16_t* w, int64_t w_ld, const float* off, float c, float coff,
                                                             const int32_t* idx, const void* val, int val_dtype, int k, float itau, float tau2, int N, int V, int d,
                                                             const float* lse, const float* part, int nvb, float* loss, float* saved) {
-    __shared__ int s_idx[512];
-    __shared__ float s_t[512], s_q[512], s_sum[4];
+    __shared__ __attribute__((aligned(16))) int s_idx[512];
+    __shared__ __attribute__((aligned(16))) float s_t[512], s_q[512];
+    __shared__ float s_z[512], s_sum[4];
     const int t = (int)threadIdx.x, lane = t & 63, wv = t >> 6, r = (int)blockIdx.x;
-    const int sub = t >> 4, l = t & 15;
+    const int sub = t / LS, l = t & (LS - 1);
     float* sv = saved + (int64_t)r * (1 + 2 * k);
     const int32_t* ir = idx + (int64_t)r * k;
-    // the slots in LDS: class (-1: empty) and the teacher's logit
-    for (int j = t; j < k; j += 256) {
-        const int v = ir[j];
+    // the slots in LDS: class (-1: empty) and the teacher's logit; up to the next four: empty ones
+    for (int j = t; j < ((k + 3) & ~3); j += 256) {
+        const int v = j < k ? ir[j] : -1;
         s_idx[j] = (unsigned)v < (unsigned)V ? v : -1;
-        s_t[j] = load_elem(val, (int64_t)r * k + j, val_dtype) * itau;
+        s_t[j] = j < k ? load_elem(val, (int64_t)r * k + j, val_dtype) * itau : 0.f;
+        s_q[j] = 0.f;
     }
-    float lse_r;
-    if (part) {  // few pairs a row: joined here instead of in a launch of their own
-        float pm = 0.f, ps = 0.f;
+    float pm = 0.f, ps = 0.f;
+    if (part) {
         if (lane < nvb) {
             pm = part[(int64_t)lane * N + r];
             ps = part[((int64_t)nvb + lane) * N + r];
         }
-        for (int o = 1; o < 64; o *= 2) {
-            const float m2 = __shfl_xor(pm, o), s2 = __shfl_xor(ps, o);
-            const bool up = lane & o;  // (the same order in every lane: the lower lane's pair first)
-            float a0 = up ? m2 : pm, b0 = up ? s2 : ps;
-            lse_join(a0, b0, up ? pm : m2, up ? ps : s2);
-            pm = a0;
-            ps = b0;
-        }
-        lse_r = ps == 0.f ? -INFINITY : (pm + __builtin_amdgcn_logf(ps)) * kLn2;
-    } else lse_r = lse[r];
-    const float l2 = lse_r * kLog2e;
+    } else pm = lse[r];
     __syncthreads();
-    // the teacher's maximum and sum, by every wave for itself
-    float m = -INFINITY, s = 0.f;
-    for (int j = lane; j < k; j += 64)
-        if (s_idx[j] >= 0) m = m != m || s_t[j] != s_t[j] ? NAN : fmaxf(m, s_t[j]);
-    for (int o = 32; o; o >>= 1) {
-        const float m2 = __shfl_xor(m, o);
-        m = m != m || m2 != m2 ? NAN : fmaxf(m, m2);
-    }
-    const bool some = m != -INFINITY && l2 != -INFINITY;  // (no filled slot, or nothing but -inf in them, or no class left)
-    for (int j = lane; j < k; j += 64)
-        if (s_idx[j] >= 0) s += expf(s_t[j] - m);
-    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-    const float ls = logf(s);
-    float sum = 0.f;
-    constexpr int U = 4;  // slots of 16 lanes in flight
+    constexpr int U = 4;  // slots of LS lanes in flight
     const uint16_t* xr = x + r * x_ld;
-    for (int j0 = 0; j0 < k; j0 += 16 * U) {
+    for (int j0 = 0; j0 < k; j0 += 256 / LS * U) {
         float z[U];
         int v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * 16 + sub;
-            v[u] = some && j < k ? s_idx[j] : -1;
+            const int j = j0 + u * (256 / LS) + sub;
+            v[u] = j < k ? s_idx[j] : -1;
             z[u] = 0.f;
         }
-        for (int f = l * 8; f < d; f += 128) {
+        for (int f = l * 8; f < d; f += LS * 8) {
             const u32x4 xv = *reinterpret_cast<const u32x4*>(xr + f);
             u32x4 wr[U];
 #pragma unroll
@@ -1433,24 +1417,56 @@ __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, i
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * 16 + sub;
-            for (int o = 8; o; o >>= 1) z[u] += __shfl_xor(z[u], o);
-            if (j < k && l == 0) {
-                float z2 = -INFINITY, q = 0.f;
-                if (v[u] >= 0) {
-                    const float ov = off ? off[v[u]] : 0.f;
-                    z2 = ov == -INFINITY ? -INFINITY : fmaf(z[u], c, ov * coff);
-                    const float lq = s_t[j] - m - ls;
-                    q = expf(lq);
-                    if (q != 0.f) sum += q * (lq - (z2 - l2) * kLn2);
-                }
-                sv[1 + j] = z2;
-                s_q[j] = q;
+            const int j = j0 + u * (256 / LS) + sub;
+            z[u] = row16_sum(z[u]);
+            if (LS == 64) {
+                z[u] += __shfl_xor(z[u], 16);
+                z[u] += __shfl_xor(z[u], 32);
             }
+            if (j < k && l == 0) s_z[j] = z[u];
         }
     }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
+    float lse_r = pm;
+    if (part) {  // few pairs a row: joined here instead of in a launch of their own
+        for (int o = 1; o < 64; o *= 2) {
+            const float m2 = __shfl_xor(pm, o), s2 = __shfl_xor(ps, o);
+            const bool up = lane & o;  // (the same order in every lane: the lower lane's pair first)
+            float a0 = up ? m2 : pm, b0 = up ? s2 : ps;
+            lse_join(a0, b0, up ? pm : m2, up ? ps : s2);
+            pm = a0;
+            ps = b0;
+        }
+        lse_r = ps == 0.f ? -INFINITY : (pm + __builtin_amdgcn_logf(ps)) * kLn2;
+    }
+    const float l2 = lse_r * kLog2e;
+    // the teacher's maximum and sum, by every wave for itself
+    float m = -INFINITY, s = 0.f;
+    for (int j = lane; j < k; j += 64)
+        if (s_idx[j] >= 0) m = m != m || s_t[j] != s_t[j] ? NAN : fmaxf(m, s_t[j]);
+    for (int o = 32; o; o >>= 1) {
+        const float m2 = __shfl_xor(m, o);
+        m = m != m || m2 != m2 ? NAN : fmaxf(m, m2);
+    }
+    const bool some = m != -INFINITY && l2 != -INFINITY;  // (no filled slot, or nothing but -inf in them, or no class left)
+    for (int j = lane; j < k; j += 64)
+        if (s_idx[j] >= 0) s += expf(s_t[j] - m);
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+    const float ls = logf(s);
+    __syncthreads();
+    float sum = 0.f;
+    for (int j = t; j < k; j += 256) {
+        const int v = some ? s_idx[j] : -1;
+        float z2 = -INFINITY;
+        if (v >= 0) {
+            const float ov = off ? off[v] : 0.f;
+            z2 = ov == -INFINITY ? -INFINITY : fmaf(s_z[j], c, ov * coff);
+            const float lq = s_t[j] - m - ls, q = expf(lq);
+            if (q != 0.f) sum += q * (lq - (z2 - l2) * kLn2);
+            s_q[j] = q;
+        }
+        sv[1 + j] = z2;
+    }
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
     if (lane == 0) s_sum[wv] = sum;
     __syncthreads();
     if (t == 0) {
@@ -1461,10 +1477,15 @@ __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, i
         const int v = s_idx[j];
         float q = s_q[j];
         bool first = some && v >= 0;
-        for (int o = 0; o < k; ++o) {
-            const bool same = s_idx[o] == v;
-            first = first && !(same && o < j);
-            q += same && o > j ? s_q[o] : 0.f;
+        for (int o = 0; o < k; o += 4) {
+            const int4 vo = *reinterpret_cast<const int4*>(s_idx + o);
+            const f32x4 qo = *reinterpret_cast<const f32x4*>(s_q + o);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool same = (e == 0 ? vo.x : e == 1 ? vo.y : e == 2 ? vo.z : vo.w) == v;
+                first = first && !(same && o + e < j);
+                q += same && o + e > j ? qo[e] : 0.f;
+            }
         }
         sv[1 + k + j] = first ? q : -1.f;
     }
@@ -1606,7 +1627,8 @@ static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool backward) {
         if (rt * ft <= (rt == 2 ? 6 : rt == 1 ? 4 : 8) && few_lds(rt, (int)d) <= 160 * 1024) {
             p.few = rt;
             const double nch = (double)(up(V, 32) / 32);
-            p.few_wgs = (int)std::max(1., std::min(std::min(nch, 256.), std::sqrt(nch * 1.9e6 / (double)(N * d))));
+            const double most = rt * (ft == 3 ? 4 : ft) <= 2 && few_lds(rt, (int)d) <= 80 * 1024 ? 512. : 256.;  // two a CU where they fit
+            p.few_wgs = (int)std::max(1., std::min(std::min(nch, most), std::sqrt(nch * 1.9e6 / (double)(N * d))));  // (a slice of dx costs what its traffic does)
             p.bwd_bytes = std::max(p.bwd_bytes, 256 + (int64_t)p.few_wgs * N * d * 4);
         }
     }
@@ -1711,7 +1733,7 @@ static int launch_few(const FewArgs& a, int dtype, int rt, int wgs, uint16_t* dx
 #undef CDET_GO
     CDET_LAUNCH_CHECK();
     if (!dx) return 0;
-    const unsigned nb = (unsigned)div_up((int64_t)a.N * (a.d / 4), 32);
+    const unsigned nb = (unsigned)div_up((int64_t)a.N * (a.d / 4), 8);
     if (dtype == CDET_BF16) class_few_sum_kernel<CDET_BF16><<<dim3(nb), dim3(256), 0, s>>>(a.slab, wgs, a.N, a.d, dx, dx_ld, a.outscale);
     else class_few_sum_kernel<CDET_F16><<<dim3(nb), dim3(256), 0, s>>>(a.slab, wgs, a.N, a.d, dx, dx_ld, a.outscale);
     CDET_LAUNCH_CHECK();
@@ -1881,12 +1903,14 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         a.dz = (uint16_t*)(ws + p.o_dz);
         a.dz_ld = p.g.piece;
         a.dz_rows = p.rows32;
-        a.idx = p.big_f ? nullptr : idx;
+        // few slots are written by the tile's own workgroup (every tile reads its rows' slots: 1656 x 400 x 160 with k = 24 13.5 us against 7.4 and a launch of 3.1, with k = 128 36)
+        const bool apart = p.big_f || k > 8;
+        a.idx = apart ? nullptr : idx;
         a.saved = saved;
         a.k = k;
         int rc = launch_logits<true>(a, q->dtype, p.big_f, s);
         if (rc) return rc;
-        if (idx && p.big_f) {
+        if (idx && apart) {
             const unsigned nb = (unsigned)div_up((int64_t)N * k, 256);
             if (q->dtype == CDET_BF16) class_teacher_dz_kernel<CDET_BF16><<<dim3(nb), dim3(256), 0, s>>>(idx, saved, lse2, coef, k, N, v0, Vp, a.dz, a.dz_ld);
             else class_teacher_dz_kernel<CDET_F16><<<dim3(nb), dim3(256), 0, s>>>(idx, saved, lse2, coef, k, N, v0, Vp, a.dz, a.dz_ld);
@@ -1990,11 +2014,17 @@ extern "C" int cdet_linear_distill_fwd(const cdet_linear_loss_desc* d, const voi
     if (rc) return rc;
     const dim3 nb((unsigned)d->N), nt(256);
     const LogitArgs a = logit_args(d);
-#define CDET_GO(DT_)                                                                                                                                        \
-    class_teacher_kernel<DT_><<<nb, nt, 0, (hipStream_t)stream>>>((const uint16_t*)x, d->x_ld, (const uint16_t*)w, d->w_ld, d->offset, a.c, a.coff, idx, val, val_dtype, \
+#define CDET_GO(DT_, LS_)                                                                                                                                   \
+    class_teacher_kernel<DT_, LS_><<<nb, nt, 0, (hipStream_t)stream>>>((const uint16_t*)x, d->x_ld, (const uint16_t*)w, d->w_ld, d->offset, a.c, a.coff, idx, val, val_dtype, \
                                                                  k, 1.f / d->tau, d->tau * d->tau, d->N, d->V, d->d, lse, part, p.nvb, loss, saved)
-    if (d->dtype == CDET_BF16) CDET_GO(CDET_BF16);
-    else CDET_GO(CDET_F16);
+    const bool wide = k <= 16 && d->d > 128;
+    if (d->dtype == CDET_BF16) {
+        if (wide) CDET_GO(CDET_BF16, 64);
+        else CDET_GO(CDET_BF16, 16);
+    } else {
+        if (wide) CDET_GO(CDET_F16, 64);
+        else CDET_GO(CDET_F16, 16);
+    }
 #undef CDET_GO
     CDET_LAUNCH_CHECK();
     return 0;
