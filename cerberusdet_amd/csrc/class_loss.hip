@@ -59,8 +59,8 @@ __device__ __forceinline__ int xcd_order(int b, int n) {  // consecutive logical
 // The staged stream of a workgroup's tiles and the multiplications on it. acc[mt][nt] = A B^T over K (any K; K % 8 == 0 for K-contiguous operands); C row of
 // register i: grp * MT*32 + mt*32 + 8*(i>>2) + 4*(lane>>5) + (i&3), C column: wave * NT*32 + nt*32 + (lane&31). The stream runs three stages ahead of the
 // multiplications, across the end of a tile: what `next` opens is fetched while the last tile is finished and its results are stored.
-// WALK = false: one tile only, without the branches of the crossing.
-template <int DT, int MT, int NT, bool ATR, bool BTR, bool WALK>
+// WALK = false: one tile only, without the branches of the crossing. KM (ATR, no walk): open() takes a bit per k; what takes no part is not read from A.
+template <int DT, int MT, int NT, bool ATR, bool BTR, bool WALK, bool KM>
 struct Pipe {
     static constexpr int ABYTES = MT * 64 * 64, BBYTES = NT * 128 * 64, STAGE = ABYTES + BBYTES;
     static constexpr int NA = MT / 2, NB = NT, NPW = NA + NB;  // DMA instructions (1 KiB) of a wave per step
@@ -73,6 +73,8 @@ struct Pipe {
     int krem;            // K of the opened tile left to be fetched
     int fslot, rslot;    // stages to be written / read next (byte offsets)
     int sure;            // memory phases whose next stage is known to be there
+    mask_t km;           // KM: word of the fourth stage from now; w[]: of the next three
+    uint32_t w[3];
 
     __device__ __forceinline__ void init(unsigned char* s, int64_t a_ld, int64_t b_ld) {
         smem = s;
@@ -106,14 +108,28 @@ struct Pipe {
         return tr ? (id >> 2) * 64 + 8 * ((lane & 7) ^ (((lane >> 4) & 1) << 2)) : 16 * id + (lane >> 2);
     }
     // the tile that is fetched from now on (rows beyond a_rows / b_rows, and everything beyond K, read as zero; a_rows 0: nothing is read)
-    __device__ __forceinline__ void open(const uint16_t* a, int a_rows, const uint16_t* b, int b_rows, int K) {
+    __device__ __forceinline__ void open(const uint16_t* a, int a_rows, const uint16_t* b, int b_rows, int K, const uint32_t* k_mask = nullptr) {
 #pragma unroll
-        for (int i = 0; i < NA; ++i) ka[i] = row_of(ATR, i) < a_rows ? k_of(ATR, i) : 0x40000000;
+        for (int i = 0; i < NA; ++i) ka[i] = KM ? (row_of(ATR, i) < a_rows ? 1 << k_of(ATR, i) : 0) : row_of(ATR, i) < a_rows ? k_of(ATR, i) : 0x40000000;
 #pragma unroll
         for (int i = 0; i < NB; ++i) kb[i] = row_of(BTR, i) < b_rows ? k_of(BTR, i) : 0x40000000;
         ap = a;
         bp = b;
         krem = K;
+        if (KM) {
+            km = as_mask(k_mask);
+            w[0] = km[0];
+            w[1] = km[1];
+            w[2] = km[2];
+            km += 3;
+        }
+    }
+    __device__ __forceinline__ uint32_t read_word() { return KM ? *km++ : 0u; }  // (the masks are longer than their numbers by what is read ahead)
+    __device__ __forceinline__ void push_word(uint32_t word) {
+        if (!KM) return;
+        w[0] = w[1];
+        w[1] = w[2];
+        w[2] = word;
     }
     template <class Next>
     __device__ __forceinline__ void fetch(Next&& next) {
@@ -121,9 +137,11 @@ struct Pipe {
         const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)ap, 0, LCAP, 0x00020000);
         const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)bp, 0, LCAP, 0x00020000);
         unsigned char* dst = smem + fslot + wave8 * 1024;
+        const int word = KM ? (int)(krem >= LBK ? w[0] : krem > 0 ? w[0] & ((1u << krem) - 1) : 0u) : 0;
 #pragma unroll
         for (int i = 0; i < NA; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(dst + i * 8192), 16, (int)(ka[i] < krem ? va[i] : LSENT), 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(dst + i * 8192), 16,
+                                                     (int)((KM ? (ka[i] & word) != 0 : ka[i] < krem) ? va[i] : LSENT), 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < NB; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void*)(dst + ABYTES + i * 8192), 16, (int)(kb[i] < krem ? vb[i] : LSENT), 0, 0, 0);
@@ -134,9 +152,10 @@ struct Pipe {
     }
     template <class Next>
     __device__ __forceinline__ void prime(Next&& next) {
-        fetch(next);
-        fetch(next);
-        fetch(next);
+        for (int f = 0; f < 3; ++f) {
+            fetch(next);
+            push_word(read_word());
+        }
     }
     __device__ __forceinline__ void start() {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * NPW) : "memory");
@@ -168,6 +187,8 @@ struct Pipe {
         for (int st = 0; st < steps; ++st) {
             u32x4 a[2][MT], b[2][NT];
             u32x2 al[2][MT], ah[2][MT], bl[2][NT], bh[2][NT];
+            if (KM) asm volatile("" : "+s"(w[0]), "+s"(w[1]), "+s"(w[2]));
+            const uint32_t word = read_word();
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
@@ -192,6 +213,7 @@ struct Pipe {
                 --sure;
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             } else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * NPW) : "memory");
+            push_word(word);
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -252,7 +274,8 @@ struct Pipe {
 // tiles, no phases: a wave multiplies one half of a step while it reads the next half's fragments, one barrier a step, RING - 1 stages ahead. (As phases of
 // 8 waves, like the large tile, the two products of 997 x 1201 x 320's gradients took 16.1 us, so 13.7; a deeper ring does not help.) Same interface as Pipe; column = wave * NT*32 + nt*32 + (lane&31),
 // wave = 0, 1; run() leaves the LDS free. Rows and classes that take no part are not read: open() takes a bit per row of B, and (KM) per k of A -- a launch
-// less than copies without them, which the large tile is given instead: in its loop the test costs 3 % of the gradients' products.
+// less than a copy of x without them, which the large tile is given instead: in its loop the test costs 2 - 3 % of a product, more than the copy of x does;
+// for w (KEPT, below) it is the copy that costs more.
 template <int DT, int MT, int NT, bool ATR, bool BTR, int RING, bool KM>
 struct Quad {
     static constexpr int ABYTES = MT * 64 * 64, BBYTES = NT * 64 * 64, STAGE = ABYTES + BBYTES;
@@ -464,7 +487,7 @@ struct Quad {
 };
 constexpr int QRING = 4;
 template <int DT, int MT, int NT, bool ATR, bool BTR, bool WALK, bool KM>
-using Product = std::conditional_t<MT == 4, Pipe<DT, MT, NT, ATR, BTR, WALK>, Quad<DT, MT, NT, ATR, BTR, QRING, KM>>;
+using Product = std::conditional_t<MT == 4, Pipe<DT, MT, NT, ATR, BTR, WALK, KM>, Quad<DT, MT, NT, ATR, BTR, QRING, KM>>;
 template <int MT> constexpr int kLinThreads = MT == 4 ? 512 : 256;
 template <int MT, int NT> constexpr int kLinCols = MT == 4 ? NT * 128 : NT * 64;  // B rows of a tile (A rows: MT * 64)
 
@@ -793,9 +816,9 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_logits_kernel(const 
 // ---- second product of the backward: a piece's dw tiles and dx tiles in one launch -----------------------------------------------------------------
 struct GradArgs {
     const uint16_t* x;    // [N][x_ld]; large tile: with zeros in the rows that take no part
-    const uint16_t* w;    // [Vp][w_ld], first class of the piece; large tile: with zeros in left-out classes
+    const uint16_t* w;    // [Vp][w_ld], first class of the piece
     const uint16_t* dz;   // [rows32][dz_ld]
-    const uint32_t *live, *kept;  // small tile: bit per row, takes part; per class of the piece, not left out. The others are not read: 0 * inf and NaN stay out
+    const uint32_t *live, *kept;  // bit per row, takes part (small tile); per class of the piece, not left out. The others are not read: 0 * inf and NaN stay out
     int64_t x_ld, w_ld, dz_ld;
     int N, rows32, d, Vp; // Vp: classes of the piece
     int vk;               // columns of dz that hold numbers (Vp rounded up to the tile)
@@ -813,7 +836,8 @@ struct GradArgs {
     const float* outscale;
 };
 
-template <int DT, int MT, int NT>
+// KEPT: classes can be left out, whose weights are not read (1021 x 32003 x 512: 2 us in the loop, a copy of w with zeros there 10; 494 x 63581 x 984 50)
+template <int DT, int MT, int NT, bool KEPT>
 __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_grads_kernel(const GradArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr int BM = MT * 64, BN = kLinCols<MT, NT>;
@@ -883,11 +907,11 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_grads_kernel(const G
     const int f0 = (L % a.ntd) * BM, r0 = (L / a.ntd % a.ntr) * BN, s = L / a.ntd / a.ntr;
     const int k0 = min(s * a.kper, a.Vp), k = min(a.kper, a.Vp - k0);
     {
-        Product<DT, MT, NT, true, false, false, MT == 2> p;
+        Product<DT, MT, NT, true, false, false, KEPT> p;
         auto none = []() {};
         p.init(smem, a.w_ld, a.dz_ld);
         const uint16_t *w = a.w + (int64_t)k0 * a.w_ld + f0, *dz = a.dz + (int64_t)r0 * a.dz_ld + k0;
-        if constexpr (MT == 4) p.open(w, a.d - f0, dz, a.rows32 - r0, k);
+        if constexpr (!KEPT) p.open(w, a.d - f0, dz, a.rows32 - r0, k);
         else p.open(w, a.d - f0, dz, a.rows32 - r0, k, a.kept + (k0 >> 5));
         p.prime(none);
         p.start();
@@ -961,7 +985,7 @@ __global__ __launch_bounds__(1024) void class_lse_kernel(const float* part, int 
 }
 
 // What the backward needs of every row -- lse, coefficient, whether it takes part -- and which classes are not left out; and, for the large tile, x with
-// zeros in the rows that take no part and, where classes can be left out, w of the first piece with zeros in those (0 * inf and NaN stay out).
+// zeros in the rows that take no part (0 * inf and NaN stay out).
 // A row's coefficient is g_r times what brings the largest |g| of the rows that take part to 1.984375 (fp16: times 2^12): the entries of dz that matter
 // most, g (p - 1) at the labels of rows with the largest weight (of all rows, under a mean), then lie at the top of a binade, where rounding to 16 bits
 // costs half of what it does at its bottom; and dz stays inside fp16's range. Every workgroup finds the maximum for itself (N up to 32768: 16 bytes a row
@@ -979,10 +1003,10 @@ struct PrepArgs {
     const float* off;           // [V] or null
     float *lse2, *coef, *outscale;
     uint32_t *live, *kept;
-    const uint16_t *x, *w;      // null: no copy
-    int64_t x_ld, w_ld;
-    int d8, Vp;
-    u32x4 *xo, *wo;
+    const uint16_t* x;          // null: no copy
+    int64_t x_ld;
+    int d8;
+    u32x4* xo;
 };
 __device__ __forceinline__ bool prep_live(const PrepArgs& a, int64_t r) {
     const float l = a.lse[r * a.lse_stride];
@@ -1035,20 +1059,7 @@ __global__ __launch_bounds__(1024) void class_prep_kernel(const PrepArgs a) {
             const int64_t r = i / a.d8, c = i - r * a.d8;
             a.xo[i] = prep_live(a, r) ? *reinterpret_cast<const u32x4*>(a.x + r * a.x_ld + c * 8) : u32x4{0, 0, 0, 0};
         }
-    if (a.w)
-        for (int64_t i = t; i < (int64_t)a.Vp * a.d8; i += nt) {
-            const int64_t v = i / a.d8, c = i - v * a.d8;
-            a.wo[i] = a.off[v] != -INFINITY ? *reinterpret_cast<const u32x4*>(a.w + v * a.w_ld + c * 8) : u32x4{0, 0, 0, 0};
-        }
 }
-// a later piece's weights with zeros in the left-out classes
-__global__ __launch_bounds__(256) void class_weights_kernel(const uint16_t* w, int64_t ld, const float* off, int V, int d8, u32x4* out) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)V * d8; i += (int64_t)gridDim.x * 256) {
-        const int64_t v = i / d8, c = i - v * d8;
-        out[i] = off[v] != -INFINITY ? *reinterpret_cast<const u32x4*>(w + v * ld + c * 8) : u32x4{0, 0, 0, 0};
-    }
-}
-// slices' slabs -> 16-bit, in a fixed order; blockIdx.y: which of two
 struct SumArgs {
     const float* slab[2];
     uint16_t* out[2];
@@ -1578,7 +1589,7 @@ struct LinPlan {
     int nvb, rows32;
     GradShape g;
     int64_t o_part, o_zlab, o_lse, fwd_bytes;
-    int64_t o_lse2, o_coef, o_scale, o_live, o_kept, o_x, o_w, o_dz, o_slab, o_wslab, bwd_bytes;
+    int64_t o_lse2, o_coef, o_scale, o_live, o_kept, o_x, o_dz, o_slab, o_wslab, bwd_bytes;
     int few, few_wgs;  // backward of few rows: 0, or row tiles of class_few_kernel; its workgroups (workspace: the scale, 256 bytes, and their slices)
 };
 static const int kFewRows = 128;
@@ -1617,7 +1628,6 @@ static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool backward) {
     p.o_live = take(up(N, 256) / 8 + 64);  // (bits; 64 bytes more than they need are read)
     p.o_kept = take(up(V, 256) / 8 + 64);
     p.o_x = p.big_f || shape.big ? take(N * d * 2) : 0;
-    p.o_w = (p.big_f || shape.big) && q->offset ? take((int64_t)shape.piece * d * 2) : 0;
     p.o_dz = take((int64_t)p.rows32 * shape.piece * 2);
     p.o_slab = p.direct ? 0 : take((int64_t)shape.splits * N * d * 4);
     p.o_wslab = shape.wsplits > 1 ? take((int64_t)shape.wsplits * shape.piece * d * 4) : 0;
@@ -1684,21 +1694,24 @@ static int launch_logits(LogitArgs a, int dtype, bool big, hipStream_t s) {
     CDET_LAUNCH_CHECK();
     return 0;
 }
-static int launch_grads(const GradArgs& a, int dtype, bool big, hipStream_t s) {
+static int launch_grads(const GradArgs& a, int dtype, bool big, bool kept, hipStream_t s) {
     const unsigned n = (unsigned)(a.ndw + a.ndx);
-#define CDET_GO(DT_, MT_, NT_, LDS_)                                                          \
-    do {                                                                                      \
-        static std::atomic<uint64_t> seen{0};                                                 \
-        allow_lds(seen, class_grads_kernel<DT_, MT_, NT_>, LDS_);                             \
-        class_grads_kernel<DT_, MT_, NT_><<<dim3(n), dim3(kLinThreads<MT_>), LDS_, s>>>(a);   \
+#define CDET_GO(DT_, MT_, KEPT_, LDS_)                                                          \
+    do {                                                                                        \
+        static std::atomic<uint64_t> seen{0};                                                   \
+        allow_lds(seen, class_grads_kernel<DT_, MT_, 2, KEPT_>, LDS_);                          \
+        class_grads_kernel<DT_, MT_, 2, KEPT_><<<dim3(n), dim3(kLinThreads<MT_>), LDS_, s>>>(a); \
     } while (0)
-    if (dtype == CDET_BF16) {
-        if (big) CDET_GO(CDET_BF16, 4, 2, LDS_BIG);
-        else CDET_GO(CDET_BF16, 2, 2, LDS_SMALL);
-    } else {
-        if (big) CDET_GO(CDET_F16, 4, 2, LDS_BIG);
-        else CDET_GO(CDET_F16, 2, 2, LDS_SMALL);
-    }
+#define CDET_GRADS(DT_)                                                                         \
+    do {                                                                                        \
+        if (big && kept) CDET_GO(DT_, 4, true, LDS_BIG);                                        \
+        else if (big) CDET_GO(DT_, 4, false, LDS_BIG);                                          \
+        else if (kept) CDET_GO(DT_, 2, true, LDS_SMALL);                                        \
+        else CDET_GO(DT_, 2, false, LDS_SMALL);                                                 \
+    } while (0)
+    if (dtype == CDET_BF16) CDET_GRADS(CDET_BF16);
+    else CDET_GRADS(CDET_F16);
+#undef CDET_GRADS
 #undef CDET_GO
     CDET_LAUNCH_CHECK();
     return 0;
@@ -1832,24 +1845,18 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
     pa.live = (uint32_t*)(ws + p.o_live);
     pa.kept = (uint32_t*)(ws + p.o_kept);
     pa.x_ld = q->x_ld;
-    pa.w_ld = q->w_ld;
     pa.d8 = d / 8;
-    const bool copy_x = p.big_f || p.g.big, copy_w = copy_x && q->offset;
+    const bool copy_x = p.big_f || p.g.big;
     if (copy_x) {
         pa.x = (const uint16_t*)x;
         pa.xo = (u32x4*)(ws + p.o_x);
-    }
-    if (copy_w) {
-        pa.w = (const uint16_t*)w;
-        pa.Vp = std::min(V, p.g.piece);
-        pa.wo = (u32x4*)(ws + p.o_w);
     }
     if (N > 32768) {
         class_max_kernel<<<dim3(1), dim3(1024), 0, s>>>(pa, os + 1);
         CDET_LAUNCH_CHECK();
         pa.gmax = os + 1;
     }
-    const int64_t most = std::max<int64_t>(std::max(N, V), copy_x ? ((int64_t)N + pa.Vp) * (d / 8) : 0);
+    const int64_t most = std::max<int64_t>(std::max(N, V), copy_x ? (int64_t)N * (d / 8) : 0);
     class_prep_kernel<<<dim3((unsigned)std::min<int64_t>(N > 8192 ? 1024 : 256, div_up(most, 1024))), dim3(1024), 0, s>>>(pa);
     CDET_LAUNCH_CHECK();
     const int bt = p.g.big ? 256 : 128;
@@ -1886,15 +1893,6 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         a.w = (const uint16_t*)w + (int64_t)v0 * q->w_ld;
         a.off = q->offset ? q->offset + v0 : nullptr;
         a.live = pa.live;
-        if (copy_w) {
-            if (v0) {
-                class_weights_kernel<<<dim3((unsigned)std::min<int64_t>(2048, div_up((int64_t)Vp * (d / 8), 256))), dim3(256), 0, s>>>(a.w, q->w_ld, a.off, Vp, d / 8,
-                                                                                                                                  (u32x4*)(ws + p.o_w));
-                CDET_LAUNCH_CHECK();
-            }
-            a.w = (const uint16_t*)(ws + p.o_w);
-            a.w_ld = d;
-        }
         a.V = Vp;
         a.label = label;
         a.v_first = v0;
@@ -1946,7 +1944,7 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         g.slab = (float*)(ws + p.o_slab);
         g.add = v0 > 0;
         g.outscale = os;
-        rc = launch_grads(g, q->dtype, p.g.big != 0, s);
+        rc = launch_grads(g, q->dtype, p.g.big != 0, q->offset != nullptr, s);
         if (rc) return rc;
         const bool ends = v0 + Vp >= V;
         sum.slab[1] = g.wslab;

@@ -186,6 +186,39 @@ def test_linear_ce_bad_values_in_left_out_places(dtype):
     assert torch.all(bad[2][~live] == 0) and torch.all(bad[3][::5] == 0)
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("N,V,d", [(2600, 3900, 40), (1100, 30000, 72), (40000, 4500, 16), (140, 2000, 64)])
+def test_bad_values_in_left_out_places_of_every_tile(N, V, d, dtype):
+    """The same over the large tile, slices and pieces of the class list, and for the distillation: same bits as with clean numbers there."""
+    ops = _ops()
+    x, w, labels = ce_case(N, V, d, dtype, seed=70)
+    off = 0.1 * _rand(V, seed=71)
+    off[::50] = -math.inf
+    off[32:96] = -math.inf
+    off[-1] = -math.inf
+    out = off == -math.inf
+    labels[out[labels]] = -1
+    labels[::9] = -1
+    idx, val = teacher(N, V, 10, 72, empty=False)
+    idx[::9] = -1
+    idx = torch.where(out[idx.long().clamp(min=0)], -1, idx).int()
+    none = (idx < 0).all(1)
+    xb, wb = x.clone(), w.clone()
+    xb[(labels < 0) & none] = math.nan
+    wb[out] = math.inf
+    wb[out.nonzero()[::2, 0]] = math.nan
+    for a, b in zip(run_ce(x, w, labels, offset=off)[2:], run_ce(xb, wb, labels, offset=off)[2:]):
+        assert torch.equal(a, b)
+    got = []
+    for xs, ws in ((x, w), (xb, wb)):
+        loss, saved = ops.linear_distill_fwd(xs, ws, idx, val, offset=off)
+        got.append((loss, *ops.linear_distill_bwd(xs, ws, idx, saved, offset=off)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and torch.all(torch.isfinite(a))
+    ref = reference(x, w, labels, offset=off)
+    check_grads(*run_ce(xb, wb, labels, offset=off)[2:], ref, x)
+
+
 def test_linear_ce_nothing_left():
     """Every class left out, every row ignored, no rows at all: losses and gradients of 0."""
     x, w, labels = ce_case(9, 20, 16, BF)
