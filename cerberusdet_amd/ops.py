@@ -389,6 +389,9 @@ def det_loss(feats, gt, nc, gains, strides, grad_scale=1.0, grad_dtype=None, wan
 # ---------------------------------------------------------------------------------------------------------------
 # Losses over a long class list (csrc/class_loss.hip, csrc/topk_distill.hip). Bad arguments raise ValueError before anything is launched. The messages are
 # put together only when they are raised: for a single row these calls are as long as what the host does around the launch.
+_INF = float("inf")
+
+
 def _bad(msg):
     raise ValueError(msg)
 
@@ -445,7 +448,7 @@ def _linear_loss_desc(x, w, offset, scale, tau, label64=0):
     if not 1 <= V <= 1 << 24 or N > 1 << 24:
         _bad(f"1 .. 2^24 classes and at most 2^24 rows, got {V} and {N}")
     scale, tau = float(scale), float(tau)
-    if not 0.0 < tau < float("inf") or not abs(scale) < float("inf"):
+    if not 0.0 < tau < _INF or not abs(scale) < _INF:
         _bad(f"tau = {tau} must be positive, scale = {scale} finite")
     if offset is not None:
         _on(gpu, "offset", offset)
@@ -517,8 +520,8 @@ def linear_ce_bwd(x, w, labels, lse, drow=None, offset=None, scale=1.0, want_dx=
     ref = C.byref(d)
     dev = x.device
     with _Device(dev.index) as s:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
-        dw = torch.empty(w.shape, dtype=x.dtype, device=dev) if want_dw else None
+        dx = torch.empty(d.N, d.d, dtype=x.dtype, device=dev) if want_dx else None  # (sizes one by one: a torch.Size takes the call twice as long)
+        dw = torch.empty(d.V, d.d, dtype=x.dtype, device=dev) if want_dw else None
         ws = torch.empty(lib.cdet_linear_loss_ws_bytes(ref, 1), dtype=torch.uint8, device=dev)
         L.check(lib.cdet_linear_ce_bwd(ref, xs.data_ptr(), wsrc.data_ptr(), labels.data_ptr(), lse.data_ptr(), ptr(g), gs, ptr(dx), d.d, ptr(dw), d.d, ws.data_ptr(), s),
                 "cdet_linear_ce_bwd")
@@ -539,7 +542,7 @@ def linear_distill_fwd(x, w, idx, val, tau=1.0, offset=None, scale=1.0):
     dev = x.device
     with _Device(dev.index) as s:
         loss = torch.empty(d.N, dtype=torch.float32, device=dev)
-        saved = torch.empty((d.N, 1 + 2 * k), dtype=torch.float32, device=dev)
+        saved = torch.empty(d.N, 1 + 2 * k, dtype=torch.float32, device=dev)
         ws = torch.empty(lib.cdet_linear_loss_ws_bytes(ref, 0), dtype=torch.uint8, device=dev)
         L.check(lib.cdet_linear_distill_fwd(ref, xs.data_ptr(), wsrc.data_ptr(), k, idx.data_ptr(), val.data_ptr(), _DT[val.dtype], loss.data_ptr(), saved.data_ptr(),
                                             ws.data_ptr(), s), "cdet_linear_distill_fwd")
@@ -559,8 +562,8 @@ def linear_distill_bwd(x, w, idx, saved, drow=None, tau=1.0, offset=None, scale=
     ref = C.byref(d)
     dev = x.device
     with _Device(dev.index) as s:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
-        dw = torch.empty(w.shape, dtype=x.dtype, device=dev) if want_dw else None
+        dx = torch.empty(d.N, d.d, dtype=x.dtype, device=dev) if want_dx else None  # (sizes one by one: a torch.Size takes the call twice as long)
+        dw = torch.empty(d.V, d.d, dtype=x.dtype, device=dev) if want_dw else None
         ws = torch.empty(lib.cdet_linear_loss_ws_bytes(ref, 1), dtype=torch.uint8, device=dev)
         L.check(lib.cdet_linear_distill_bwd(ref, xs.data_ptr(), wsrc.data_ptr(), k, idx.data_ptr(), saved.data_ptr(), ptr(g), gs, ptr(dx), d.d, ptr(dw), d.d,
                                             ws.data_ptr(), s), "cdet_linear_distill_bwd")
@@ -594,7 +597,7 @@ def topk_distill(logits, idx, val, tau=1.0, drow=None, grad_scale=1.0, grad_dtyp
     rows = shape[:-1]
     idx, val = _teacher(idx, val, rows, gpu)
     tau = float(tau)
-    if not 0.0 < tau < float("inf"):
+    if not 0.0 < tau < _INF:
         _bad(f"tau = {tau} must be positive")
     grad_dtype = grad_dtype or (logits.dtype if out is None else out.dtype)
     if grad_dtype is not logits.dtype and grad_dtype is not torch.float32:
@@ -609,10 +612,10 @@ def topk_distill(logits, idx, val, tau=1.0, drow=None, grad_scale=1.0, grad_dtyp
             if out.shape != shape or out.dtype != grad_dtype or (P > 1 and out.stride(0) < G * V):
                 _bad(f"out must be {tuple(shape)} {grad_dtype} without overlapping pixels")
         elif want_grad:
-            out = torch.empty(shape, dtype=grad_dtype, device=dev)
+            out = torch.empty(*shape, dtype=grad_dtype, device=dev)
         gld = _pixel_pitch(out, "out", P, G, V) if out is not None else 0
         d = L.TopkDistillDesc(P, G, V, idx.shape[-1], _DT[logits.dtype], _DT[val.dtype], _DT[grad_dtype], ld, gld, tau, float(grad_scale))
-        loss = torch.empty(rows, dtype=torch.float32, device=dev)
+        loss = torch.empty(*rows, dtype=torch.float32, device=dev)
         L.check(lib.cdet_topk_distill(C.byref(d), logits.data_ptr(), idx.data_ptr(), val.data_ptr(), ptr(g), loss.data_ptr(), ptr(out), s), "cdet_topk_distill")
     return loss, out
 
