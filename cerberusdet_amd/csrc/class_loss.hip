@@ -1097,8 +1097,8 @@ __global__ __launch_bounds__(256) void class_zero_kernel(uint16_t* p, int64_t ro
 //   do not: 128 x 131072 x 320 87 us with one, 110 with two);
 //   dw block = dz x, written out;  dx += dz w, in registers until the end: one fp32 slice a workgroup (class_few_sum_kernel adds them in their order).
 // A wave owns FT tiles of 32 features in the last two; RT tiles of 32 rows. Bound by memory for long lists, w in and dw out: backward of 1 x 131072 x 960
-// 113 us = 4.5 TB/s (by tiles of 128 x 128: 183), 32 x 131072 x 512 72 us (98), 128 x 131072 x 320 87 us (100); of short ones by three waits for LDS and
-// one for memory: 96 x 365 x 320 15 + 4 us of kernels (21).
+// 109 us = 4.6 TB/s (by tiles of 128 x 128: 183), 32 x 131072 x 512 72 us (98), 128 x 131072 x 320 88 us (100); of short ones by a chain of waits: 96 x 365 x
+// 320 15 + 4 us of kernels (21). Two workgroups a CU where registers and LDS leave room: 10 x 57842 x 264 25 us, with one 32.
 struct FewArgs {
     const uint16_t *x, *w;
     int64_t x_ld, w_ld;
@@ -1165,6 +1165,21 @@ __global__ __launch_bounds__(512, RT * FT <= 2 ? 4 : 2) void class_few_kernel(co
     int sv[kFewSlots];
 #pragma unroll
     for (int u = 0; u < kFewSlots; ++u) sv[u] = a.idx && tid + 512 * u < a.N * a.k ? a.idx[tid + 512 * u] : -1;
+    // x, zeros in the rows that take no part (known later) and behind the last feature
+    u32x4 xv[RT * 4];
+    auto load_x = [&](int p) {
+#pragma unroll
+        for (int i = 0; i < RT * 4; ++i) {
+            const int r = wave + 8 * i;
+            xv[i] = p * 8 < a.d && r < a.N ? *reinterpret_cast<const u32x4*>(a.x + r * a.x_ld + p * 8) : u32x4{0, 0, 0, 0};
+        }
+    };
+    auto keep = [&](int p) {
+        if (p < nft * 4)
+#pragma unroll
+            for (int i = 0; i < RT * 4; ++i) *reinterpret_cast<u32x4*>(xs + (wave + 8 * i) * S + p * 16) = l2s[wave + 8 * i] != INFINITY ? xv[i] : u32x4{0, 0, 0, 0};
+    };
+    load_x(lane);
     if (tid < RT * 32) {  // the rows, as class_prep_kernel has them
         const int r = tid;
         float l = r < a.N ? a.lse[r * a.lse_stride] : 0.f, g = r < a.N ? (a.drow ? a.drow[(int64_t)r * a.drow_stride] : 1.f) : 0.f;
@@ -1185,16 +1200,10 @@ __global__ __launch_bounds__(512, RT * FT <= 2 ? 4 : 2) void class_few_kernel(co
     m = m > 0.f ? fminf(fmaxf(m, 1e-30f), 1e37f) : 1.f;
     const float down = 1.984375f * a.spread / m, os = a.gain * m / (1.984375f * a.spread);
     if (blockIdx.x == 0 && tid == 0) *a.outscale = os;
-#pragma unroll 1
-    for (int p = lane; p < nft * 4; p += 64) {  // x, zeros in the rows that take no part and behind the last feature
-        u32x4 xv[RT * 4];
-#pragma unroll
-        for (int i = 0; i < RT * 4; ++i) {
-            const int r = wave + 8 * i;
-            xv[i] = p * 8 < a.d && l2s[r] != INFINITY ? *reinterpret_cast<const u32x4*>(a.x + r * a.x_ld + p * 8) : u32x4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int i = 0; i < RT * 4; ++i) *reinterpret_cast<u32x4*>(xs + (wave + 8 * i) * S + p * 16) = xv[i];
+    keep(lane);
+    for (int p = lane + 64; p < nft * 4; p += 64) {
+        load_x(p);
+        keep(p);
     }
     __builtin_amdgcn_sched_barrier(0);
     f32x16 acc[RT][FT];
