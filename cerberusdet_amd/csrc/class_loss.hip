@@ -1097,8 +1097,8 @@ __global__ __launch_bounds__(256) void class_zero_kernel(uint16_t* p, int64_t ro
 //   do not: 128 x 131072 x 320 87 us with one, 110 with two);
 //   dw block = dz x, written out;  dx += dz w, in registers until the end: one fp32 slice a workgroup (class_few_sum_kernel adds them in their order).
 // A wave owns FT tiles of 32 features in the last two; RT tiles of 32 rows. Bound by memory for long lists, w in and dw out: backward of 1 x 131072 x 960
-// 109 us = 4.6 TB/s (by tiles of 128 x 128: 183), 32 x 131072 x 512 72 us (98), 128 x 131072 x 320 88 us (100); of short ones by a chain of waits: 96 x 365 x
-// 320 15 + 4 us of kernels (21). Two workgroups a CU where registers and LDS leave room: 10 x 57842 x 264 25 us, with one 32.
+// 109 us = 4.6 TB/s (by tiles of 128 x 128: 183), 32 x 131072 x 512 72 us (98), 128 x 131072 x 320 90 us (100); of short ones by a chain of waits: 96 x 365 x
+// 320 15 + 4 us of kernels (21). Two workgroups a CU where registers and LDS leave room: 16 x 131072 x 400 50 us, with one 59.
 struct FewArgs {
     const uint16_t *x, *w;
     int64_t x_ld, w_ld;
@@ -1121,9 +1121,9 @@ struct FewArgs {
     float* outscale;
 };
 constexpr int kFewSlots = 8;
-static inline int few_lds(int RT, int d) {
+static inline int few_lds(int RT, int N, int d) {  // (x: rows up to the next 16)
     const int S = (d + 31) / 32 * 64 + 16;
-    return (RT * 32 + 32) * S + 32768 + RT * 32 * 80 + 32 * (RT * 64 + 16) + (RT * 32 * 4 + 64) * 4;
+    return ((N + 15) / 16 * 16 + 32) * S + 32768 + RT * 32 * 80 + 32 * (RT * 64 + 16) + (RT * 32 * 4 + 64) * 4;
 }
 __device__ __forceinline__ u32x4 few_row(const unsigned char* p) { return *reinterpret_cast<const u32x4*>(p); }
 // features f0 .. +31 as fragment rows, K = lines k0 .. +15 of S bytes
@@ -1146,7 +1146,8 @@ __global__ __launch_bounds__(512, RT * FT <= 2 ? 4 : 2) void class_few_kernel(co
     constexpr bool TWO = RT <= 2;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, h = lane >> 5;
     const int nft = (a.d + 31) >> 5, S = nft * 64 + 16, nch = (a.V + 31) >> 5, step = (int)gridDim.x;
-    unsigned char *xs = smem, *ws = xs + RT * 32 * S, *red = ws + 32 * S, *dzr = red + 32768, *dzc = dzr + RT * 32 * 80, *lor = red, *loc = red + RT * 32 * 80;
+    const int lines = (a.N + 15) & ~15;
+    unsigned char *xs = smem, *ws = xs + lines * S, *red = ws + 32 * S, *dzr = red + 32768, *dzc = dzr + RT * 32 * 80, *lor = red, *loc = red + RT * 32 * 80;
     float *l2s = reinterpret_cast<float*>(dzc + 32 * CS), *gs = l2s + RT * 32, *gm = gs + RT * 32, *offs = gm + RT * 32;
     int* labs = reinterpret_cast<int*>(offs + 64);
     int ch = (int)blockIdx.x;
@@ -1177,7 +1178,8 @@ __global__ __launch_bounds__(512, RT * FT <= 2 ? 4 : 2) void class_few_kernel(co
     auto keep = [&](int p) {
         if (p < nft * 4)
 #pragma unroll
-            for (int i = 0; i < RT * 4; ++i) *reinterpret_cast<u32x4*>(xs + (wave + 8 * i) * S + p * 16) = l2s[wave + 8 * i] != INFINITY ? xv[i] : u32x4{0, 0, 0, 0};
+            for (int i = 0; i < RT * 4; ++i)
+                if (wave + 8 * i < lines) *reinterpret_cast<u32x4*>(xs + (wave + 8 * i) * S + p * 16) = l2s[wave + 8 * i] != INFINITY ? xv[i] : u32x4{0, 0, 0, 0};
     };
     load_x(lane);
     if (tid < RT * 32) {  // the rows, as class_prep_kernel has them
@@ -1228,7 +1230,7 @@ __global__ __launch_bounds__(512, RT * FT <= 2 ? 4 : 2) void class_few_kernel(co
         f32x16 z;
 #pragma unroll
         for (int e = 0; e < 16; ++e) z[e] = 0.f;
-        const unsigned char *wz = ws + l31 * S + h * 16, *xz = xs + (t0 * 32 + l31) * S + h * 16;
+        const unsigned char *wz = ws + l31 * S + h * 16, *xz = xs + min(t0 * 32 + l31, lines - 1) * S + h * 16;  // (rows behind the last: any, their dz is 0)
 #pragma unroll 4
         for (int s = kp; s < 2 * nft; s += KP) z = lmfma<DT>(few_row(wz + s * 32), few_row(xz + s * 32), z);
 #pragma unroll
@@ -1317,6 +1319,7 @@ __global__ __launch_bounds__(512, RT * FT <= 2 ? 4 : 2) void class_few_kernel(co
                 for (int e = 0; e < 16; ++e) o16[e] = 0.f;
 #pragma unroll
                 for (int t = 0; t < 2 * RT; ++t) {
+                    if (t * 16 >= lines) break;
                     const u32x4 xt = few_tr(xs, S, t * 16, f0, lane);
                     o16 = lmfma<DT>(xt, few_row(dzc + l31 * CS + t * 32 + h * 16), o16);
                     if (TWO) o16 = lmfma<DT>(xt, few_row(loc + l31 * CS + t * 32 + h * 16), o16);
@@ -1643,10 +1646,10 @@ static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool backward) {
     p.bwd_bytes = o;
     if (N <= kFewRows) {
         const int rt = N <= 32 ? 1 : N <= 64 ? 2 : 4, ft = (int)up(up(d, 32) / 32, 8) / 8;
-        if (rt * ft <= (rt == 2 ? 6 : rt == 1 ? 4 : 8) && few_lds(rt, (int)d) <= 160 * 1024) {
+        if (rt * ft <= (rt == 2 ? 6 : rt == 1 ? 4 : 8) && few_lds(rt, (int)N, (int)d) <= 160 * 1024) {
             p.few = rt;
             const double nch = (double)(up(V, 32) / 32);
-            const double most = rt * (ft == 3 ? 4 : ft) <= 2 && few_lds(rt, (int)d) <= 80 * 1024 ? 512. : 256.;  // two a CU where they fit
+            const double most = rt * (ft == 3 ? 4 : ft) <= 2 && few_lds(rt, (int)N, (int)d) <= 80 * 1024 ? 512. : 256.;  // two a CU where they fit
             p.few_wgs = (int)std::max(1., std::min(std::min(nch, most), std::sqrt(nch * 1.9e6 / (double)(N * d))));  // (a slice of dx costs what its traffic does)
             p.bwd_bytes = std::max(p.bwd_bytes, 256 + (int64_t)p.few_wgs * N * d * 4);
         }
@@ -1727,7 +1730,7 @@ static int launch_grads(const GradArgs& a, int dtype, bool big, bool kept, hipSt
 }
 
 static int launch_few(const FewArgs& a, int dtype, int rt, int wgs, uint16_t* dx, int64_t dx_ld, hipStream_t s) {
-    const size_t lds = (size_t)few_lds(rt, a.d);
+    const size_t lds = (size_t)few_lds(rt, a.N, a.d);
     const int nft = (a.d + 31) / 32;
 #define CDET_GO(DT_, RT_, FT_)                                                                        \
     do {                                                                                              \

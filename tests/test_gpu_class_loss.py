@@ -290,7 +290,8 @@ def test_linear_distill(N, V, d, k, dtype):
 
 
 FEW = [(1, 33, 8), (2, 32, 256), (31, 31, 264), (32, 97, 960), (32, 9001, 512), (33, 64, 608), (64, 700, 40), (60, 20000, 264), (65, 65, 320), (128, 1000, 256), (97, 12000, 304), (1, 40000, 520),
-       (33, 70, 616), (70, 70, 328), (32, 70, 968)]  # (the last three: a row of features more than the few rows' kernel holds)
+       (33, 70, 616), (70, 70, 328), (32, 70, 968),
+       (16, 70, 1024), (16, 40, 1032), (17, 40, 960), (48, 70, 736), (48, 70, 744), (64, 70, 608), (64, 70, 616), (80, 70, 480), (80, 70, 488), (128, 70, 320)]  # as much as its LDS holds, and more
 
 
 @pytest.mark.parametrize("dtype", [BF, F16])
