@@ -1,7 +1,7 @@
 // Distillation from a teacher's top k logits on logits that are in memory: loss and gradient of every row in one launch.
 //   p = softmax(z / tau) over the row's V logits, q = softmax of the teacher's filled slots / tau
 //   loss = tau^2 sum_j q_j (log q_j - log p[idx_j]),   dz_v = drow * grad_scale * tau * (p_v - sum_{j: idx_j == v} q_j)
-// Bound by memory: logits once in, gradient once out. A row of up to 32768 logits stays in the registers of its 1, 4, 8 or 16 waves (td_wide_kernel), so the
+// Bound by memory: logits once in, gradient once out. A row of up to 32768 logits stays in the registers of its 1, 2, 4, 8 or 16 waves, so the
 // maximum, the sum and the gradient are taken from one read (td_wave_kernel, td_wide_kernel); one of up to 256 KiB is held as it is stored
 // (td_held_kernel); a longer one is read again for its gradient (td_long_kernel). Above 2048 logits the gradient is written dense and then, behind a
 // barrier, the k named entries are written again with their q; shorter rows put q together in LDS first. Rows of at most 128 logits (box distributions,
@@ -122,13 +122,15 @@ __device__ __forceinline__ void td_sync() {
 struct TdSlots {
     float *q, *lq, *z;
     int* v;
-    __device__ TdSlots(float* lds, int k) : q(lds), lq(lds + k), z(lds + 2 * k), v(reinterpret_cast<int*>(lds + 3 * k)) {}
+    static __host__ __device__ constexpr int up(int k) { return (k + 3) & ~3; }  // (empty ones up to the next four)
+    __device__ TdSlots(float* lds, int k) : q(lds), lq(lds + up(k)), z(lds + 2 * up(k)), v(reinterpret_cast<int*>(lds + 3 * up(k))) {}
 };
 // fills it; t = thread of the row. False: no filled slot, or nothing but -inf in them
 template <int DT, int NW>
 __device__ __forceinline__ bool td_teacher(const TdArgs& a, int64_t row, int t, const typename TdElem<DT>::T* z, TdSlots s, float* scratch) {
     constexpr int NT = NW * 64;
     float m = -INFINITY;
+    if (t < TdSlots::up(a.k) - a.k) s.v[a.k + t] = -1;
     for (int j = t; j < a.k; j += NT) {
         int v = a.idx[row * a.k + j];
         const float x = load_elem(a.val, row * a.k + j, a.vdt) * a.itau;
@@ -168,10 +170,19 @@ __device__ __forceinline__ void td_finish(const TdArgs& a, int64_t row, int t, b
         if (q != 0.f) sum += q * (s.lq[j] - (e2 - l2s) * kTdLn2);
         if (!dz) continue;
         bool first = true;
-        for (int o = 0; o < a.k; ++o) {
-            const bool same = s.v[o] == v;
-            first = first && !(same && o < j);
-            q += same && o > j ? s.q[o] : 0.f;
+        for (int o = 0; o < a.k; o += 4) {
+            const int4 c = *reinterpret_cast<const int4*>(s.v + o);
+            const int named[4] = {c.x, c.y, c.z, c.w};
+            bool hit = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hit = hit || (named[e] == v && o + e != j);
+            if (hit)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool same = named[e] == v;
+                    first = first && !(same && o + e < j);
+                    q += same && o + e > j ? s.q[o + e] : 0.f;
+                }
         }
         if (first) dz[v] = TdElem<GDT>::put((__builtin_amdgcn_exp2f(e2) * inv - q) * g);
     }
@@ -350,13 +361,14 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
 }
 
 // V <= 32768: a row's logits in registers, up to NCH chunks of CH per thread, NW waves a row; loss, maximum and sum from one read. Bound by memory:
-// 16800 x 8192 fp32 212 us = 5.2 TB/s, 4200 x 32768 210 us.
+// 16800 x 8192 fp32 210 us = 5.2 TB/s, 4200 x 32768 210 us; shorter 16-bit rows by what a row waits for, so as few waves as hold one: 20000 x 3001 bf16
+// 49 us with 2, 75 with 4.
 template <int DT, int GDT, int NW>
 __global__ __launch_bounds__(NW * 64, NW == 16 ? 8 : 1) void td_wide_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
     typedef typename TdElem<GDT>::T TG;
     constexpr int NT = NW * 64, CH = 16 / sizeof(T), NCH = 32 / CH;
-    extern __shared__ float lds[];
+    extern __shared__ __attribute__((aligned(16))) float lds[];
     __shared__ float scratch[16];
     const int t = (int)threadIdx.x, V = a.V;
     const int64_t row = blockIdx.x;
@@ -424,13 +436,15 @@ __global__ __launch_bounds__(NW * 64, NW == 16 ? 8 : 1) void td_wide_kernel(cons
 }
 
 // longer rows, as they are stored (16 waves a row, NCH chunks of 16 bytes a thread): two exponentials a logit instead of a second read.
-// 8192 x 65536 bf16 396 us = 5.4 TB/s; NCH = 16 leaves one row a CU, whose loads and stores take turns: 4096 x 131072 bf16 475 us = 4.5 TB/s.
+// 8192 x 65536 bf16 388 us = 5.5 TB/s; NCH = 16 leaves one row a CU, whose loads and stores take turns: 4096 x 131072 bf16 479 us = 4.5 TB/s (walking over
+// its rows, the next one's loads under this one's stores: 535).
 template <int DT, int GDT, int NCH>
 __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
     typedef typename TdElem<GDT>::T TG;
     constexpr int NW = 16, NT = 1024, CH = 16 / sizeof(T);
-    extern __shared__ float lds[];
+    constexpr uint32_t NINF = DT == CDET_F32 ? 0xff800000u : DT == CDET_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
     __shared__ float scratch[16];
     const int t = (int)threadIdx.x, V = a.V;
     const int64_t row = blockIdx.x;
@@ -438,31 +452,25 @@ __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const T
     const T* z;
     TG* dz;
     td_row(a, row, z, dz);
-    const T ninf = TdElem<DT>::put(-INFINITY);
     u32x4 v[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int e0 = (i * NT + t) * CH;
-        TdVec<T, CH> x;
-        if (e0 + CH <= V) x = *reinterpret_cast<const TdVec<T, CH>*>(z + e0);
-        else {
-#pragma unroll
-            for (int e = 0; e < CH; ++e) x.v[e] = ninf;
-            if (e0 < V)
-#pragma unroll
-                for (int e = 0; e < CH; ++e)
-                    if (e0 + e < V) x.v[e] = z[e0 + e];
+        v[i] = u32x4{NINF, NINF, NINF, NINF};
+        if (e0 + CH <= V) {
+            const TdVec<T, CH> x = *reinterpret_cast<const TdVec<T, CH>*>(z + e0);
+            __builtin_memcpy(&v[i], &x, 16);
         }
-        __builtin_memcpy(&v[i], &x, 16);
     }
+    const float vt = t < V % CH ? TdElem<DT>::get(z[V - V % CH + t]) : -INFINITY;  // what is left behind the last whole chunk: a logit a thread
     auto logit = [&](int i, int e) {
         if (DT == CDET_F32) return __uint_as_float(v[i][e]);
         return TdElem<DT>::get((T)(v[i][(e >> 1) & 3] >> (16 * (e & 1))));
     };
     // each pass unpacks the chunks anew: without this the compiler keeps 128 fp32 values a thread from the first pass on
     auto anew = [&](int i) { asm volatile("" : "+v"(v[i])); };
-    bool on = td_teacher<DT, NW>(a, row, t, z, slots, scratch);
-    float m = -INFINITY;
+    const bool some = td_teacher<DT, NW>(a, row, t, z, slots, scratch);
+    float m = vt;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
         if (i * NT * CH < V) {
@@ -471,9 +479,9 @@ __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const T
             for (int e = 0; e < CH; ++e) m = fmaxf(m, logit(i, e));
         }
     m = td_reduce<NW, true>(m, scratch);
-    on = on && m != -INFINITY;
+    const bool on = some && m != -INFINITY;
     const float mu = __builtin_isinf(m) ? 0.f : m, muc = mu * a.c;
-    float s = 0.f;
+    float s = td_exp2<DT>(vt, mu, a.c, muc);
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
         if (i * NT * CH < V) {
@@ -483,27 +491,28 @@ __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const T
         }
     s = td_reduce<NW, false>(s, scratch);
     const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s);
-    const float g = a.gs * (a.drow ? a.drow[row] : 1.f), f = inv * g;
+    const float g = a.gs * (a.drow ? a.drow[row] : 1.f);
     if (dz) {
+        float f = inv * g, mg = mu, mgc = muc;
+        int u = t;
+        asm volatile("" : "+v"(u));  // (addresses are computed anew: no register is kept for them)
+        if (!on) {  // zeros, whatever the logits are
+            f = mg = mgc = 0.f;
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) v[i] = u32x4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int e0 = (i * NT + t) * CH;
-            if (e0 >= V) continue;
-            anew(i);
-            float o[CH];
-            if (on) {  // (uniform)
+            const int e0 = (i * NT + u) * CH;
+            if (i * NT * CH < V) {
+                anew(i);
+                float o[CH];
 #pragma unroll
-                for (int e = 0; e < CH; ++e) o[e] = td_exp2<DT>(logit(i, e), mu, a.c, muc) * f;
-            } else {
-#pragma unroll
-                for (int e = 0; e < CH; ++e) o[e] = 0.f;
+                for (int e = 0; e < CH; ++e) o[e] = td_exp2<DT>(logit(i, e), mg, a.c, mgc) * f;
+                if (e0 + CH <= V) td_put<GDT, CH>(dz + e0, o);
             }
-            if (e0 + CH <= V) td_put<GDT, CH>(dz + e0, o);
-            else
-#pragma unroll
-                for (int e = 0; e < CH; ++e)
-                    if (e0 + e < V) dz[e0 + e] = TdElem<GDT>::put(o[e]);
         }
+        if (u < V % CH) dz[V - V % CH + u] = TdElem<GDT>::put(td_exp2<DT>(on ? vt : 0.f, mg, a.c, mgc) * f);
     }
     td_sync<NW>();
     td_finish<GDT, NW>(a, row, t, on, dz, mu, inv, l2s, g, slots, scratch);
@@ -516,7 +525,7 @@ __global__ __launch_bounds__(1024) void td_long_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
     typedef typename TdElem<GDT>::T TG;
     constexpr int NW = 16, NT = 1024, CH = 16 / sizeof(T), U = 16 / CH;  // U chunks (16 logits) at a time
-    extern __shared__ float lds[];
+    extern __shared__ __attribute__((aligned(16))) float lds[];
     __shared__ float scratch[16];
     const int t = (int)threadIdx.x, V = a.V;
     const int64_t row = blockIdx.x;
@@ -714,7 +723,7 @@ __global__ __launch_bounds__(256) void td_narrow_kernel(const TdArgs a) {
 
 template <int DT, int GDT>
 static int td_launch(const TdArgs& a, hipStream_t s) {
-    const size_t lds = (size_t)a.k * 16;
+    const size_t lds = (size_t)TdSlots::up(a.k) * 16;
 #define CDET_NARROW(L, E)                                                                                          \
     do {                                                                                                           \
         const dim3 grid((unsigned)((a.rows + 256 / L - 1) / (256 / L)));                                           \
@@ -735,6 +744,7 @@ static int td_launch(const TdArgs& a, hipStream_t s) {
         else if (a.V <= 1024) td_wave_kernel<DT, GDT, 16><<<grid, dim3(256), 4 * row, s>>>(a);
         else td_wave_kernel<DT, GDT, 32><<<grid, dim3(256), 4 * row, s>>>(a);
     }
+    else if (a.V <= 4096) td_wide_kernel<DT, GDT, 2><<<dim3((unsigned)a.rows), dim3(128), lds, s>>>(a);
     else if (a.V <= 8192) td_wide_kernel<DT, GDT, 4><<<dim3((unsigned)a.rows), dim3(256), lds, s>>>(a);
     else if (a.V <= 16384) td_wide_kernel<DT, GDT, 8><<<dim3((unsigned)a.rows), dim3(512), lds, s>>>(a);
     else if (a.V <= 32768) td_wide_kernel<DT, GDT, 16><<<dim3((unsigned)a.rows), dim3(1024), lds, s>>>(a);
