@@ -458,6 +458,32 @@ def test_topk_distill_row_tails(V, dtype):
     assert torch.equal(loss, got[0]) and torch.equal(part, got[1]) and torch.equal(same[:, :V], z)
 
 
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("V,k", [(700, 9), (2051, 9), (3001, 33), (4097, 30), (9001, 30), (20003, 7), (33001, 9), (65535, 30), (65541, 31), (100001, 6), (131079, 5)])
+def test_topk_distill_odd_values_of_every_type(V, k, dtype):
+    """Rows that hold NaN and have no teacher, rows of nothing but -inf, -inf in the tail, one class in every slot, over all forms by length."""
+    z = (2 * _rand(7, V, seed=54)).to(dtype)
+    idx, val = teacher(7, V, k, 55, empty=False)
+    idx[0] = V - 1
+    idx[1, 1:4] = V - 2
+    z[2, -5:] = -math.inf
+    idx[2] = torch.where(idx[2] >= V - 5, 0, idx[2])
+    z[3] = -math.inf
+    idx[4] = -1
+    z[4] = math.nan
+    idx[5, 1:] = -1
+    got = _ops().topk_distill(z, idx, val, tau=1.0)
+    assert torch.all(got[0][3:5] == 0) and torch.all(got[1][3:5] == 0)
+    zr = z.clone()
+    zr[4] = 0
+    check_map(got, zr, idx, val, 1.0, None)
+    same = z.clone()
+    loss, _ = _ops().topk_distill(same, idx, val, tau=1.0, out=same)
+    assert torch.equal(loss, got[0]) and torch.equal(same, got[1])
+    only, none = _ops().topk_distill(z, idx, val, tau=1.0, want_grad=False)
+    assert none is None and torch.equal(only, got[0])
+
+
 @pytest.mark.parametrize("P,V,k", [(9, 100, 300), (5, 1, 200), (6, 2048, 512), (3, 2040, 511)])
 def test_topk_distill_more_slots_than_classes_and_the_most(P, V, k):
     z = 2.5 * _rand(P, V, seed=47)
