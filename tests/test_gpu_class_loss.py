@@ -739,6 +739,72 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(loss[P - 3:], few[0]) and torch.equal(dz[P - 3:], few[1])
 
 
+def test_few_rows_far_and_pitched():
+    """Rows of x and w more than 2^31 elements from the first; dx and dw with pitches above d and a workspace full of ones: what lies behind a row stays."""
+    import ctypes as C
+
+    from cerberusdet_amd import _lib as L
+
+    ops, ld, N, V, d = _ops(), (1 << 22) - 8, 100, 600, 64
+    x, w, labels = ce_case(N, V, d, BF, seed=190)
+    loss, lse, dx, dw = run_ce(x, w, labels)
+    big = torch.empty(V, ld, dtype=BF, device=DEV)
+    big[:N, :d], big[:, 128:128 + d] = x, w
+    for a, b in zip((loss, lse, dx, dw), run_ce(big[:N, :d], big[:, 128:128 + d], labels)):
+        assert torch.equal(a, b)
+    del big
+    lib = L.load()
+    desc = L.LinearLossDesc(N, V, d, L.BF16, d, d, 1.0, 1.0, None, 1)
+    bx, bw = torch.full((N, d + 24), 9.0, dtype=BF, device=DEV), torch.full((V, d + 8), 9.0, dtype=BF, device=DEV)
+    size = lib.cdet_linear_loss_ws_bytes(C.byref(desc), 1)
+    ws = torch.empty(size + 512, dtype=torch.uint8, device=DEV).fill_(255)
+    L.check(lib.cdet_linear_ce_bwd(C.byref(desc), x.data_ptr(), w.data_ptr(), labels.data_ptr(), lse.data_ptr(), None, 0, bx.data_ptr(), d + 24, bw.data_ptr(), d + 8,
+                                   ws.data_ptr(), ops.stream()))
+    assert torch.equal(bx[:, :d], dx) and torch.equal(bw[:, :d], dw) and torch.all(bx[:, d:] == 9) and torch.all(bw[:, d:] == 9) and torch.all(ws[size:] == 255)
+
+
+@pytest.mark.parametrize("N,V,d,k", [(1, 5000, 264, 9), (37, 900, 320, 20), (100, 700, 64, 5)])
+def test_few_rows_captured(N, V, d, k):
+    """Losses and gradients of few rows captured and replayed on new numbers, eager calls of other sizes in between; and on two streams at once."""
+    ops = _ops()
+    x, w, labels = ce_case(N, V, d, BF, seed=200)
+    idx, val = teacher(N, V, k, 201, empty=False)
+
+    def step(x, w):
+        loss, lse = ops.linear_ce_fwd(x, w, labels)
+        kd, saved = ops.linear_distill_fwd(x, w, idx, val, tau=2.0)
+        return [loss, lse, *ops.linear_ce_bwd(x, w, labels, lse), kd, *ops.linear_distill_bwd(x, w, idx, saved, tau=2.0)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(x, w)
+    for turn in range(4):
+        x.copy_(_rand(N, d, seed=210 + turn, dtype=BF))
+        run_ce(*ce_case(33 + turn, 77, 40, BF, seed=220))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step(x, w)):
+            assert torch.equal(a, b), turn
+    y = _rand(N, d, seed=230, dtype=BF)
+    want = step(x, w), step(y, w)
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        outs = []
+        for s, inp in zip(streams, (x, y)):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                outs.append(step(inp, w))
+        torch.cuda.synchronize()
+        for a, b in zip(want, outs):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
 def test_used_together():
     """A student classifier learns from labels and from a teacher's top logits in one backward; the fused distillation is that of its own logits."""
     from cerberusdet_amd.utils import loss as UL
