@@ -11,7 +11,7 @@
 //
 // One product for all three (Pipe): an 8-wave workgroup, 256 x 256 outputs, K in steps of 32 through a ring of four LDS stages filled by LDS-DMA. The two
 // halves of the workgroup run half a step apart: while one multiplies, the other reads its fragments. What bounds it is the chip's power: 4096 x 4096 x 8192
-// runs at 1230 - 1250 TF/s on random bf16 numbers and at 1740 on zeros (hipBLASLt on the same random numbers: 1300). Small problems take 128 x 128 tiles of
+// runs at 1230 - 1250 TF/s on random bf16 numbers and at 1740 on zeros (a library's product on the same random numbers: 1300). Small problems take 128 x 128 tiles of
 // 4 waves (Quad), where a workgroup's own latency counts; the backward of at most 128 rows has a form of its own (class_few_kernel).
 // Operand "A" (fragment rows) is what must come out contiguous: a lane ends up with four consecutive A rows of one B row. So A = classes in the first
 // product (a lane holds classes of ONE row of x: the softmax statistics are sums inside the lane), A = features in the other two. An operand whose
