@@ -118,6 +118,9 @@ __device__ __forceinline__ void td_sync() {
     }
 }
 
+// what exponents are taken relative to: the maximum, or 0 where there is nothing but -inf and NaN -- a sum of 0 then says that nothing is left, NaN stays NaN
+__device__ __forceinline__ float td_base(float m) { return m == -INFINITY ? 0.f : m; }
+
 // a row's teacher in LDS: class (-1: an empty slot), q, log q, and the student's logit there (taken before the gradient may overwrite it)
 struct TdSlots {
     float *q, *lq, *z;
@@ -125,7 +128,7 @@ struct TdSlots {
     static __host__ __device__ constexpr int up(int k) { return (k + 3) & ~3; }  // (empty ones up to the next four)
     __device__ TdSlots(float* lds, int k) : q(lds), lq(lds + up(k)), z(lds + 2 * up(k)), v(reinterpret_cast<int*>(lds + 3 * up(k))) {}
 };
-// fills it; t = thread of the row. False: no filled slot, or nothing but -inf in them
+// fills it; t = thread of the row. False: no filled slot, or nothing but -inf in them (the sum is 0; NaN makes it NaN, which the maximum would not show)
 template <int DT, int NW>
 __device__ __forceinline__ bool td_teacher(const TdArgs& a, int64_t row, int t, const typename TdElem<DT>::T* z, TdSlots s, float* scratch) {
     constexpr int NT = NW * 64;
@@ -142,7 +145,7 @@ __device__ __forceinline__ bool td_teacher(const TdArgs& a, int64_t row, int t, 
             m = fmaxf(m, x);
         }
     }
-    m = td_reduce<NW, true>(m, scratch);
+    m = td_base(td_reduce<NW, true>(m, scratch));
     float sum = 0.f;
     for (int j = t; j < a.k; j += NT)
         if (s.v[j] >= 0) sum += expf(s.lq[j] - m);
@@ -153,7 +156,7 @@ __device__ __forceinline__ bool td_teacher(const TdArgs& a, int64_t row, int t, 
         s.lq[j] = lq;
         s.q[j] = s.v[j] >= 0 ? expf(lq) : 0.f;
     }
-    return m != -INFINITY;
+    return sum != 0.f;
 }
 
 // the row's loss, and the named entries of its gradient (a class named twice takes both q; the slot that names it first writes)
@@ -272,8 +275,7 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
         }
     }
     m = td_reduce<1, true>(m, nullptr);
-    tm = td_reduce<1, true>(tm, nullptr);
-    const bool on = m != -INFINITY && tm != -INFINITY;
+    tm = td_base(td_reduce<1, true>(tm, nullptr));
     const float mu = __builtin_isinf(m) ? 0.f : m, muc = mu * a.c;
     float s = 0.f, ts = 0.f;
 #pragma unroll
@@ -295,6 +297,7 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
         }
     s = td_reduce<1, false>(s, nullptr);
     ts = td_reduce<1, false>(ts, nullptr);
+    const bool on = s != 0.f && ts != 0.f;
     const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s), its = 1.f / ts, lts = __builtin_amdgcn_logf(ts);
     td_sync<1>();  // every slot has read its logit: from here on the row says which slot names a class (k: none; of several, one of them)
     uint16_t* const own = reinterpret_cast<uint16_t*>(rb);
@@ -402,7 +405,6 @@ __global__ __launch_bounds__(NW * 64, NW == 16 ? 8 : 1) void td_wide_kernel(cons
 #pragma unroll
             for (int e = 0; e < CH; ++e) m = fmaxf(m, v[i][e]);
     m = td_reduce<NW, true>(m, scratch);
-    on = on && m != -INFINITY;
     const float mu = __builtin_isinf(m) ? 0.f : m, muc = mu * a.c;
     float s = 0.f;
 #pragma unroll
@@ -414,6 +416,7 @@ __global__ __launch_bounds__(NW * 64, NW == 16 ? 8 : 1) void td_wide_kernel(cons
                 s += v[i][e];
             }
     s = td_reduce<NW, false>(s, scratch);
+    on = on && s != 0.f;
     const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s);
     const float g = a.gs * (a.drow ? a.drow[row] : 1.f), f = inv * g;
     if (dz) {
@@ -479,7 +482,6 @@ __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const T
             for (int e = 0; e < CH; ++e) m = fmaxf(m, logit(i, e));
         }
     m = td_reduce<NW, true>(m, scratch);
-    const bool on = some && m != -INFINITY;
     const float mu = __builtin_isinf(m) ? 0.f : m, muc = mu * a.c;
     float s = td_exp2<DT>(vt, mu, a.c, muc);
 #pragma unroll
@@ -490,6 +492,7 @@ __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const T
             for (int e = 0; e < CH; ++e) s += td_exp2<DT>(logit(i, e), mu, a.c, muc);
         }
     s = td_reduce<NW, false>(s, scratch);
+    const bool on = some && s != 0.f;
     const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s);
     const float g = a.gs * (a.drow ? a.drow[row] : 1.f);
     if (dz) {
@@ -562,10 +565,10 @@ __global__ __launch_bounds__(1024) void td_long_kernel(const TdArgs a) {
             for (int e = 0; e < CH; ++e) s += __builtin_amdgcn_exp2f((v[u][e] - mu) * a.c);
     }
     const float all = td_reduce<NW, true>(m, scratch);
-    on = on && all != -INFINITY;
     const float mu = __builtin_isinf(all) ? 0.f : all, muc = mu * a.c;
     s = s == 0.f ? 0.f : s * __builtin_amdgcn_exp2f(((__builtin_isinf(m) ? 0.f : m) - mu) * a.c);
     s = td_reduce<NW, false>(s, scratch);
+    on = on && s != 0.f;
     const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s);
     const float g = a.gs * (a.drow ? a.drow[row] : 1.f), f = inv * g;
     if (dz) {
@@ -645,9 +648,8 @@ __global__ __launch_bounds__(256) void td_narrow_kernel(const TdArgs a) {
         tm = fmaxf(tm, tx[j]);
     }
     m = td_lanes<L, true>(m);
-    tm = td_lanes<L, true>(tm);
+    tm = td_base(td_lanes<L, true>(tm));
     const float mu = __builtin_isinf(m) ? 0.f : m;
-    const bool on = tm != -INFINITY && m != -INFINITY;
     float s = 0.f, ts = 0.f, p[E], lq[S], q[S];
 #pragma unroll
     for (int j = 0; j < S; ++j) {
@@ -663,6 +665,7 @@ __global__ __launch_bounds__(256) void td_narrow_kernel(const TdArgs a) {
     }
     s = td_lanes<L, false>(s);
     ts = td_lanes<L, false>(ts);
+    const bool on = s != 0.f && ts != 0.f;
     const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s), itq = 1.f / ts, lts = __builtin_amdgcn_logf(ts);
     float *lp = s_lp[r], *sq = s_q[r];
 #pragma unroll

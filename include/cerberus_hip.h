@@ -519,7 +519,8 @@ int cdet_linear_distill_bwd(const cdet_linear_loss_desc* d, const void* x, const
  * logits each -- the class logits of a head map (G = 1), its four 16-bin box distributions (G = 4, V = 16). Distribution g of pixel p starts at
  * logits + (p * ld + g * V) elements (pass the pointer of the first channel); its gradient, d(sum_r drow_r loss_r) / d logit * grad_scale, at
  * dlogits + (p * grad_ld + g * V). idx / val [P * G, k], drow [P * G] or NULL (ones), loss [P * G]. Everything else in a pixel's pitch is left as it is.
- * logits: fp32 / bf16 / fp16, any alignment of whole elements; -inf = a class left out. dlogits may be NULL (loss only) and may BE logits (same type
+ * logits: fp32 / bf16 / fp16, any alignment of whole elements; -inf = a class left out. NaN in a row that takes part, in its logits or in a filled slot,
+ * gives a loss of NaN. dlogits may be NULL (loss only) and may BE logits (same type
  * and pitch). */
 typedef struct {
     int32_t P, G, V, k;
