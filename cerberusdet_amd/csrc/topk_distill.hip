@@ -47,12 +47,10 @@ template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) 
     T v[N];
 };
 
-// exponent of a logit relative to the row's maximum, log2 units. fp32: the difference first, so that the error does not grow with |z|; 16-bit logits and
-// gradients need no more than one fused rounding of z c (2^-24 |z c| against 2^-9)
-template <int DT>
-__device__ __forceinline__ float td_exp2(float z, float mu, float c, float muc) {
-    return __builtin_amdgcn_exp2f(DT == CDET_F32 ? (z - mu) * c : fmaf(z, c, -muc));
-}
+// exponential of a logit relative to the row's maximum, the one form that sums, loss and gradient share: the difference first, so that the error does not grow
+// with |z| (one fused rounding of z c, for 16-bit logits, put the sum and the named entries 13 nats apart at -1e9, and z c leaves fp32's range before z does;
+// no slower but in td_held_kernel, which has its own)
+__device__ __forceinline__ float td_exp2(float z, float mu, float c) { return __builtin_amdgcn_exp2f((z - mu) * c); }
 typedef __attribute__((ext_vector_type(2))) float tdf2;
 typedef __attribute__((ext_vector_type(2))) __bf16 tdb2;
 typedef __attribute__((ext_vector_type(2))) _Float16 tdh2;
@@ -169,8 +167,8 @@ __device__ __forceinline__ void td_finish(const TdArgs& a, int64_t row, int t, b
         const int v = s.v[j];
         if (!on || v < 0) continue;
         float q = s.q[j];
-        const float e2 = (s.z[j] - mu) * a.c;
-        if (q != 0.f) sum += q * (s.lq[j] - (e2 - l2s) * kTdLn2);
+        const float below = s.z[j] - mu;
+        if (q != 0.f) sum += q * (s.lq[j] - (below * a.itau - l2s * kTdLn2));  // (not by way of log2 units, which end before fp32 does)
         if (!dz) continue;
         bool first = true;
         for (int o = 0; o < a.k; o += 4) {
@@ -187,7 +185,7 @@ __device__ __forceinline__ void td_finish(const TdArgs& a, int64_t row, int t, b
                     q += same && o + e > j ? s.q[o + e] : 0.f;
                 }
         }
-        if (first) dz[v] = TdElem<GDT>::put((__builtin_amdgcn_exp2f(e2) * inv - q) * g);
+        if (first) dz[v] = TdElem<GDT>::put((__builtin_amdgcn_exp2f(below * a.c) * inv - q) * g);
     }
     sum = td_reduce<NW, false>(sum, scratch);
     if (t == 0) a.loss[row] = on ? sum * a.tau2 : 0.f;
@@ -276,17 +274,17 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
     }
     m = td_reduce<1, true>(m, nullptr);
     tm = td_base(td_reduce<1, true>(tm, nullptr));
-    const float mu = __builtin_isinf(m) ? 0.f : m, muc = mu * a.c;
+    const float mu = __builtin_isinf(m) ? 0.f : m;
     float s = 0.f, ts = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
         if (i * 64 * CH < V)
 #pragma unroll
             for (int e = 0; e < CH; ++e) {
-                v[i][e] = td_exp2<DT>(v[i][e], mu, a.c, muc);
+                v[i][e] = td_exp2(v[i][e], mu, a.c);
                 s += v[i][e];
             }
-    vt = td_exp2<DT>(vt, mu, a.c, muc);
+    vt = td_exp2(vt, mu, a.c);
     s += vt;
     for (int j = t; j < k; j += 64)
         if (sv[j] >= 0) {
@@ -314,9 +312,9 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
     for (int j = t; j < k; j += 64) {
         const float q = on && sv[j] >= 0 ? sq[j] * its : 0.f;
         sq[j] = q;
-        if (q != 0.f) sum += q * (slq[j] - lts - (sz[j] - mu) * a.c + l2s);
+        if (q != 0.f) sum += q * ((slq[j] - lts + l2s) * kTdLn2 - (sz[j] - mu) * a.itau);  // (td_finish)
     }
-    sum = td_reduce<1, false>(sum, nullptr) * kTdLn2;
+    sum = td_reduce<1, false>(sum, nullptr);
     if (t == 0) a.loss[row] = on ? sum * a.tau2 : 0.f;
     if (!dz) return;
     td_sync<1>();
@@ -405,14 +403,14 @@ __global__ __launch_bounds__(NW * 64, NW == 16 ? 8 : 1) void td_wide_kernel(cons
 #pragma unroll
             for (int e = 0; e < CH; ++e) m = fmaxf(m, v[i][e]);
     m = td_reduce<NW, true>(m, scratch);
-    const float mu = __builtin_isinf(m) ? 0.f : m, muc = mu * a.c;
+    const float mu = __builtin_isinf(m) ? 0.f : m;
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
         if (i * NT * CH < V)
 #pragma unroll
             for (int e = 0; e < CH; ++e) {
-                v[i][e] = td_exp2<DT>(v[i][e], mu, a.c, muc);
+                v[i][e] = td_exp2(v[i][e], mu, a.c);
                 s += v[i][e];
             }
     s = td_reduce<NW, false>(s, scratch);
@@ -440,7 +438,9 @@ __global__ __launch_bounds__(NW * 64, NW == 16 ? 8 : 1) void td_wide_kernel(cons
 
 // longer rows, as they are stored (16 waves a row, NCH chunks of 16 bytes a thread): two exponentials a logit instead of a second read.
 // 8192 x 65536 bf16 388 us = 5.5 TB/s; NCH = 16 leaves one row a CU, whose loads and stores take turns: 4096 x 131072 bf16 479 us = 4.5 TB/s (walking over
-// its rows, the next one's loads under this one's stores: 535).
+// its rows, the next one's loads under this one's stores: 535). That form's time shows its instructions, so 16-bit rows take an exponent in one: z c - mu c,
+// with the rounding of mu c (at most 1/2) taken back out of the sum (as (z - mu) c: 505 us, fp16 511 against 467). Where mu c is beyond 2^24 two 16-bit logits
+// are the same or 2^12 and more apart, and a power of two that makes the product exact stands in for c.
 template <int DT, int GDT, int NCH>
 __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
@@ -482,21 +482,28 @@ __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const T
             for (int e = 0; e < CH; ++e) m = fmaxf(m, logit(i, e));
         }
     m = td_reduce<NW, true>(m, scratch);
-    const float mu = __builtin_isinf(m) ? 0.f : m, muc = mu * a.c;
-    float s = td_exp2<DT>(vt, mu, a.c, muc);
+    const float mu = __builtin_isinf(m) ? 0.f : m;
+    float c = a.c, muc = mu * c;
+    if (DT != CDET_F32 && !(fabsf(muc) <= 16777216.f)) {
+        c = __builtin_amdgcn_ldexpf(1.f, 23 - __builtin_amdgcn_frexp_expf(mu));
+        muc = mu * c;
+    }
+    auto power = [&](float z, float mu, float muc) { return DT == CDET_F32 ? td_exp2(z, mu, c) : __builtin_amdgcn_exp2f(fmaf(z, c, -muc)); };
+    float s = power(vt, mu, muc);
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
         if (i * NT * CH < V) {
             anew(i);
 #pragma unroll
-            for (int e = 0; e < CH; ++e) s += td_exp2<DT>(logit(i, e), mu, a.c, muc);
+            for (int e = 0; e < CH; ++e) s += power(logit(i, e), mu, muc);
         }
     s = td_reduce<NW, false>(s, scratch);
     const bool on = some && s != 0.f;
+    const float g = a.gs * (a.drow ? a.drow[row] : 1.f), dense = g / s;
+    if (DT != CDET_F32) s *= __builtin_amdgcn_exp2f(-fmaf(mu, c, -muc));
     const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s);
-    const float g = a.gs * (a.drow ? a.drow[row] : 1.f);
     if (dz) {
-        float f = inv * g, mg = mu, mgc = muc;
+        float f = dense, mg = mu, mgc = muc;
         int u = t;
         asm volatile("" : "+v"(u));  // (addresses are computed anew: no register is kept for them)
         if (!on) {  // zeros, whatever the logits are
@@ -511,11 +518,11 @@ __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const T
                 anew(i);
                 float o[CH];
 #pragma unroll
-                for (int e = 0; e < CH; ++e) o[e] = td_exp2<DT>(logit(i, e), mg, a.c, mgc) * f;
+                for (int e = 0; e < CH; ++e) o[e] = power(logit(i, e), mg, mgc) * f;
                 if (e0 + CH <= V) td_put<GDT, CH>(dz + e0, o);
             }
         }
-        if (u < V % CH) dz[V - V % CH + u] = TdElem<GDT>::put(td_exp2<DT>(on ? vt : 0.f, mg, a.c, mgc) * f);
+        if (u < V % CH) dz[V - V % CH + u] = TdElem<GDT>::put(power(on ? vt : 0.f, mg, mgc) * f);
     }
     td_sync<NW>();
     td_finish<GDT, NW>(a, row, t, on, dz, mu, inv, l2s, g, slots, scratch);
@@ -565,7 +572,7 @@ __global__ __launch_bounds__(1024) void td_long_kernel(const TdArgs a) {
             for (int e = 0; e < CH; ++e) s += __builtin_amdgcn_exp2f((v[u][e] - mu) * a.c);
     }
     const float all = td_reduce<NW, true>(m, scratch);
-    const float mu = __builtin_isinf(all) ? 0.f : all, muc = mu * a.c;
+    const float mu = __builtin_isinf(all) ? 0.f : all;
     s = s == 0.f ? 0.f : s * __builtin_amdgcn_exp2f(((__builtin_isinf(m) ? 0.f : m) - mu) * a.c);
     s = td_reduce<NW, false>(s, scratch);
     on = on && s != 0.f;
@@ -577,7 +584,7 @@ __global__ __launch_bounds__(1024) void td_long_kernel(const TdArgs a) {
             load(e0, v);
             float o[CH];
 #pragma unroll
-            for (int e = 0; e < CH; ++e) o[e] = on ? td_exp2<DT>(v[e], mu, a.c, muc) * f : 0.f;
+            for (int e = 0; e < CH; ++e) o[e] = on ? td_exp2(v[e], mu, a.c) * f : 0.f;
             if (e0 + CH <= V) td_put<GDT, CH>(dz + e0, o);
             else
 #pragma unroll
@@ -604,7 +611,7 @@ __device__ __forceinline__ void td_get(const void* base, int64_t at, int n, floa
     }
 }
 
-// V <= L E, k <= L S: L lanes a row, E neighbouring classes and S slots a lane. A row's slots meet its classes in LDS: log p of every class, and {q, 1} of the slot
+// V <= L E, k <= L S: L lanes a row, E neighbouring classes and S slots a lane. A row's slots meet its classes in LDS: how far every class is below the maximum, and {q, 1} of the slot
 // that named it last; as many owned classes as filled slots means that no class was named twice. Few elements a lane leave it bound by its instructions, so a
 // lane takes four neighbours (6, 8 in longer rows) and, where k <= L, one slot: 268800 x 4 x 16 fp32, k = 16: 56 us = 5.1 TB/s, with a class and a slot a lane
 // and 16 lanes a row 82; 268800 x 80, k = 10: 31 us, with eight slots on each of two lanes 50.
@@ -613,7 +620,7 @@ __global__ __launch_bounds__(256) void td_narrow_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
     typedef typename TdElem<GDT>::T TG;
     constexpr int ROWS = 256 / L, W = L * E + 4;  // (4: rows start in different banks)
-    __shared__ __attribute__((aligned(16))) float s_lp[ROWS][W];
+    __shared__ __attribute__((aligned(16))) float s_z[ROWS][W];  // below the maximum
     __shared__ __attribute__((aligned(16))) float s_q[ROWS][2 * W];
     const int lane = (int)threadIdx.x & 63, l = (int)threadIdx.x & (L - 1), r = (int)threadIdx.x / L, V = a.V, k = a.k;
     const int64_t row = (int64_t)blockIdx.x * ROWS + r;
@@ -659,18 +666,18 @@ __global__ __launch_bounds__(256) void td_narrow_kernel(const TdArgs a) {
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        v[e] = (v[e] - mu) * a.c;
-        p[e] = __builtin_amdgcn_exp2f(v[e]);
+        v[e] -= mu;
+        p[e] = __builtin_amdgcn_exp2f(v[e] * a.c);
         s += p[e];
     }
     s = td_lanes<L, false>(s);
     ts = td_lanes<L, false>(ts);
     const bool on = s != 0.f && ts != 0.f;
     const float inv = 1.f / s, l2s = __builtin_amdgcn_logf(s), itq = 1.f / ts, lts = __builtin_amdgcn_logf(ts);
-    float *lp = s_lp[r], *sq = s_q[r];
+    float *below = s_z[r], *sq = s_q[r];
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
-        *reinterpret_cast<float2*>(lp + l * E + e) = float2{v[e] - l2s, v[e + 1] - l2s};
+        *reinterpret_cast<float2*>(below + l * E + e) = float2{v[e], v[e + 1]};
         *reinterpret_cast<f32x4*>(sq + 2 * (l * E + e)) = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     td_sync<1>();  // (a row's lanes are in one wave)
@@ -678,14 +685,13 @@ __global__ __launch_bounds__(256) void td_narrow_kernel(const TdArgs a) {
 #pragma unroll
     for (int j = 0; j < S; ++j)
         if (ti[j] >= 0) {
-            lq[j] -= lts;
             q[j] *= itq;
-            if (q[j] != 0.f) sum += q[j] * (lq[j] - lp[ti[j]]);
+            if (q[j] != 0.f) sum += q[j] * ((lq[j] - lts + l2s) * kTdLn2 - below[ti[j]] * a.itau);  // (td_finish)
             *reinterpret_cast<float2*>(sq + 2 * ti[j]) = float2{q[j], 1.f};
             more += 1.f;
         }
     td_sync<1>();
-    sum = td_lanes<L, false>(sum) * kTdLn2;
+    sum = td_lanes<L, false>(sum);
     float qs[E];
 #pragma unroll
     for (int e = 0; e < E; e += 2) {

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_class_loss import BF, DEV, F16, F32, _ops, _rand, ce_case, check_map, teacher
+from test_gpu_class_loss import BF, DEV, F16, F32, U, _ops, _rand, _randint, ce_case, check_map, check_rows, map_reference, teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,67 @@ def test_nan_is_the_same_for_the_fused_projection():
     logits, _ = _ops().topk_distill(x.float() @ w.float().T, idx, val)
     for loss in (fused, logits):
         assert loss[:3].isnan().all() and torch.all(loss[3:5] == 0) and loss[5].isfinite()
+
+
+def check_far(got, z, idx, val, tau):
+    """An exponent e = (z - max) log2(e) / tau takes four roundings of its own size, exp2 and log2 one or two; a sum of V terms adds up at most 48 + V / 1024 of
+    them in a chain. Terms that count (p > 2^-150) have |e| < 150, and sum p |e| ln 2 <= ln V + 1: u (4 (ln V + 1) + V / 1024 + 64) of the sum, 700 u of one p."""
+    loss, dz = got
+    V, k = z.shape[-1], idx.shape[-1]
+    wl, wd, mag = map_reference(z, idx, val, tau, None)
+    logp = torch.log_softmax(z.double() / tau, -1).gather(-1, idx.long().clamp(0, V - 1))
+    logp = torch.where(torch.isfinite(logp), logp, 0.0).abs().amax(-1)
+    rel = U * (4 * (math.log(V) + 1) + V / 1024 + 64)
+    # log p: four roundings of itself and the sum's; log q: the same of the teacher's logits, below 32; k products added up
+    check_rows(loss, wl, tau * tau * 2 * (rel + U * (8 * logp + 8 * 32 + k + 32)))
+    h = 0.0 if dz.dtype == F32 else torch.finfo(dz.dtype).eps / 2
+    # exp2's results end at 2^-126 (below that the hardware gives 0): p is off by no more than that; and half a smallest step of the gradient's type
+    tol = 1.01 * (h * wd.abs() + (rel + 700 * U) * mag + tau * 2.0 ** -126) + 2 * torch.finfo(dz.dtype).tiny * torch.finfo(dz.dtype).eps
+    err = (dz.double() - wd).abs()
+    assert torch.all(err <= tol), (err / tol).max().item()
+
+
+FAR = [(F32, 1.0e5), (F32, -1.0e30), (F32, -3.3e38), (BF, 1.0e3), (BF, -1.0e5), (BF, -1.0e9), (BF, 1.0e30), (BF, -3.3e38), (F16, 1.0e3), (F16, -6.0e4)]
+
+
+@pytest.mark.parametrize("dtype,base", FAR)
+@pytest.mark.parametrize("V", FORMS)
+def test_far_logits_cost_nothing(V, dtype, base):
+    """Rows around one far value: loss and gradient are as exact as near 0, for neighbours of the type (tau of their distance) and for ties (tau = 1)."""
+    k = 6
+    step = 2.0 ** (math.floor(math.log2(abs(base))) - {F32: 23, BF: 7, F16: 10}[dtype])
+    near = torch.tensor(base, dtype=dtype, device=DEV).double() + step * _randint(6, (7, V), 320)
+    z = near.to(dtype)
+    idx, val = distinct(7, V, k, 321)
+    idx[1] = z[1].float().argmax().int()  # all slots on the largest
+    z[2] = z[2, 0]
+    z[3, 1::3] = -math.inf
+    idx[3] = idx[3] // 3 * 3
+    idx[4, 2:] = -1
+    for tau in (1.0, step) if 2.0 ** -20 < step < 1e12 else (1.0,):
+        v = val * tau  # (the teacher's distribution stays)
+        check_far(_ops().topk_distill(z, idx, v, tau=tau), z, idx, v, tau)
+        check_far(_ops().topk_distill(z, idx, v, tau=tau, grad_dtype=F32), z, idx, v, tau)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("V", FORMS)
+def test_masks_of_the_lowest_value(V, dtype):
+    """Classes masked with the type's lowest number: no probability beside others, all of it where nothing else is left; a teacher that names one has the loss
+    that the formula gives, which is finite."""
+    low = torch.finfo(dtype).min
+    z = (2 * _rand(6, V, seed=330)).to(dtype)
+    idx, val = distinct(6, V, 4, 331)
+    z[0, ::2] = low
+    idx[0] = idx[0] | 1
+    z[1] = low
+    z[2] = low
+    z[2, 1::2] = -math.inf
+    idx[2] = idx[2] // 2 * 2
+    z[3, idx[3, 0].long()] = low
+    val[3, 0] -= 12.0  # (tau^2 q 3.4e38 / tau stays in range)
+    z[4] = torch.finfo(dtype).max
+    for tau in (1.0, 2.0):
+        got = _ops().topk_distill(z, idx, val, tau=tau)
+        assert got[0].isfinite().all() and got[1].isfinite().all()
+        check_far(got, z, idx, val, tau)
