@@ -128,3 +128,54 @@ def test_masks_of_the_lowest_value(V, dtype):
         got = _ops().topk_distill(z, idx, val, tau=tau)
         assert got[0].isfinite().all() and got[1].isfinite().all()
         check_far(got, z, idx, val, tau)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("V", [60, 1500, 9001, 70001, 140000])
+def test_gradient_of_16_bit_logits_under_a_loss_scale(V, dtype):
+    """The gradient through autograd is rounded to the logits' type once, behind the incoming gradient: what a loss scale lifts into fp16's range is there."""
+    from cerberusdet_amd.utils import loss as UL
+
+    z = _rand(5, V, seed=340).to(dtype)
+    idx, val = distinct(5, V, 7, 341)
+    weight = torch.tensor([1.0, 0.5, -2.0, 0.0, 1.37], device=DEV) * 2.0 ** 13
+    leaf = z.clone().requires_grad_()
+    (UL.topk_distillation(leaf, idx, val, tau=2.0, reduction="none") * weight).sum().backward()
+    wl, wd, mag = map_reference(z, idx, val, 2.0, weight)
+    rel = U * (4 * (math.log(V) + 1) + V / 1024 + 64 + 64)  # check_far's; logits within 6 / tau of the maximum's 6: 4 roundings of an exponent below 9
+    h = 0.0 if dtype == F32 else torch.finfo(dtype).eps / 2
+    tol = 1.01 * (h * wd.abs() + rel * mag) + torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    err = (leaf.grad.double() - wd).abs()
+    assert leaf.grad.dtype == dtype and torch.all(err <= tol), (err / tol).max().item()
+
+
+@pytest.mark.parametrize("dtype,P,taped", [(BF, 1000, True), (F16, 1000, False), (F32, 1000, True), (F32, 300, False)])
+def test_forward_holds_no_gradient_map(dtype, P, taped):
+    """Long or 16-bit maps are read again by the backward, and a loss without one makes no gradient: neither keeps a map of the logits' size."""
+    from cerberusdet_amd.utils import loss as UL
+
+    z = _rand(P, 40000, seed=350, dtype=dtype).requires_grad_()
+    idx, val = distinct(P, 40000, 4, 351)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    with torch.set_grad_enabled(taped):
+        loss = UL.topk_distillation(z, idx, val)
+    assert torch.cuda.max_memory_allocated() - before < z.numel()
+    if not taped:
+        return
+    with torch.no_grad():
+        z.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):  # (what the backward reads may not change: refused)
+        loss.backward()
+
+
+def test_topk_distillation_twice_through_one_graph():
+    from cerberusdet_amd.utils import loss as UL
+
+    z = _rand(50, 300, seed=360).requires_grad_()
+    idx, val = teacher(50, 300, 6, 361)
+    loss = UL.topk_distillation(z, idx, val, tau=1.5)
+    a, = torch.autograd.grad(loss, z, retain_graph=True)
+    b, = torch.autograd.grad(3 * loss, z)
+    assert torch.allclose(3 * a, b, rtol=4 * 2.0 ** -23, atol=0)
