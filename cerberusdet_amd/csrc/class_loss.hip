@@ -934,7 +934,8 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_grads_kernel(const G
 // ---- small launches ----------------------------------------------------------------------------------------------------------------------------------
 // rows' (maximum, sum) pairs -> lse: C rows a workgroup (a power of two), 1024 / C threads a row that take every (1024 / C)th pair, joined in a tree of
 // fixed order
-__device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2) {  // a sum of 0 has no maximum; one of inf or NaN stays
+// a sum of 0 has no maximum; one of inf, whose maximum is written as 0, stays inf beside any other (and does not become inf * 0), NaN stays NaN
+__device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2) {
     if (s2 == 0.f) return;
     if (s == 0.f) {
         m = m2;
@@ -942,7 +943,7 @@ __device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2)
         return;
     }
     const float mn = fmaxf(m, m2);
-    s = s * __builtin_amdgcn_exp2f(m - mn) + s2 * __builtin_amdgcn_exp2f(m2 - mn);
+    s = (s == INFINITY ? s : s * __builtin_amdgcn_exp2f(m - mn)) + (s2 == INFINITY ? s2 : s2 * __builtin_amdgcn_exp2f(m2 - mn));
     m = mn;
 }
 __global__ __launch_bounds__(1024) void class_lse_kernel(const float* part, int nvb, int N, int V, int C, const void* label, int label64, const float* zlab, float* loss,

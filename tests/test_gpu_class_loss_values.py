@@ -179,3 +179,32 @@ def test_topk_distillation_twice_through_one_graph():
     a, = torch.autograd.grad(loss, z, retain_graph=True)
     b, = torch.autograd.grad(3 * loss, z)
     assert torch.allclose(3 * a, b, rtol=4 * 2.0 ** -23, atol=0)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("N,V", [(1, 300), (70, 4000), (70, 20000), (2600, 3900), (300, 60000)])
+def test_an_infinite_logit_beside_far_ones(N, V, dtype):
+    """One class's logit overflows to +inf, another one far down the list is 300: the log-sum-exp is +inf (not NaN), and so is the loss of every other class."""
+    d = 16
+    x, w = torch.zeros(N, d, dtype=dtype, device=DEV), torch.zeros(V, d, dtype=dtype, device=DEV)
+    x[:, 0] = 2.0
+    off = 0.1 * _rand(V, seed=370)
+    for a, b in ((1, V - 1), (V - 1, 1), (V // 2, 3)):
+        w[:, 0] = 0
+        w[a, 0] = 3.0
+        o = off.clone()
+        o[b] = 300.0
+        labels = torch.full((N,), b, device=DEV)
+        loss, lse = _ops().linear_ce_fwd(x, w, labels, offset=o, scale=1e38)
+        assert torch.all(lse == math.inf) and torch.all(loss == math.inf)
+        idx = torch.full((N, 2), b, dtype=torch.int32, device=DEV)
+        idx[:, 1] = 7
+        loss, saved = _ops().linear_distill_fwd(x, w, idx, torch.zeros(N, 2, device=DEV), offset=o, scale=1e38)
+        assert torch.all(loss == math.inf)
+        none = torch.full_like(idx, -1)
+        loss, saved = _ops().linear_distill_fwd(x, w, none, torch.zeros(N, 2, device=DEV), offset=o, scale=1e38)
+        assert torch.all(loss == 0) and torch.all(saved[:, 0] == math.inf)
+    w[V // 2 + 5, 1] = math.nan  # NaN beside an infinite one stays NaN
+    x[:, 1] = 1.0
+    loss, lse = _ops().linear_ce_fwd(x, w, torch.full((N,), 1, device=DEV), offset=off, scale=1e38)
+    assert lse.isnan().all() and loss.isnan().all()
