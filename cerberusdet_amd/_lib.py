@@ -90,7 +90,7 @@ class LinearLossDesc(C.Structure):
 
 class TopkDistillDesc(C.Structure):
     _fields_ = [("P", i32), ("G", i32), ("V", i32), ("k", i32), ("dtype", i32), ("val_dtype", i32), ("grad_dtype", i32), ("ld", i64), ("grad_ld", i64),
-                ("tau", f32), ("grad_scale", f32)]
+                ("tau", f32), ("grad_scale", f32), ("part", vp)]
 
 
 class WgradItem(C.Structure):

@@ -20,6 +20,7 @@ struct TdArgs {
     const void* val;
     const float* drow;
     float* loss;
+    uint8_t* part;  // null, or 1 where the row takes part
     int64_t ld, gld;
     int64_t rows;
     int G, V, k, vdt;
@@ -116,6 +117,10 @@ __device__ __forceinline__ void td_sync() {
     }
 }
 
+__device__ __forceinline__ void td_row_out(const TdArgs& a, int64_t row, bool on, float sum) {
+    a.loss[row] = on ? sum * a.tau2 : 0.f;
+    if (a.part) a.part[row] = on;
+}
 // what exponents are taken relative to: the maximum, or 0 where there is nothing but -inf and NaN -- a sum of 0 then says that nothing is left, NaN stays NaN
 __device__ __forceinline__ float td_base(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -188,7 +193,7 @@ __device__ __forceinline__ void td_finish(const TdArgs& a, int64_t row, int t, b
         if (first) dz[v] = TdElem<GDT>::put((__builtin_amdgcn_exp2f(below * a.c) * inv - q) * g);
     }
     sum = td_reduce<NW, false>(sum, scratch);
-    if (t == 0) a.loss[row] = on ? sum * a.tau2 : 0.f;
+    if (t == 0) td_row_out(a, row, on, sum);
 }
 
 template <typename T, typename TG>
@@ -315,7 +320,7 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
         if (q != 0.f) sum += q * ((slq[j] - lts + l2s) * kTdLn2 - (sz[j] - mu) * a.itau);  // (td_finish)
     }
     sum = td_reduce<1, false>(sum, nullptr);
-    if (t == 0) a.loss[row] = on ? sum * a.tau2 : 0.f;
+    if (t == 0) td_row_out(a, row, on, sum);
     if (!dz) return;
     td_sync<1>();
     for (int j = t; j < k; j += 64)
@@ -727,7 +732,7 @@ __global__ __launch_bounds__(256) void td_narrow_kernel(const TdArgs a) {
             for (int e = 0; e < E; ++e)
                 if (e < nv) dz[l * E + e] = TdElem<GDT>::put(o[e]);
     }
-    if (l == 0) a.loss[row] = on ? sum * a.tau2 : 0.f;
+    if (l == 0) td_row_out(a, row, on, sum);
 }
 
 template <int DT, int GDT>
@@ -792,6 +797,7 @@ extern "C" int cdet_topk_distill(const cdet_topk_distill_desc* d, const void* lo
     a.val = val;
     a.drow = drow;
     a.loss = loss;
+    a.part = d->part;
     a.ld = d->ld;
     a.gld = d->grad_ld;
     a.rows = (int64_t)d->P * d->G;

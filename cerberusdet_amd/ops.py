@@ -577,11 +577,12 @@ def _pixel_pitch(t, what, P, G, V):
     return st[0] if P > 1 else G * V
 
 
-def topk_distill(logits, idx, val, tau=1.0, drow=None, grad_scale=1.0, grad_dtype=None, want_grad=True, out=None):
+def topk_distill(logits, idx, val, tau=1.0, drow=None, grad_scale=1.0, grad_dtype=None, want_grad=True, out=None, part=None):
     """The same distillation on logits in memory, loss and gradient in one call (like det_loss): logits [P, V], or [P, G, V] for G distributions a pixel (a
     head map's box bins), fp32 / bf16 / fp16, unit stride along V, distributions of a pixel back to back, any pixel pitch -- a channel slice of an NHWC map
     as it lies, e.g. view.torch().flatten(0, 2). idx / val [.., k]; drow: weights of the rows. Returns (loss [..] fp32, dlogits | None): the gradient of
-    sum(drow * loss) * grad_scale in grad_dtype (the logits' or fp32) -- in `out` if given (a slice of a gradient map, or the logits themselves)."""
+    sum(drow * loss) * grad_scale in grad_dtype (the logits' or fp32) -- in `out` if given (a slice of a gradient map, or the logits themselves).
+    part: a bool tensor [..] that is told which rows take part (a filled slot above -inf, a class above -inf)."""
     lib = L.load()
     if not isinstance(logits, torch.Tensor) or logits.dim() not in (2, 3) or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         _bad("logits must be [P, V] or [P, G, V] fp32, bf16 or fp16")
@@ -603,6 +604,10 @@ def topk_distill(logits, idx, val, tau=1.0, drow=None, grad_scale=1.0, grad_dtyp
     if grad_dtype is not logits.dtype and grad_dtype is not torch.float32:
         _bad(f"grad_dtype must be {logits.dtype} or fp32")
     g, gs = _row_grad(drow, rows, gpu)
+    if part is not None:
+        _on(gpu, "part", part)
+        if part.shape != rows or part.dtype != torch.bool or not part.is_contiguous():
+            _bad(f"part must be contiguous {list(rows)} bool, got {tuple(part.shape)} {part.dtype}")
     dev = logits.device
     with _Device(gpu) as s:
         if g is not None and gs == 0 and P * G != 1:
@@ -614,7 +619,7 @@ def topk_distill(logits, idx, val, tau=1.0, drow=None, grad_scale=1.0, grad_dtyp
         elif want_grad:
             out = torch.empty(*shape, dtype=grad_dtype, device=dev)
         gld = _pixel_pitch(out, "out", P, G, V) if out is not None else 0
-        d = L.TopkDistillDesc(P, G, V, idx.shape[-1], _DT[logits.dtype], _DT[val.dtype], _DT[grad_dtype], ld, gld, tau, float(grad_scale))
+        d = L.TopkDistillDesc(P, G, V, idx.shape[-1], _DT[logits.dtype], _DT[val.dtype], _DT[grad_dtype], ld, gld, tau, float(grad_scale), ptr(part))
         loss = torch.empty(*rows, dtype=torch.float32, device=dev)
         L.check(lib.cdet_topk_distill(C.byref(d), logits.data_ptr(), idx.data_ptr(), val.data_ptr(), ptr(g), loss.data_ptr(), ptr(out), s), "cdet_topk_distill")
     return loss, out

@@ -4,6 +4,8 @@ loss.py:179-181]. The whole computation -- anchors, DFL decode, task-aligned ass
 w.r.t. the head maps -- is one call into csrc/det_loss.hip; autograd sees a single node."""
 from __future__ import annotations
 
+import math
+
 import torch
 
 from .torch_utils import get_hyperparameter
@@ -121,11 +123,12 @@ class _LinearDistillFn(torch.autograd.Function):
         loss, saved = ops.linear_distill_fwd(x, w, idx, val, tau=tau, offset=offset, scale=scale)
         ctx.save_for_backward(x, w, idx, offset, saved)
         ctx.tau, ctx.scale = tau, scale
-        return loss
+        ctx.mark_non_differentiable(saved)
+        return loss, saved
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
+    def backward(ctx, g, _):
         from .. import ops
 
         x, w, idx, offset, saved = ctx.saved_tensors
@@ -144,11 +147,11 @@ class _TopkDistillFn(torch.autograd.Function):
     lifts into fp16's range -- and never kept or multiplied as a map. Small fp32 maps, bound by the host, have it made in the forward's one call and multiplied."""
 
     @staticmethod
-    def forward(ctx, logits, idx, val, tau, ahead):
+    def forward(ctx, logits, idx, val, tau, ahead, part):
         from .. import ops
 
         ctx.tau = tau
-        loss, ctx.dz = ops.topk_distill(logits, idx, val, tau=tau, want_grad=ahead)
+        loss, ctx.dz = ops.topk_distill(logits, idx, val, tau=tau, want_grad=ahead, part=part)
         if not ahead:
             ctx.save_for_backward(logits, idx, val)
         return loss
@@ -157,32 +160,33 @@ class _TopkDistillFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         if ctx.dz is not None:
-            return ctx.dz * g[..., None], None, None, None, None
+            return ctx.dz * g[..., None], None, None, None, None, None
         from .. import ops
 
         logits, idx, val = ctx.saved_tensors
-        return ops.topk_distill(logits, idx, val, tau=ctx.tau, drow=g.float())[1], None, None, None, None
+        return ops.topk_distill(logits, idx, val, tau=ctx.tau, drow=g.float())[1], None, None, None, None, None
 
 
 def linear_cross_entropy(x, w, labels, offset=None, scale=1.0, reduction="mean"):
     """Cross entropy of a linear classifier over a long class list, differentiable in x [N, d] and w [V, d] (bf16 / fp16); the N x V logits are never in
-    memory. Labels outside of 0 .. V-1 leave their row out; "mean" is over the rows that are left. See ops.linear_ce_fwd."""
-    loss, _ = _LinearCeFn.apply(x, w, labels, offset, float(scale))
-    return _reduced(loss, (labels >= 0) & (labels < w.shape[0]), reduction)
+    memory. Labels outside of 0 .. V-1 leave their row out; "mean" is over the rows that take part. See ops.linear_ce_fwd."""
+    loss, lse = _LinearCeFn.apply(x, w, labels, offset, float(scale))
+    return _reduced(loss, (labels.clamp(0, w.shape[0] - 1) == labels) & (lse != -math.inf), reduction)
 
 
 def linear_distillation(x, w, idx, val, tau=1.0, offset=None, scale=1.0, reduction="mean"):
     """Distillation of that classifier from a teacher's top k logits (idx [N, k] int32, val [N, k]), differentiable in x and w. See ops.linear_distill_fwd."""
-    loss = _LinearDistillFn.apply(x, w, idx, val, float(tau), offset, float(scale))
-    return _reduced(loss, ((idx >= 0) & (idx < w.shape[0])).any(1), reduction)
+    loss, saved = _LinearDistillFn.apply(x, w, idx, val, float(tau), offset, float(scale))
+    return _reduced(loss, saved[:, 0] != math.inf, reduction)  # (the forward's mark of a row that takes no part)
 
 
 def topk_distillation(logits, idx, val, tau=1.0, reduction="mean"):
     """Distillation of logits [P, V] or [P, G, V] in memory from a teacher's top k, differentiable in the logits, which the backward reads again. See
     ops.topk_distill."""
     ahead = logits.dtype == torch.float32 and logits.numel() <= _AHEAD and logits.requires_grad and torch.is_grad_enabled()
-    loss = _TopkDistillFn.apply(logits, idx, val, float(tau), ahead)
-    return _reduced(loss, ((idx >= 0) & (idx < logits.shape[-1])).any(-1), reduction)
+    part = torch.empty(logits.shape[:-1], dtype=torch.bool, device=logits.device) if reduction == "mean" else None
+    loss = _TopkDistillFn.apply(logits, idx, val, float(tau), ahead, part)
+    return _reduced(loss, part, reduction)
 
 
 class HeadDistillation:

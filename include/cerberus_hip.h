@@ -518,7 +518,8 @@ int cdet_linear_distill_bwd(const cdet_linear_loss_desc* d, const void* x, const
 /* linear_distill's loss on logits that are in memory, loss AND gradient in one call (like cdet_det_loss): P pixels (rows) of G distributions of V
  * logits each -- the class logits of a head map (G = 1), its four 16-bin box distributions (G = 4, V = 16). Distribution g of pixel p starts at
  * logits + (p * ld + g * V) elements (pass the pointer of the first channel); its gradient, d(sum_r drow_r loss_r) / d logit * grad_scale, at
- * dlogits + (p * grad_ld + g * V). idx / val [P * G, k], drow [P * G] or NULL (ones), loss [P * G]. Everything else in a pixel's pitch is left as it is.
+ * dlogits + (p * grad_ld + g * V). idx / val [P * G, k], drow [P * G] or NULL (ones), loss [P * G]. Everything else in a pixel's pitch is left as it is. A row takes part if it has
+ * a filled slot that is not -inf and a logit that is not.
  * logits: fp32 / bf16 / fp16, any alignment of whole elements; -inf = a class left out. NaN in a row that takes part, in its logits or in a filled slot,
  * gives a loss of NaN. dlogits may be NULL (loss only) and may BE logits (same type
  * and pitch). */
@@ -527,6 +528,7 @@ typedef struct {
     int32_t dtype, val_dtype, grad_dtype;
     int64_t ld, grad_ld;
     float tau, grad_scale;
+    uint8_t* part;                 /* optional [P * G]: 1 where the row takes part, else 0           */
 } cdet_topk_distill_desc;
 int cdet_topk_distill(const cdet_topk_distill_desc* d, const void* logits, const int32_t* idx, const void* val, const float* drow, float* loss, void* dlogits,
                       void* stream);

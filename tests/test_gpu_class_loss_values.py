@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_class_loss import BF, DEV, F16, F32, U, _ops, _rand, _randint, ce_case, check_map, check_rows, map_reference, teacher
+from test_gpu_class_loss import BF, DEV, F16, F32, U, _ops, _rand, _randint, ce_case, check_grads, check_map, check_rows, map_reference, reference, teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -208,3 +208,109 @@ def test_an_infinite_logit_beside_far_ones(N, V, dtype):
     x[:, 1] = 1.0
     loss, lse = _ops().linear_ce_fwd(x, w, torch.full((N,), 1, device=DEV), offset=off, scale=1e38)
     assert lse.isnan().all() and loss.isnan().all()
+
+
+def test_means_over_the_rows_that_take_part():
+    """reduction="mean" divides by the rows that the kernels count: not by those whose filled slots hold nothing but -inf, or that have no class left."""
+    from cerberusdet_amd.utils import loss as UL
+
+    x, w, labels = ce_case(20, 50, 16, BF, seed=380)
+    idx, val = distinct(20, 50, 4, 381)
+    val[3] = -math.inf
+    val[5, 1:] = -math.inf
+    idx[7] = -1
+    idx[9, :2] = -2
+    val[9, 2:] = -math.inf
+    part = torch.ones(20, dtype=torch.bool, device=DEV)
+    part[[3, 7, 9]] = False
+    xl = x.clone().requires_grad_()
+    mean = UL.linear_distillation(xl, w, idx, val, tau=2.0)
+    rows = UL.linear_distillation(x, w, idx, val, tau=2.0, reduction="none")
+    assert torch.allclose(mean, rows[part].sum() / 17, rtol=1e-6) and torch.all(rows[~part] == 0)
+    mean.backward()
+    m = torch.full((1,), 1 / 17, device=DEV)
+    check_grads(xl.grad, None, reference(x, w, idx=idx, val=val, tau=2.0, drow=m), x, tau=2.0)
+    for z in (2 * _rand(20, 50, seed=382), 2 * _rand(20, 1000, seed=383), 2 * _rand(20, 3000, seed=384), 2 * _rand(20, 40000, seed=385), 2 * _rand(20, 80000, seed=386)):
+        z[11] = -math.inf
+        here = part.clone()
+        here[11] = False
+        val2 = val.clone()
+        val2[12] = math.nan  # NaN takes part
+        for v, n in ((val, 16), (val2, 16)):
+            leaf = z.clone().requires_grad_()
+            mean = UL.topk_distillation(leaf, idx, v, tau=2.0)
+            rows = UL.topk_distillation(z, idx, v, tau=2.0, reduction="none")
+            assert torch.all(rows[~here] == 0)
+            if v is val:
+                assert torch.allclose(mean, rows[here].sum() / n, rtol=1e-6)
+                mean.backward()
+                assert torch.allclose(leaf.grad * n, _ops().topk_distill(z, idx, v, tau=2.0)[1], rtol=1e-5, atol=1e-7)
+            else:
+                assert mean.isnan()
+    two = 2 * _rand(6, 4, 16, seed=387)
+    idx, val = teacher(24, 16, 3, 388)
+    two[2, 1] = -math.inf
+    idx, val = idx.view(6, 4, 3), val.view(6, 4, 3)
+    val[4, 2] = -math.inf
+    live = (((idx >= 0) & (idx < 16)) & (val > -math.inf)).any(-1)
+    live[2, 1] = False
+    rows = UL.topk_distillation(two, idx, val, reduction="none")
+    assert torch.allclose(UL.topk_distillation(two, idx, val), rows.sum() / live.sum(), rtol=1e-6)
+    none = UL.linear_cross_entropy(x, w, labels, offset=torch.full((50,), -math.inf, device=DEV))
+    assert none == 0
+
+
+@pytest.mark.parametrize("V", FORMS)
+def test_rows_that_take_part_are_told(V):
+    z = 2 * _rand(9, V, seed=395)
+    idx, val = distinct(9, V, 3, 396)
+    z[1] = -math.inf
+    z[2] = math.nan
+    idx[3] = -1
+    val[4] = -math.inf
+    val[5, 0] = math.nan
+    part = torch.zeros(10, dtype=torch.bool, device=DEV)
+    loss, _ = _ops().topk_distill(z, idx, val, part=part[:9], want_grad=False)
+    assert part.tolist() == [True, False, True, False, False, True, True, True, True, False]
+    for bad in (part, part[:9].int(), torch.zeros(18, dtype=torch.bool, device=DEV)[::2], torch.zeros(9, dtype=torch.bool)):
+        with pytest.raises(ValueError):
+            _ops().topk_distill(z, idx, val, part=bad)
+
+
+@pytest.mark.parametrize("N", [9000, 300000])
+def test_captured_means_of_many_rows(N):
+    """The means of as many rows as a library's sum takes several workgroups for, captured and replayed on new numbers with eager work in between."""
+    from cerberusdet_amd.utils import loss as UL
+
+    V, k = 40, 3
+    z, w, x = 2 * _rand(N, V, seed=400), _rand(V, 16, seed=401, dtype=BF), _rand(N, 16, seed=402, dtype=BF)
+    idx, val = teacher(N, V, k, 403)
+    labels = _randint(V, (N,), 404)
+
+    def step(x, w, z, labels, idx, val):
+        x, w, z = (t.detach().requires_grad_() for t in (x, w, z))
+        total = UL.linear_cross_entropy(x, w, labels) + UL.linear_distillation(x, w, idx, val) + UL.topk_distillation(z, idx, val, tau=2.0)
+        total = total + UL.topk_distillation(z, idx, val, reduction="sum") / N
+        return [total.detach(), *torch.autograd.grad(total, (x, w, z))]
+
+    data = (x, w, z, labels, idx, val)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*data)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(*data)
+    for turn in range(6):
+        x.copy_(_rand(N, 16, seed=410 + turn, dtype=BF))
+        z.copy_(_rand(N, V, seed=420 + turn))
+        labels.copy_(_randint(V + 9, (N,), 430 + turn) - 4)
+        graph.replay()
+        got = [o.clone() for o in outs]
+        want = step(*data)
+        _rand(N, 8, seed=440 + turn).sum()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), turn
