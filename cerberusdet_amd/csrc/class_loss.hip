@@ -41,6 +41,9 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 typedef const __attribute__((address_space(4))) uint32_t* mask_t;
 __device__ __forceinline__ mask_t as_mask(const uint32_t* p) { return (mask_t)(uintptr_t)p; }
 
+// a class's offset in log2 units; -inf leaves the class out, in every form: an offset of -inf, or a mask near fp32's lowest number
+__device__ __forceinline__ float class_offset(float off, float coff) { return off < -2.3e38f ? -INFINITY : off * coff; }
+
 template <int DT>
 __device__ __forceinline__ f32x16 lmfma(const u32x4& a, const u32x4& b, const f32x16& c) {
     if (DT == CDET_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -496,7 +499,7 @@ struct LogitArgs {
     const uint16_t* x;
     const uint16_t* w;
     int64_t x_ld, w_ld;
-    const float* off;     // [V] class offsets, or null; -inf leaves the class out
+    const float* off;     // [V] class offsets, or null (class_offset)
     float c, coff;        // z / tau in units of log2: acc * c + off * coff
     int N, V, d;          // V, w, off: of the piece in the backward
     int ntv, ntr;         // tiles
@@ -634,10 +637,9 @@ __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_logits_kernel(const 
         int v = v0, r;
         if (WALK && t != L) place(t, v, r);
         v += (int)threadIdx.x;
-        return v < a.V ? a.off[v] : -INFINITY;
+        return v < a.V ? class_offset(a.off[v], a.coff) : -INFINITY;
     };
     auto note = [&](float* dst, float o) {
-        o *= a.coff;
         dst[threadIdx.x] = o;
         const bool out = __ballot(o == -INFINITY) != 0;
         if (p.lane == 0) reinterpret_cast<int*>(dst + BM)[p.wave8] = out;
@@ -1002,6 +1004,7 @@ struct PrepArgs {
     float gain, spread;
     const float* gmax;          // null: find it
     const float* off;           // [V] or null
+    float coff;                 // as LogitArgs
     float *lse2, *coef, *outscale;
     uint32_t *live, *kept;
     const uint16_t* x;          // null: no copy
@@ -1051,7 +1054,7 @@ __global__ __launch_bounds__(1024) void class_prep_kernel(const PrepArgs a) {
         a.coef[r] = on ? g * down : 0.f;
     }
     for (int64_t v = t; v - (t & 63) < a.V; v += nt) {
-        const uint64_t bits = __ballot(v < a.V && (!a.off || a.off[v] != -INFINITY));
+        const uint64_t bits = __ballot(v < a.V && (!a.off || class_offset(a.off[v], a.coff) != -INFINITY));
         if ((t & 63) == 0) *reinterpret_cast<uint64_t*>(a.kept + (v >> 5)) = bits;
     }
     if (t == 0) *a.outscale = a.gain * m / (1.984375f * a.spread);
@@ -1161,7 +1164,7 @@ __global__ __launch_bounds__(512, RT * FT <= 2 ? 4 : 2) void class_few_kernel(co
             const int p = lane + 64 * i, v = b * 32 + p / (FT * 4), col = (wave * FT * 4 + p % (FT * 4)) * 8;
             wr[i] = v < a.V && col < a.d ? *reinterpret_cast<const u32x4*>(a.w + v * a.w_ld + col) : u32x4{0, 0, 0, 0};
         }
-        if (tid < 32) on = b * 32 + tid >= a.V ? -INFINITY : a.off ? a.off[b * 32 + tid] : 0.f;
+        if (tid < 32) on = b * 32 + tid >= a.V ? -INFINITY : a.off ? class_offset(a.off[b * 32 + tid], a.coff) : 0.f;
     };
     fetch(ch);
     int sv[kFewSlots];
@@ -1259,7 +1262,7 @@ __global__ __launch_bounds__(512, RT * FT <= 2 ? 4 : 2) void class_few_kernel(co
             const float2 s = sums[t];
             const int r = t * 32 + r31, at = labs[r] - ch * 32 - 2 * cp;
             const float l2 = l2s[r], g = gs[r] * down, mag = fabsf(g), l2g = l2 - __builtin_amdgcn_logf(mag);
-            float d0 = __builtin_amdgcn_exp2f(fmaf(s.x, a.c, o.x * a.coff) - l2g), d1 = __builtin_amdgcn_exp2f(fmaf(s.y, a.c, o.y * a.coff) - l2g);
+            float d0 = __builtin_amdgcn_exp2f(fmaf(s.x, a.c, o.x) - l2g), d1 = __builtin_amdgcn_exp2f(fmaf(s.y, a.c, o.y) - l2g);
             d0 -= at == 0 ? mag : 0.f;
             d1 -= at == 1 ? mag : 0.f;
             d0 = o.x == -INFINITY || l2 == INFINITY ? 0.f : g < 0.f ? -d0 : d0;
@@ -1482,8 +1485,8 @@ __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, i
         const int v = some ? s_idx[j] : -1;
         float z2 = -INFINITY;
         if (v >= 0) {
-            const float ov = off ? off[v] : 0.f;
-            z2 = ov == -INFINITY ? -INFINITY : fmaf(s_z[j], c, ov * coff);
+            const float ov = off ? class_offset(off[v], coff) : 0.f;
+            z2 = ov == -INFINITY ? -INFINITY : fmaf(s_z[j], c, ov);
             const float lq = s_t[j] - m - ls, q = expf(lq);
             if (q != 0.f) sum += q * (lq - (z2 - l2) * kLn2);
             s_q[j] = q;
@@ -1852,6 +1855,7 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
     pa.gain = q->scale * (idx ? q->tau : 1.f);
     pa.spread = spread;
     pa.off = q->offset;
+    pa.coff = kLog2e / q->tau;
     pa.lse2 = lse2;
     pa.coef = coef;
     pa.outscale = os;

@@ -488,8 +488,8 @@ int cdet_det_loss(const cdet_loss_desc* d, const void* f0, const void* f1, const
  *   dx = scale * dz w, dw = scale * dz^T x
  * x [N, d] and w [V, d]: bf16 / fp16, unit stride along d, row pitches in elements (multiples of 8; 0 repeats one row), 16-byte aligned, d % 8 == 0.
  * Sums, softmax statistics and losses are fp32; dz is rounded to the 16-bit type once before it is multiplied with w and x.
- *   offset  optional [V] fp32 (class priors); -inf leaves a class out, whatever its weights hold: p = 0, dw = 0. The
- *           offset itself has no gradient.
+ *   offset  optional [V] fp32 (class priors); -inf leaves a class out, whatever its weights hold: p = 0, dw = 0. So does a mask below -2.3e38 (fp32's
+ *           lowest number). The offset itself has no gradient.
  *   labels  [N] int64 / int32; outside of 0 .. V-1 (-100, say): the row takes no part -- loss 0, gradient 0, whatever the row of x holds. A row
  *           whose classes are all left out takes no part either; a label that is left out beside others that are not has loss +inf.
  *   idx     [N, k] int32 classes of the teacher's largest logits, val [N, k] their values; outside of 0 .. V-1: an empty slot. A class may be named

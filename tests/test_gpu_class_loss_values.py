@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_class_loss import BF, DEV, F16, F32, U, _ops, _rand, _randint, ce_case, check_grads, check_map, check_rows, map_reference, reference, teacher
+from test_gpu_class_loss import BF, DEV, F16, F32, U, _ops, _rand, _randint, ce_case, check_grads, check_map, check_rows, map_reference, reference, run_ce, teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -314,3 +314,34 @@ def test_captured_means_of_many_rows(N):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b), turn
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("N,V,d", [(5, 70, 16), (100, 700, 64), (140, 2000, 64), (2600, 3900, 40)])
+def test_offsets_of_the_lowest_value_leave_out(N, V, d, dtype):
+    """A class masked with fp32's lowest number is left out like one of -inf, in every form: the same bits, whatever its weights hold."""
+    ops = _ops()
+    x, w, labels = ce_case(N, V, d, dtype, seed=390)
+    idx, val = distinct(N, V, 6, 391)
+    out = torch.zeros(V, dtype=torch.bool, device=DEV)
+    out[::9] = True
+    labels[1:] = torch.where(out[labels[1:]], -100, labels[1:])
+    labels[0] = 9  # a left-out class beside others: loss +inf, the gradient reaches the others only
+    idx[2:] = torch.where(out[idx[2:].long()], -1, idx[2:])
+    idx[1, 0] = 18
+    wb = w.clone()
+    wb[out] = math.nan
+    base = 0.1 * _rand(V, seed=392)
+    got = []
+    for low in (-math.inf, torch.finfo(F32).min, -3e38):
+        off = torch.where(out, low, base)
+        got.append(list(run_ce(x, wb, labels, offset=off)))
+        for tau in (4.0, 0.5):
+            kd, saved = ops.linear_distill_fwd(x, wb, idx, val, tau=tau, offset=off)
+            got[-1] += [kd, *ops.linear_distill_bwd(x, wb, idx, saved, tau=tau, offset=off)]
+    assert got[0][0][0] == math.inf and got[0][4][1] == math.inf and got[0][2].isfinite().all() and torch.all(got[0][3][out] == 0)
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert torch.equal(a, b)
+    loss, lse, dx, dw = run_ce(x, w, labels, offset=torch.full((V,), torch.finfo(F32).min, device=DEV))
+    assert torch.all(loss == 0) and torch.all(dx == 0) and torch.all(dw == 0)
