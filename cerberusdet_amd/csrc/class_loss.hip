@@ -1668,7 +1668,8 @@ static int lin_check(const cdet_linear_loss_desc* q, const char* who) {
     CDET_CHECK_ARG(q->d >= 8 && q->d % 8 == 0 && q->d <= 65536, "%s: d = %d must be a multiple of 8 in 8 .. 65536", who, q->d);
     CDET_CHECK_ARG(q->x_ld >= 0 && q->x_ld % 8 == 0 && q->x_ld < (1 << 22) && q->w_ld >= 0 && q->w_ld % 8 == 0 && q->w_ld < (1 << 22),
                    "%s: row pitches %lld, %lld must be multiples of 8 elements below 2^22", who, (long long)q->x_ld, (long long)q->w_ld);
-    CDET_CHECK_ARG(q->tau > 0.f && q->tau < INFINITY && q->scale == q->scale && q->scale - q->scale == 0.f, "%s: tau %g must be positive, scale %g finite", who, q->tau, q->scale);
+    // (scale / tau and 1 / tau in log2 units, and tau^2, are fp32 numbers)
+    CDET_CHECK_ARG(q->tau >= 1e-18f && q->tau <= 1e18f && fabsf(q->scale / q->tau) <= 1e38f, "%s: tau %g (1e-18 .. 1e18) or scale %g (at most 1e38 tau)", who, q->tau, q->scale);
     return 0;
 }
 static inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }

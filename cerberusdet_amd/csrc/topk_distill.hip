@@ -782,7 +782,7 @@ extern "C" int cdet_topk_distill(const cdet_topk_distill_desc* d, const void* lo
     CDET_CHECK_ARG(d->P >= 0 && d->G >= 1 && d->V >= 1 && d->V <= (1 << 24) && (int64_t)d->P * d->G < ((int64_t)1 << 31), "cdet_topk_distill: P %d, G %d, V %d", d->P,
                    d->G, d->V);
     CDET_CHECK_ARG(d->k >= 1 && d->k <= 512, "cdet_topk_distill: k = %d (1 .. 512)", d->k);
-    CDET_CHECK_ARG(d->tau > 0.f && d->tau < INFINITY, "cdet_topk_distill: tau %g must be positive", d->tau);
+    CDET_CHECK_ARG(d->tau >= 1e-18f && d->tau <= 1e18f, "cdet_topk_distill: tau %g (1e-18 .. 1e18)", d->tau);  // (1 / tau and tau^2 are fp32 numbers)
     CDET_CHECK_ARG(d->ld >= 0, "cdet_topk_distill: negative pitch");
     if (d->P == 0) return 0;
     CDET_CHECK_ARG(logits && idx && val && loss, "cdet_topk_distill: logits, idx, val and loss must be given");

@@ -389,7 +389,6 @@ def det_loss(feats, gt, nc, gains, strides, grad_scale=1.0, grad_dtype=None, wan
 # ---------------------------------------------------------------------------------------------------------------
 # Losses over a long class list (csrc/class_loss.hip, csrc/topk_distill.hip). Bad arguments raise ValueError before anything is launched. The messages are
 # put together only when they are raised: for a single row these calls are as long as what the host does around the launch.
-_INF = float("inf")
 
 
 def _bad(msg):
@@ -448,8 +447,8 @@ def _linear_loss_desc(x, w, offset, scale, tau, label64=0):
     if not 1 <= V <= 1 << 24 or N > 1 << 24:
         _bad(f"1 .. 2^24 classes and at most 2^24 rows, got {V} and {N}")
     scale, tau = float(scale), float(tau)
-    if not 0.0 < tau < _INF or not abs(scale) < _INF:
-        _bad(f"tau = {tau} must be positive, scale = {scale} finite")
+    if not 1e-18 <= tau <= 1e18 or not abs(scale / tau) <= 1e38:
+        _bad(f"tau = {tau} must be in 1e-18 .. 1e18, scale = {scale} at most 1e38 tau")
     if offset is not None:
         _on(gpu, "offset", offset)
         if offset.shape != (V,) or offset.dtype != torch.float32:
@@ -598,8 +597,8 @@ def topk_distill(logits, idx, val, tau=1.0, drow=None, grad_scale=1.0, grad_dtyp
     rows = shape[:-1]
     idx, val = _teacher(idx, val, rows, gpu)
     tau = float(tau)
-    if not 0.0 < tau < _INF:
-        _bad(f"tau = {tau} must be positive")
+    if not 1e-18 <= tau <= 1e18:
+        _bad(f"tau = {tau} must be in 1e-18 .. 1e18")
     grad_dtype = grad_dtype or (logits.dtype if out is None else out.dtype)
     if grad_dtype is not logits.dtype and grad_dtype is not torch.float32:
         _bad(f"grad_dtype must be {logits.dtype} or fp32")
