@@ -1399,7 +1399,8 @@ __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, i
     __shared__ __attribute__((aligned(16))) int s_idx[512];
     __shared__ __attribute__((aligned(16))) float s_t[512], s_q[512];
     __shared__ float s_z[512], s_sum[4];
-    const int t = (int)threadIdx.x, lane = t & 63, wv = t >> 6, r = (int)blockIdx.x;
+    const int t = (int)threadIdx.x, lane = t & 63, wv = t >> 6, r = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+    if (r >= N) return;
     const int sub = t / LS, l = t & (LS - 1);
     float* sv = saved + (int64_t)r * (1 + 2 * k);
     const int32_t* ir = idx + (int64_t)r * k;
@@ -1521,14 +1522,14 @@ __global__ __launch_bounds__(256) void class_teacher_kernel(const uint16_t* x, i
 template <int DT>
 __global__ __launch_bounds__(256) void class_teacher_dz_kernel(const int32_t* idx, const float* saved, const float* lse2, const float* coef, int k, int N, int v_first,
                                                                int Vp, uint16_t* dz, int64_t dz_ld) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)N * k) return;
-    const int v = idx[i];
-    if (v < v_first || v - v_first >= Vp) return;
-    const int r = (int)(i / k), j = (int)(i - (int64_t)r * k);
-    TeacherDz t;
-    t.load(saved, lse2, coef, k, r, j);
-    t.store<DT>(dz + r * dz_ld + (v - v_first));
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)N * k; i += (int64_t)gridDim.x * 256) {
+        const int v = idx[i];
+        if (v < v_first || v - v_first >= Vp) continue;
+        const int r = (int)(i / k), j = (int)(i - (int64_t)r * k);
+        TeacherDz t;
+        t.load(saved, lse2, coef, k, r, j);
+        t.store<DT>(dz + r * dz_ld + (v - v_first));
+    }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------------------------------
@@ -1927,7 +1928,7 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         int rc = launch_logits<true>(a, q->dtype, p.big_f, s);
         if (rc) return rc;
         if (idx && apart) {
-            const unsigned nb = (unsigned)div_up((int64_t)N * k, 256);
+            const unsigned nb = (unsigned)std::min<int64_t>(div_up((int64_t)N * k, 256), 1 << 18);
             if (q->dtype == CDET_BF16) class_teacher_dz_kernel<CDET_BF16><<<dim3(nb), dim3(256), 0, s>>>(idx, saved, lse2, coef, k, N, v0, Vp, a.dz, a.dz_ld);
             else class_teacher_dz_kernel<CDET_F16><<<dim3(nb), dim3(256), 0, s>>>(idx, saved, lse2, coef, k, N, v0, Vp, a.dz, a.dz_ld);
             CDET_LAUNCH_CHECK();
@@ -2028,7 +2029,7 @@ extern "C" int cdet_linear_distill_fwd(const cdet_linear_loss_desc* d, const voi
     const float* part = few ? (const float*)((char*)ws + p.o_part) : nullptr;
     const int rc = lin_forward(d, p, x, w, nullptr, nullptr, lse, (char*)ws, (hipStream_t)stream);
     if (rc) return rc;
-    const dim3 nb((unsigned)d->N), nt(256);
+    const dim3 nb((unsigned)std::min(d->N, 1 << 20), (unsigned)div_up(d->N, 1 << 20)), nt(256);  // (a grid's row holds less than 2^32 threads)
     const LogitArgs a = logit_args(d);
 #define CDET_GO(DT_, LS_)                                                                                                                                   \
     class_teacher_kernel<DT_, LS_><<<nb, nt, 0, (hipStream_t)stream>>>((const uint16_t*)x, d->x_ld, (const uint16_t*)w, d->w_ld, d->offset, a.c, a.coff, idx, val, val_dtype, \

@@ -22,7 +22,7 @@ struct TdArgs {
     float* loss;
     uint8_t* part;  // null, or 1 where the row takes part
     int64_t ld, gld;
-    int64_t rows;
+    int64_t rows, row0;  // row0: the launch's first
     int G, V, k, vdt;
     float c, itau, tau2, gs;  // log2(e) / tau, 1 / tau, tau^2, grad_scale * tau
 };
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
     constexpr int CH = 16 / sizeof(T), NCH = PER / CH;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int t = (int)threadIdx.x & 63, V = a.V, k = a.k;
-    const int64_t row = (int64_t)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
+    const int64_t row = a.row0 + (int64_t)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
     if (row >= a.rows) return;  // (whole waves, and no barrier of the workgroup follows)
     float* const base = lds + ((int)threadIdx.x >> 6) * (td_wave_lds<T>(k, V) / 4);
     float *const sq = base, *const slq = base + k + 1, *const sz = slq + k;  // (sq[k] = 0: what a class takes that no slot names)
@@ -377,7 +377,7 @@ __global__ __launch_bounds__(NW * 64, NW == 16 ? 8 : 1) void td_wide_kernel(cons
     extern __shared__ __attribute__((aligned(16))) float lds[];
     __shared__ float scratch[16];
     const int t = (int)threadIdx.x, V = a.V;
-    const int64_t row = blockIdx.x;
+    const int64_t row = a.row0 + blockIdx.x;
     const TdSlots slots(lds, a.k);
     const T* z;
     TG* dz;
@@ -455,7 +455,7 @@ __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const T
     extern __shared__ __attribute__((aligned(16))) float lds[];
     __shared__ float scratch[16];
     const int t = (int)threadIdx.x, V = a.V;
-    const int64_t row = blockIdx.x;
+    const int64_t row = a.row0 + blockIdx.x;
     const TdSlots slots(lds, a.k);
     const T* z;
     TG* dz;
@@ -543,7 +543,7 @@ __global__ __launch_bounds__(1024) void td_long_kernel(const TdArgs a) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
     __shared__ float scratch[16];
     const int t = (int)threadIdx.x, V = a.V;
-    const int64_t row = blockIdx.x;
+    const int64_t row = a.row0 + blockIdx.x;
     const TdSlots slots(lds, a.k);
     const T* z;
     TG* dz;
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(256) void td_narrow_kernel(const TdArgs a) {
     __shared__ __attribute__((aligned(16))) float s_z[ROWS][W];  // below the maximum
     __shared__ __attribute__((aligned(16))) float s_q[ROWS][2 * W];
     const int lane = (int)threadIdx.x & 63, l = (int)threadIdx.x & (L - 1), r = (int)threadIdx.x / L, V = a.V, k = a.k;
-    const int64_t row = (int64_t)blockIdx.x * ROWS + r;
+    const int64_t row = a.row0 + (int64_t)blockIdx.x * ROWS + r;
     const bool here = row < a.rows;
     const T* z;
     TG* dz;
@@ -736,11 +736,11 @@ __global__ __launch_bounds__(256) void td_narrow_kernel(const TdArgs a) {
 }
 
 template <int DT, int GDT>
-static int td_launch(const TdArgs& a, hipStream_t s) {
+static int td_launch_rows(const TdArgs& a, int64_t rows, hipStream_t s) {
     const size_t lds = (size_t)TdSlots::up(a.k) * 16;
 #define CDET_NARROW(L, E)                                                                                          \
     do {                                                                                                           \
-        const dim3 grid((unsigned)((a.rows + 256 / L - 1) / (256 / L)));                                           \
+        const dim3 grid((unsigned)((rows + 256 / L - 1) / (256 / L)));                                           \
         if (a.k <= L) td_narrow_kernel<DT, GDT, L, E, 1><<<grid, dim3(256), 0, s>>>(a);                            \
         else td_narrow_kernel<DT, GDT, L, E, E><<<grid, dim3(256), 0, s>>>(a);                                     \
     } while (0)
@@ -752,20 +752,31 @@ static int td_launch(const TdArgs& a, hipStream_t s) {
     else if (narrow <= 128) CDET_NARROW(16, 8);
 #undef CDET_NARROW
     else if (a.V <= 2048) {
-        const dim3 grid((unsigned)((a.rows + 3) / 4));
+        const dim3 grid((unsigned)((rows + 3) / 4));
         const size_t row = td_wave_lds<typename TdElem<DT>::T>(a.k, a.V);
         if (a.V <= 512) td_wave_kernel<DT, GDT, 8><<<grid, dim3(256), 4 * row, s>>>(a);
         else if (a.V <= 1024) td_wave_kernel<DT, GDT, 16><<<grid, dim3(256), 4 * row, s>>>(a);
         else td_wave_kernel<DT, GDT, 32><<<grid, dim3(256), 4 * row, s>>>(a);
     }
-    else if (a.V <= 4096) td_wide_kernel<DT, GDT, 2><<<dim3((unsigned)a.rows), dim3(128), lds, s>>>(a);
-    else if (a.V <= 8192) td_wide_kernel<DT, GDT, 4><<<dim3((unsigned)a.rows), dim3(256), lds, s>>>(a);
-    else if (a.V <= 16384) td_wide_kernel<DT, GDT, 8><<<dim3((unsigned)a.rows), dim3(512), lds, s>>>(a);
-    else if (a.V <= 32768) td_wide_kernel<DT, GDT, 16><<<dim3((unsigned)a.rows), dim3(1024), lds, s>>>(a);
-    else if (DT != CDET_F32 && a.V <= 65536) td_held_kernel<DT, GDT, 8><<<dim3((unsigned)a.rows), dim3(1024), lds, s>>>(a);
-    else if (a.V <= (DT == CDET_F32 ? 65536 : 131072)) td_held_kernel<DT, GDT, 16><<<dim3((unsigned)a.rows), dim3(1024), lds, s>>>(a);
-    else td_long_kernel<DT, GDT><<<dim3((unsigned)a.rows), dim3(1024), lds, s>>>(a);
+    else if (a.V <= 4096) td_wide_kernel<DT, GDT, 2><<<dim3((unsigned)rows), dim3(128), lds, s>>>(a);
+    else if (a.V <= 8192) td_wide_kernel<DT, GDT, 4><<<dim3((unsigned)rows), dim3(256), lds, s>>>(a);
+    else if (a.V <= 16384) td_wide_kernel<DT, GDT, 8><<<dim3((unsigned)rows), dim3(512), lds, s>>>(a);
+    else if (a.V <= 32768) td_wide_kernel<DT, GDT, 16><<<dim3((unsigned)rows), dim3(1024), lds, s>>>(a);
+    else if (DT != CDET_F32 && a.V <= 65536) td_held_kernel<DT, GDT, 8><<<dim3((unsigned)rows), dim3(1024), lds, s>>>(a);
+    else if (a.V <= (DT == CDET_F32 ? 65536 : 131072)) td_held_kernel<DT, GDT, 16><<<dim3((unsigned)rows), dim3(1024), lds, s>>>(a);
+    else td_long_kernel<DT, GDT><<<dim3((unsigned)rows), dim3(1024), lds, s>>>(a);
     CDET_LAUNCH_CHECK();
+    return 0;
+}
+
+// (a launch of at most 2^31 threads)
+template <int DT, int GDT>
+static int td_launch(TdArgs a, hipStream_t s) {
+    const int64_t most = a.V > 2048 ? 1 << 21 : 1 << 25;
+    for (a.row0 = 0; a.row0 < a.rows; a.row0 += most) {
+        const int rc = td_launch_rows<DT, GDT>(a, a.rows - a.row0 < most ? a.rows - a.row0 : most, s);
+        if (rc) return rc;
+    }
     return 0;
 }
 

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_class_loss import BF, DEV, F16, F32, U, _ops, _rand, _randint, ce_case, check_grads, check_map, check_rows, map_reference, reference, run_ce, teacher
+from test_gpu_class_loss import BF, DEV, F16, F32, U, _ops, _rand, _randint, ce_case, check_grads, check_map, check_rows, loss_tol, map_reference, reference, run_ce, teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -345,3 +345,37 @@ def test_offsets_of_the_lowest_value_leave_out(N, V, d, dtype):
             assert torch.equal(a, b)
     loss, lse, dx, dw = run_ce(x, w, labels, offset=torch.full((V,), torch.finfo(F32).min, device=DEV))
     assert torch.all(loss == 0) and torch.all(dx == 0) and torch.all(dw == 0)
+
+
+# more rows than one launch of each form takes, and than a grid holds threads for
+@pytest.mark.parametrize("P,V,dtype", [((1 << 28) + 3, 60, F32), ((1 << 26) + 1, 130, BF), ((1 << 22) + 1, 16400, BF), ((1 << 21) + 7, 70001, BF)])
+def test_topk_distill_of_the_most_rows(P, V, dtype):
+    """Rows that repeat one pattern (the logits by stride 0): every row's loss is its first occurrence's, to the bit."""
+    z = (2 * _rand(1, V, seed=450)).to(dtype)
+    idx = torch.arange(P, dtype=torch.int32, device=DEV).remainder_(4)[:, None]
+    val = torch.zeros(P, 1, device=DEV)
+    loss, _ = _ops().topk_distill(z.expand(P, V), idx, val, want_grad=False)
+    wl = -torch.log_softmax(z[0].double(), 0)[:4]
+    assert torch.all((loss[:4].double() - wl).abs() <= 2 * U * (4 * (math.log(V) + 1) + V / 1024 + 64 + 8 * wl))
+    whole = P // 4 * 4
+    assert torch.all(loss[:whole].view(-1, 4) == loss[:4]) and torch.equal(loss[whole:], loss[:P - whole])
+
+
+def test_linear_distill_of_the_most_rows():
+    """2^24 rows (one x by stride 0) of 17 slots: every row the same loss and dx; dw their sum."""
+    ops = _ops()
+    N, V, d, k = 1 << 24, 16, 8, 17
+    x, w, _ = ce_case(1, V, d, BF, seed=460)
+    idx, val = teacher(1, V, k, 461, empty=False)
+    loss, saved = ops.linear_distill_fwd(x.expand(N, d), w, idx.expand(N, k), val.expand(N, k))
+    assert torch.all(loss == loss[0]) and torch.all(saved[:, 0] == saved[0, 0])
+    ref = reference(x, w, idx=idx, val=val)
+    check_rows(loss[:1], ref["loss"], 2 * loss_tol(ref, d) + 64 * U * 16)
+    dx, dw = ops.linear_distill_bwd(x.expand(N, d), w, idx.expand(N, k), saved, torch.full((1,), 2.0 ** -24, device=DEV))
+    assert torch.all(dx == dx[0])
+    one = torch.full((1,), 2.0 ** -24, device=DEV)
+    check_grads(dx[:1], None, reference(x, w, idx=idx, val=val, drow=one), x)
+    # 2^24 equal terms: at most 2^24 u = 1 of the sum in a chain, but the tiles' chains are shorter than 2^24 / 64 = 2^18: 2^-6, and dz's and dw's roundings
+    want = reference(x, w, idx=idx, val=val)["dw"]
+    mag = reference(x, w, idx=idx, val=val)["dz"].abs().T @ x.double().abs()
+    assert torch.all((dw.double() - want).abs() <= mag * (2.0 ** -6 + 2.0 ** -7) + 2.0 ** -8 * want.abs())
