@@ -132,6 +132,7 @@ def train(hyp, opt, device, train_dataset=None, val_dataset=None):
     from cerberusdet_amd import val as validate
     from cerberusdet_amd.models import CerberusDet
     from cerberusdet_amd.trainers import Averaging
+    from cerberusdet_amd.trainers.averaging import on_group
 
     tasks = opt.tasks.split(",")
     data_nc = [int(v) for v in opt.nc.split(",")]  # classes in the label files
@@ -182,7 +183,7 @@ def train(hyp, opt, device, train_dataset=None, val_dataset=None):
         reduce_precision_like_reference(model)
     if WORLD_SIZE > 1:
         for t in list(model.state_dict().values()):  # what DDP's constructor does in the reference (train.py:182-184)
-            dist.broadcast(t, src=0)
+            on_group(dist.broadcast, t, src=0)
         model.mark_weights_changed()
     iters = {t: iter(d) for t, d in train_dataset.items()}
     # --skip-batches (reference trainers/averaging.py:50-54,144-146): a task with a shorter dataset is visited every
@@ -273,7 +274,7 @@ def train(hyp, opt, device, train_dataset=None, val_dataset=None):
                     save_training_checkpoint(wdir / "best.pt", model, trainer, epoch, best_fitness, best_fitness_per_task, stopper.best_epoch)
         if WORLD_SIZE > 1:  # every rank leaves the loop together (reference train.py:251-257 broadcasts the stop flag)
             flag = torch.tensor([int(stop)], device=device)
-            dist.broadcast(flag, src=0)
+            on_group(dist.broadcast, flag, src=0)
             stop = bool(flag.item())
         if stop:
             if RANK in (-1, 0):
