@@ -1543,7 +1543,8 @@ static inline bool big_tiles(int64_t rows, int64_t cols) { return rows > 128 && 
 // two; a tile 6 (8, 5) steps more than its K / 32 (the large one 12 where the two are compared: the estimate is short where
 // its tiles are short); a launch is as long as the busiest of an XCD's 32 CUs (64 places), the longer kind of tile first, and 4
 // more; slabs of slices move at 4 MB/us.
-// dz of a piece stays within 192 MiB, so that it lives in the 256 MiB cache between its three uses.
+// dz of a piece stays within 192 MiB, so that it lives in the 256 MiB cache between its three uses -- up to 49152 rows: a piece has at least 2048 classes
+// (as far as there are that many), so beyond that dz takes 4 KiB a row and goes through memory, which the estimate does not price.
 // 4096 x 65536 x 640: 4 pieces of 4 slices, by equal lengths, took 4 x 219 us for the products, 3 pieces of 5 take 3 x 242. 8400 x 1203 x 1024: dw on 20
 // tiles of 8400 rows took 200 us of backward, in 6 slices of the rows 104.
 struct GradShape {

@@ -23,3 +23,13 @@ def test_what_leaves_fp32_with_tau_or_scale_is_refused(tau, scale):
         assert lib.cdet_topk_distill(C.byref(_tdesc(tau=tau)), P, P, P, P, P, 2 * P, None) == -1001
         with pytest.raises(ValueError, match="GPU|tau"):
             ops.topk_distill(torch.zeros(4, 10), torch.zeros(4, 3, dtype=torch.int32), torch.zeros(4, 3), tau=tau)
+
+
+@pytest.mark.parametrize("N", [200, 8192, 49152, 49153, 268800, 1 << 20, 1 << 24])
+def test_workspace_of_many_rows(N):
+    """dz of a piece: 192 MiB, or 4 KiB a row where 2048 classes take more; beside it (d = 8) less than 64 bytes a row and 8 MiB."""
+    lib = L.load()
+    for V in (300, 2048, 4500, 131072, 1 << 24):
+        size = lib.cdet_linear_loss_ws_bytes(C.byref(_desc(N=N, V=V, d=8, x_ld=8, w_ld=8)), 1)
+        rows = (N + 31) // 32 * 32
+        assert 0 < size <= min(max(192 << 20, 4096 * rows), rows * 2 * ((V + 255) // 256 * 256)) + 64 * N + (8 << 20)
