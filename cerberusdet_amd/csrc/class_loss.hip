@@ -166,7 +166,8 @@ struct Pipe {
         __builtin_amdgcn_sched_barrier(0);
     }
     __device__ __forceinline__ u32x4 frag_n(int base, int t, int kk) const { return *reinterpret_cast<const u32x4*>(smem + ((base + t * 2048) ^ (kk << 5))); }
-    // transpose reads are asm: in front of the builtin the compiler waits for every DMA in flight. Their registers become values behind the phase's own wait
+    // transpose reads are asm: in front of the builtin the compiler waits for every DMA in flight. Their registers become values behind the phase's own wait;
+    // that the compiler moves none of them before it is checked in the build's assembly (tests/test_class_loss_registers_cpu.py)
     __device__ __forceinline__ void frag_t(int base, int t, int kk, u32x2& lo, u32x2& hi) const {
         const int o = (int)(unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem + (((base + (t >> 1) * 4096) ^ ((t & 1) << 6)) + kk * 2048);
         asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(lo) : "v"(o));
