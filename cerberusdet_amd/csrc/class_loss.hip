@@ -7,7 +7,9 @@
 // Forward: one matrix product whose epilogue keeps, per row and per 128 (64) classes, the running maximum and the sum of exponentials; a second launch
 // joins those pairs per row in a fixed order. Backward: per piece of the class list the product is computed again, its epilogue turns the logits
 // into dz (16-bit, one [N, piece] buffer), and one launch computes the piece's dw and adds the piece to dx. dz is relative to the largest row gradient
-// (class_prep_kernel): p of a 10^5-class list times 1 / N is far below fp16's smallest number.
+// (class_prep_kernel): p of a 10^5-class list times 1 / N is far below fp16's smallest number. That rounding is the price of multiplying dz on the matrix
+// cores once: relative to 64 bits dx and dw are off by 0.0018 - 0.0024 (bf16) and 0.00026 - 0.00029 (fp16), by 0.0017 and 0.00021 with dz in fp32, whose rounding
+// of the results alone remains; dz as two 16-bit numbers would double both gradient products, half of a training pass (up to 64 rows they are not what counts).
 //
 // One product for all three (Pipe): an 8-wave workgroup, 256 x 256 outputs, K in steps of 32 through a ring of four LDS stages filled by LDS-DMA. The two
 // halves of the workgroup run half a step apart: while one multiplies, the other reads its fragments. What bounds it is the chip's power: 4096 x 4096 x 8192
@@ -839,6 +841,7 @@ struct GradArgs {
     const float* outscale;
 };
 
+// (The large tile has 256 registers a lane, and its two forms spill 2 and 5 of them where a tile is added to its slab.)
 // KEPT: classes can be left out, whose weights are not read (1021 x 32003 x 512: 2 us in the loop, a copy of w with zeros there 10; 494 x 63581 x 984 50)
 template <int DT, int MT, int NT, bool KEPT>
 __global__ __launch_bounds__(kLinThreads<MT>, 2) void class_grads_kernel(const GradArgs a) {
@@ -1102,8 +1105,8 @@ __global__ __launch_bounds__(256) void class_zero_kernel(uint16_t* p, int64_t ro
 //   do not: 128 x 131072 x 320 87 us with one, 110 with two);
 //   dw block = dz x, written out;  dx += dz w, in registers until the end: one fp32 slice a workgroup (class_few_sum_kernel adds them in their order).
 // A wave owns FT tiles of 32 features in the last two; RT tiles of 32 rows. Bound by memory for long lists, w in and dw out: backward of 1 x 131072 x 960
-// 109 us = 4.6 TB/s (by tiles of 128 x 128: 183), 32 x 131072 x 512 72 us (98), 128 x 131072 x 320 90 us (100); of short ones by a chain of waits: 96 x 365 x
-// 320 15 + 4 us of kernels (21). Two workgroups a CU where registers and LDS leave room: 16 x 131072 x 400 50 us, with one 59.
+// 104 us = 4.8 TB/s (by tiles of 128 x 128: 180), 32 x 131072 x 512 68 us (97), 128 x 131072 x 320 90 us (97); of short ones by a chain of waits: 96 x 365 x
+// 320 15 + 4 us of kernels (21). Two workgroups a CU where registers and LDS leave room: 16 x 131072 x 400 50 us, with one 59, by tiles 89.
 struct FewArgs {
     const uint16_t *x, *w;
     int64_t x_ld, w_ld;
@@ -1536,7 +1539,8 @@ __global__ __launch_bounds__(256) void class_teacher_dz_kernel(const int32_t* id
 // ---- host --------------------------------------------------------------------------------------------------------------------------------------------
 static inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 // 256 x 256 tiles read 131 FLOP per byte staged, 128 x 128 tiles half of that, so the large ones are taken wherever they fill most of the 256 CUs
-// (130 x 65536 x 1024 forward 34 us against 42) and the rows more than half of one (1 x 131072 x 1024: 50 against 43)
+// (forward with d = 320, large against small: 96 tiles 17.8 us and 13.7, 150 tiles 16.8 and 18.6, 256 tiles 19.1 and 23.0; d = 1024, 130 x 65536 36 and 43) and the
+// rows more than half of one (1 x 131072 x 1024: 51 and 44, 128 rows 65 and 61)
 static inline bool big_tiles(int64_t rows, int64_t cols) { return rows > 128 && (up(rows, 256) / 256) * (up(cols, 256) / 256) >= 160; }
 
 // The backward's shape: tile, pieces that the class list is cut into, and slices of a piece's classes for dx and of the rows for dw, whose tiles may be few
@@ -1611,6 +1615,8 @@ struct LinPlan {
     int64_t o_lse2, o_coef, o_scale, o_live, o_kept, o_x, o_dz, o_slab, o_wslab, bwd_bytes;
     int few, few_wgs;  // backward of few rows: 0, or row tiles of class_few_kernel; its workgroups (workspace: the scale, 256 bytes, and their slices)
 };
+// (backward by class_few_kernel and by tiles, V x d = 5000 x 320: 8 rows 11.5 and 23 us, 64 23.3 and 26.1, 96 25.9 and 26.1, 128 28.3 and 26.8; 50000 x 320: 24 and
+// 42, 46 and 48, 46.5 and 50.5, 51.3 and 53.3; 365 x 128, 128 rows: 13.4 and 16.4)
 static const int kFewRows = 128;
 static LinPlan lin_plan(const cdet_linear_loss_desc* q, bool backward) {
     LinPlan p = {};
@@ -1922,7 +1928,8 @@ static int lin_backward(const cdet_linear_loss_desc* q, const void* x, const voi
         a.dz = (uint16_t*)(ws + p.o_dz);
         a.dz_ld = p.g.piece;
         a.dz_rows = p.rows32;
-        // few slots are written by the tile's own workgroup (every tile reads its rows' slots: 1656 x 400 x 160 with k = 24 13.5 us against 7.4 and a launch of 3.1, with k = 128 36)
+        // few slots are written by the tile's own workgroup; every tile reads its rows' slots (backward of 997 x 1201 x 320, in the tile and apart: k = 4 26.2 us and
+        // 27.8, k = 8 26.7 and 27.6, k = 12 27.6 and 28.0, k = 16 28.7 and 28.3, k = 48 34.0 and 28.7; 200 x 1201 x 64, 1656 x 400 x 160, 500 x 5000 x 256 alike)
         const bool apart = p.big_f || k > 8;
         a.idx = apart ? nullptr : idx;
         a.saved = saved;
@@ -2036,6 +2043,7 @@ extern "C" int cdet_linear_distill_fwd(const cdet_linear_loss_desc* d, const voi
 #define CDET_GO(DT_, LS_)                                                                                                                                   \
     class_teacher_kernel<DT_, LS_><<<nb, nt, 0, (hipStream_t)stream>>>((const uint16_t*)x, d->x_ld, (const uint16_t*)w, d->w_ld, d->offset, a.c, a.coff, idx, val, val_dtype, \
                                                                  k, 1.f / d->tau, d->tau * d->tau, d->N, d->V, d->d, lse, part, p.nvb, loss, saved)
+    // (forward of 6000 x 4000, 64 lanes a slot and 16: d = 320, k = 16 49.1 us and 52.1, k = 24 54.7 and 52.9; d = 192, k = 16 42.5 and 43.1; d = 128, k = 16 39.3 and 37.8)
     const bool wide = k <= 16 && d->d > 128;
     if (d->dtype == CDET_BF16) {
         if (wide) CDET_GO(CDET_BF16, 64);

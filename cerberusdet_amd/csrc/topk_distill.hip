@@ -205,9 +205,9 @@ __device__ __forceinline__ void td_row(const TdArgs& a, int64_t row, const T*& z
 
 // V <= 2048: a wave a row, four rows a workgroup, the logits in registers (up to PER a lane) and, as they are stored, in LDS: the slots find theirs there, and
 // then leave their numbers (16 bits) there for the dense gradient to take their q along -- no gather from and no second write to memory (67200 x 1203 fp32,
-// k = 32 scattered classes: 123 us = 5.4 TB/s, with them 170). LDS of 32 bits an element leaves 16-bit rows half of the waves (67200 x 2048 bf16: 101 us =
+// k = 32 scattered classes: 122 us = 5.4 TB/s, with them 170). LDS of 32 bits an element leaves 16-bit rows half of the waves (67200 x 2048 bf16: 101 us =
 // 5.4 TB/s, so 144). What a row holds behind its last whole 16 bytes goes a logit a lane (67200 x 1203: as a partial chunk 134 us). PER = 32 for all
-// lengths: 67200 x 365 fp32 55 us, with 8 44. 16-bit rows of odd lengths pay for addresses off by 2 bytes: 67200 x 1203 bf16 85 us, x 1204 67.
+// lengths: 67200 x 365 bf16 54 us, with 8 51; x 700 65, with 16 63. Addresses off by 2 bytes cost little: 67200 x 1203 bf16 75 us, x 1204 74.
 __host__ __device__ constexpr int td_wave_slots(int k) { return (14 * k + 4 + 15) & ~15; }  // bytes of a row: q (k + 1), log q, the student's logits, classes,
 template <typename T>
 __host__ __device__ constexpr int td_wave_lds(int k, int V) {  // and the logits as they are stored (16 KiB at most)
@@ -367,8 +367,8 @@ __global__ __launch_bounds__(256) void td_wave_kernel(const TdArgs a) {
 }
 
 // V <= 32768: a row's logits in registers, up to NCH chunks of CH per thread, NW waves a row; loss, maximum and sum from one read. Bound by memory:
-// 16800 x 8192 fp32 210 us = 5.2 TB/s, 4200 x 32768 210 us; shorter 16-bit rows by what a row waits for, so as few waves as hold one: 20000 x 3001 bf16
-// 49 us with 2, 75 with 4.
+// 16800 x 8192 fp32 225 us = 4.9 TB/s, 4200 x 32768 223 us; shorter 16-bit rows by what a row waits for, so as few waves as hold one: bf16 with 2 and 4
+// 20000 x 2100 57 and 79 us, x 3001 63 and 79, x 4096 75 and 79.
 template <int DT, int GDT, int NW>
 __global__ __launch_bounds__(NW * 64, NW == 16 ? 8 : 1) void td_wide_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
@@ -442,9 +442,9 @@ __global__ __launch_bounds__(NW * 64, NW == 16 ? 8 : 1) void td_wide_kernel(cons
 }
 
 // longer rows, as they are stored (16 waves a row, NCH chunks of 16 bytes a thread): two exponentials a logit instead of a second read.
-// 8192 x 65536 bf16 388 us = 5.5 TB/s; NCH = 16 leaves one row a CU, whose loads and stores take turns: 4096 x 131072 bf16 479 us = 4.5 TB/s (walking over
+// 8192 x 65536 bf16 415 us = 5.2 TB/s; NCH = 16 leaves one row a CU, whose loads and stores take turns: 4096 x 131072 bf16 487 us = 4.4 TB/s (walking over
 // its rows, the next one's loads under this one's stores: 535). That form's time shows its instructions, so 16-bit rows take an exponent in one: z c - mu c,
-// with the rounding of mu c (at most 1/2) taken back out of the sum (as (z - mu) c: 505 us, fp16 511 against 467). Where mu c is beyond 2^24 two 16-bit logits
+// with the rounding of mu c (at most 1/2) taken back out of the sum (as (z - mu) c: 505 us, so 482; fp16 511 and 467). Where mu c is beyond 2^24 two 16-bit logits
 // are the same or 2^12 and more apart, and a power of two that makes the product exact stands in for c.
 template <int DT, int GDT, int NCH>
 __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const TdArgs a) {
@@ -534,7 +534,7 @@ __global__ __launch_bounds__(1024, NCH <= 8 ? 8 : 4) void td_held_kernel(const T
 }
 
 // rows that do not fit the registers: one pass for a running maximum and sum, a second one for the gradient; 16 waves a row
-// (1024 x 131072 fp32 312 us = 5.2 TB/s over its three passes)
+// (1024 x 131072 fp32 315 us = 5.1 TB/s over its three passes)
 template <int DT, int GDT>
 __global__ __launch_bounds__(1024) void td_long_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
@@ -619,7 +619,8 @@ __device__ __forceinline__ void td_get(const void* base, int64_t at, int n, floa
 // V <= L E, k <= L S: L lanes a row, E neighbouring classes and S slots a lane. A row's slots meet its classes in LDS: how far every class is below the maximum, and {q, 1} of the slot
 // that named it last; as many owned classes as filled slots means that no class was named twice. Few elements a lane leave it bound by its instructions, so a
 // lane takes four neighbours (6, 8 in longer rows) and, where k <= L, one slot: 268800 x 4 x 16 fp32, k = 16: 56 us = 5.1 TB/s, with a class and a slot a lane
-// and 16 lanes a row 82; 268800 x 80, k = 10: 31 us, with eight slots on each of two lanes 50.
+// and 16 lanes a row 82; 268800 x 80 fp32, k = 10: 40 us (eight slots on each of two lanes took 1.6 times
+// as long).
 template <int DT, int GDT, int L, int E, int S>
 __global__ __launch_bounds__(256) void td_narrow_kernel(const TdArgs a) {
     typedef typename TdElem<DT>::T T;
