@@ -2006,7 +2006,8 @@ extern "C" int64_t cdet_linear_loss_ws_bytes(const cdet_linear_loss_desc* d, int
 #define CDET_LIN_GRADS(who)                                                                                                                            \
     CDET_CHECK_ARG((!dx || (al16(dx) && dx_ld >= d->d && dx_ld % 8 == 0)) && (!dw || (al16(dw) && dw_ld >= d->d && dw_ld % 8 == 0)),                     \
                    who ": dx / dw must be 16-byte aligned with row pitches that are multiples of 8 and at least d");                                   \
-    CDET_CHECK_ARG(drow_stride == 0 || drow_stride == 1, who ": drow_stride must be 0 or 1");
+    CDET_CHECK_ARG(drow_stride == 0 || drow_stride == 1, who ": drow_stride must be 0 or 1");                                                           \
+    CDET_CHECK_ARG((!dx || dx != x) && (!dw || dw != w), who ": dx / dw may not take the place of x / w");
 
 extern "C" int cdet_linear_ce_fwd(const cdet_linear_loss_desc* d, const void* x, const void* w, const void* labels, float* loss, float* lse, void* ws, void* stream) {
     CDET_LIN_COMMON("cdet_linear_ce_fwd")

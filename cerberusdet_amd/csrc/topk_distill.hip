@@ -802,6 +802,16 @@ extern "C" int cdet_topk_distill(const cdet_topk_distill_desc* d, const void* lo
     CDET_CHECK_ARG(dlogits != logits || (d->grad_dtype == d->dtype && d->grad_ld == d->ld), "cdet_topk_distill: in place needs the logits' type and pitch");
     const int es = elem_size(d->dtype), gs = elem_size(d->grad_dtype);
     CDET_CHECK_ARG(((uintptr_t)logits % es) == 0 && ((uintptr_t)dlogits % gs) == 0, "cdet_topk_distill: logits / dlogits must be aligned to their elements");
+    if (dlogits && dlogits != logits) {  // beside the logits (another slice of their map, say), not half over them: rows are read while others are written
+        const uintptr_t z = (uintptr_t)logits, g = (uintptr_t)dlogits;
+        const int64_t zp = d->ld * es, gp = d->grad_ld * gs, zw = (int64_t)d->G * d->V * es, gw = (int64_t)d->G * d->V * gs;
+        bool apart = g >= z + (uintptr_t)((d->P - 1) * zp + zw) || z >= g + (uintptr_t)((d->P - 1) * gp + gw);
+        if (!apart && zp == gp) {
+            const int64_t in = ((int64_t)(g - z) % zp + zp) % zp;  // where in a pixel of the logits the gradient starts
+            apart = in >= zw && in + gw <= zp;
+        }
+        CDET_CHECK_ARG(apart, "cdet_topk_distill: the gradient overlaps the logits without being in their place");
+    }
     TdArgs a;
     a.z = logits;
     a.dz = dlogits;

@@ -498,7 +498,8 @@ int cdet_det_loss(const cdet_loss_desc* d, const void* f0, const void* f1, const
  *   lse     [N] log-sum-exp of the row;  saved [N, 1 + 2 k] fp32: what linear_distill's backward needs (opaque)
  *   tau     1e-18 .. 1e18; |scale| at most 1e38 tau
  *   drow    gradient of the rows' losses, fp32: [N] (drow_stride 1), one value (0), or NULL (ones)
- *   dx, dw  16-bit like x and w, either may be NULL; whole [V, d] of dw is written, the pitches' tails are not touched
+ *   dx, dw  16-bit like x and w, either may be NULL; whole [V, d] of dw is written, the pitches' tails are not touched. They must
+ *           not overlap x or w
  * ws: cdet_linear_loss_ws_bytes(d, backward) bytes, 16-byte aligned; contents need not survive between calls. N = 0 is allowed (dw = 0). */
 typedef struct {
     int32_t N, V, d;
@@ -519,11 +520,11 @@ int cdet_linear_distill_bwd(const cdet_linear_loss_desc* d, const void* x, const
 /* linear_distill's loss on logits that are in memory, loss AND gradient in one call (like cdet_det_loss): P pixels (rows) of G distributions of V
  * logits each -- the class logits of a head map (G = 1), its four 16-bin box distributions (G = 4, V = 16). Distribution g of pixel p starts at
  * logits + (p * ld + g * V) elements (pass the pointer of the first channel); its gradient, d(sum_r drow_r loss_r) / d logit * grad_scale, at
- * dlogits + (p * grad_ld + g * V). idx / val [P * G, k], drow [P * G] or NULL (ones), loss [P * G]. Everything else in a pixel's pitch is left as it is. A row takes part if it has
- * a filled slot that is not -inf and a logit that is not.
+ * dlogits + (p * grad_ld + g * V). idx / val [P * G, k], drow [P * G] or NULL (ones), loss [P * G]. Everything else in a pixel's pitch is left as it is.
+ * A row takes part if it has a filled slot that is not -inf and a logit that is not.
  * logits: fp32 / bf16 / fp16, any alignment of whole elements; -inf = a class left out. NaN in a row that takes part, in its logits or in a filled slot,
- * gives a loss of NaN. dlogits may be NULL (loss only) and may BE logits (same type
- * and pitch). */
+ * gives a loss of NaN. dlogits may be NULL (loss only) and may BE logits (same type and pitch); it may lie beside each pixel's logits (another slice of
+ * their map) and may not overlap them in any other way. */
 typedef struct {
     int32_t P, G, V, k;
     int32_t dtype, val_dtype, grad_dtype;

@@ -379,3 +379,25 @@ def test_linear_distill_of_the_most_rows():
     want = reference(x, w, idx=idx, val=val)["dw"]
     mag = reference(x, w, idx=idx, val=val)["dz"].abs().T @ x.double().abs()
     assert torch.all((dw.double() - want).abs() <= mag * (2.0 ** -6 + 2.0 ** -7) + 2.0 ** -8 * want.abs())
+
+
+@pytest.mark.parametrize("dtype,gdt", [(F32, F32), (BF, BF), (BF, F32)])
+@pytest.mark.parametrize("V", [16, 203, 3001])
+def test_gradient_beside_the_logits_in_one_map(V, dtype, gdt):
+    """Logits and gradient as slices of one buffer: back to back a pixel, and one behind the other; a gradient shifted over the logits is refused."""
+    ops, P, k = _ops(), 40, 5
+    z = (2 * _rand(P, V, seed=470)).to(dtype)
+    idx, val = distinct(P, V, k, 471)
+    loss, dz = ops.topk_distill(z, idx, val, grad_dtype=gdt)
+    wide = dtype.itemsize * ((V + 3) // 4 * 4)
+    pitch = wide + gdt.itemsize * (V + 8)
+    pitch += -pitch % 16
+    raw = torch.zeros(P, pitch, dtype=torch.uint8, device=DEV)
+    zs, gs = raw.view(dtype)[:, :V], raw[:, wide:].view(gdt)[:, 2:2 + V] if dtype == gdt else raw[:, wide + (-wide % 4):].view(gdt)[:, 2:2 + V]
+    zs.copy_(z)
+    got, out = ops.topk_distill(zs, idx, val, out=gs)
+    assert torch.equal(got, loss) and torch.equal(gs, dz) and torch.equal(zs, z)
+    if dtype == gdt:
+        with pytest.raises(RuntimeError, match="overlaps"):
+            ops.topk_distill(zs, idx, val, out=raw.view(dtype)[:, 1:1 + V])
+        assert torch.equal(zs, z)
