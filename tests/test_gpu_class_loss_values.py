@@ -401,3 +401,48 @@ def test_gradient_beside_the_logits_in_one_map(V, dtype, gdt):
         with pytest.raises(RuntimeError, match="overlaps"):
             ops.topk_distill(zs, idx, val, out=raw.view(dtype)[:, 1:1 + V])
         assert torch.equal(zs, z)
+
+
+@pytest.mark.parametrize("dtype,V", [(BF, 900), (F16, 9001), (F32, 70000)])
+def test_backward_from_the_logits_captured_and_on_two_streams(dtype, V):
+    """The gradient that the backward makes, captured and replayed on new logits with eager work in between; forward and backward of two streams at once."""
+    from cerberusdet_amd.utils import loss as UL
+
+    P, k = (40000 if V < 1000 else 600), 4
+    z = (2 * _rand(P, V, seed=480)).to(dtype)
+    assert dtype != F32 or z.numel() > UL._AHEAD
+    idx, val = teacher(P, V, k, 481)
+
+    def step(z):
+        leaf = z.detach().requires_grad_()
+        loss = UL.topk_distillation(leaf, idx, val, tau=2.0)
+        return [loss.detach(), *torch.autograd.grad(64.0 * loss, leaf)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(z)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(z)
+    for turn in range(4):
+        z.copy_(2 * _rand(P, V, seed=482 + turn))
+        graph.replay()
+        got = [o.clone() for o in outs]
+        want = step(z)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
+    zs = [z, z.flip(1).contiguous()]
+    want = [step(t) for t in zs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = []
+        for s, t in zip(streams, zs):
+            with torch.cuda.stream(s):
+                got.append(step(t))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
