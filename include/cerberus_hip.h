@@ -496,7 +496,7 @@ int cdet_det_loss(const cdet_loss_desc* d, const void* f0, const void* f1, const
  *           twice (its slots count separately). q = softmax of val / tau over the filled slots; a row without any takes no part; one that
  *           names a left-out class beside others has loss +inf (and that class no gradient). k <= 512.
  *   lse     [N] log-sum-exp of the row;  saved [N, 1 + 2 k] fp32: what linear_distill's backward needs (opaque)
- *   tau     1e-18 .. 1e18; |scale| at most 1e38 tau
+ *   tau     1e-18 .. 1e18; |scale| at most 1e38 tau. Logits are carried in log2 units: |z / tau| beyond 2.3e38 is infinite
  *   drow    gradient of the rows' losses, fp32: [N] (drow_stride 1), one value (0), or NULL (ones)
  *   dx, dw  16-bit like x and w, either may be NULL; whole [V, d] of dw is written, the pitches' tails are not touched. They must
  *           not overlap x or w
