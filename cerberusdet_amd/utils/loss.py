@@ -192,8 +192,8 @@ def topk_distillation(logits, idx, val, tau=1.0, reduction="mean"):
 class HeadDistillation:
     """Distillation of a task's Detect head from a teacher's head maps of the same strides: `HeadDistillation(model, k, tau)(preds, teacher_preds, task)` ->
     (scalar, items[2]), items = (box, cls). Box: the four reg_max-bin distributions of every pixel against the teacher's; cls: the class logits against the
-    teacher's k largest. Both are means over the pixels of all maps (box: and their four distributions), weighted by `box` and `cls`. preds: three NCHW maps as Loss takes them (the model's NHWC
-    buffers are read in place)."""
+    teacher's k largest. Both are means over the pixels of all maps (box: and their four distributions), weighted by `box` and `cls`. preds: three NCHW maps
+    as Loss takes them (the model's NHWC buffers are read in place)."""
 
     def __init__(self, model, k=16, tau=2.0, box=1.0, cls=1.0):
         self.k, self.tau, self.box, self.cls = int(k), float(tau), float(box), float(cls)
